@@ -1,0 +1,249 @@
+// C ABI entry points of the gated delta rule (include/ftc_causal_product.h): argument checking, workspaces and the
+// sequence of launches.  The kernels: ftc_delta_{prepare,scan,outputs,gradients,step}.hip.
+#include "ftc_delta_kernel.h"
+
+namespace ftc {
+namespace delta {
+namespace {
+
+// Calls of up to this many positions run position by position: a chunk's three launches take as long however
+// few of its 64 positions there are.
+constexpr int64_t kStepMost = 8;
+constexpr int64_t kMostRowStride = 1 << 22;  // elements between positions: a chunk's offsets stay below 2 GiB
+
+struct Sizes {
+    int64_t N, H, Hk, L, E, M;
+    int64_t chunks() const { return (L + kRows - 1) / kRows; }
+    int64_t col_blocks() const { return (M + kCols - 1) / kCols; }
+    int64_t tiles() const { return E <= 64 ? 4 : 8; }
+    int64_t units() const { return N * H * chunks(); }  // chunks of all chains
+    // floats (all multiples of 64)
+    int64_t factors() const { return units() * kFactors * kRows; }
+    int64_t t() const { return units() * 3 * kRows * kRows / 2; }
+    int64_t s() const { return units() * col_blocks() * tiles() * 256; }
+    int64_t z() const { return units() * col_blocks() * 4 * 256; }
+    int64_t zdu() const { return units() * col_blocks() * kRows; }
+    int64_t kept() const { return 4 * (factors() + t() + s() + z()); }
+    int64_t backward() const { return 4 * (s() + z() + zdu()); }
+};
+
+int check_sizes(const Sizes &s) {
+    if (s.N < 0 || s.H < 0 || s.Hk < 0 || s.L < 0 || s.E < 0 || s.M < 0) return fail(FTC_ERR_INVALID, "negative size");
+    if (s.H > 0 && (s.Hk == 0 || s.H % s.Hk != 0))
+        return fail(FTC_ERR_INVALID, "the number of value heads (%lld) must be a multiple of the number of key heads (%lld)",
+                    (long long)s.H, (long long)s.Hk);
+    if (s.E < 1 || s.E > kMaxE || s.M < 1 || s.M > 512)
+        return fail(FTC_ERR_UNSUPPORTED, "the gated delta rule takes key rows of 1 to 128 values and value rows of 1 to "
+                    "512, got %lld and %lld", (long long)s.E, (long long)s.M);
+    if (s.N > 0x7fffffff || s.H > 0x7fffffff || s.L > 0x7fffff00 ||
+        (s.N * s.H > 0 && (s.N * s.H > 0x7fffffff || s.N * s.H * s.col_blocks() > 0x7fffffff / (s.chunks() + 1))))
+        return fail(FTC_ERR_UNSUPPORTED, "too many chains, positions and columns for one call");
+    return FTC_OK;
+}
+
+int check_rows(const ftc_tensor4 *t, const char *name, int64_t N, int64_t H, int64_t L, int64_t X, int dtype) {
+    if (!t) return fail(FTC_ERR_INVALID, "%s is null", name);
+    if (t->dtype != FTC_F32 && t->dtype != FTC_BF16)
+        return fail(FTC_ERR_INVALID, "%s has dtype code %d, expected FTC_F32 or FTC_BF16", name, (int)t->dtype);
+    if (dtype >= 0 && t->dtype != dtype)
+        return fail(FTC_ERR_INVALID, "%s has dtype code %d, expected %d", name, (int)t->dtype, dtype);
+    if (t->size[0] != N || t->size[1] != H || t->size[2] != L || t->size[3] != X)
+        return fail(FTC_ERR_INVALID, "%s has shape (%lld,%lld,%lld,%lld), expected (%lld,%lld,%lld,%lld)", name,
+                    (long long)t->size[0], (long long)t->size[1], (long long)t->size[2], (long long)t->size[3],
+                    (long long)N, (long long)H, (long long)L, (long long)X);
+    if (N * H * L == 0) return FTC_OK;
+    if (!t->ptr) return fail(FTC_ERR_INVALID, "%s has a null data pointer", name);
+    if (X > 1 && t->stride[3] != 1)
+        return fail(FTC_ERR_INVALID, "%s must be contiguous in its last dimension (stride %lld)", name,
+                    (long long)t->stride[3]);
+    if (L > 1 && (t->stride[2] < 0 || t->stride[2] > kMostRowStride))
+        return fail(FTC_ERR_UNSUPPORTED, "%s has rows %lld elements apart, at most %lld are supported", name,
+                    (long long)t->stride[2], (long long)kMostRowStride);
+    return FTC_OK;
+}
+int check_state(const ftc_tensor4 *t, const char *name, const Sizes &s) {
+    if (!t) return FTC_OK;
+    if (t->dtype != FTC_F32) return fail(FTC_ERR_INVALID, "%s must be FTC_F32", name);
+    if (t->size[0] != s.N || t->size[1] != s.H || t->size[2] != s.E || t->size[3] != s.M)
+        return fail(FTC_ERR_INVALID, "%s has shape (%lld,%lld,%lld,%lld), expected (%lld,%lld,%lld,%lld)", name,
+                    (long long)t->size[0], (long long)t->size[1], (long long)t->size[2], (long long)t->size[3],
+                    (long long)s.N, (long long)s.H, (long long)s.E, (long long)s.M);
+    if (s.N * s.H == 0) return FTC_OK;
+    if (!t->ptr) return fail(FTC_ERR_INVALID, "%s has a null data pointer", name);
+    if (s.M > 1 && t->stride[3] != 1) return fail(FTC_ERR_INVALID, "%s must be contiguous in its last dimension", name);
+    return FTC_OK;
+}
+
+bool reads_wide(const Operand &o) {
+    const int bytes = o.dtype == FTC_F32 ? 4 : 2, lot = 16 / bytes;
+    return o.width % lot == 0 && ((uintptr_t)o.ptr & 15) == 0 && o.stride_n % lot == 0 && o.stride_h % lot == 0 &&
+           o.stride_l % lot == 0;
+}
+Scalars scalars(const ftc_tensor4 *t) {
+    return t ? Scalars{t->ptr, t->stride[0], t->stride[1], t->stride[2], t->dtype} : Scalars{};
+}
+StateRef state(const ftc_tensor4 *t) {
+    return t ? StateRef{(float *)t->ptr, t->stride[0], t->stride[1], t->stride[2]} : StateRef{};
+}
+OperandOut rows_out(const ftc_tensor4 *t) { return t ? as_operand_out(t) : OperandOut{}; }
+
+// The inputs that both directions have
+int read_inputs(const ftc_tensor4 *q, const ftc_tensor4 *k, const ftc_tensor4 *v, const ftc_tensor4 *g, const ftc_tensor4 *b,
+                Sizes *s, DeltaArgs *p) {
+    if (!q || !v) return fail(FTC_ERR_INVALID, "queries or values is null");
+    *s = Sizes{v->size[0], v->size[1], q->size[1], v->size[2], q->size[3], v->size[3]};
+    if (int rc = check_sizes(*s)) return rc;
+    if (int rc = check_rows(q, "queries", s->N, s->Hk, s->L, s->E, -1)) return rc;
+    if (int rc = check_rows(k, "keys", s->N, s->Hk, s->L, s->E, q->dtype)) return rc;
+    if (int rc = check_rows(v, "values", s->N, s->H, s->L, s->M, q->dtype)) return rc;
+    if (int rc = check_rows(g, "log_decay", s->N, s->H, s->L, 1, -1)) return rc;
+    if (int rc = check_rows(b, "beta", s->N, s->H, s->L, 1, -1)) return rc;
+    p->q = as_operand(q), p->k = as_operand(k), p->v = as_operand(v);
+    p->g = scalars(g), p->b = scalars(b);
+    p->N = (int32_t)s->N, p->H = (int32_t)s->H, p->Hk = (int32_t)s->Hk, p->L = (int32_t)s->L;
+    p->E = (int32_t)s->E, p->M = (int32_t)s->M;
+    p->chunks = (int32_t)s->chunks(), p->col_blocks = (int32_t)s->col_blocks();
+    p->vec_q = reads_wide(p->q), p->vec_k = reads_wide(p->k);
+    return FTC_OK;
+}
+void place_kept(const Sizes &s, void *kept, DeltaArgs *p) {
+    p->factors = (float *)kept;
+    p->s = p->factors + s.factors();
+    p->z = p->s + s.s();
+    p->t = (uint16_t *)(p->z + s.z());
+}
+int launched(const char *name) {
+    note_kernel(name);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? FTC_OK : fail(FTC_ERR_HIP, "%s: %s", name, hipGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace delta
+}  // namespace ftc
+
+using namespace ftc;
+using namespace ftc::delta;
+
+extern "C" {
+
+static int64_t delta_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M, int what) {
+    const Sizes s{N, H, Hk, L, E, M};
+    if (int rc = check_sizes(s)) return rc;
+    return what == 1 ? s.backward() : s.kept();
+}
+int64_t ftc_gated_delta_rule_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M) {
+    const int64_t bytes = delta_bytes(N, H, Hk, L, E, M, 0);
+    return bytes > 0 && L <= kStepMost ? 0 : bytes;
+}
+int64_t ftc_gated_delta_rule_kept_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M) {
+    return delta_bytes(N, H, Hk, L, E, M, 0);
+}
+int64_t ftc_gated_delta_rule_backward_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M) {
+    return delta_bytes(N, H, Hk, L, E, M, 1);
+}
+
+int ftc_gated_delta_rule(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,
+                         const ftc_tensor4 *log_decay, const ftc_tensor4 *beta, const int64_t *lengths, float scale,
+                         int32_t normalize, const ftc_tensor4 *initial_state, const ftc_tensor4 *out,
+                         const ftc_tensor4 *final_state, void *kept, size_t kept_bytes, void *workspace,
+                         size_t workspace_bytes, void *stream) {
+    Sizes s;
+    DeltaArgs p = {};
+    if (int rc = read_inputs(queries, keys, values, log_decay, beta, &s, &p)) return rc;
+    if (int rc = check_rows(out, "out", s.N, s.H, s.L, s.M, queries->dtype)) return rc;
+    if (int rc = check_state(initial_state, "initial_state", s)) return rc;
+    if (int rc = check_state(final_state, "final_state", s)) return rc;
+    if (s.N * s.H == 0) return FTC_OK;
+    p.out = rows_out(out), p.initial = state(initial_state), p.final_ = state(final_state);
+    p.lengths = lengths, p.scale = scale, p.normalize = normalize != 0;
+    if (s.L == 0 && !final_state) return FTC_OK;
+    if (!kept && s.L <= kStepMost) {
+        delta_steps(p, (hipStream_t)stream);
+        return launched("delta_step_kernel");
+    }
+    if (s.L == 0) {  // the state as it came
+        delta_steps(p, (hipStream_t)stream);
+        return launched("delta_step_kernel");
+    }
+    const int64_t need = s.kept();
+    void *const at = kept ? kept : workspace;
+    if (!at || (int64_t)(kept ? kept_bytes : workspace_bytes) < need)
+        return fail(FTC_ERR_WORKSPACE, "ftc_gated_delta_rule needs %lld bytes", (long long)need);
+    if ((uintptr_t)at & 255) return fail(FTC_ERR_WORKSPACE, "the workspace must be 256-byte aligned");
+    place_kept(s, at, &p);
+    const bool bf16 = queries->dtype == FTC_BF16;
+    delta_prepare(p, bf16, (hipStream_t)stream);
+    delta_scan(p, bf16, (hipStream_t)stream);
+    delta_outputs(p, bf16, (hipStream_t)stream);
+    return launched("delta_scan_kernel");
+}
+
+int ftc_gated_delta_rule_backward(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,
+                                  const ftc_tensor4 *log_decay, const ftc_tensor4 *beta, const int64_t *lengths,
+                                  float scale, int32_t normalize, const void *kept, size_t kept_bytes,
+                                  const ftc_tensor4 *grad_out, const ftc_tensor4 *grad_final_state,
+                                  const ftc_tensor4 *grad_queries, const ftc_tensor4 *grad_keys,
+                                  const ftc_tensor4 *grad_values, const ftc_tensor4 *grad_log_decay,
+                                  const ftc_tensor4 *grad_beta, const ftc_tensor4 *grad_initial_state, void *workspace,
+                                  size_t workspace_bytes, void *stream) {
+    Sizes s;
+    DeltaArgs p = {};
+    if (int rc = read_inputs(queries, keys, values, log_decay, beta, &s, &p)) return rc;
+    if (int rc = check_rows(grad_out, "grad_out", s.N, s.H, s.L, s.M, queries->dtype)) return rc;
+    if (int rc = check_state(grad_final_state, "grad_final_state", s)) return rc;
+    if (int rc = check_state(grad_initial_state, "grad_initial_state", s)) return rc;
+    struct {
+        const ftc_tensor4 *t;
+        const char *name;
+        int64_t heads, width;
+        int dtype;
+    } const grads[] = {{grad_queries, "grad_queries", s.Hk, s.E, queries->dtype}, {grad_keys, "grad_keys", s.Hk, s.E, queries->dtype},
+                       {grad_values, "grad_values", s.H, s.M, queries->dtype}, {grad_log_decay, "grad_log_decay", s.H, 1, log_decay->dtype},
+                       {grad_beta, "grad_beta", s.H, 1, beta->dtype}};
+    for (const auto &g : grads)
+        if (g.t)
+            if (int rc = check_rows(g.t, g.name, s.N, g.heads, s.L, g.width, g.dtype)) return rc;
+    if (s.N * s.H == 0 || (s.L == 0 && !grad_initial_state)) return FTC_OK;
+    if (s.L == 0) return fail(FTC_ERR_INVALID, "a call of no positions has no backward");
+    if (!kept || (int64_t)kept_bytes < s.kept())
+        return fail(FTC_ERR_WORKSPACE, "ftc_gated_delta_rule_backward needs the %lld bytes that the forward kept",
+                    (long long)s.kept());
+    if (!workspace || (int64_t)workspace_bytes < s.backward())
+        return fail(FTC_ERR_WORKSPACE, "ftc_gated_delta_rule_backward needs %lld bytes of workspace", (long long)s.backward());
+    if (((uintptr_t)kept | (uintptr_t)workspace) & 255)
+        return fail(FTC_ERR_WORKSPACE, "the workspace must be 256-byte aligned");
+    p.lengths = lengths, p.scale = scale, p.normalize = normalize != 0;
+    place_kept(s, (void *)kept, &p);
+    p.ds = (float *)workspace, p.de = p.ds + s.s(), p.zdu = p.de + s.z();
+    p.go = as_operand(grad_out);
+    p.gq = rows_out(grad_queries), p.gk = rows_out(grad_keys), p.gv = rows_out(grad_values);
+    p.gg = scalars(grad_log_decay), p.gb = scalars(grad_beta);
+    p.grad_final = state(grad_final_state), p.grad_initial = state(grad_initial_state);
+    const bool bf16 = queries->dtype == FTC_BF16;
+    delta_pull(p, bf16, (hipStream_t)stream);
+    delta_scan_back(p, bf16, (hipStream_t)stream);
+    if (grad_queries || grad_keys || grad_log_decay || grad_beta) delta_gradients(p, bf16, (hipStream_t)stream);
+    return launched("delta_gradients_kernel");
+}
+
+int ftc_gated_delta_step(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,
+                         const ftc_tensor4 *log_decay, const ftc_tensor4 *beta, float scale, int32_t normalize,
+                         const ftc_tensor4 *state_in_out, const ftc_tensor4 *out, void *stream) {
+    Sizes s;
+    DeltaArgs p = {};
+    if (int rc = read_inputs(queries, keys, values, log_decay, beta, &s, &p)) return rc;
+    if (int rc = check_rows(out, "out", s.N, s.H, s.L, s.M, queries->dtype)) return rc;
+    if (!state_in_out) return fail(FTC_ERR_INVALID, "state is null");
+    if (int rc = check_state(state_in_out, "state", s)) return rc;
+    if (s.N * s.H == 0 || s.L == 0) return FTC_OK;
+    if ((s.N > 1 && state_in_out->stride[0] == 0) || (s.H > 1 && state_in_out->stride[1] == 0) ||
+        (s.E > 1 && state_in_out->stride[2] < s.M))
+        return fail(FTC_ERR_INVALID, "state is written and must not overlap itself");
+    p.out = rows_out(out), p.initial = p.final_ = state(state_in_out);
+    p.scale = scale, p.normalize = normalize != 0;
+    delta_steps(p, (hipStream_t)stream);
+    return launched("delta_step_kernel");
+}
+
+}  // extern "C"

@@ -46,6 +46,12 @@ EXPORTED_SYMBOLS = (
     "ftc_layer_norm_stats_split",
     "ftc_linear_split",
     "ftc_linear_split_normed",
+    "ftc_gated_delta_rule_workspace_bytes",
+    "ftc_gated_delta_rule_kept_bytes",
+    "ftc_gated_delta_rule",
+    "ftc_gated_delta_rule_backward_workspace_bytes",
+    "ftc_gated_delta_rule_backward",
+    "ftc_gated_delta_step",
 )
 
 
@@ -140,6 +146,19 @@ def load():
     lib.ftc_causal_linear_attention_wide_backward.restype = ctypes.c_int
     lib.ftc_causal_linear_attention_wide_backward.argtypes = [t4] * 3 + [ctypes.c_void_p] + [t4] * 6 + [
         ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    for name in ("ftc_gated_delta_rule_workspace_bytes", "ftc_gated_delta_rule_kept_bytes",
+                 "ftc_gated_delta_rule_backward_workspace_bytes"):
+        f = getattr(lib, name)
+        f.restype = ctypes.c_int64
+        f.argtypes = [ctypes.c_int64] * 6
+    scalars = [ctypes.c_void_p, ctypes.c_float, ctypes.c_int32]  # lengths, scale, normalize
+    memory = [ctypes.c_void_p, ctypes.c_size_t]
+    lib.ftc_gated_delta_rule.restype = ctypes.c_int
+    lib.ftc_gated_delta_rule.argtypes = [t4] * 5 + scalars + [t4] * 3 + memory * 2 + [ctypes.c_void_p]
+    lib.ftc_gated_delta_rule_backward.restype = ctypes.c_int
+    lib.ftc_gated_delta_rule_backward.argtypes = [t4] * 5 + scalars + memory + [t4] * 8 + memory + [ctypes.c_void_p]
+    lib.ftc_gated_delta_step.restype = ctypes.c_int
+    lib.ftc_gated_delta_step.argtypes = [t4] * 5 + scalars[1:] + [t4] * 2 + [ctypes.c_void_p]
     lib.ftc_causal_dot_plan.restype = ctypes.c_int
     lib.ftc_causal_dot_plan.argtypes = [t4] * 3 + [ctypes.c_int, ctypes.c_char_p, ctypes.c_size_t]
     _lib = lib

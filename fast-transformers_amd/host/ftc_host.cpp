@@ -712,6 +712,160 @@ Tensor encoder(const Tensor &x, const std::vector<Layer> &layers, const std::opt
     return out;
 }
 
+// ---- the gated delta rule (delta_rule/__init__.py) ----
+// Its memory comes from torch's allocator with every call (in a captured graph from the graph's own pool), so
+// calls on different streams and replays of different graphs never share any.
+struct DeltaTensors {
+    Tensor q, k, v, g, b;
+    ftc_tensor4 dq, dk, dv, dg, db;
+};
+// rows with unit inner stride whose positions are at most 2^22 elements apart
+Tensor delta_rows(const Tensor &t, const char *name, const Tensor &like) {
+    if (t.dim() != 4 || t.device() != like.device())
+        error(std::string("gated_delta_rule: ") + name + " must be 4-dimensional (N, H, L, X), on the device of the queries");
+    if ((t.size(3) > 1 && t.stride(3) != 1) || (t.size(2) > 1 && t.stride(2) > (1 << 22))) return t.contiguous();
+    return t;
+}
+// (N, H, L) -> the (N, H, L, 1) that the library takes
+Tensor delta_scalars(const Tensor &t, const char *name, const Tensor &like) {
+    if (t.dim() != 3 || t.device() != like.device())
+        error(std::string("gated_delta_rule: ") + name + " must be 3-dimensional (N, H, L), on the device of the queries");
+    const Tensor rows = t.unsqueeze(3);
+    return rows.size(2) > 1 && rows.stride(2) > (1 << 22) ? rows.contiguous() : rows;
+}
+ftc_tensor4 delta_describe(const Tensor &t, const char *name) {
+    if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16)
+        error(std::string("gated_delta_rule: ") + name + " must be float32 or bfloat16, got " +
+              py::str(py::cast(t.scalar_type())).cast<std::string>());
+    return describe(t);
+}
+DeltaTensors delta_tensors(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &log_decay,
+                           const Tensor &beta) {
+    if (!queries.is_cuda()) error("gated_delta_rule: queries are on " + queries.device().str() + ", expected a GPU tensor");
+    DeltaTensors t;
+    t.q = delta_rows(queries, "queries", queries), t.k = delta_rows(keys, "keys", queries);
+    t.v = delta_rows(values, "values", queries);
+    t.g = delta_scalars(log_decay, "log_decay", queries), t.b = delta_scalars(beta, "beta", queries);
+    t.dq = delta_describe(t.q, "queries"), t.dk = delta_describe(t.k, "keys"), t.dv = delta_describe(t.v, "values");
+    t.dg = delta_describe(t.g, "log_decay"), t.db = delta_describe(t.b, "beta");
+    return t;
+}
+struct DeltaState {
+    Tensor t;
+    ftc_tensor4 d;
+    const ftc_tensor4 *p = nullptr;
+    DeltaState(const OptTensor &from, const char *name, const Tensor &like) {
+        if (!from) return;
+        if (from->dim() != 4 || from->scalar_type() != at::kFloat || from->device() != like.device())
+            error(std::string("gated_delta_rule: ") + name + " must be a float32 tensor (N, H, E, M) on the device of the queries");
+        t = from->size(3) > 1 && from->stride(3) != 1 ? from->contiguous() : *from;
+        d = describe(t), p = &d;
+    }
+};
+const int64_t *delta_lengths(const OptTensor &lengths, const Tensor &q) {
+    if (!lengths) return nullptr;
+    if (lengths->scalar_type() != at::kLong || lengths->device() != q.device() || lengths->dim() != 1 ||
+        lengths->size(0) != q.size(0) || !lengths->is_contiguous())
+        error("gated_delta_rule: lengths must be a contiguous int64 tensor of N values on the device of the queries");
+    return lengths->const_data_ptr<int64_t>();
+}
+Tensor delta_memory(int64_t bytes, const char *what, const Tensor &like) {
+    check(bytes, what);
+    return at::empty({bytes}, like.options().dtype(at::kByte));
+}
+
+// (out, final state or None, what the backward needs or None)
+std::tuple<Tensor, OptTensor, OptTensor> delta_rule(const Tensor &queries, const Tensor &keys, const Tensor &values,
+                                                    const Tensor &log_decay, const Tensor &beta,
+                                                    const OptTensor &initial_state, const OptTensor &lengths, double scale,
+                                                    bool normalize, bool return_state, bool keep) {
+    const at::NoGradGuard no_grad;
+    const DeltaTensors t = delta_tensors(queries, keys, values, log_decay, beta);
+    const c10::DeviceGuard guard(t.q.device());
+    const int64_t N = t.v.size(0), H = t.v.size(1), Hk = t.q.size(1), L = t.v.size(2), E = t.q.size(3), M = t.v.size(3);
+    const DeltaState s0(initial_state, "initial_state", t.q);
+    const int64_t *const len = delta_lengths(lengths, t.q);
+    // (N, L, H, M) storage, as the next projection takes it
+    const Tensor out = at::empty({N, L, H, M}, t.v.options()).permute({0, 2, 1, 3});
+    OptTensor s1;
+    if (return_state) s1 = at::empty({N, H, E, M}, t.v.options().dtype(at::kFloat));
+    const Tensor memory = keep ? delta_memory(ftc_gated_delta_rule_kept_bytes(N, H, Hk, L, E, M), "ftc_gated_delta_rule_kept_bytes", t.q)
+                               : delta_memory(ftc_gated_delta_rule_workspace_bytes(N, H, Hk, L, E, M),
+                                              "ftc_gated_delta_rule_workspace_bytes", t.q);
+    const ftc_tensor4 dout = describe(out);
+    const Out d1(s1, "final_state");
+    hipStream_t const stream = c10::hip::getCurrentHIPStream(t.q.device().index()).stream();
+    void *const kept = keep ? memory.data_ptr() : nullptr;
+    void *const ws = keep ? nullptr : memory.data_ptr();
+    const int rc = native([&] {
+        return ftc_gated_delta_rule(&t.dq, &t.dk, &t.dv, &t.dg, &t.db, len, (float)scale, normalize, s0.p, &dout, d1.p,
+                                    kept, (size_t)memory.numel(), ws, (size_t)memory.numel(), stream);
+    });
+    check(rc, "ftc_gated_delta_rule");
+    return {out, s1, keep ? OptTensor(memory) : OptTensor()};
+}
+
+// gradients of queries, keys, values, log_decay, beta and the initial state (None where not needed)
+std::vector<OptTensor> delta_rule_backward(const Tensor &queries, const Tensor &keys, const Tensor &values,
+                                           const Tensor &log_decay, const Tensor &beta, const OptTensor &lengths,
+                                           double scale, bool normalize, const Tensor &kept, const Tensor &grad_out,
+                                           const OptTensor &grad_final_state, const std::vector<bool> &needed) {
+    const at::NoGradGuard no_grad;
+    const DeltaTensors t = delta_tensors(queries, keys, values, log_decay, beta);
+    const c10::DeviceGuard guard(t.q.device());
+    const int64_t N = t.v.size(0), H = t.v.size(1), Hk = t.q.size(1), L = t.v.size(2), E = t.q.size(3), M = t.v.size(3);
+    const Tensor go = delta_rows(grad_out, "grad_out", t.q);
+    const DeltaState g1(grad_final_state, "grad_final_state", t.q);
+    const int64_t *const len = delta_lengths(lengths, t.q);
+    std::vector<OptTensor> grads(6);
+    const Tensor *const inputs[] = {&queries, &keys, &values, &log_decay, &beta};
+    for (int i = 0; i < 5; i++)  // (stored as a projection's output is: positions before heads)
+        if (needed[i]) {
+            const Tensor &x = *inputs[i];
+            grads[i] = x.dim() == 4 ? at::empty({x.size(0), x.size(2), x.size(1), x.size(3)}, x.options()).permute({0, 2, 1, 3})
+                                    : at::empty({x.size(0), x.size(2), x.size(1)}, x.options()).permute({0, 2, 1});
+        }
+    if (needed[5]) grads[5] = at::empty({N, H, E, M}, t.q.options().dtype(at::kFloat));
+    auto wide = [](const OptTensor &x) { return x ? OptTensor(x->unsqueeze(3)) : OptTensor(); };
+    const Out gq(grads[0], "grad_queries"), gk(grads[1], "grad_keys"), gv(grads[2], "grad_values"),
+        gg(wide(grads[3]), "grad_log_decay"), gb(wide(grads[4]), "grad_beta"), g0(grads[5], "grad_initial_state");
+    const ftc_tensor4 dgo = delta_describe(go, "grad_out");
+    const Tensor ws = delta_memory(ftc_gated_delta_rule_backward_workspace_bytes(N, H, Hk, L, E, M),
+                                   "ftc_gated_delta_rule_backward_workspace_bytes", t.q);
+    hipStream_t const stream = c10::hip::getCurrentHIPStream(t.q.device().index()).stream();
+    const void *const held = kept.const_data_ptr();
+    void *const at = ws.data_ptr();
+    const int rc = native([&] {
+        return ftc_gated_delta_rule_backward(&t.dq, &t.dk, &t.dv, &t.dg, &t.db, len, (float)scale, normalize, held,
+                                             (size_t)kept.numel(), &dgo, g1.p, gq.p, gk.p, gv.p, gg.p, gb.p, g0.p, at,
+                                             (size_t)ws.numel(), stream);
+    });
+    check(rc, "ftc_gated_delta_rule_backward");
+    return grads;
+}
+
+// One token: queries, keys (N, Hk, E), values (N, H, M), log_decay, beta (N, H), state (N, H, E, M) in place
+Tensor delta_step(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &log_decay,
+                  const Tensor &beta, const Tensor &state, double scale, bool normalize) {
+    const at::NoGradGuard no_grad;
+    if (queries.dim() != 3 || keys.dim() != 3 || values.dim() != 3 || log_decay.dim() != 2 || beta.dim() != 2)
+        error("gated_delta_step: expected queries and keys (N, Hk, E), values (N, H, M), log_decay and beta (N, H)");
+    const DeltaTensors t = delta_tensors(queries.unsqueeze(2), keys.unsqueeze(2), values.unsqueeze(2),
+                                         log_decay.unsqueeze(2), beta.unsqueeze(2));
+    const c10::DeviceGuard guard(t.q.device());
+    if (state.size(-1) > 1 && state.stride(-1) != 1)
+        error("gated_delta_step: state is updated in place and must be contiguous in its last dimension");
+    const DeltaState s(state, "state", t.q);
+    const Tensor out = at::empty(values.sizes(), values.options());
+    const ftc_tensor4 dout = describe(out.unsqueeze(2));
+    hipStream_t const stream = c10::hip::getCurrentHIPStream(t.q.device().index()).stream();
+    const int rc = native([&] {
+        return ftc_gated_delta_step(&t.dq, &t.dk, &t.dv, &t.dg, &t.db, (float)scale, normalize, s.p, &dout, stream);
+    });
+    check(rc, "ftc_gated_delta_step");
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ftc_host, m) {
@@ -729,4 +883,7 @@ PYBIND11_MODULE(_ftc_host, m) {
     py::class_<Layer>(m, "Layer").def(
         py::init<Linear, Linear, Linear, Linear, Linear, Linear, Norm, Norm, double>());
     m.def("encoder", &encoder);
+    m.def("delta_rule", &delta_rule);
+    m.def("delta_rule_backward", &delta_rule_backward);
+    m.def("delta_step", &delta_step);
 }

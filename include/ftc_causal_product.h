@@ -333,6 +333,56 @@ int ftc_linear_split_normed(const void *x, const float *x_scale, int64_t tokens,
                             const float *bias, int64_t features, int64_t k, const float *rows, const float *stats,
                             const float *gamma, const float *beta, float *out, void *stream);
 
+/*
+ * The gated delta rule: linear attention whose state fades and whose write corrects what the state holds for
+ * the key.  Beside ftc_causal_dot_product_state; no counterpart in the reference.  Per chain of a value head, on a
+ * state S of E x M in fp32:
+ *
+ *   S' = exp(g_l) S_{l-1},  z_l = v_l - S'^T k_l,  S_l = S' + k_l (beta_l z_l)^T,  out_l = scale S_l^T q_l
+ *
+ * queries, keys: (N,Hk,L,E); values, out: (N,H,L,M) of the same dtype, FTC_F32 or FTC_BF16; H is a multiple of Hk,
+ * value head h reads key head h / (H / Hk).  log_decay (g), beta: (N,H,L,1), either dtype.  normalize: q and k are
+ * divided by sqrt(|x|^2 + 1e-6) first.  lengths: N int64 values on the device, or NULL; positions at or past
+ * lengths[n] leave the state as it is, their rows are not looked at and their outputs are zero.  initial_state
+ * (NULL: zeros), final_state (NULL: not wanted): (N,H,E,M), FTC_F32, unit stride along M; they may be one tensor.
+ * Log decays may be -infinity (the state is forgotten).  Sizes: E from 1 to 128, M from 1 to 512, L from 0 on;
+ * rows at most 2^22 elements apart; anything else returns FTC_ERR_UNSUPPORTED.
+ *
+ * kept: memory of ftc_gated_delta_rule_kept_bytes that the backward reads (the states before every 64th
+ * position among it), or NULL for a forward without one, which then needs `workspace`.  Neither needs
+ * initialisation, both are 256-byte aligned.
+ */
+int64_t ftc_gated_delta_rule_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M);
+int64_t ftc_gated_delta_rule_kept_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M);
+int ftc_gated_delta_rule(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,
+                         const ftc_tensor4 *log_decay, const ftc_tensor4 *beta, const int64_t *lengths, float scale,
+                         int32_t normalize, const ftc_tensor4 *initial_state, const ftc_tensor4 *out,
+                         const ftc_tensor4 *final_state, void *kept, size_t kept_bytes, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/*
+ * Its gradients, given grad_out and grad_final_state (NULL: zeros) and what the forward kept.  The inputs are
+ * those of the forward; gradients have their inputs' dtypes (grad_initial_state: FTC_F32), those of positions past
+ * a sequence's end are zero, and one that is not wanted may be NULL.  L >= 1.
+ */
+int64_t ftc_gated_delta_rule_backward_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M);
+int ftc_gated_delta_rule_backward(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,
+                                  const ftc_tensor4 *log_decay, const ftc_tensor4 *beta, const int64_t *lengths,
+                                  float scale, int32_t normalize, const void *kept, size_t kept_bytes,
+                                  const ftc_tensor4 *grad_out, const ftc_tensor4 *grad_final_state,
+                                  const ftc_tensor4 *grad_queries, const ftc_tensor4 *grad_keys,
+                                  const ftc_tensor4 *grad_values, const ftc_tensor4 *grad_log_decay,
+                                  const ftc_tensor4 *grad_beta, const ftc_tensor4 *grad_initial_state, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+
+/*
+ * One position of the rule (or a few) for sequences that are being generated: tensors as above, `state` is
+ * updated in place.  One launch, no workspace.
+ */
+int ftc_gated_delta_step(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,
+                         const ftc_tensor4 *log_decay, const ftc_tensor4 *beta, float scale, int32_t normalize,
+                         const ftc_tensor4 *state, const ftc_tensor4 *out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
