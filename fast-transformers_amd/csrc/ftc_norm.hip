@@ -1,0 +1,604 @@
+// The norms around a block, its gate and residual in one pass over the rows, and their gradients.
+//
+//   n = norm_after(block),  y = n w_a + b_a,  x = residual + scale act(gate) y,  h = norm_before(x) w_b + b_b
+//   norm: (r - mean) / sqrt(variance + eps), or r / sqrt(mean of squares + eps), or r itself
+//
+// Backward, with x^ the normalised x and the norms' statistics from the forward:
+//   dx = grad_x + rstd (w_b grad_h - [mean of it] - x^ mean(w_b grad_h x^)),   grad_residual = dx
+//   dy = scale act(gate) dx,   grad_gate = scale act'(gate) y dx,   grad_block = the same of the first norm, from dy
+//   gradients of w_b, b_b, w_a, b_a: sums over the rows of grad_h x^, grad_h, dy n, dy
+//
+// What bounds it is memory: every row is read once and written once, held in registers in between (x is made again in
+// the backward from the same rows that it has to read anyway: a stored x in 16 bits would spoil the gradients of w_b).
+// A team of 16 to 1024 lanes takes a row, eight values a lane at a time; the workgroup walks its rows and keeps the
+// sums for the parameters in registers, leaves them in the workspace, and a second kernel adds them up in a fixed
+// order.  A gate that several rows share is summed the same way: a workgroup's rows all belong to one of its rows.
+// All arithmetic is fp32; results are rounded once.
+#include <algorithm>
+
+#include "ftc_common.h"
+
+namespace ftc {
+namespace norm {
+namespace {
+
+constexpr int kLot = 8;  // values of a row that a lane takes at a time
+
+struct Params {
+    const void *weight, *bias;
+    int32_t kind, weight_dtype, bias_dtype;  // kind: enum ftc_norm_kind
+};
+struct Rows {
+    void *ptr;
+    int64_t stride;
+    int32_t dtype;
+};
+struct Args {
+    Rows block, residual, gate, x, h, grad_x, grad_h, grad_block, grad_residual, grad_gate;
+    Params after, before;
+    float *stats;        // four floats a row: mean and 1 / deviation of the first norm and of the second
+    float *sums;         // partial sums for the parameters, [workgroup][kSums][D]
+    float *gate_sums;    // ... and for a shared gate, [gate row][part][D]
+    int64_t rows, gate_rows, every;  // every: rows that have the same gate row
+    int64_t segment;                 // rows that the backward sums together: `every` of a shared gate, else all
+    int32_t D, parts, activation, shared;  // parts: workgroups per segment; shared: several rows have one gate row
+    float scale, eps;
+};
+enum { kAfterWeight, kAfterBias, kBeforeWeight, kBeforeBias, kSums };
+
+struct Lot {
+    float x[kLot];
+};
+template <bool VEC>
+__device__ __forceinline__ Lot load_lot(const void *base, int dtype, int64_t at, int left) {
+    Lot r;
+    if (VEC) {
+        if (dtype == FTC_F32) {
+            const float4 a = *(const float4 *)((const float *)base + at), b = *(const float4 *)((const float *)base + at + 4);
+            r.x[0] = a.x, r.x[1] = a.y, r.x[2] = a.z, r.x[3] = a.w, r.x[4] = b.x, r.x[5] = b.y, r.x[6] = b.z, r.x[7] = b.w;
+        } else {
+            const uint4 a = *(const uint4 *)((const uint16_t *)base + at);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                r.x[2 * i] = __uint_as_float(w[i] << 16), r.x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kLot; i++) r.x[i] = i < left ? load_as_f32(base, dtype, at + i) : 0.f;
+    }
+    return r;
+}
+template <bool VEC>
+__device__ __forceinline__ void store_lot(void *base, int dtype, int64_t at, int left, const Lot &r) {
+    if (VEC) {
+        if (dtype == FTC_F32) {
+            *(float4 *)((float *)base + at) = make_float4(r.x[0], r.x[1], r.x[2], r.x[3]);
+            *(float4 *)((float *)base + at + 4) = make_float4(r.x[4], r.x[5], r.x[6], r.x[7]);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                w[i] = (uint32_t)f32_to_bf16(r.x[2 * i]) | ((uint32_t)f32_to_bf16(r.x[2 * i + 1]) << 16);
+            *(uint4 *)((uint16_t *)base + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kLot; i++)
+            if (i < left) store_from_f32(base, dtype, at + i, r.x[i]);
+    }
+}
+
+// Sums over a team of LPR lanes, two at a time, in every lane; `turn` alternates between the two halves of `mem`
+// so that one barrier is enough.
+template <int LPR>
+__device__ __forceinline__ void team_sum(float &a, float &b, float (*mem)[2][16], int &turn) {
+#pragma unroll
+    for (int d = 1; d < (LPR < 64 ? LPR : 64); d *= 2) a += __shfl_xor(a, d), b += __shfl_xor(b, d);
+    if (LPR > 64) {
+        constexpr int kWaves = LPR / 64;
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) mem[turn][0][wave] = a, mem[turn][1][wave] = b;
+        __syncthreads();
+        a = 0.f, b = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) a += mem[turn][0][w], b += mem[turn][1][w];
+        turn ^= 1;
+    }
+}
+
+__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + expf(-g)); }
+__device__ __forceinline__ float activate(float g, int activation) {
+    return activation == FTC_GATE_PLAIN ? g : activation == FTC_GATE_SIGMOID ? sigmoid(g) : g * sigmoid(g);
+}
+__device__ __forceinline__ float activate_slope(float g, int activation) {
+    if (activation == FTC_GATE_PLAIN) return 1.f;
+    const float s = sigmoid(g);
+    return activation == FTC_GATE_SIGMOID ? s * (1.f - s) : s * (1.f + g * (1.f - s));
+}
+
+// One lot of a norm's weight and bias
+template <bool VEC>
+__device__ __forceinline__ void params_lot(const Params &p, int col, int left, Lot &w, Lot &b) {
+    if (p.weight) w = load_lot<VEC>(p.weight, p.weight_dtype, col, left);
+    else
+#pragma unroll
+        for (int i = 0; i < kLot; i++) w.x[i] = 1.f;
+    if (p.bias) b = load_lot<VEC>(p.bias, p.bias_dtype, col, left);
+    else
+#pragma unroll
+        for (int i = 0; i < kLot; i++) b.x[i] = 0.f;
+}
+
+// LPR lanes take a row, NV lots each; THREADS / LPR rows at a time
+template <int LPR, int NV, bool VEC>
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Args p) {
+    constexpr int kThreads = LPR > 256 ? LPR : 256, kTeams = kThreads / LPR;
+    __shared__ float mem[2][2][16];
+    const int team = threadIdx.x / LPR, lane = threadIdx.x % LPR;
+    int turn = 0;
+    const float per = 1.f / (float)p.D;
+    auto column = [&](int v) { return kLot * (lane + LPR * v); };
+
+    // Mean (layer norm) and 1 / deviation of the row in r
+    auto statistics = [&](const Lot (&r)[NV], const Params &n, float &mean, float &rstd) {
+        mean = 0.f, rstd = 1.f;
+        if (n.kind == FTC_NORM_NONE) return;
+        float none = 0.f;
+        if (n.kind == FTC_NORM_LAYER) {
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int i = 0; i < kLot; i++) mean += r[v].x[i];  // (zeros past the row's end)
+            team_sum<LPR>(mean, none, mem, turn);
+            mean *= per;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; v++)
+#pragma unroll
+            for (int i = 0; i < kLot; i++)
+                if (column(v) + i < p.D) sum = fmaf(r[v].x[i] - mean, r[v].x[i] - mean, sum);
+        team_sum<LPR>(sum, none, mem, turn);
+        rstd = 1.f / sqrtf(sum * per + p.eps);
+    };
+
+    for (int64_t base = (int64_t)blockIdx.x * kTeams; base < p.rows; base += (int64_t)gridDim.x * kTeams) {
+        const int64_t row = base + team, gate_row = p.every == 1 ? row : row / p.every;
+        const bool live = row < p.rows;
+        Lot r[NV];
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int col = column(v);
+            if (live && col < p.D) r[v] = load_lot<VEC>(p.block.ptr, p.block.dtype, row * p.block.stride + col, p.D - col);
+            else
+#pragma unroll
+                for (int i = 0; i < kLot; i++) r[v].x[i] = 0.f;
+        }
+        float mean_a, rstd_a, mean_b, rstd_b;
+        statistics(r, p.after, mean_a, rstd_a);
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int col = column(v);
+            if (!live || col >= p.D) continue;
+            if (p.after.kind != FTC_NORM_NONE) {
+                Lot w, b;
+                params_lot<VEC>(p.after, col, p.D - col, w, b);
+#pragma unroll
+                for (int i = 0; i < kLot; i++) r[v].x[i] = fmaf((r[v].x[i] - mean_a) * rstd_a, w.x[i], b.x[i]);
+            }
+            if (p.gate.ptr) {
+                const Lot g = load_lot<VEC>(p.gate.ptr, p.gate.dtype, gate_row * p.gate.stride + col, p.D - col);
+#pragma unroll
+                for (int i = 0; i < kLot; i++) r[v].x[i] *= activate(g.x[i], p.activation);
+            }
+            if (p.residual.ptr) {
+                const Lot d = load_lot<VEC>(p.residual.ptr, p.residual.dtype, row * p.residual.stride + col, p.D - col);
+#pragma unroll
+                for (int i = 0; i < kLot; i++) r[v].x[i] = fmaf(p.scale, r[v].x[i], d.x[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLot; i++) r[v].x[i] *= p.scale;
+            }
+            if (!VEC)
+#pragma unroll
+                for (int i = 0; i < kLot; i++) r[v].x[i] = col + i < p.D ? r[v].x[i] : 0.f;
+            store_lot<VEC>(p.x.ptr, p.x.dtype, row * p.x.stride + col, p.D - col, r[v]);
+        }
+        statistics(r, p.before, mean_b, rstd_b);
+        if (p.h.ptr && live)
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int col = column(v);
+                if (col >= p.D) continue;
+                Lot w, b;
+                params_lot<VEC>(p.before, col, p.D - col, w, b);
+#pragma unroll
+                for (int i = 0; i < kLot; i++) r[v].x[i] = fmaf((r[v].x[i] - mean_b) * rstd_b, w.x[i], b.x[i]);
+                store_lot<VEC>(p.h.ptr, p.h.dtype, row * p.h.stride + col, p.D - col, r[v]);
+            }
+        if (p.stats && live && lane == 0)
+            *(float4 *)(p.stats + 4 * row) = make_float4(mean_a, rstd_a, mean_b, rstd_b);
+    }
+}
+
+template <int LPR, int NV, bool VEC>
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_kernel(Args p) {
+    constexpr int kThreads = LPR > 256 ? LPR : 256, kTeams = kThreads / LPR;
+    __shared__ float mem[2][2][16];
+    __shared__ float fold_mem[kTeams > 1 ? kTeams * LPR * kLot * NV : 1];
+    const int team = threadIdx.x / LPR, lane = threadIdx.x % LPR;
+    int turn = 0;
+    const float per = 1.f / (float)p.D;
+    auto column = [&](int v) { return kLot * (lane + LPR * v); };
+    // the teams' sums to one row of floats
+    auto leave = [&](Lot (&sum)[NV], float *to) {
+        if (kTeams > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int i = 0; i < kLot; i++) fold_mem[(team * LPR * NV + lane * NV + v) * kLot + i] = sum[v].x[i];
+            __syncthreads();
+            if (team) return;
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int i = 0; i < kLot; i++) {
+                    float s = sum[v].x[i];
+#pragma unroll
+                    for (int t = 1; t < kTeams; t++) s += fold_mem[(t * LPR * NV + lane * NV + v) * kLot + i];
+                    sum[v].x[i] = s;
+                }
+        }
+#pragma unroll
+        for (int v = 0; v < NV; v++)
+            if (column(v) < p.D) store_lot<VEC>(to, FTC_F32, column(v), p.D - column(v), sum[v]);
+    };
+
+    Lot dwa[NV] = {}, dba[NV] = {}, dwb[NV] = {}, dbb[NV] = {};
+    // segments of rows (one per gate row), the part of them that is this workgroup's
+    const int part = blockIdx.x % p.parts;
+    for (int64_t seg = blockIdx.x / p.parts; seg * p.segment < p.rows; seg += gridDim.x / p.parts) {
+        const int64_t first = seg * p.segment, end = min(p.rows, first + p.segment);
+        Lot dgate[NV] = {};
+        for (int64_t base = first + (int64_t)part * kTeams; base < end; base += (int64_t)p.parts * kTeams) {
+            const int64_t row = base + team, gate_row = p.shared ? seg : row;
+            const bool live = row < end;
+            float mean_a = 0.f, rstd_a = 1.f, mean_b = 0.f, rstd_b = 1.f;
+            if (live && p.stats) {
+                const float4 s = *(const float4 *)(p.stats + 4 * row);
+                mean_a = s.x, rstd_a = s.y, mean_b = s.z, rstd_b = s.w;
+            }
+            Lot n[NV], dx[NV], gate[NV], xh[NV];
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int col = column(v), left = p.D - col;
+#pragma unroll
+                for (int i = 0; i < kLot; i++) n[v].x[i] = dx[v].x[i] = xh[v].x[i] = gate[v].x[i] = 0.f;
+                if (!live || col >= p.D) continue;
+                n[v] = load_lot<VEC>(p.block.ptr, p.block.dtype, row * p.block.stride + col, left);
+                if (p.gate.ptr) gate[v] = load_lot<VEC>(p.gate.ptr, p.gate.dtype, gate_row * p.gate.stride + col, left);
+                if (p.before.kind != FTC_NORM_NONE) {
+                    if (p.residual.ptr) xh[v] = load_lot<VEC>(p.residual.ptr, p.residual.dtype, row * p.residual.stride + col, left);
+                    if (p.grad_h.ptr) dx[v] = load_lot<VEC>(p.grad_h.ptr, p.grad_h.dtype, row * p.grad_h.stride + col, left);
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int col = column(v), left = p.D - col;
+                if (!live || col >= p.D) continue;
+#pragma unroll
+                for (int i = 0; i < kLot; i++) n[v].x[i] = VEC || i < left ? (n[v].x[i] - mean_a) * rstd_a : 0.f;
+                if (p.before.kind == FTC_NORM_NONE) continue;
+                Lot w, b;
+                params_lot<VEC>(p.after, col, left, w, b);
+#pragma unroll
+                for (int i = 0; i < kLot; i++) {
+                    const float y = fmaf(n[v].x[i], w.x[i], b.x[i]);
+                    const float a = p.gate.ptr ? activate(gate[v].x[i], p.activation) * y : y;
+                    xh[v].x[i] = VEC || i < left ? (fmaf(p.scale, a, xh[v].x[i]) - mean_b) * rstd_b : 0.f;
+                }
+                params_lot<VEC>(p.before, col, left, w, b);
+#pragma unroll
+                for (int i = 0; i < kLot; i++) {
+                    dwb[v].x[i] = fmaf(dx[v].x[i], xh[v].x[i], dwb[v].x[i]);
+                    dbb[v].x[i] += dx[v].x[i];
+                    dx[v].x[i] *= w.x[i];
+                    s0 += dx[v].x[i];
+                    s1 = fmaf(dx[v].x[i], xh[v].x[i], s1);
+                }
+            }
+            if (p.before.kind != FTC_NORM_NONE) {
+                team_sum<LPR>(s0, s1, mem, turn);
+                s0 = p.before.kind == FTC_NORM_LAYER ? s0 * per : 0.f, s1 *= per;
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+#pragma unroll
+                    for (int i = 0; i < kLot; i++) dx[v].x[i] = rstd_b * ((dx[v].x[i] - s0) - xh[v].x[i] * s1);
+            }
+            float t0 = 0.f, t1 = 0.f;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int col = column(v), left = p.D - col;
+                if (!live || col >= p.D) continue;
+                if (p.grad_x.ptr) {
+                    const Lot g = load_lot<VEC>(p.grad_x.ptr, p.grad_x.dtype, row * p.grad_x.stride + col, left);
+#pragma unroll
+                    for (int i = 0; i < kLot; i++) dx[v].x[i] += g.x[i];
+                }
+                if (!VEC)
+#pragma unroll
+                    for (int i = 0; i < kLot; i++) dx[v].x[i] = i < left ? dx[v].x[i] : 0.f;
+                if (p.grad_residual.ptr)
+                    store_lot<VEC>(p.grad_residual.ptr, p.grad_residual.dtype, row * p.grad_residual.stride + col, left, dx[v]);
+                Lot w, b;
+                params_lot<VEC>(p.after, col, left, w, b);
+                if (p.gate.ptr) {
+                    Lot d;
+#pragma unroll
+                    for (int i = 0; i < kLot; i++) {
+                        const float y = fmaf(n[v].x[i], w.x[i], b.x[i]), g = gate[v].x[i];
+                        d.x[i] = p.scale * activate_slope(g, p.activation) * y * dx[v].x[i];
+                        dx[v].x[i] *= p.scale * activate(g, p.activation);
+                        dgate[v].x[i] += d.x[i];
+                    }
+                    if (p.grad_gate.ptr && !p.shared)
+                        store_lot<VEC>(p.grad_gate.ptr, p.grad_gate.dtype, row * p.grad_gate.stride + col, left, d);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kLot; i++) dx[v].x[i] *= p.scale;
+                }
+                if (p.after.kind == FTC_NORM_NONE) continue;
+#pragma unroll
+                for (int i = 0; i < kLot; i++) {
+                    dwa[v].x[i] = fmaf(dx[v].x[i], n[v].x[i], dwa[v].x[i]);
+                    dba[v].x[i] += dx[v].x[i];
+                    dx[v].x[i] *= w.x[i];
+                    t0 += dx[v].x[i];
+                    t1 = fmaf(dx[v].x[i], n[v].x[i], t1);
+                }
+            }
+            if (p.after.kind != FTC_NORM_NONE) {
+                team_sum<LPR>(t0, t1, mem, turn);
+                t0 = p.after.kind == FTC_NORM_LAYER ? t0 * per : 0.f, t1 *= per;
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+#pragma unroll
+                    for (int i = 0; i < kLot; i++) dx[v].x[i] = rstd_a * ((dx[v].x[i] - t0) - n[v].x[i] * t1);
+            }
+            if (p.grad_block.ptr && live)
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+                    if (column(v) < p.D)
+                        store_lot<VEC>(p.grad_block.ptr, p.grad_block.dtype, row * p.grad_block.stride + column(v),
+                                       p.D - column(v), dx[v]);
+        }
+        if (p.shared && p.gate_sums) leave(dgate, p.gate_sums + (seg * p.parts + part) * p.D);
+    }
+    float *const to = p.sums + (int64_t)blockIdx.x * kSums * p.D;
+    if (p.sums && p.after.weight) leave(dwa, to + kAfterWeight * p.D);
+    if (p.sums && p.after.bias) leave(dba, to + kAfterBias * p.D);
+    if (p.sums && p.before.weight) leave(dwb, to + kBeforeWeight * p.D);
+    if (p.sums && p.before.bias) leave(dbb, to + kBeforeBias * p.D);
+}
+
+// out[row][col] = sum over `count` rows of floats, `stride` apart, in a fixed order: 8 lots of them by 32 columns
+struct Fold {
+    const float *from;
+    void *to;
+    int64_t to_stride, from_stride;  // between results; a result's terms start `from_stride` floats apart
+    int32_t dtype, results, count, stride;
+};
+struct FoldArgs {
+    Fold fold[kSums + 1];
+    int32_t D, folds;
+};
+__global__ __launch_bounds__(256) void fold_rows_kernel(FoldArgs p) {
+    __shared__ float mem[8][32];
+    const int x = threadIdx.x % 32, lot = threadIdx.x / 32, col = blockIdx.x * 32 + x;
+    const Fold f = p.fold[blockIdx.y];
+    for (int r = blockIdx.z; r < f.results; r += gridDim.z) {
+        float sum = 0.f;
+        if (col < p.D)
+            for (int i = lot; i < f.count; i += 8) sum += f.from[r * f.from_stride + (int64_t)i * f.stride + col];
+        __syncthreads();
+        mem[lot][x] = sum;
+        __syncthreads();
+        if (lot == 0 && col < p.D) {
+            float all = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) all += mem[k][x];
+            store_from_f32(f.to, f.dtype, r * f.to_stride + col, all);
+        }
+    }
+}
+
+// ---- host ----
+constexpr int64_t kMostWidth = 16384;
+constexpr int kLeastNormed = 3;
+
+struct Plan {
+    int lpr, teams;
+    int64_t groups, parts;  // workgroups, workgroups per segment
+};
+Plan plan_of(int64_t D, int64_t rows, int64_t segment, bool backward) {
+    Plan q;
+    q.lpr = D <= 128 ? 16 : D <= 1024 ? 64 : D <= 8192 ? 256 : 1024;
+    q.teams = q.lpr > 256 ? 1 : 256 / q.lpr;
+    // four workgroups a compute unit; the backward leaves sums with each of them: two
+    const int64_t most = backward ? 512 : 1024, segments = (rows + segment - 1) / segment;
+    q.parts = std::min((segment + q.teams - 1) / q.teams, std::max<int64_t>(1, most / segments));
+    q.groups = std::min(segments, std::max<int64_t>(1, most / q.parts)) * q.parts;
+    return q;
+}
+
+template <int LPR, int NV>
+void launch(const Args &p, const Plan &q, bool vec, bool backward, hipStream_t stream) {
+    const dim3 grid((uint32_t)q.groups), block(LPR > 256 ? LPR : 256);
+    if (backward) {
+        if (vec) residual_norm_backward_kernel<LPR, NV, true><<<grid, block, 0, stream>>>(p);
+        else residual_norm_backward_kernel<LPR, NV, false><<<grid, block, 0, stream>>>(p);
+    } else {
+        if (vec) residual_norm_kernel<LPR, NV, true><<<grid, block, 0, stream>>>(p);
+        else residual_norm_kernel<LPR, NV, false><<<grid, block, 0, stream>>>(p);
+    }
+}
+void dispatch(const Args &p, const Plan &q, bool vec, bool backward, hipStream_t stream) {
+    if (p.D <= 128) launch<16, 1>(p, q, vec, backward, stream);
+    else if (p.D <= 512) launch<64, 1>(p, q, vec, backward, stream);
+    else if (p.D <= 1024) launch<64, 2>(p, q, vec, backward, stream);
+    else if (p.D <= 2048) launch<256, 1>(p, q, vec, backward, stream);
+    else if (p.D <= 4096) launch<256, 2>(p, q, vec, backward, stream);
+    else if (p.D <= 8192) launch<256, 4>(p, q, vec, backward, stream);
+    else launch<1024, 2>(p, q, vec, backward, stream);
+}
+
+int read_rows(const ftc_rows *r, const char *name, bool wanted, Rows *to) {
+    *to = Rows{};
+    if (!r || !r->ptr) return wanted ? fail(FTC_ERR_INVALID, "%s is null", name) : FTC_OK;
+    if (r->dtype != FTC_F32 && r->dtype != FTC_BF16)
+        return fail(FTC_ERR_INVALID, "%s has dtype code %d, expected FTC_F32 or FTC_BF16", name, (int)r->dtype);
+    *to = Rows{r->ptr, r->stride, r->dtype};
+    return FTC_OK;
+}
+int read_norm(const ftc_norm &n, const char *name, Params *to) {
+    if (n.kind < FTC_NORM_NONE || n.kind > FTC_NORM_LAYER) return fail(FTC_ERR_INVALID, "%s has kind %d", name, (int)n.kind);
+    for (int32_t d : {n.weight_dtype, n.bias_dtype})
+        if (d != FTC_F32 && d != FTC_BF16) return fail(FTC_ERR_INVALID, "%s has dtype code %d", name, (int)d);
+    const bool none = n.kind == FTC_NORM_NONE;
+    *to = Params{none ? nullptr : n.weight, none ? nullptr : n.bias, n.kind, n.weight_dtype, n.bias_dtype};
+    return FTC_OK;
+}
+int read_call(const ftc_residual_norm_call *c, Args *p) {
+    if (!c) return fail(FTC_ERR_INVALID, "the call is null");
+    if (c->rows < 0 || c->width < 1 || c->width > kMostWidth || c->rows > 0x7fffffff)
+        return fail(c->rows < 0 ? FTC_ERR_INVALID : FTC_ERR_UNSUPPORTED,
+                    "rows of 1 to %lld values are supported, and fewer than 2^31 of them", (long long)kMostWidth);
+    if (c->activation < FTC_GATE_PLAIN || c->activation > FTC_GATE_SILU)
+        return fail(FTC_ERR_INVALID, "the gate's activation has code %d", (int)c->activation);
+    p->rows = c->rows, p->D = (int32_t)c->width, p->activation = c->activation, p->scale = c->scale, p->eps = c->eps;
+    if (int rc = read_rows(&c->block, "block", c->rows > 0, &p->block)) return rc;
+    if (int rc = read_rows(&c->residual, "residual", false, &p->residual)) return rc;
+    if (int rc = read_rows(&c->gate, "gate", false, &p->gate)) return rc;
+    if (int rc = read_norm(c->after, "the norm after the block", &p->after)) return rc;
+    if (int rc = read_norm(c->before, "the norm before the next block", &p->before)) return rc;
+    // (a layer norm of two values, or the mean square's of one, has gradients that are all cancellation: eps / r^2 of
+    // what is subtracted, which is the rounding of fp32)
+    if (c->width < kLeastNormed && (p->after.kind != FTC_NORM_NONE || p->before.kind != FTC_NORM_NONE))
+        return fail(FTC_ERR_UNSUPPORTED, "rows of at least %d values are normalised", kLeastNormed);
+    p->gate_rows = p->gate.ptr ? c->gate_rows : 0;
+    if (p->gate.ptr && (p->gate_rows < 1 || c->rows % p->gate_rows))
+        return fail(FTC_ERR_INVALID, "the gate has %lld rows, which do not divide the block's %lld",
+                    (long long)c->gate_rows, (long long)c->rows);
+    return FTC_OK;
+}
+void set_segments(Args *p) {
+    p->shared = p->gate.ptr && p->gate_rows < p->rows;
+    p->every = p->gate.ptr ? p->rows / p->gate_rows : 1;
+    p->segment = p->shared ? p->every : p->rows;
+}
+bool wide(const Args &p) {
+    if (p.D % kLot) return false;
+    const Rows *const all[] = {&p.block, &p.residual, &p.gate, &p.x, &p.h, &p.grad_x, &p.grad_h, &p.grad_block,
+                               &p.grad_residual, &p.grad_gate};
+    for (const Rows *r : all)
+        if (r->ptr && (((uintptr_t)r->ptr & 15) || r->stride % kLot)) return false;
+    for (const void *q : {p.after.weight, p.after.bias, p.before.weight, p.before.bias})
+        if (q && ((uintptr_t)q & 15)) return false;
+    return true;
+}
+Plan backward_plan(const Args &p) { return plan_of(p.D, p.rows, p.segment, true); }
+int64_t sums_floats(const Args &p, const Plan &q) { return q.groups * kSums * p.D; }
+int64_t gate_floats(const Args &p, const Plan &q) { return p.shared ? p.gate_rows * q.parts * p.D : 0; }
+int launched(const char *name) {
+    note_kernel(name);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? FTC_OK : fail(FTC_ERR_HIP, "%s: %s", name, hipGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace norm
+}  // namespace ftc
+
+using namespace ftc;
+using namespace ftc::norm;
+
+extern "C" {
+
+int ftc_residual_norm(const ftc_residual_norm_call *call, const ftc_rows *x, const ftc_rows *h, float *stats, void *stream) {
+    Args p = {};
+    if (int rc = read_call(call, &p)) return rc;
+    if (int rc = read_rows(x, "x", p.rows > 0, &p.x)) return rc;
+    if (int rc = read_rows(h, "h", p.rows > 0 && p.before.kind != FTC_NORM_NONE, &p.h)) return rc;
+    if (p.before.kind == FTC_NORM_NONE && p.h.ptr) return fail(FTC_ERR_INVALID, "h is given without the norm that makes it");
+    if (p.rows == 0) return FTC_OK;
+    p.stats = stats;
+    set_segments(&p);
+    const Plan q = plan_of(p.D, p.rows, p.rows, false);
+    dispatch(p, q, wide(p), false, (hipStream_t)stream);
+    return launched("residual_norm_kernel");
+}
+
+int64_t ftc_residual_norm_backward_workspace_bytes(const ftc_residual_norm_call *call) {
+    Args p = {};
+    if (int rc = read_call(call, &p)) return rc;
+    if (p.rows == 0) return 0;
+    set_segments(&p);
+    const Plan q = backward_plan(p);
+    return 4 * (sums_floats(p, q) + gate_floats(p, q));
+}
+
+int ftc_residual_norm_backward(const ftc_residual_norm_call *call, const float *stats, const ftc_rows *grad_x,
+                               const ftc_rows *grad_h, const ftc_rows *grad_block, const ftc_rows *grad_residual,
+                               const ftc_rows *grad_gate, void *grad_after_weight, void *grad_after_bias,
+                               void *grad_before_weight, void *grad_before_bias, void *workspace, size_t workspace_bytes,
+                               void *stream) {
+    Args p = {};
+    if (int rc = read_call(call, &p)) return rc;
+    if (int rc = read_rows(grad_x, "grad_x", false, &p.grad_x)) return rc;
+    if (int rc = read_rows(grad_h, "grad_h", false, &p.grad_h)) return rc;
+    if (int rc = read_rows(grad_block, "grad_block", false, &p.grad_block)) return rc;
+    if (int rc = read_rows(grad_residual, "grad_residual", false, &p.grad_residual)) return rc;
+    if (int rc = read_rows(grad_gate, "grad_gate", false, &p.grad_gate)) return rc;
+    if (p.grad_gate.ptr && !p.gate.ptr) return fail(FTC_ERR_INVALID, "grad_gate is given without a gate");
+    if (p.rows == 0) return FTC_OK;
+    if (!stats && (p.after.kind != FTC_NORM_NONE || p.before.kind != FTC_NORM_NONE))
+        return fail(FTC_ERR_INVALID, "stats is null");
+    set_segments(&p);
+    const Plan q = backward_plan(p);
+    if (!workspace || (int64_t)workspace_bytes < 4 * (sums_floats(p, q) + gate_floats(p, q)))
+        return fail(FTC_ERR_WORKSPACE, "ftc_residual_norm_backward needs %lld bytes",
+                    (long long)(4 * (sums_floats(p, q) + gate_floats(p, q))));
+    if ((uintptr_t)workspace & 255) return fail(FTC_ERR_WORKSPACE, "the workspace must be 256-byte aligned");
+    p.stats = const_cast<float *>(stats);
+    p.sums = (float *)workspace, p.gate_sums = p.shared ? p.sums + sums_floats(p, q) : nullptr;
+    p.parts = (int32_t)q.parts;
+    FoldArgs f = {};
+    f.D = p.D;
+    struct {
+        const void *param;
+        void *grad;
+        int32_t dtype;
+    } const params[kSums] = {{p.after.weight, grad_after_weight, p.after.weight_dtype}, {p.after.bias, grad_after_bias, p.after.bias_dtype},
+                             {p.before.weight, grad_before_weight, p.before.weight_dtype}, {p.before.bias, grad_before_bias, p.before.bias_dtype}};
+    for (int i = 0; i < kSums; i++)
+        if (params[i].param && params[i].grad)
+            f.fold[f.folds++] = Fold{p.sums + i * p.D, params[i].grad, 0, 0, params[i].dtype, 1, (int32_t)q.groups, kSums * p.D};
+    if (!f.folds) p.sums = nullptr;
+    int results = 1;
+    if (p.shared && p.grad_gate.ptr) {
+        results = (int)std::min<int64_t>(p.gate_rows, 4096);
+        f.fold[f.folds++] = Fold{p.gate_sums, p.grad_gate.ptr, p.grad_gate.stride, q.parts * p.D, p.grad_gate.dtype,
+                                 (int32_t)p.gate_rows, (int32_t)q.parts, p.D};
+    } else {
+        p.gate_sums = nullptr;
+    }
+    dispatch(p, q, wide(p), true, (hipStream_t)stream);
+    if (f.folds)
+        fold_rows_kernel<<<dim3((uint32_t)((p.D + 31) / 32), (uint32_t)f.folds, (uint32_t)results), 256, 0, (hipStream_t)stream>>>(f);
+    return launched("residual_norm_backward_kernel");
+}
+
+}  // extern "C"

@@ -52,7 +52,26 @@ EXPORTED_SYMBOLS = (
     "ftc_gated_delta_rule_backward_workspace_bytes",
     "ftc_gated_delta_rule_backward",
     "ftc_gated_delta_step",
+    "ftc_residual_norm",
+    "ftc_residual_norm_backward_workspace_bytes",
+    "ftc_residual_norm_backward",
 )
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("stride", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class Norm(ctypes.Structure):
+    _fields_ = [("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("kind", ctypes.c_int32),
+                ("weight_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32)]
+
+
+class ResidualNormCall(ctypes.Structure):
+    _fields_ = [("block", Rows), ("residual", Rows), ("gate", Rows), ("after", Norm), ("before", Norm),
+                ("rows", ctypes.c_int64), ("gate_rows", ctypes.c_int64), ("width", ctypes.c_int64),
+                ("activation", ctypes.c_int32), ("scale", ctypes.c_float), ("eps", ctypes.c_float)]
+
 
 
 class Tensor4(ctypes.Structure):
@@ -159,6 +178,14 @@ def load():
     lib.ftc_gated_delta_rule_backward.argtypes = [t4] * 5 + scalars + memory + [t4] * 8 + memory + [ctypes.c_void_p]
     lib.ftc_gated_delta_step.restype = ctypes.c_int
     lib.ftc_gated_delta_step.argtypes = [t4] * 5 + scalars[1:] + [t4] * 2 + [ctypes.c_void_p]
+    call, rows = ctypes.POINTER(ResidualNormCall), ctypes.POINTER(Rows)
+    lib.ftc_residual_norm.restype = ctypes.c_int
+    lib.ftc_residual_norm.argtypes = [call, rows, rows, ctypes.c_void_p, ctypes.c_void_p]
+    lib.ftc_residual_norm_backward_workspace_bytes.restype = ctypes.c_int64
+    lib.ftc_residual_norm_backward_workspace_bytes.argtypes = [call]
+    lib.ftc_residual_norm_backward.restype = ctypes.c_int
+    lib.ftc_residual_norm_backward.argtypes = [call, ctypes.c_void_p] + [rows] * 5 + [ctypes.c_void_p] * 5 + [
+        ctypes.c_size_t, ctypes.c_void_p]
     lib.ftc_causal_dot_plan.restype = ctypes.c_int
     lib.ftc_causal_dot_plan.argtypes = [t4] * 3 + [ctypes.c_int, ctypes.c_char_p, ctypes.c_size_t]
     _lib = lib

@@ -866,6 +866,112 @@ Tensor delta_step(const Tensor &queries, const Tensor &keys, const Tensor &value
     return out;
 }
 
+// ---- the norms around a block (norms/__init__.py) ----
+int32_t norm_dtype(const Tensor &t, const char *name) {
+    if (t.scalar_type() == at::kFloat) return FTC_F32;
+    if (t.scalar_type() == at::kBFloat16) return FTC_BF16;
+    error(std::string("residual_norm: ") + name + " must be float32 or bfloat16, got " +
+          py::str(py::cast(t.scalar_type())).cast<std::string>());
+}
+// Rows of the last dimension, one stride between them (a copy where the leading dimensions have several)
+struct NormRows {
+    Tensor t;
+    ftc_rows r{nullptr, 0, FTC_F32};
+    NormRows(const OptTensor &from, const char *name) {
+        if (!from) return;
+        const int64_t D = from->size(-1);
+        t = from->dim() == 2 ? *from : from->reshape({D ? from->numel() / D : 0, D});
+        if (D > 1 && t.stride(1) != 1) t = t.contiguous();
+        r = ftc_rows{t.numel() ? t.data_ptr() : nullptr, t.stride(0), norm_dtype(t, name)};
+    }
+};
+struct NormCall {
+    NormRows block, residual, gate;
+    Tensor keep[4];
+    ftc_residual_norm_call call{};
+    NormCall(const Tensor &b, const OptTensor &res, const OptTensor &g, int after, const OptTensor &aw, const OptTensor &ab,
+             int before, const OptTensor &bw, const OptTensor &bb, int activation, double scale, double eps)
+        : block(b, "block"), residual(res, "residual"), gate(g, "gate") {
+        if (!b.is_cuda()) error("residual_norm: block is on " + b.device().str() + ", expected a GPU tensor");
+        for (const Tensor *x : {&residual.t, &gate.t})
+            if (x->defined() && x->device() != b.device()) error("residual_norm: all tensors must be on one device");
+        call.block = block.r, call.residual = residual.r, call.gate = gate.r;
+        call.rows = block.t.size(0), call.width = block.t.size(1), call.gate_rows = gate.t.defined() ? gate.t.size(0) : 0;
+        if ((residual.t.defined() && residual.t.sizes() != block.t.sizes()) ||
+            (gate.t.defined() && gate.t.size(1) != call.width))
+            error("residual_norm: residual and gate must have rows like the block's");
+        auto norm = [&](int kind, const OptTensor &w, const OptTensor &bias, Tensor *held) {
+            ftc_norm n{nullptr, nullptr, kind, FTC_F32, FTC_F32};
+            auto vector = [&](const Tensor &x, Tensor &at) {
+                if (x.dim() != 1 || x.size(0) != call.width || x.device() != b.device())
+                    error("residual_norm: a norm's weight and bias are vectors of the rows' width on the block's device");
+                at = x.contiguous();
+                return at.const_data_ptr();
+            };
+            if (w) n.weight = vector(*w, held[0]), n.weight_dtype = norm_dtype(*w, "weight");
+            if (bias) n.bias = vector(*bias, held[1]), n.bias_dtype = norm_dtype(*bias, "bias");
+            return n;
+        };
+        call.after = norm(after, aw, ab, keep), call.before = norm(before, bw, bb, keep + 2);
+        call.activation = activation, call.scale = (float)scale, call.eps = (float)eps;
+    }
+};
+
+// (x, h or None, statistics for the backward or None)
+std::tuple<Tensor, OptTensor, OptTensor> residual_norm(const Tensor &block, const OptTensor &residual, const OptTensor &gate,
+                                                       int after, const OptTensor &aw, const OptTensor &ab, int before,
+                                                       const OptTensor &bw, const OptTensor &bb, int activation,
+                                                       double scale, double eps, bool keep) {
+    const at::NoGradGuard no_grad;
+    const NormCall c(block, residual, gate, after, aw, ab, before, bw, bb, activation, scale, eps);
+    const c10::DeviceGuard guard(block.device());
+    const Tensor x = at::empty(block.sizes(), residual ? residual->options() : block.options());
+    OptTensor h, stats;
+    if (before != FTC_NORM_NONE) h = at::empty(block.sizes(), block.options());
+    if (keep && (after != FTC_NORM_NONE || before != FTC_NORM_NONE))
+        stats = at::empty({c.call.rows, 4}, block.options().dtype(at::kFloat));
+    const NormRows xr(x, "x"), hr(h, "h");
+    hipStream_t const stream = c10::hip::getCurrentHIPStream(block.device().index()).stream();
+    float *const st = stats ? stats->data_ptr<float>() : nullptr;
+    const int rc = native([&] { return ftc_residual_norm(&c.call, &xr.r, h ? &hr.r : nullptr, st, stream); });
+    check(rc, "ftc_residual_norm");
+    return {x, h, stats};
+}
+
+// gradients of block, residual, gate, after's weight and bias, before's weight and bias (None where not needed)
+std::vector<OptTensor> residual_norm_backward(const Tensor &block, const OptTensor &residual, const OptTensor &gate, int after,
+                                              const OptTensor &aw, const OptTensor &ab, int before, const OptTensor &bw,
+                                              const OptTensor &bb, int activation, double scale, double eps,
+                                              const OptTensor &stats, const OptTensor &grad_x, const OptTensor &grad_h,
+                                              const std::vector<bool> &needed) {
+    const at::NoGradGuard no_grad;
+    const NormCall c(block, residual, gate, after, aw, ab, before, bw, bb, activation, scale, eps);
+    const c10::DeviceGuard guard(block.device());
+    const NormRows gx(grad_x, "grad_x"), gh(grad_h, "grad_h");
+    std::vector<OptTensor> grads(7);
+    const OptTensor inputs[] = {block, residual, gate, aw, ab, bw, bb};
+    for (int i = 0; i < 7; i++)
+        if (needed[i] && inputs[i]) {
+            grads[i] = at::empty(inputs[i]->sizes(), inputs[i]->options());
+            // (no rows, or a norm that is not there: nothing is written)
+            if (c.call.rows == 0 || (i >= 3 && (i < 5 ? after : before) == FTC_NORM_NONE)) grads[i]->zero_();
+        }
+    const NormRows gb(grads[0], "grad_block"), gr(grads[1], "grad_residual"), gg(grads[2], "grad_gate");
+    auto ptr = [](const OptTensor &t) { return t ? t->data_ptr() : nullptr; };
+    const Tensor ws = delta_memory(ftc_residual_norm_backward_workspace_bytes(&c.call),
+                                   "ftc_residual_norm_backward_workspace_bytes", block);
+    hipStream_t const stream = c10::hip::getCurrentHIPStream(block.device().index()).stream();
+    const float *const st = stats ? stats->const_data_ptr<float>() : nullptr;
+    void *const at = ws.data_ptr(), *const p3 = ptr(grads[3]), *const p4 = ptr(grads[4]), *const p5 = ptr(grads[5]),
+               *const p6 = ptr(grads[6]);
+    const int rc = native([&] {
+        return ftc_residual_norm_backward(&c.call, st, &gx.r, &gh.r, &gb.r, &gr.r, &gg.r, p3, p4, p5, p6, at,
+                                          (size_t)ws.numel(), stream);
+    });
+    check(rc, "ftc_residual_norm_backward");
+    return grads;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ftc_host, m) {
@@ -886,4 +992,6 @@ PYBIND11_MODULE(_ftc_host, m) {
     m.def("delta_rule", &delta_rule);
     m.def("delta_rule_backward", &delta_rule_backward);
     m.def("delta_step", &delta_step);
+    m.def("residual_norm", &residual_norm);
+    m.def("residual_norm_backward", &residual_norm_backward);
 }

@@ -383,6 +383,48 @@ int ftc_gated_delta_step(const ftc_tensor4 *queries, const ftc_tensor4 *keys, co
                          const ftc_tensor4 *log_decay, const ftc_tensor4 *beta, float scale, int32_t normalize,
                          const ftc_tensor4 *state, const ftc_tensor4 *out, void *stream);
 
+/*
+ * The norms around a block with its gate and residual, in one pass over the rows (beside the encoder's layer
+ * norms above; no counterpart in the reference).  Per row of `width` values:
+ *
+ *   y = norm_after(block),   x = residual + scale act(gate) y,   h = norm_before(x)
+ *
+ * A norm is (r - mean) / sqrt(variance + eps) weight + bias (layer), r / sqrt(mean of squares + eps) weight + bias
+ * (rms) or r (none); weight and bias may be NULL.  act: the gate itself, its sigmoid, or gate * sigmoid(gate).  A
+ * gate of gate_rows rows serves rows / gate_rows rows each, in order; residual and gate are absent with ptr NULL.
+ * Every tensor is FTC_F32 or FTC_BF16 by itself, rows of contiguous values `stride` elements apart; width from 1
+ * to 16384, of rows that are normalised from 3.  x and h must not overlap the inputs.  stats: NULL, or four floats a row for the backward.
+ */
+enum ftc_norm_kind { FTC_NORM_NONE = 0, FTC_NORM_RMS = 1, FTC_NORM_LAYER = 2 };
+enum ftc_gate_activation { FTC_GATE_PLAIN = 0, FTC_GATE_SIGMOID = 1, FTC_GATE_SILU = 2 };
+typedef struct ftc_rows {
+    void *ptr;
+    int64_t stride;
+    int32_t dtype;
+} ftc_rows;
+typedef struct ftc_norm {
+    const void *weight, *bias;
+    int32_t kind, weight_dtype, bias_dtype;
+} ftc_norm;
+typedef struct ftc_residual_norm_call {
+    ftc_rows block, residual, gate;
+    ftc_norm after, before;
+    int64_t rows, gate_rows, width;
+    int32_t activation;
+    float scale, eps;
+} ftc_residual_norm_call;
+int ftc_residual_norm(const ftc_residual_norm_call *call, const ftc_rows *x, const ftc_rows *h, float *stats, void *stream);
+/*
+ * Its gradients from grad_x and grad_h (either may be NULL: zeros).  Gradients of the parameters have their
+ * parameters' dtypes; one that is not wanted may be NULL.  Sums are in a fixed order.
+ */
+int64_t ftc_residual_norm_backward_workspace_bytes(const ftc_residual_norm_call *call);
+int ftc_residual_norm_backward(const ftc_residual_norm_call *call, const float *stats, const ftc_rows *grad_x,
+                               const ftc_rows *grad_h, const ftc_rows *grad_block, const ftc_rows *grad_residual,
+                               const ftc_rows *grad_gate, void *grad_after_weight, void *grad_after_bias,
+                               void *grad_before_weight, void *grad_before_bias, void *workspace,
+                               size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
