@@ -13,18 +13,22 @@ constexpr int64_t kMostRowStride = 1 << 22;  // elements between positions: a ch
 
 struct Sizes {
     int64_t N, H, Hk, L, E, M;
+    int32_t dtype;
     int64_t chunks() const { return (L + kRows - 1) / kRows; }
     int64_t col_blocks() const { return (M + kCols - 1) / kCols; }
     int64_t tiles() const { return E <= 64 ? 4 : 8; }
+    int64_t pieces() const { return dtype == FTC_F32 ? 3 : 1; }
     int64_t units() const { return N * H * chunks(); }  // chunks of all chains
     // floats (all multiples of 64)
     int64_t factors() const { return units() * kFactors * kRows; }
-    int64_t t() const { return units() * 3 * kRows * kRows / 2; }
+    int64_t t() const { return units() * kTFrags * 3 * 256; }
+    int64_t keys() const { return N * Hk * chunks() * 2 * tiles() * pieces() * 256; }
     int64_t s() const { return units() * col_blocks() * tiles() * 256; }
     int64_t z() const { return units() * col_blocks() * 4 * 256; }
-    int64_t zdu() const { return units() * col_blocks() * kRows; }
-    int64_t kept() const { return 4 * (factors() + t() + s() + z()); }
-    int64_t backward() const { return 4 * (s() + z() + zdu()); }
+    int64_t dots() const { return units() * col_blocks() * kRows; }
+    // T, keys, factors, states, Z; to be kept for the backward also the transpose of T and O
+    int64_t forward(bool keep) const { return 4 * (factors() + (keep ? 2 : 1) * (t() + z()) + 2 * keys() + s()); }
+    int64_t backward() const { return 4 * (s() + z() + 2 * dots() + keys()); }
 };
 
 int check_sizes(const Sizes &s) {
@@ -91,7 +95,7 @@ OperandOut rows_out(const ftc_tensor4 *t) { return t ? as_operand_out(t) : Opera
 int read_inputs(const ftc_tensor4 *q, const ftc_tensor4 *k, const ftc_tensor4 *v, const ftc_tensor4 *g, const ftc_tensor4 *b,
                 Sizes *s, DeltaArgs *p) {
     if (!q || !v) return fail(FTC_ERR_INVALID, "queries or values is null");
-    *s = Sizes{v->size[0], v->size[1], q->size[1], v->size[2], q->size[3], v->size[3]};
+    *s = Sizes{v->size[0], v->size[1], q->size[1], v->size[2], q->size[3], v->size[3], q->dtype};
     if (int rc = check_sizes(*s)) return rc;
     if (int rc = check_rows(q, "queries", s->N, s->Hk, s->L, s->E, -1)) return rc;
     if (int rc = check_rows(k, "keys", s->N, s->Hk, s->L, s->E, q->dtype)) return rc;
@@ -106,11 +110,16 @@ int read_inputs(const ftc_tensor4 *q, const ftc_tensor4 *k, const ftc_tensor4 *v
     p->vec_q = reads_wide(p->q), p->vec_k = reads_wide(p->k);
     return FTC_OK;
 }
-void place_kept(const Sizes &s, void *kept, DeltaArgs *p) {
-    p->factors = (float *)kept;
-    p->s = p->factors + s.factors();
-    p->z = p->s + s.s();
-    p->t = (uint16_t *)(p->z + s.z());
+void place_forward(const Sizes &s, void *at, bool keep, DeltaArgs *p) {
+    float *next = (float *)at;
+    auto take = [&](int64_t floats) {
+        float *const here = next;
+        next += floats;
+        return here;
+    };
+    p->factors = take(s.factors()), p->s = take(s.s()), p->z = take(s.z());
+    p->t = (uint16_t *)take(s.t()), p->kr = (uint16_t *)take(s.keys()), p->kc = (uint16_t *)take(s.keys());
+    if (keep) p->o = take(s.z()), p->tt = (uint16_t *)take(s.t());
 }
 int launched(const char *name) {
     note_kernel(name);
@@ -127,20 +136,22 @@ using namespace ftc::delta;
 
 extern "C" {
 
-static int64_t delta_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M, int what) {
-    const Sizes s{N, H, Hk, L, E, M};
+static int64_t delta_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M, int32_t dtype, int what) {
+    const Sizes s{N, H, Hk, L, E, M, dtype};
+    if (dtype != FTC_F32 && dtype != FTC_BF16) return fail(FTC_ERR_INVALID, "unknown dtype code %d", (int)dtype);
     if (int rc = check_sizes(s)) return rc;
-    return what == 1 ? s.backward() : s.kept();
+    return what == 2 ? s.backward() : s.forward(what == 1);
 }
-int64_t ftc_gated_delta_rule_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M) {
-    const int64_t bytes = delta_bytes(N, H, Hk, L, E, M, 0);
+int64_t ftc_gated_delta_rule_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M, int32_t dtype) {
+    const int64_t bytes = delta_bytes(N, H, Hk, L, E, M, dtype, 0);
     return bytes > 0 && L <= kStepMost ? 0 : bytes;
 }
-int64_t ftc_gated_delta_rule_kept_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M) {
-    return delta_bytes(N, H, Hk, L, E, M, 0);
+int64_t ftc_gated_delta_rule_kept_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M, int32_t dtype) {
+    return delta_bytes(N, H, Hk, L, E, M, dtype, 1);
 }
-int64_t ftc_gated_delta_rule_backward_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M) {
-    return delta_bytes(N, H, Hk, L, E, M, 1);
+int64_t ftc_gated_delta_rule_backward_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M,
+                                                      int32_t dtype) {
+    return delta_bytes(N, H, Hk, L, E, M, dtype, 2);
 }
 
 int ftc_gated_delta_rule(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,
@@ -166,12 +177,12 @@ int ftc_gated_delta_rule(const ftc_tensor4 *queries, const ftc_tensor4 *keys, co
         delta_steps(p, (hipStream_t)stream);
         return launched("delta_step_kernel");
     }
-    const int64_t need = s.kept();
+    const int64_t need = s.forward(kept != nullptr);
     void *const at = kept ? kept : workspace;
     if (!at || (int64_t)(kept ? kept_bytes : workspace_bytes) < need)
         return fail(FTC_ERR_WORKSPACE, "ftc_gated_delta_rule needs %lld bytes", (long long)need);
     if ((uintptr_t)at & 255) return fail(FTC_ERR_WORKSPACE, "the workspace must be 256-byte aligned");
-    place_kept(s, at, &p);
+    place_forward(s, at, kept != nullptr, &p);
     const bool bf16 = queries->dtype == FTC_BF16;
     delta_prepare(p, bf16, (hipStream_t)stream);
     delta_scan(p, bf16, (hipStream_t)stream);
@@ -206,17 +217,18 @@ int ftc_gated_delta_rule_backward(const ftc_tensor4 *queries, const ftc_tensor4 
             if (int rc = check_rows(g.t, g.name, s.N, g.heads, s.L, g.width, g.dtype)) return rc;
     if (s.N * s.H == 0 || (s.L == 0 && !grad_initial_state)) return FTC_OK;
     if (s.L == 0) return fail(FTC_ERR_INVALID, "a call of no positions has no backward");
-    if (!kept || (int64_t)kept_bytes < s.kept())
+    if (!kept || (int64_t)kept_bytes < s.forward(true))
         return fail(FTC_ERR_WORKSPACE, "ftc_gated_delta_rule_backward needs the %lld bytes that the forward kept",
-                    (long long)s.kept());
+                    (long long)s.forward(true));
     if (!workspace || (int64_t)workspace_bytes < s.backward())
         return fail(FTC_ERR_WORKSPACE, "ftc_gated_delta_rule_backward needs %lld bytes of workspace", (long long)s.backward());
     if (((uintptr_t)kept | (uintptr_t)workspace) & 255)
         return fail(FTC_ERR_WORKSPACE, "the workspace must be 256-byte aligned");
     p.lengths = lengths, p.scale = scale, p.normalize = normalize != 0;
-    place_kept(s, (void *)kept, &p);
-    p.ds = (float *)workspace, p.de = p.ds + s.s(), p.zdu = p.de + s.z();
-    p.go = as_operand(grad_out);
+    place_forward(s, (void *)kept, true, &p);
+    p.ds = (float *)workspace, p.de = p.ds + s.s(), p.dots = p.de + s.z(), p.written = p.dots + s.dots();
+    p.qc = (uint16_t *)(p.written + s.dots());
+    p.go = as_operand(grad_out), p.vec_go = reads_wide(p.go);
     p.gq = rows_out(grad_queries), p.gk = rows_out(grad_keys), p.gv = rows_out(grad_values);
     p.gg = scalars(grad_log_decay), p.gb = scalars(grad_beta);
     p.grad_final = state(grad_final_state), p.grad_initial = state(grad_initial_state);

@@ -4,141 +4,171 @@
 //   P_ij = beta_j (dO_i . Z_j) D_ij rq_i rk_j  (j <= i),   R_ij = -beta_j (dE_i . Z_j) D_ij rk_i rk_j  (j < i)
 //
 //   dq_i = rq_i e^{G_i} S dO_i + sum_j P_ij k_j
-//   dk+_i = -rk_i e^{G_i} S dE_i + sum_j R_ij k_j                  (k_i as it reads the state: with e^{+G_i})
-//   dk-_j = rk_j beta_j e^{G_64 - G_j} dS Z_j + sum_i P_ij q_i + sum_i R_ij k_i      (as it is written: e^{-G_j})
-//   dbeta_j = Z_j . dU_j - sum_{i > j} D_ij (k^_i . k^_j) (dE_i . Z_j)
-//   dG_i = q_i . dq_i + k_i . dk+_i - k_i . dk-_i,  dG_64 += sum_j k_j . (first term of dk-_j) + e^{G_64} <S, dS>
-//   dg_l = sum of dG_i over i >= l in the chunk
+//   dk_i = -rk_i e^{G_i} S dE_i + sum_j R_ij k_j                               (k_i as it reads the state: e^{+G_i})
+//          + rk_i beta_i e^{G_64 - G_i} dS Z_i + sum_j P_ji q_j + sum_j R_ji k_j           (as it is written: e^{-G_i})
 //   (normalised rows: dq - q (q . dq) / |q|^2, the same for k)
 //
-// A workgroup of four wavefronts takes a chunk of one key head and its value heads one after the other, so that the
+// The other gradients need no more products than the reverse scan has made, since
+//   q_i . dq_i = dO_i . O_i,   k_i . dk_i = -dE_i . (V_i - Z_i) as it reads and dE_i . Z_i as it is written:
+//   dbeta_i = dE_i . Z_i / beta_i          (all terms of dE_i have the factor beta_i)
+//   dG_i = dO_i . O_i - dE_i . V_i,   dg_l = sum of dG_i over i >= l in the chunk + <state after it, its gradient>
+// (the last is e^{G_64} <S, dS> + what the chunk's keys write, taken anew in every chunk: nothing adds up over chunks).
+//
+// A workgroup of eight wavefronts takes a chunk of one key head and its value heads one after the other, so that the
 // gradients of shared keys are summed in registers, in one order.  Phase 1 walks the columns of the state, 32 at a
-// time through LDS; a wavefront has all 64 positions of a quarter of the key columns, and a quarter of the tiles of
-// dO Z^T and dE Z^T.  Phase 2 multiplies the 64 x 64 matrices with the rows.
+// time through LDS, the next 32 on their way meanwhile; a wavefront has 32 positions of a quarter of the key
+// columns, and some of the tiles of dO Z^T and dE Z^T.  Phase 2 multiplies the 64 x 64 matrices with the rows.
+// Gradients of bf16 rows are made of values in two pieces (2^-17 of them is left out, against half a step of 2^-8 that the
+// rounding of the results takes).
 #include "ftc_delta_kernel.h"
 
 namespace ftc {
 namespace delta {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kSquare = Plane<128>::kBytes;  // a plane of 64 x 64
-
-// A fragment-ordered block of 16 columns (TILES tiles of 16 rows) -> planes with a row per column
-template <int TILES, int RB>
-__device__ __forceinline__ void transpose_in(const float *from, lds_char *planes, int plane_bytes, int row0, int unit) {
-    const int t = unit / 64, l = unit % 64;
-    const f32x4 x = *(const f32x4a *)(from + 4 * unit);
-    store_pieces(planes + Plane<RB>::addr(row0 + (l & 15), 4 * t + (l >> 4)), plane_bytes, x);
-}
+constexpr int kThreads = 512;
 
 template <typename T, int KE>
 __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) {
-    constexpr int RB = 64 * KE, PIECES = Elem<T>::kPieces, ET = 2 * KE, EW = ET / 4;
-    constexpr int kMB = 32;                                          // columns of the state at a time
+    constexpr int PIECES = Elem<T>::kPieces, NP = PIECES == 1 ? 2 : 3;
+    constexpr int RB = 64 * KE, ET = 2 * KE, EW = ET / 4, RT = 2;
+    constexpr int kMB = 32;                                           // columns of the state at a time
     constexpr int kGo = kRows * 64, kSq = kMB * 128, kSt = kMB * RB;  // bytes of a plane of dO, of Z or dE, of a state
-    constexpr int kPhase1 = PIECES * kGo + 6 * kSq + 6 * kSt;
-    constexpr int kRowsPlane = Plane<RB>::kBytes;
-    constexpr int kPhase2 = 2 * PIECES * kRowsPlane + 6 * kSquare;
-    constexpr int kBytes = kPhase1 > kPhase2 ? kPhase1 : kPhase2;
+    constexpr int kRowsPlane = Plane<RB>::kBytes, kSquare = Plane<128>::kBytes;
+    constexpr int kQK = 2 * PIECES * kRowsPlane, kPhase1 = PIECES * kGo + 2 * NP * kSq + 2 * NP * kSt;
+    constexpr bool kResident = PIECES == 1;  // rows of q and k stay in LDS; else they come after phase 1
+    constexpr int kPR = 2 * NP * kSquare;
+    constexpr int kBytes = kResident ? kQK + (kPhase1 > kPR ? kPhase1 : kPR) : (kPhase1 > kQK + kPR ? kPhase1 : kQK + kPR);
     __shared__ __align__(16) char mem[kBytes];
     __shared__ __align__(16) float f_mem[kFactors * kRows];
-    __shared__ float dots_mem[4][4][kRows];   // per wavefront: q.dq, k.dk+, k.dk-, k.(first term of dk-)
-    __shared__ float total_mem[2][kRows];     // q.dq and k.dk of all value heads
-    __shared__ float beta_mem[4][kRows];      // per row of tiles: the second term of dbeta
-    __shared__ float state_mem[4];            // per wavefront: its share of <S, dS>
+    __shared__ float dot_mem[2][2][kRows];  // per half of the columns staged together: dE . Z, dE . V
+    __shared__ float total_mem[2][kRows];  // q . dq and k . dk of all value heads
+    __shared__ float state_mem[8];         // per wavefront: its share of <S, dS>
     lds_char *const lds = (lds_char *)mem;
-    lds_char *const gop = lds, *const zp = gop + PIECES * kGo, *const dep = zp + 3 * kSq, *const sp = dep + 3 * kSq,
-                    *const dsp = sp + 3 * kSt;
-    lds_char *const qp = lds, *const kp = qp + PIECES * kRowsPlane, *const pp = kp + PIECES * kRowsPlane,
-                    *const rp = pp + 3 * kSquare;
+    lds_char *const qp = lds, *const kp = qp + PIECES * kRowsPlane;
+    lds_char *const gop = lds + (kResident ? kQK : 0), *const zp = gop + PIECES * kGo, *const dep = zp + NP * kSq,
+                    *const sp = dep + NP * kSq, *const dsp = sp + NP * kSt;
+    lds_char *const pp = lds + kQK, *const rp = pp + NP * kSquare;
     lds_float *const fp = (lds_float *)f_mem;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    const int G = p.H / p.Hk;
-    const int chunk = (int)(blockIdx.x % (uint32_t)p.chunks), nk = (int)(blockIdx.x / (uint32_t)p.chunks);
-    const int n = nk / p.Hk, hk = nk % p.Hk;
+    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6), c = lane & 15, q = lane >> 4;
+    const int e0 = EW * (wave & 3), t0 = RT * (wave >> 2);  // the wavefront's tiles of key columns and of positions
+    const int G = scalar(p.H / p.Hk);
+    const int nk = scalar((int)(blockIdx.x / (uint32_t)p.chunks)), chunk = (int)blockIdx.x - nk * p.chunks;
+    const int n = scalar(nk / p.Hk), hk = nk - n * p.Hk;
     const int64_t l0 = (int64_t)chunk * kRows;
-    const int rows = min((int64_t)kRows, p.L - l0);  // of the chunk in memory
+    const int rows = (int)min((int64_t)kRows, p.L - l0);  // of the chunk in memory
     auto grad_at = [&](const Scalars &x, int h, int i) { return n * x.sn + h * x.sh + (l0 + i) * x.sl; };
+    const Where first = where_of(p, n * p.H + hk * G, chunk);
+    const int valid = first.valid;  // (the same for all heads of a sequence)
 
-    f32x4 dQ[4][EW] = {}, dK[4][EW] = {};
+    f32x4 dQ[RT][EW] = {}, dK[RT][EW] = {};
+    auto stage_rows = [&]() {
+        RowTile<T, 32 * KE, kThreads> tile;
+        tile.load(chunk_rows(p.q, n, hk, l0, Elem<T>::kBytes), (uint32_t)p.q.stride_l * Elem<T>::kBytes, p.E, valid,
+                  p.vec_q, tid);
+        tile.template store<RB>(qp, tid);
+        tile.load(chunk_rows(p.k, n, hk, l0, Elem<T>::kBytes), (uint32_t)p.k.stride_l * Elem<T>::kBytes, p.E, valid,
+                  p.vec_k, tid);
+        tile.template store<RB>(kp, tid);
+    };
+
+    // ---- what phase 1 stages: dO's rows by the first 256 threads, the others' fragments by all ----
+    RowTile<T, kMB, 256> go;
+    f32x4 zr, er, sr[ET / 4], dr[ET / 4];
+    uint32_t vr[4];
+    auto request = [&](int h, int m0) {
+        const int64_t at = ((int64_t)(n * p.H + h) * p.chunks + chunk) * p.col_blocks;
+        if (tid < 256) {
+            Operand shifted = p.go;
+            shifted.ptr = (const char *)p.go.ptr + (int64_t)m0 * kCols * Elem<T>::kBytes;
+            go.load(chunk_rows(shifted, n, h, l0, Elem<T>::kBytes), (uint32_t)p.go.stride_l * Elem<T>::kBytes,
+                    p.M - m0 * kCols, valid, p.vec_go, tid);
+        }
+        const int block = m0 + (tid >> 8), unit = tid & 255, row = 4 * (unit >> 4 & 15), col = block * kCols + c;
+        {
+            const __amdgpu_buffer_rsrc_t rs = chunk_rows(p.v, n, h, l0, Elem<T>::kBytes);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t from = row + r < valid && col < p.M
+                    ? (uint32_t)(row + r) * ((uint32_t)p.v.stride_l * Elem<T>::kBytes) + (uint32_t)(col * Elem<T>::kBytes) : kOutside;
+                vr[r] = Elem<T>::kBytes == 4 ? __builtin_amdgcn_raw_buffer_load_b32(rs, from, 0, 0)
+                                             : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, from, 0, 0);
+            }
+        }
+        zr = er = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (block < p.col_blocks) {
+            zr = *(const f32x4a *)(p.z + (at + block) * (4 * 256) + 4 * unit);
+            er = *(const f32x4a *)(p.de + (at + block) * (4 * 256) + 4 * unit);
+        }
+#pragma unroll
+        for (int u = 0; u < ET / 4; u++) {
+            sr[u] = dr[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (block < p.col_blocks) {
+                sr[u] = *(const f32x4a *)(p.s + (at + block) * (ET * 256) + 4 * (unit + 256 * u));
+                dr[u] = *(const f32x4a *)(p.ds + (at + block) * (ET * 256) + 4 * (unit + 256 * u));
+            }
+        }
+    };
+    // a fragment's place in planes with a row per column: four positions (or key columns) of column c
+    auto put = [&](f32x4 &dot_z, f32x4 &dot_v) {
+        if (tid < 256) go.template store<64>(gop, tid);
+        const int row = 16 * (tid >> 8) + c, t = (tid & 255) >> 6;
+        float dot = 0.f;
+        store_pieces<NP>(zp + Plane<128>::addr(row, 4 * t + q), kSq, zr);
+        store_pieces<NP>(dep + Plane<128>::addr(row, 4 * t + q), kSq, er);
+        dot_z += er * zr;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            dot_v[r] = fmaf(er[r], __uint_as_float(Elem<T>::kBytes == 4 ? vr[r] : vr[r] << 16), dot_v[r]);
+#pragma unroll
+        for (int u = 0; u < ET / 4; u++) {
+            store_pieces<NP>(sp + Plane<RB>::addr(row, 4 * (t + 4 * u) + q), kSt, sr[u]);
+            store_pieces<NP>(dsp + Plane<RB>::addr(row, 4 * (t + 4 * u) + q), kSt, dr[u]);
+            dot += (sr[u][0] * dr[u][0] + sr[u][1] * dr[u][1]) + (sr[u][2] * dr[u][2] + sr[u][3] * dr[u][3]);
+        }
+        return dot;
+    };
+    // the tiles of the square matrices, transposed: rows j of tile tj, columns i of tile ti
+    auto tile_of = [&](int x, int &ti, int &tj) {
+        const int id = wave + 8 * x;
+        ti = id < 2 ? 0 : id < 4 ? 1 : id < 8 ? 2 : 3, tj = id < 4 ? id & 1 : id & 3;
+        return id < 12;
+    };
+
+    if (valid > 0) {
+        request(hk * G, 0);
+        if (kResident) stage_rows();
+    }
     if (tid < kRows) total_mem[0][tid] = total_mem[1][tid] = 0.f;
-
     for (int g = 0; g < G; g++) {
         const int h = hk * G + g;
-        const Where w = where_of(p, n * p.H + h, chunk);
-        if (w.valid == 0) {  // (the same for all heads of a sequence)
+        if (valid == 0) {
             if (tid < rows) {
                 if (p.gg.ptr) store_from_f32(p.gg.ptr, p.gg.dtype, grad_at(p.gg, h, tid), 0.f);
                 if (p.gb.ptr) store_from_f32(p.gb.ptr, p.gb.dtype, grad_at(p.gb, h, tid), 0.f);
             }
             continue;
         }
-        const float *const factors = p.factors + w.at * (kFactors * kRows);
-        for (int i = tid; i < kFactors * kRows; i += kThreads) fp[i] = factors[i];
+        const int64_t at = (int64_t)(n * p.H + h) * p.chunks + chunk;
+        for (int i = tid; i < kFactors * kRows; i += kThreads) fp[i] = p.factors[at * (kFactors * kRows) + i];
 
         // ---- phase 1 ----
-        f32x4 F[3] = {}, N[3] = {};                                   // (dO Z^T)^T, (dE Z^T)^T: rows j, columns i
-        f32x4 aQ[4][EW] = {}, aP[4][EW] = {}, aM[4][EW] = {};         // S dO, S dE, dS Z
+        f32x4 F[2] = {}, N[2] = {};                                    // (dO Z^T)^T, (dE Z^T)^T
+        f32x4 aQ[RT][EW] = {}, aP[RT][EW] = {}, aM[RT][EW] = {};       // S dO, S dE, dS Z
+        f32x4 dot_z = {0.f, 0.f, 0.f, 0.f}, dot_v = {0.f, 0.f, 0.f, 0.f};
         float state_dot = 0.f;
-        auto tile_of = [&](int x, int &ti, int &tj) {
-            const int id = wave + 4 * x;
-            ti = id < 2 ? 0 : id < 4 ? 1 : id < 8 ? 2 : 3, tj = id < 4 ? id & 1 : id & 3;
-        };
-        const __amdgpu_buffer_rsrc_t go_rows = chunk_rows(p.go, w.n, w.h, l0, Elem<T>::kBytes);
         for (int m0 = 0; m0 < p.col_blocks; m0 += 2) {
-            RowTile<T, kMB, kThreads> go;
-            // (32 columns from 16 m0 on: the offset goes into the rows' base)
-            {
-                Operand shifted = p.go;
-                shifted.ptr = (const char *)p.go.ptr + (int64_t)m0 * kCols * Elem<T>::kBytes;
-                const bool vec = (p.M - m0 * kCols) % (Elem<T>::kBytes == 4 ? 4 : 8) == 0 &&
-                                 (((uintptr_t)shifted.ptr | (uint64_t)(shifted.stride_n * Elem<T>::kBytes) |
-                                   (uint64_t)(shifted.stride_h * Elem<T>::kBytes) |
-                                   (uint64_t)(shifted.stride_l * Elem<T>::kBytes)) & 15) == 0;
-                go.load(chunk_rows(shifted, w.n, w.h, l0, Elem<T>::kBytes), (uint32_t)p.go.stride_l * Elem<T>::kBytes,
-                        p.M - m0 * kCols, w.valid, vec, tid);
-            }
             __syncthreads();  // (what was staged before has been read)
-            go.template store<64>(gop, tid);
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const int block = m0 + b;
-                const bool there = block < p.col_blocks;
-                const int64_t at = w.at * p.col_blocks + (there ? block : m0);
-                const float *const z = p.z + at * (4 * 256), *const de = p.de + at * (4 * 256),
-                            *const s = p.s + at * (ET * 256), *const ds = p.ds + at * (ET * 256);
-                if (there) {
-                    transpose_in<4, 128>(z, zp, kSq, 16 * b, tid);
-                    transpose_in<4, 128>(de, dep, kSq, 16 * b, tid);
-#pragma unroll
-                    for (int u = 0; u < ET / 4; u++) {
-                        const int unit = tid + kThreads * u, t = unit / 64, l = unit % 64;
-                        const f32x4 x = *(const f32x4a *)(s + 4 * unit), y = *(const f32x4a *)(ds + 4 * unit);
-                        state_dot += (x[0] * y[0] + x[1] * y[1]) + (x[2] * y[2] + x[3] * y[3]);
-                        store_pieces(sp + Plane<RB>::addr(16 * b + (l & 15), 4 * t + (l >> 4)), kSt, x);
-                        store_pieces(dsp + Plane<RB>::addr(16 * b + (l & 15), 4 * t + (l >> 4)), kSt, y);
-                    }
-                } else {  // zeros: dO's columns past M are zero too
-                    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                    const int t = tid / 64, l = tid % 64;
-                    store_pieces(zp + Plane<128>::addr(16 * b + (l & 15), 4 * t + (l >> 4)), kSq, zero);
-                    store_pieces(dep + Plane<128>::addr(16 * b + (l & 15), 4 * t + (l >> 4)), kSq, zero);
-#pragma unroll
-                    for (int u = 0; u < ET / 4; u++) {
-                        const int unit = tid + kThreads * u, tt = unit / 64;
-                        store_pieces(sp + Plane<RB>::addr(16 * b + (l & 15), 4 * tt + (l >> 4)), kSt, zero);
-                        store_pieces(dsp + Plane<RB>::addr(16 * b + (l & 15), 4 * tt + (l >> 4)), kSt, zero);
-                    }
-                }
-            }
+            state_dot += put(dot_z, dot_v);
             __syncthreads();
+            if (m0 + 2 < p.col_blocks) request(h, m0 + 2);
+            else if (g + 1 < G) request(h + 1, 0);
 #pragma unroll
-            for (int x = 0; x < 3; x++) {
+            for (int x = 0; x < 2; x++) {
                 int ti, tj;
-                tile_of(x, ti, tj);
-                Frag zf[3], of[PIECES], ef[3];
+                if (!tile_of(x, ti, tj)) continue;
+                Frag zf[NP], of[PIECES], ef[NP];
                 columns_of<128>(zp, tj, 0, c, q, zf, kSq);
 #pragma unroll
                 for (int k = 0; k < PIECES; k++) of[k] = Plane<64>::rows(gop + k * kGo, ti, 0, c, q);
@@ -146,19 +176,19 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
                 columns_of<128>(dep, ti, 0, c, q, ef, kSq);
                 N[x] = product(zf, ef, N[x]);
             }
-            Frag sf[EW][3], df[EW][3];
+            Frag sf[EW][NP], df[EW][NP];
 #pragma unroll
             for (int e = 0; e < EW; e++) {
-                columns_of<RB>(sp, EW * wave + e, 0, c, q, sf[e], kSt);
-                columns_of<RB>(dsp, EW * wave + e, 0, c, q, df[e], kSt);
+                columns_of<RB>(sp, e0 + e, 0, c, q, sf[e], kSt);
+                columns_of<RB>(dsp, e0 + e, 0, c, q, df[e], kSt);
             }
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                Frag of[PIECES], ef[3], zf[3];
+            for (int t = 0; t < RT; t++) {
+                Frag of[PIECES], ef[NP], zf[NP];
 #pragma unroll
-                for (int k = 0; k < PIECES; k++) of[k] = Plane<64>::rows(gop + k * kGo, t, 0, c, q);
-                columns_of<128>(dep, t, 0, c, q, ef, kSq);
-                columns_of<128>(zp, t, 0, c, q, zf, kSq);
+                for (int k = 0; k < PIECES; k++) of[k] = Plane<64>::rows(gop + k * kGo, t0 + t, 0, c, q);
+                columns_of<128>(dep, t0 + t, 0, c, q, ef, kSq);
+                columns_of<128>(zp, t0 + t, 0, c, q, zf, kSq);
 #pragma unroll
                 for (int e = 0; e < EW; e++) {
                     aQ[t][e] = product(of, sf[e], aQ[t][e]);
@@ -167,80 +197,59 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
                 }
             }
         }
-        (void)go_rows;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) state_dot += __shfl_xor(state_dot, d);
+#pragma unroll
+        for (int r = 0; r < 4; r++) dot_z[r] = sum16(dot_z[r]), dot_v[r] = sum16(dot_v[r]);
+        settle();
         if (lane == 0) state_mem[wave] = state_dot;
+        if (c == 0)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                dot_mem[wave >> 2][0][16 * (wave & 3) + 4 * q + r] = dot_z[r];
+                dot_mem[wave >> 2][1][16 * (wave & 3) + 4 * q + r] = dot_v[r];
+            }
+        // (by the wavefront that sums the decays: on its way during phase 2)
+        float o = 0.f, written = 0.f;
+        if (wave == 0)
+            for (int b = 0; b < p.col_blocks; b++) {
+                o += p.dots[(at * p.col_blocks + b) * kRows + lane];
+                written += p.written[(at * p.col_blocks + b) * 64 + lane];
+            }
 
         // ---- phase 2 ----
         __syncthreads();
-        {
-            RowTile<T, 32 * KE, kThreads> tile;
-            tile.load(chunk_rows(p.q, w.n, w.hk, l0, Elem<T>::kBytes), (uint32_t)p.q.stride_l * Elem<T>::kBytes, p.E,
-                      w.valid, p.vec_q, tid);
-            tile.template store<RB>(qp, tid);
-            tile.load(chunk_rows(p.k, w.n, w.hk, l0, Elem<T>::kBytes), (uint32_t)p.k.stride_l * Elem<T>::kBytes, p.E,
-                      w.valid, p.vec_k, tid);
-            tile.template store<RB>(kp, tid);
-        }
-        __syncthreads();
+        if (!kResident) stage_rows();
 #pragma unroll
-        for (int x = 0; x < 3; x++) {
+        for (int x = 0; x < 2; x++) {
             int ti, tj;
-            tile_of(x, ti, tj);
-            f32x4 kk = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < KE; s++) {
-                Frag a[PIECES], b[PIECES];
-                rows_of<RB>(kp, tj, s, c, q, a);
-                rows_of<RB>(kp, ti, s, c, q, b);
-                kk = product(a, b, kk);
-            }
+            if (!tile_of(x, ti, tj)) continue;
             const int i = 16 * ti + c, j0 = 16 * tj + 4 * q;
             const float rk_i = fp[kRk * kRows + i], rq_i = fp[kRq * kRows + i];
-            f32x4 pt, rt, bt;
+            f32x4 pt, rt;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int j = j0 + r;
                 const float d = j <= i ? expf((fp[kHigh * kRows + i] - fp[kHigh * kRows + j]) +
-                                              (fp[kLow * kRows + i] - fp[kLow * kRows + j])) * fp[kRk * kRows + j] : 0.f;
-                const float b = fp[kBeta * kRows + j];
-                pt[r] = j <= i ? b * F[x][r] * d * rq_i : 0.f;
-                const float n_ij = j < i ? N[x][r] * d * rk_i : 0.f;
-                rt[r] = -b * n_ij;
-                bt[r] = sum16(n_ij * kk[r]);
+                                              (fp[kLow * kRows + i] - fp[kLow * kRows + j])) *
+                                             (fp[kRk * kRows + j] * fp[kBeta * kRows + j]) : 0.f;
+                pt[r] = j <= i ? F[x][r] * d * rq_i : 0.f;
+                rt[r] = j < i ? -N[x][r] * d * rk_i : 0.f;
             }
-            store_pieces(pp + Plane<128>::addr(i, 4 * tj + q), kSquare, pt);
-            store_pieces(rp + Plane<128>::addr(i, 4 * tj + q), kSquare, rt);
-            if (c == 0)
-#pragma unroll
-                for (int r = 0; r < 4; r++) beta_mem[ti][j0 + r] = bt[r];
+            store_pieces<NP>(pp + Plane<128>::addr(i, 4 * tj + q), kSquare, pt);
+            store_pieces<NP>(rp + Plane<128>::addr(i, 4 * tj + q), kSquare, rt);
         }
-        // the values of q and k at the places of the accumulators
-        auto row_value = [&](const lds_char *planes, int row, int col) {
-            float v = 0.f;
 #pragma unroll
-            for (int k = PIECES - 1; k >= 0; k--)
-                v += bf16_to_f32(*(const __attribute__((address_space(3))) uint16_t *)(
-                    planes + k * kRowsPlane + Plane<RB>::addr(row, col >> 2) + 2 * (col & 3)));
-            return v;
-        };
-        float first[4][4];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int t = 0; t < RT; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int row = 16 * t + 4 * q + r;
-                const float rise = fp[kRise * kRows + row], fall = fp[kFall * kRows + row], rk = fp[kRk * kRows + row];
-                float dot = 0.f;
+                const int row = 16 * (t0 + t) + 4 * q + r;
+                const float read_q = fp[kReadQ * kRows + row], read_k = fp[kReadK * kRows + row], write = fp[kWrite * kRows + row];
 #pragma unroll
                 for (int e = 0; e < EW; e++) {
-                    aQ[t][e][r] *= rise * fp[kRq * kRows + row];
-                    aP[t][e][r] *= -rise * rk;
-                    aM[t][e][r] *= fall * rk * fp[kBeta * kRows + row];
-                    dot = fmaf(row_value(kp, row, 16 * (EW * wave + e) + c), aM[t][e][r], dot);
+                    dQ[t][e][r] = fmaf(read_q, aQ[t][e][r], dQ[t][e][r]);
+                    dK[t][e][r] += write * aM[t][e][r] - read_k * aP[t][e][r];
                 }
-                first[t][r] = sum16(dot);
             }
         __syncthreads();
 #pragma unroll
@@ -248,84 +257,56 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
             Frag kf[EW][PIECES], qf[EW][PIECES];
 #pragma unroll
             for (int e = 0; e < EW; e++) {
-                columns_of<RB>(kp, EW * wave + e, s, c, q, kf[e]);
-                columns_of<RB>(qp, EW * wave + e, s, c, q, qf[e]);
+                columns_of<RB>(kp, e0 + e, s, c, q, kf[e]);
+                columns_of<RB>(qp, e0 + e, s, c, q, qf[e]);
             }
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                Frag f[3];
-                if (t >= 2 * s) {  // rows i of tile t: columns j up to it
-                    rows_of<128>(pp, t, s, c, q, f);
+            for (int t = 0; t < RT; t++) {
+                Frag f[NP];
+                if (t0 + t >= 2 * s) {  // rows i: columns j up to it
+                    rows_of<128>(pp, t0 + t, s, c, q, f);
 #pragma unroll
-                    for (int e = 0; e < EW; e++) aQ[t][e] = product(f, kf[e], aQ[t][e]);
-                    rows_of<128>(rp, t, s, c, q, f);
+                    for (int e = 0; e < EW; e++) dQ[t][e] = product(f, kf[e], dQ[t][e]);
+                    rows_of<128>(rp, t0 + t, s, c, q, f);
 #pragma unroll
-                    for (int e = 0; e < EW; e++) aP[t][e] = product(f, kf[e], aP[t][e]);
+                    for (int e = 0; e < EW; e++) dK[t][e] = product(f, kf[e], dK[t][e]);
                 }
-                if (t < 2 * s + 2) {  // columns j of tile t: rows i from it on
-                    columns_of<128>(pp, t, s, c, q, f);
+                if (t0 + t < 2 * s + 2) {  // columns j: rows i from it on
+                    columns_of<128>(pp, t0 + t, s, c, q, f);
 #pragma unroll
-                    for (int e = 0; e < EW; e++) aM[t][e] = product(f, qf[e], aM[t][e]);
-                    columns_of<128>(rp, t, s, c, q, f);
+                    for (int e = 0; e < EW; e++) dK[t][e] = product(f, qf[e], dK[t][e]);
+                    columns_of<128>(rp, t0 + t, s, c, q, f);
 #pragma unroll
-                    for (int e = 0; e < EW; e++) aM[t][e] = product(f, kf[e], aM[t][e]);
+                    for (int e = 0; e < EW; e++) dK[t][e] = product(f, kf[e], dK[t][e]);
                 }
             }
         }
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int row = 16 * t + 4 * q + r;
-                float dq = 0.f, dp = 0.f, dm = 0.f;
-#pragma unroll
-                for (int e = 0; e < EW; e++) {
-                    const int col = 16 * (EW * wave + e) + c;
-                    const float kv = row_value(kp, row, col);
-                    dq = fmaf(row_value(qp, row, col), aQ[t][e][r], dq);
-                    dp = fmaf(kv, aP[t][e][r], dp);
-                    dm = fmaf(kv, aM[t][e][r], dm);
-                }
-                dq = sum16(dq), dp = sum16(dp), dm = sum16(dm);
-                if (c == 0) {
-                    dots_mem[wave][0][row] = dq, dots_mem[wave][1][row] = dp, dots_mem[wave][2][row] = dm;
-                    dots_mem[wave][3][row] = first[t][r];
-                }
-#pragma unroll
-                for (int e = 0; e < EW; e++) dQ[t][e][r] += aQ[t][e][r], dK[t][e][r] += aP[t][e][r] + aM[t][e][r];
-            }
-        __syncthreads();
         if (wave == 0) {
-            float dot[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                dot[k] = (dots_mem[0][k][lane] + dots_mem[1][k][lane]) + (dots_mem[2][k][lane] + dots_mem[3][k][lane]);
-            total_mem[0][lane] += dot[0], total_mem[1][lane] += dot[1] + dot[2];
-            double sum = (double)dot[0] + (double)dot[1] - (double)dot[2], all = dot[3];
+            const float z = dot_mem[0][0][lane] + dot_mem[1][0][lane], v = dot_mem[0][1][lane] + dot_mem[1][1][lane];
+            total_mem[0][lane] += o, total_mem[1][lane] += 2.f * z - v;
+            double sum = (double)o - (double)v, all = written, state = 0.0;
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-            all += (double)fp[kRise * kRows + kRows - 1] *
-                   (((double)state_mem[0] + (double)state_mem[1]) + ((double)state_mem[2] + (double)state_mem[3]));
+#pragma unroll
+            for (int i = 0; i < 8; i++) state += state_mem[i];
+            all += (double)fp[kRise * kRows + kRows - 1] * state;
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) {  // sums from here to the end
                 const double other = __shfl_down(sum, d);
                 if (lane + d < 64) sum += other;
             }
-            if (p.gg.ptr && lane < rows)
-                store_from_f32(p.gg.ptr, p.gg.dtype, grad_at(p.gg, h, lane), lane < w.valid ? (float)(sum + all) : 0.f);
-        } else if (wave == 1 && p.gb.ptr && lane < rows) {
-            float sum = 0.f;
-            for (int b = 0; b < p.col_blocks; b++) sum += p.zdu[(w.at * p.col_blocks + b) * kRows + lane];
-            // (tiles of column block lane / 16: rows of tiles from it on)
-            float less = 0.f;
-            for (int t = lane / 16; t < 4; t++) less += beta_mem[t][lane];
-            store_from_f32(p.gb.ptr, p.gb.dtype, grad_at(p.gb, h, lane), lane < w.valid ? sum - less : 0.f);
+            if (lane < rows) {
+                if (p.gg.ptr)
+                    store_from_f32(p.gg.ptr, p.gg.dtype, grad_at(p.gg, h, lane), lane < valid ? (float)(sum + all) : 0.f);
+                if (p.gb.ptr)
+                    store_from_f32(p.gb.ptr, p.gb.dtype, grad_at(p.gb, h, lane),
+                                   lane < valid ? z / fp[kBeta * kRows + lane] : 0.f);
+            }
         }
         __syncthreads();
     }
 
-    const Where w = where_of(p, n * p.H + hk * G, chunk);
-    if (w.valid > 0 && p.normalize) {  // (q, k, the factors of the last head: those of q and k are alike)
+    if (valid > 0 && p.normalize) {  // (the factors of the last head: those of q and k are alike)
         auto row_value = [&](const lds_char *planes, int row, int col) {
             float v = 0.f;
 #pragma unroll
@@ -335,29 +316,29 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
             return v;
         };
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int t = 0; t < RT; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int row = 16 * t + 4 * q + r;
+                const int row = 16 * (t0 + t) + 4 * q + r;
                 const float rq = fp[kRq0 * kRows + row], rk = fp[kRk * kRows + row];
                 const float fq = total_mem[0][row] * rq * rq, fk = total_mem[1][row] * rk * rk;
 #pragma unroll
                 for (int e = 0; e < EW; e++) {
-                    const int col = 16 * (EW * wave + e) + c;
+                    const int col = 16 * (e0 + e) + c;
                     dQ[t][e][r] = fmaf(-fq, row_value(qp, row, col), dQ[t][e][r]);
                     dK[t][e][r] = fmaf(-fk, row_value(kp, row, col), dK[t][e][r]);
                 }
             }
     }
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+    for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const int row = 16 * t + 4 * q + r;
+            const int row = 16 * (t0 + t) + 4 * q + r;
             if (row >= rows) continue;
 #pragma unroll
             for (int e = 0; e < EW; e++) {
-                const int col = 16 * (EW * wave + e) + c;
+                const int col = 16 * (e0 + e) + c;
                 if (col >= p.E) continue;
                 if (p.gq.ptr)
                     store_from_f32(p.gq.ptr, p.gq.dtype,

@@ -21,8 +21,9 @@
 // column c.  Two such tiles, rows 0 to 15 and 16 to 31, are the eight values of one k-step of the next product's
 // right operand if the left one takes its k in the same order: slots 0 to 3 are k = 4 q + r, slots 4 to 7
 // k = 16 + 4 q + r.  So a wavefront that owns 16 columns of the state goes through a chunk's three
-// products without an exchange.  What it leaves in memory it leaves in the order of its registers ("fragments":
-// per tile 64 lanes x 4 values).
+// products without an exchange.  What the kernels leave for each other lies in the order of the registers
+// ("fragments"): of results, per tile 64 lanes x 4 floats; of left operands, per tile, k-step and piece 64 lanes x 8
+// bf16, so that the scan needs neither LDS nor barriers.
 #pragma once
 #include "ftc_wg_kernel.h"
 
@@ -51,15 +52,18 @@ constexpr float kNormEps = 1e-6f;
 enum Factor {
     kRise,   // e^{G_i}
     kFall,   // e^{G_64 - G_i}
-    kBeta,   // beta_i (0 past the sequence's end)
+    kBeta,   // beta_i (0 past the sequence's end, at least 2^-64 in size before it)
     kRk,     // 1 / |k_i|, or 1
     kRq,     // scale / |q_i|, or scale
     kRq0,    // 1 / |q_i|, or 1
     kHigh,   // G_i in two floats: its differences are wanted to 24 bits, whatever its size
     kLow,
+    kReadK,  // rk e^{G_i}: k_i as it reads the state
+    kReadQ,  // rq e^{G_i}
+    kWriteK, // rk e^{G_64 - G_i}: as it is written
+    kWrite,  // ... times beta_i
     kFactors
 };
-
 struct Scalars {  // one value per position: log decays, beta and their gradients
     void *ptr;
     int64_t sn, sh, sl;
@@ -73,13 +77,16 @@ struct DeltaArgs {
     StateRef initial, final_;
     OperandOut out;
     int32_t N, H, Hk, L, E, M, chunks, col_blocks;  // col_blocks: of 16 columns
-    int32_t vec_q, vec_k;    // rows can be read 16 bytes at a time
+    int32_t vec_q, vec_k, vec_go;  // rows can be read 16 bytes at a time
     int32_t normalize;
     float scale;
     float *factors;          // [chain][chunk][kFactors][64]
-    uint16_t *t;             // T: [chain][chunk][3 pieces][64][64]
-    float *s;                // states before each chunk, fragments: [chain][chunk][col block][2 KE tiles][64][4]
-    float *z;                // Z, fragments: [chain][chunk][col block][4 tiles][64][4]
+    // left operands' fragments, [chain][chunk][number][pieces][64][8]
+    uint16_t *t, *tt;        // T and its transpose (may be absent): six with 3 pieces, those not above the diagonal
+    uint16_t *kr, *kc, *qc;  // of key chains: rows of k, columns of k and (backward) of q
+    // results' fragments
+    float *s;                // states before each chunk: [chain][chunk][col block][2 KE tiles][64][4]
+    float *z, *o;            // Z and (may be absent) O: [chain][chunk][col block][4 tiles][64][4]
     // backward
     Operand go;
     OperandOut gq, gk, gv;
@@ -87,7 +94,8 @@ struct DeltaArgs {
     StateRef grad_final, grad_initial;
     float *ds;               // the gradient of the state after each chunk, as s
     float *de;               // A^T dO, then dE, as z
-    float *zdu;              // sum over a column block of Z dU: [chain][chunk][col block][64]
+    float *dots;             // dO . O of every position, column block by column block: [chain][chunk][col block][64]
+    float *written;          // shares of what a chunk's keys write of <state, its gradient>: the same, [64 lanes]
 };
 
 // ---- rows in LDS ----
@@ -120,17 +128,25 @@ __device__ __forceinline__ f32x4 mfma16(const Frag &a, const Frag &b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mfma::bf16x8, a),
                                                    __builtin_bit_cast(mfma::bf16x8, b), c, 0, 0, 0);
 }
-// acc += A B over the piece products of order <= 2, smallest first
+// acc += A B over the piece products of order <= 2 (two pieces at most: <= 1), smallest first
 template <int NA, int NB>
 __device__ __forceinline__ f32x4 product(const Frag (&a)[NA], const Frag (&b)[NB], f32x4 acc) {
 #pragma unroll
-    for (int order = 2; order >= 0; order--)
+    for (int order = NA > 2 || NB > 2 ? 2 : 1; order >= 0; order--)
 #pragma unroll
         for (int pa = 0; pa < NA; pa++) {
             const int pb = order - pa;
             if (pb >= 0 && pb < NB) acc = mfma16(a[pa], b[pb], acc);
         }
     return acc;
+}
+// Lets the last products' results arrive before a branch.  The compiler counts the instructions between a matrix
+// product and the first use of its result, but where a branch skips a block it counts those of the block on the path
+// without them too (seen in a listing: a result read two instructions after its product, and wrong rows).
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
 }
 // two tiles of a result -> the k-step that they are for the next product
 __device__ __forceinline__ void cut(const f32x4 &lo, const f32x4 &hi, Frag (&f)[3]) {
@@ -154,11 +170,15 @@ __device__ __forceinline__ void cut(const f32x4 &lo, const f32x4 &hi, Frag (&f)[
 // ---- rows from memory ----
 constexpr uint32_t kOutside = 0x80000000u;  // an offset that no buffer reaches: reads as zero
 
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // A chunk's rows of one chain.  Offsets within it stay below 2 GiB (the strides are checked for that); the
 // chunk's own place is in the 64-bit base.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const Operand &o, int64_t n, int64_t h, int64_t l0,
                                                             int bytes) {
-    const char *base = (const char *)o.ptr + (n * o.stride_n + h * o.stride_h + l0 * o.stride_l) * bytes;
+    const uint64_t at = (uint64_t)o.ptr + (uint64_t)((n * o.stride_n + h * o.stride_h + l0 * o.stride_l) * bytes);
+    // (the same in every lane; the compiler, which has made it from a division, would try the lanes one by one)
+    const char *base = (const char *)(((uint64_t)(uint32_t)scalar((int)(at >> 32)) << 32) | (uint32_t)scalar((int)(uint32_t)at));
     return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0x7fffffff, mfma::kRsrcFlags);
 }
 
@@ -250,20 +270,56 @@ __device__ __forceinline__ void columns_of(const lds_char *planes, int t, int s,
     for (int p = 0; p < PIECES; p++) f[p] = Plane<RB>::columns(planes + p * plane_bytes, t, s, c, q);
 }
 
-// Four values of consecutive columns of a row -> the planes
-__device__ __forceinline__ void store_pieces(lds_char *to, int plane_bytes, const f32x4 &x) {
-    uint32_t a[3], b[3];
-    mfma::split_pair_under_mfma(x[0], x[1], a);
-    mfma::split_pair_under_mfma(x[2], x[3], b);
+// Two values -> NP pieces.  Three add up to the value exactly; two leave 2^-17 of it (both rounded to nearest).
+template <int NP>
+__device__ __forceinline__ void pieces_of(float x0, float x1, uint32_t (&o)[NP]) {
+    if constexpr (NP == 3) {
+        mfma::split_pair_under_mfma(x0, x1, o);
+    } else {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int p = 0; p < 3; p++)
+        for (int p = 0; p < NP; p++) {
+            o[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x0, x1}, bf16x2));
+            x0 -= __uint_as_float(o[p] << 16), x1 -= __uint_as_float(o[p] & 0xffff0000u);
+        }
+    }
+}
+// Four values of consecutive columns of a row -> the planes
+template <int NP = 3>
+__device__ __forceinline__ void store_pieces(lds_char *to, int plane_bytes, const f32x4 &x) {
+    uint32_t a[NP], b[NP];
+    pieces_of<NP>(x[0], x[1], a);
+    pieces_of<NP>(x[2], x[3], b);
+#pragma unroll
+    for (int p = 0; p < NP; p++)
         *(__attribute__((address_space(3))) u32x2a *)(to + p * plane_bytes) = u32x2{a[p], b[p]};
 }
+
+// ---- left operands' fragments in memory ----
+template <int PIECES>
+__device__ __forceinline__ void load_frag(const uint16_t *from, int number, int lane, Frag (&f)[PIECES]) {
+#pragma unroll
+    for (int p = 0; p < PIECES; p++) {
+        const u32x4 r = *(const u32x4a *)(from + (number * PIECES + p) * 512 + 8 * lane);
+        f[p] = Frag{{r.x, r.y, r.z, r.w}};
+    }
+}
+template <int PIECES>
+__device__ __forceinline__ void store_frag(uint16_t *to, int number, int lane, const Frag (&f)[PIECES]) {
+#pragma unroll
+    for (int p = 0; p < PIECES; p++)
+        *(u32x4a *)(to + (number * PIECES + p) * 512 + 8 * lane) = u32x4{f[p].w[0], f[p].w[1], f[p].w[2], f[p].w[3]};
+}
+// T: row tile t has k-steps 0 .. t / 2; its transpose k-steps t / 2 .. 1
+constexpr int kTFrags = 6;
+__device__ __forceinline__ constexpr int t_number(int t, int s) { return t < 2 ? t : 2 * t - 2 + s; }
+__device__ __forceinline__ constexpr int tt_number(int t, int s) { return t < 2 ? 2 * t + s : t + 2; }
 
 // ---- places ----
 struct Where {
     int32_t chain, n, h, hk, chunk, len, valid;  // len: positions of the sequence; valid: of them in this chunk
-    int64_t at;                                  // chain * chunks + chunk
+    int64_t at, key_at;                          // chain * chunks + chunk, and of the key head's chain
 };
 __device__ __forceinline__ int sequence_length(const DeltaArgs &p, int n) {
     if (!p.lengths) return p.L;
@@ -272,11 +328,13 @@ __device__ __forceinline__ int sequence_length(const DeltaArgs &p, int n) {
 }
 __device__ __forceinline__ Where where_of(const DeltaArgs &p, int chain, int chunk) {
     Where w;
-    w.chain = chain, w.chunk = chunk, w.n = chain / p.H, w.h = chain % p.H, w.hk = w.h / (p.H / p.Hk);
-    w.len = sequence_length(p, w.n);
-    const int left = w.len - chunk * kRows;
+    w.chain = scalar(chain), w.chunk = scalar(chunk);
+    w.n = scalar(w.chain / p.H), w.h = w.chain - w.n * p.H, w.hk = scalar(w.h / (p.H / p.Hk));
+    w.len = scalar(sequence_length(p, w.n));
+    const int left = w.len - w.chunk * kRows;
     w.valid = left < 0 ? 0 : left > kRows ? kRows : left;
-    w.at = (int64_t)chain * p.chunks + chunk;
+    w.at = (int64_t)w.chain * p.chunks + w.chunk;
+    w.key_at = ((int64_t)w.n * p.Hk + w.hk) * p.chunks + w.chunk;
     return w;
 }
 __device__ __forceinline__ int chunks_of(int len) { return (len + kRows - 1) / kRows; }

@@ -1,5 +1,5 @@
 // The gated delta rule, what the chunks compute from the states before them, all chunks side by side:
-// the outputs O = diag(rq e^G) Q S + A diag(beta) Z and, for the backward, A^T dO.  Formulas and layouts:
+// the outputs O = diag(rq e^G) Q S + A diag(beta) Z and, for the backward, A^T dO and dO . O.  Formulas and layouts:
 // ftc_delta_kernel.h.
 //
 // A workgroup of four wavefronts takes one chunk and 16 CT columns per wavefront: A once for all of them, in LDS in
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kThreads) void delta_outputs_kernel(DeltaArgs p) {
     constexpr int RB = 64 * KE, PIECES = Elem<T>::kPieces, ET = 2 * KE;
     __shared__ __align__(16) char q_mem[PIECES * Plane<RB>::kBytes], k_mem[PIECES * Plane<RB>::kBytes], a_mem[3 * kAPlane];
     lds_char *const qp = (lds_char *)q_mem, *const kp = (lds_char *)k_mem, *const ap = (lds_char *)a_mem;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6), c = lane & 15, q = lane >> 4;
     const int groups = (p.col_blocks + 4 * CT - 1) / (4 * CT);
     const uint32_t id = blockIdx.x / (uint32_t)groups;
     const int first = (int)(blockIdx.x % (uint32_t)groups) * 4 * CT + wave * CT;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kThreads) void delta_outputs_kernel(DeltaArgs p) {
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 const int i0 = 16 * t + 4 * q;
-                O[t] *= *(const f32x4a *)(factors + kRise * kRows + i0) * *(const f32x4a *)(factors + kRq * kRows + i0);
+                O[t] *= *(const f32x4a *)(factors + kReadQ * kRows + i0);
                 Z[t] *= *(const f32x4a *)(factors + kBeta * kRows + i0);
             }
 #pragma unroll
@@ -115,6 +115,12 @@ __global__ __launch_bounds__(kThreads) void delta_outputs_kernel(DeltaArgs p) {
                     rows_of<128>(ap, t, s, c, q, af);
                     O[t] = product(af, uf, O[t]);
                 }
+            }
+            settle();
+            if (p.o) {
+                float *const to = p.o + (w.at * p.col_blocks + block) * (4 * 256) + 4 * lane;
+#pragma unroll
+                for (int t = 0; t < 4; t++) *(f32x4a *)(to + 256 * t) = O[t];
             }
         }
         if (col < p.M)
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(kThreads) void delta_pull_kernel(DeltaArgs p) {
     constexpr int RB = 64 * KE, PIECES = Elem<T>::kPieces;
     __shared__ __align__(16) char q_mem[PIECES * Plane<RB>::kBytes], k_mem[PIECES * Plane<RB>::kBytes], a_mem[3 * kAPlane];
     lds_char *const qp = (lds_char *)q_mem, *const kp = (lds_char *)k_mem, *const ap = (lds_char *)a_mem;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6), c = lane & 15, q = lane >> 4;
     const int groups = (p.col_blocks + 4 * CT - 1) / (4 * CT);
     const uint32_t id = blockIdx.x / (uint32_t)groups;
     const int first = (int)(blockIdx.x % (uint32_t)groups) * 4 * CT + wave * CT;
@@ -141,6 +147,13 @@ __global__ __launch_bounds__(kThreads) void delta_pull_kernel(DeltaArgs p) {
     const float *const factors = p.factors + w.at * (kFactors * kRows);
     if (w.valid == 0) return;
     stage<T, KE>(p, w, factors, qp, kp, ap, tid);
+    // the queries' fragments, by the first workgroup of the first value head
+    if (w.h % (p.H / p.Hk) == 0 && blockIdx.x % (uint32_t)groups == 0)
+        for (int i = wave; i < 4 * KE; i += 4) {
+            Frag f[PIECES];
+            columns_of<RB>(qp, i / 2, i % 2, c, q, f);
+            store_frag(p.qc + w.key_at * (4 * KE * PIECES * 512), i, lane, f);
+        }
 
     const __amdgpu_buffer_rsrc_t rows = chunk_rows(p.go, w.n, w.h, (int64_t)w.chunk * kRows, Elem<T>::kBytes);
     const uint32_t row_bytes = (uint32_t)p.go.stride_l * Elem<T>::kBytes;
@@ -168,9 +181,16 @@ __global__ __launch_bounds__(kThreads) void delta_pull_kernel(DeltaArgs p) {
                 Y[t] = product(af, gf, Y[t]);
             }
         }
-        float *const to = p.de + (w.at * p.col_blocks + block) * (4 * 256) + 4 * lane;
+        const int64_t at = w.at * p.col_blocks + block;
 #pragma unroll
-        for (int t = 0; t < 4; t++) *(f32x4a *)(to + 256 * t) = Y[t];
+        for (int t = 0; t < 4; t++) *(f32x4a *)(p.de + at * (4 * 256) + 4 * lane + 256 * t) = Y[t];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            f32x4 dot = G[t] * *(const f32x4a *)(p.o + at * (4 * 256) + 4 * lane + 256 * t);
+#pragma unroll
+            for (int r = 0; r < 4; r++) dot[r] = sum16(dot[r]);
+            if (c == 0) *(f32x4a *)(p.dots + at * kRows + 16 * t + 4 * q) = dot;
+        }
     }
 }
 

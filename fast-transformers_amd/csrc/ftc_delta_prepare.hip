@@ -39,12 +39,13 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
     constexpr int RB = 64 * KE, PIECES = Elem<T>::kPieces;
     using Tile = RowTile<T, 32 * KE, kThreads>;
     __shared__ __align__(16) char k_mem[PIECES * Plane<RB>::kBytes];
-    __shared__ __align__(16) float m_mem[kRows * kStride], t_mem[kRows * kStride], x_mem[32 * kStride];
+    // (M; at the end T's three planes)
+    __shared__ __align__(16) float m_mem[3 * Plane<128>::kBytes / 4], t_mem[kRows * kStride], x_mem[32 * kStride];
     __shared__ float k2_mem[kRows], q2_mem[kRows], high_mem[kRows], low_mem[kRows], beta_mem[kRows], rk_mem[kRows];
     lds_char *const kp = (lds_char *)k_mem;
     lds_float *const Mx = (lds_float *)m_mem, *const Tm = (lds_float *)t_mem, *const X = (lds_float *)x_mem;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6), c = lane & 15, q = lane >> 4;
     const Where w = where_of(p, (int)(blockIdx.x / (uint32_t)p.chunks), (int)(blockIdx.x % (uint32_t)p.chunks));
     if (w.valid == 0) return;  // (nobody reads what belongs to it)
     const int64_t l0 = (int64_t)w.chunk * kRows;
@@ -69,10 +70,12 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
         double g = 0.0;
         float b = 0.f;
         if (lane < w.valid) {
+            // (a beta of zero is taken as 2^-64: dbeta is found as dE . Z / beta, and all terms of dE have that factor)
             const int64_t l = l0 + lane;
             const float x = load_as_f32(p.g.ptr, p.g.dtype, w.n * p.g.sn + w.h * p.g.sh + l * p.g.sl);
             g = x < -1000.f ? -1000.0 : (double)x;
             b = load_as_f32(p.b.ptr, p.b.dtype, w.n * p.b.sn + w.h * p.b.sh + l * p.b.sl);
+            if (fabsf(b) < 0x1p-64f) b = 0x1p-64f;
         }
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -83,8 +86,13 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
         const float high = (float)g, low = (float)(g - (double)high);
         const float rk = p.normalize ? (float)(1.0 / sqrt((double)k2_mem[lane] + (double)kNormEps)) : 1.f;
         const float rq0 = p.normalize ? (float)(1.0 / sqrt((double)q2_mem[lane] + (double)kNormEps)) : 1.f;
-        factors[kRise * kRows + lane] = (float)exp(g);
-        factors[kFall * kRows + lane] = (float)exp(total - g);
+        const float rise = (float)exp(g), fall = (float)exp(total - g);
+        factors[kRise * kRows + lane] = rise;
+        factors[kFall * kRows + lane] = fall;
+        factors[kReadK * kRows + lane] = rk * rise;
+        factors[kReadQ * kRows + lane] = rq0 * p.scale * rise;
+        factors[kWriteK * kRows + lane] = rk * fall;
+        factors[kWrite * kRows + lane] = rk * fall * b;
         factors[kBeta * kRows + lane] = b;
         factors[kRk * kRows + lane] = rk;
         factors[kRq * kRows + lane] = rq0 * p.scale;
@@ -94,6 +102,18 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
         high_mem[lane] = high, low_mem[lane] = low, beta_mem[lane] = b, rk_mem[lane] = rk;
     }
     __syncthreads();
+
+    // the keys' fragments, by the first value head of the key head
+    if (w.h % (p.H / p.Hk) == 0) {
+        uint16_t *const kr = p.kr + w.key_at * (4 * KE * PIECES * 512), *const kc = p.kc + w.key_at * (4 * KE * PIECES * 512);
+        for (int i = wave; i < 4 * KE; i += 4) {
+            Frag f[PIECES];
+            rows_of<RB>(kp, i / KE, i % KE, c, q, f);
+            store_frag(kr, i, lane, f);
+            columns_of<RB>(kp, i / 2, i % 2, c, q, f);
+            store_frag(kc, i, lane, f);
+        }
+    }
 
     // M: the ten tiles on and below the diagonal
     for (int id = wave; id < 10; id += 4) {
@@ -169,18 +189,24 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
         for (int r = 0; r < 4; r++) Tm[(32 + 16 * a + 4 * q + r) * kStride + 16 * b + c] = -y[r];
     }
     __syncthreads();
-    uint16_t *const to = p.t + w.at * (3 * kRows * kRows);
+    // T in pieces where M was, and from there its fragments
+    lds_char *const tp = (lds_char *)m_mem;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int u = tid + kThreads * i, row = u / 8, col = 8 * (u % 8);
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = Tm[row * kStride + col + j];
+    for (int i = 0; i < 4; i++) {
+        const int u = tid + kThreads * i, row = u / 16, slot = u % 16;
+        const lds_float *const x = Tm + row * kStride + 4 * slot;
+        store_pieces(tp + Plane<128>::addr(row, slot), Plane<128>::kBytes, f32x4{x[0], x[1], x[2], x[3]});
+    }
+    __syncthreads();
+    for (int i = wave; i < kTFrags; i += 4) {
         Frag f[3];
-        mfma::split8<3>(x, f);
-#pragma unroll
-        for (int k = 0; k < 3; k++)
-            *(u32x4a *)(to + k * kRows * kRows + row * kRows + col) = u32x4{f[k].w[0], f[k].w[1], f[k].w[2], f[k].w[3]};
+        const int t = i < 2 ? i : 1 + i / 2, s = i < 2 ? 0 : i % 2;
+        rows_of<128>(tp, t, s, c, q, f);
+        store_frag(p.t + w.at * (kTFrags * 3 * 512), i, lane, f);
+        if (!p.tt) continue;
+        const int u = i < 4 ? i / 2 : i - 2, v = i < 4 ? i % 2 : 1;
+        columns_of<128>(tp, u, v, c, q, f);
+        store_frag(p.tt + w.at * (kTFrags * 3 * 512), i, lane, f);
     }
 }
 

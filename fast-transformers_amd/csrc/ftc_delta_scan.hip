@@ -1,84 +1,86 @@
 // The gated delta rule's state from chunk to chunk, forward (Z of every position, the state before every chunk and
 // after the last) and backward (the gradient of the state, dE = dV).  Formulas and layouts: ftc_delta_kernel.h.
 //
-// A wavefront owns 16 columns of one chain's state in registers and walks the chunks; what it multiplies with, the
-// rows of k (and q) and T, the workgroup stages in LDS, each chunk's while the one before is worked on.
+// A wavefront owns 16 columns of one chain's state in registers and walks the chunks, alone: what it multiplies with
+// it reads as fragments, straight into the registers of the operands, each one's next chunk requested as soon as this
+// chunk's is used.  A chunk is a chain of dependent products, so what bounds few chains is its latency.
 #include "ftc_delta_kernel.h"
 
 namespace ftc {
 namespace delta {
 namespace {
 
-constexpr int kTPlane = Plane<128>::kBytes;
-constexpr int kFactorFloats = kFactors * kRows;
+// Keeps the requests of a phase where they are written
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
 
-// T of a chunk: 3 planes of 64 x 64, into registers and on into LDS
-template <int NT>
-struct TTile {
-    static constexpr int kPer = 3 * kRows * 8 / NT;
-    u32x4 r[kPer];
-    __device__ __forceinline__ void load(const uint16_t *t, int tid) {
-#pragma unroll
-        for (int i = 0; i < kPer; i++) r[i] = *(const u32x4a *)(t + 8 * (tid + NT * i));
-    }
-    __device__ __forceinline__ void store(lds_char *planes, int tid) const {
-#pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            const int u = tid + NT * i, piece = u / (kRows * 8), row = (u / 8) % kRows;
-            *(__attribute__((address_space(3))) u32x4a *)(planes + piece * kTPlane + Plane<128>::addr(row, 2 * (u % 8))) =
-                r[i];
-        }
-    }
-};
-template <int NT>
-struct FactorTile {
-    static constexpr int kPer = (kFactorFloats / 4 + NT - 1) / NT;
-    f32x4 r[kPer];
-    __device__ __forceinline__ void load(const float *f, int tid) {
-#pragma unroll
-        for (int i = 0; i < kPer; i++)
-            if (tid + NT * i < kFactorFloats / 4) r[i] = *(const f32x4a *)(f + 4 * (tid + NT * i));
-    }
-    __device__ __forceinline__ void store(lds_float *to, int tid) const {
-#pragma unroll
-        for (int i = 0; i < kPer; i++)
-            if (tid + NT * i < kFactorFloats / 4)
-                *(__attribute__((address_space(3))) f32x4a *)(to + 4 * (tid + NT * i)) = r[i];
-    }
-};
 // rows 16 t + 4 q .. of a factor
-__device__ __forceinline__ f32x4 factor(const lds_float *f, int which, int t, int q) {
-    return *(const __attribute__((address_space(3))) f32x4a *)(f + which * kRows + 16 * t + 4 * q);
+__device__ __forceinline__ void load_factor(const float *f, int which, int q, f32x4 (&x)[4]) {
+#pragma unroll
+    for (int t = 0; t < 4; t++) x[t] = *(const f32x4a *)(f + which * kRows + 16 * t + 4 * q);
+}
+__device__ __forceinline__ void load_tiles(const float *from, f32x4 (&x)[4]) {
+#pragma unroll
+    for (int t = 0; t < 4; t++) x[t] = *(const f32x4a *)(from + 256 * t);
+}
+__device__ __forceinline__ void store_tiles(float *to, const f32x4 (&x)[4]) {
+#pragma unroll
+    for (int t = 0; t < 4; t++) *(f32x4a *)(to + 256 * t) = x[t];
 }
 
-// Values of rows 16 t + 4 q + r of a column
-template <typename T>
-__device__ __forceinline__ void load_column(__amdgpu_buffer_rsrc_t rs, uint32_t row_bytes, int col, int width, int valid,
-                                            int q, f32x4 (&x)[4]) {
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int row = 16 * t + 4 * q + r;
-            x[t][r] = load_one<T>(rs, row < valid && col < width ? (uint32_t)row * row_bytes + (uint32_t)(col * Elem<T>::kBytes)
-                                                                 : kOutside);
-        }
+// acc += A B with the left operand's fragment held, or read here
+template <bool HELD, int HA, int NB>
+__device__ __forceinline__ f32x4 times(const Frag (&held)[HA], const uint16_t *from, int number, int lane, const Frag (&b)[NB],
+                                       f32x4 acc) {
+    if constexpr (HELD) {
+        return product(held, b, acc);
+    } else {
+        Frag a[3];
+        load_frag(from, number, lane, a);
+        return product(a, b, acc);
+    }
 }
+
+// Workgroups go to the eight dies in turn: those of one chain to the same, whose cache they share
+__device__ __forceinline__ bool place(const DeltaArgs &p, int groups, int &chain, int &group) {
+    const uint32_t die = blockIdx.x % 8u, slot = blockIdx.x / 8u;
+    chain = (int)(slot / (uint32_t)groups * 8u + die), group = (int)(slot % (uint32_t)groups);
+    return chain < p.N * p.H;
+}
+
+// Values of rows 16 t + 4 q + r of a column, as they come from memory: what is done to them here would wait for them
+template <typename T>
+struct Column {
+    uint32_t raw[4][4];
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row_bytes, int col, int width, int valid, int q) {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = 16 * t + 4 * q + r;
+                const uint32_t at = row < valid && col < width
+                                        ? (uint32_t)row * row_bytes + (uint32_t)(col * Elem<T>::kBytes) : kOutside;
+                raw[t][r] = Elem<T>::kBytes == 4 ? __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0)
+                                                 : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, at, 0, 0);
+            }
+    }
+    __device__ __forceinline__ f32x4 values(int t) const {
+        f32x4 x;
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = __uint_as_float(Elem<T>::kBytes == 4 ? raw[t][r] : raw[t][r] << 16);
+        return x;
+    }
+};
 
 template <typename T, int KE, int NW>
-__global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaArgs p) {
-    constexpr int NT = 64 * NW, RB = 64 * KE, PIECES = Elem<T>::kPieces, ET = 2 * KE;
-    __shared__ __align__(16) char k_mem[PIECES * Plane<RB>::kBytes], t_mem[3 * kTPlane];
-    __shared__ __align__(16) float f_mem[kFactorFloats];
-    lds_char *const kp = (lds_char *)k_mem, *const tp = (lds_char *)t_mem;
-    lds_float *const fp = (lds_float *)f_mem;
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    const int groups = (p.col_blocks + NW - 1) / NW;
-    const int block = (int)(blockIdx.x % (uint32_t)groups) * NW + wave, col = kCols * block + c;
-    const Where w = where_of(p, (int)(blockIdx.x / (uint32_t)groups), 0);
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_kernel(DeltaArgs p) {
+    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512;
+    const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6), c = lane & 15, q = lane >> 4;
+    int chain, group;
+    if (!place(p, (p.col_blocks + NW - 1) / NW, chain, group)) return;
+    const int block = group * NW + wave, col = kCols * block + c;
+    if (block >= p.col_blocks) return;
+    const Where w = where_of(p, chain, 0);
     const int chunks = chunks_of(w.len);
-    const bool mine = block < p.col_blocks;
 
     f32x4 S[ET];
 #pragma unroll
@@ -91,92 +93,87 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaArgs p) {
                           : 0.f;
         }
 
-    RowTile<T, 32 * KE, NT> k_tile;
-    TTile<NT> t_tile;
-    FactorTile<NT> f_tile;
-    f32x4 V[4];
-    const uint32_t k_row = (uint32_t)p.k.stride_l * Elem<T>::kBytes, v_row = (uint32_t)p.v.stride_l * Elem<T>::kBytes;
-    auto request = [&](int chunk) {
-        const int64_t at = (int64_t)w.chain * p.chunks + chunk, l0 = (int64_t)chunk * kRows;
-        const int valid = min(kRows, w.len - chunk * kRows);
-        k_tile.load(chunk_rows(p.k, w.n, w.hk, l0, Elem<T>::kBytes), k_row, p.E, valid, p.vec_k, tid);
-        t_tile.load(p.t + at * (3 * kRows * kRows), tid);
-        f_tile.load(p.factors + at * kFactorFloats, tid);
-        load_column<T>(chunk_rows(p.v, w.n, w.h, l0, Elem<T>::kBytes), v_row, col, p.M, valid, q, V);
-    };
-    if (chunks > 0) request(0);
-    for (int chunk = 0; chunk < chunks; chunk++) {
-        const int64_t at = (int64_t)w.chain * p.chunks + chunk;
-        __syncthreads();
-        k_tile.template store<RB>(kp, tid);
-        t_tile.store(tp, tid);
-        f_tile.store(fp, tid);
-        f32x4 Z[4];
+    const uint32_t v_row = (uint32_t)p.v.stride_l * Elem<T>::kBytes;
+    // (three pieces of wide rows would not fit: read when they are used)
+    constexpr bool kHold = KE * PIECES <= 6;
+    Frag kr[4 * KE][kHold ? PIECES : 1], kc[4 * KE][kHold ? PIECES : 1], tf[kTFrags][3];
+    Column<T> V;
+    f32x4 in[4], out[4];
+    float last;
+    auto load_in = [&](int chunk) {
+        if constexpr (kHold)
 #pragma unroll
-        for (int t = 0; t < 4; t++) Z[t] = V[t];
-        __syncthreads();
-        if (chunk + 1 < chunks) request(chunk + 1);
-
-        if (p.s && mine) {
-            float *const to = p.s + (at * p.col_blocks + block) * (ET * 256) + 4 * lane;
+            for (int i = 0; i < 4 * KE; i++) load_frag(p.kr + (w.key_at + chunk) * kKeys, i, lane, kr[i]);
+    };
+    auto load_values = [&](int chunk) {
+        V.load(chunk_rows(p.v, w.n, w.h, (int64_t)chunk * kRows, Elem<T>::kBytes), v_row, col, p.M,
+               min(kRows, w.len - chunk * kRows), q);
+        load_factor(p.factors + (w.at + chunk) * (kFactors * kRows), kReadK, q, in);
+    };
+    auto load_t = [&](int chunk) {
+#pragma unroll
+        for (int i = 0; i < kTFrags; i++) load_frag(p.t + (w.at + chunk) * (kTFrags * 3 * 512), i, lane, tf[i]);
+        load_factor(p.factors + (w.at + chunk) * (kFactors * kRows), kWrite, q, out);
+        last = p.factors[(w.at + chunk) * (kFactors * kRows) + kRise * kRows + kRows - 1];
+    };
+    auto load_out = [&](int chunk) {
+        if constexpr (kHold)
+#pragma unroll
+            for (int i = 0; i < 4 * KE; i++) load_frag(p.kc + (w.key_at + chunk) * kKeys, i, lane, kc[i]);
+    };
+    if (chunks > 0) load_in(0), load_values(0), load_t(0), load_out(0);
+    for (int chunk = 0; chunk < chunks; chunk++) {
+        const int64_t at = (w.at + chunk) * p.col_blocks + block;
+        const int next = min(chunk + 1, chunks - 1);
+        {
+            float *const to = p.s + at * (ET * 256) + 4 * lane;
 #pragma unroll
             for (int t = 0; t < ET; t++) *(f32x4a *)(to + 256 * t) = S[t];
         }
         // E = V - diag(rk e^G) K S
-        f32x4 P[4] = {};
+        f32x4 P[4] = {}, Z[4] = {};
 #pragma unroll
         for (int s = 0; s < KE; s++) {
             Frag sf[3];
             cut(S[2 * s], S[2 * s + 1], sf);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                Frag kf[PIECES];
-                rows_of<RB>(kp, t, s, c, q, kf);
-                P[t] = product(kf, sf, P[t]);
-            }
+            for (int t = 0; t < 4; t++) P[t] = times<kHold>(kr[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, sf, P[t]);
         }
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const f32x4 f = factor(fp, kRise, t, q) * factor(fp, kRk, t, q);
-            P[t] = Z[t] - f * P[t];
-            Z[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int t = 0; t < 4; t++) P[t] = V.values(t) - in[t] * P[t];
+        phase();
+        load_in(next), load_values(next);
+        phase();
         // Z = T E (tiles above the diagonal are zero)
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag ef[3];
             cut(P[2 * s], P[2 * s + 1], ef);
 #pragma unroll
-            for (int t = 2 * s; t < 4; t++) {
-                Frag tf[3];
-                rows_of<128>(tp, t, s, c, q, tf);
-                Z[t] = product(tf, ef, Z[t]);
-            }
+            for (int t = 2 * s; t < 4; t++) Z[t] = product(tf[t_number(t, s)], ef, Z[t]);
         }
-        if (p.z && mine) {
-            float *const to = p.z + (at * p.col_blocks + block) * (4 * 256) + 4 * lane;
-#pragma unroll
-            for (int t = 0; t < 4; t++) *(f32x4a *)(to + 256 * t) = Z[t];
-        }
+        store_tiles(p.z + at * (4 * 256) + 4 * lane, Z);
         // S <- e^{G_64} S + K^T diag(rk beta e^{G_64 - G}) Z
-        const float last = fp[kRise * kRows + kRows - 1];
 #pragma unroll
-        for (int t = 0; t < 4; t++) Z[t] *= factor(fp, kFall, t, q) * factor(fp, kBeta, t, q) * factor(fp, kRk, t, q);
+        for (int t = 0; t < 4; t++) Z[t] *= out[t];
 #pragma unroll
         for (int t = 0; t < ET; t++) S[t] *= last;
+        phase();
+        load_t(next);
+        phase();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag uf[3];
             cut(Z[2 * s], Z[2 * s + 1], uf);
 #pragma unroll
-            for (int t = 0; t < ET; t++) {
-                Frag kf[PIECES];
-                columns_of<RB>(kp, t, s, c, q, kf);
-                S[t] = product(kf, uf, S[t]);
-            }
+            for (int t = 0; t < ET; t++)
+                S[t] = times<kHold>(kc[2 * t + s], p.kc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, uf, S[t]);
         }
+        phase();
+        load_out(next);
+        phase();
     }
-    if (p.final_.ptr && mine)
+    if (p.final_.ptr)
 #pragma unroll
         for (int t = 0; t < ET; t++)
 #pragma unroll
@@ -190,20 +187,17 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaArgs p) {
 // The same walk from the last chunk to the first, on the gradient of the state:
 //   dU = A^T dO + diag(rk e^{G_64 - G}) K dS,   dE = T^T diag(beta) dU,
 //   dS <- e^{G_64} dS + Q^T diag(rq e^G) dO - K^T diag(rk e^G) dE
+// and what the chunk's keys write of <state, its gradient>: the sum of beta Z . diag(rk e^{G_64 - G}) K dS.
 template <typename T, int KE, int NW>
-__global__ __launch_bounds__(64 * NW) void delta_scan_back_kernel(DeltaArgs p) {
-    constexpr int NT = 64 * NW, RB = 64 * KE, PIECES = Elem<T>::kPieces, ET = 2 * KE;
-    __shared__ __align__(16) char k_mem[PIECES * Plane<RB>::kBytes], q_mem[PIECES * Plane<RB>::kBytes], t_mem[3 * kTPlane];
-    __shared__ __align__(16) float f_mem[kFactorFloats];
-    lds_char *const kp = (lds_char *)k_mem, *const qp = (lds_char *)q_mem, *const tp = (lds_char *)t_mem;
-    lds_float *const fp = (lds_float *)f_mem;
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    const int groups = (p.col_blocks + NW - 1) / NW;
-    const int block = (int)(blockIdx.x % (uint32_t)groups) * NW + wave, col = kCols * block + c;
-    const Where w = where_of(p, (int)(blockIdx.x / (uint32_t)groups), 0);
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_back_kernel(DeltaArgs p) {
+    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512;
+    const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6), c = lane & 15, q = lane >> 4;
+    int chain, group;
+    if (!place(p, (p.col_blocks + NW - 1) / NW, chain, group)) return;
+    const int block = group * NW + wave, col = kCols * block + c;
+    if (block >= p.col_blocks) return;
+    const Where w = where_of(p, chain, 0);
     const int chunks = chunks_of(w.len);
-    const bool mine = block < p.col_blocks;
 
     f32x4 S[ET];
 #pragma unroll
@@ -217,126 +211,121 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_back_kernel(DeltaArgs p) {
                           : 0.f;
         }
 
-    RowTile<T, 32 * KE, NT> k_tile, q_tile;
-    TTile<NT> t_tile;
-    FactorTile<NT> f_tile;
-    f32x4 G[4], Y[4], Zn[4];
-    const uint32_t k_row = (uint32_t)p.k.stride_l * Elem<T>::kBytes, q_row = (uint32_t)p.q.stride_l * Elem<T>::kBytes,
-                   g_row = (uint32_t)p.go.stride_l * Elem<T>::kBytes;
-    auto request = [&](int chunk) {
-        const int64_t at = (int64_t)w.chain * p.chunks + chunk, l0 = (int64_t)chunk * kRows;
-        const int valid = min(kRows, w.len - chunk * kRows);
-        k_tile.load(chunk_rows(p.k, w.n, w.hk, l0, Elem<T>::kBytes), k_row, p.E, valid, p.vec_k, tid);
-        q_tile.load(chunk_rows(p.q, w.n, w.hk, l0, Elem<T>::kBytes), q_row, p.E, valid, p.vec_q, tid);
-        t_tile.load(p.t + at * (3 * kRows * kRows), tid);
-        f_tile.load(p.factors + at * kFactorFloats, tid);
-        load_column<T>(chunk_rows(p.go, w.n, w.h, l0, Elem<T>::kBytes), g_row, col, p.M, valid, q, G);
-        if (mine) {
-            const int64_t z = (at * p.col_blocks + block) * (4 * 256) + 4 * lane;
+    const uint32_t g_row = (uint32_t)p.go.stride_l * Elem<T>::kBytes, gv_row = (uint32_t)p.gv.stride_l * Elem<T>::kBytes;
+    constexpr bool kHold = KE * PIECES <= 4;
+    Frag kr[4 * KE][kHold ? PIECES : 1], kc[4 * KE][kHold ? PIECES : 1], qc[4 * KE][kHold ? PIECES : 1], tf[kTFrags][3];
+    Column<T> Gr;
+    f32x4 Y[4], Z[4], write[4], beta[4], read_q[4], read_k[4];
+    float last;
+    auto factors = [&](int chunk) { return p.factors + (w.at + chunk) * (kFactors * kRows); };
+    auto tiles = [&](int chunk) { return ((w.at + chunk) * p.col_blocks + block) * (4 * 256) + 4 * lane; };
+    auto load_in = [&](int chunk) {
+        if constexpr (kHold)
 #pragma unroll
-            for (int t = 0; t < 4; t++) Y[t] = *(const f32x4a *)(p.de + z + 256 * t);
+            for (int i = 0; i < 4 * KE; i++) load_frag(p.kr + (w.key_at + chunk) * kKeys, i, lane, kr[i]);
+        load_factor(factors(chunk), kWrite, q, write);
+        load_factor(factors(chunk), kBeta, q, beta);
+        load_tiles(p.de + tiles(chunk), Y);
+        load_tiles(p.z + tiles(chunk), Z);
+    };
+    auto load_t = [&](int chunk) {
 #pragma unroll
-            for (int t = 0; t < 4; t++) Zn[t] = *(const f32x4a *)(p.z + z + 256 * t);
+        for (int i = 0; i < kTFrags; i++) load_frag(p.tt + (w.at + chunk) * (kTFrags * 3 * 512), i, lane, tf[i]);
+        load_factor(factors(chunk), kReadQ, q, read_q);
+        load_factor(factors(chunk), kReadK, q, read_k);
+        last = factors(chunk)[kRise * kRows + kRows - 1];
+        Gr.load(chunk_rows(p.go, w.n, w.h, (int64_t)chunk * kRows, Elem<T>::kBytes), g_row, col, p.M,
+                min(kRows, w.len - chunk * kRows), q);
+    };
+    auto load_out = [&](int chunk) {
+        if constexpr (kHold) {
+#pragma unroll
+            for (int i = 0; i < 4 * KE; i++) load_frag(p.qc + (w.key_at + chunk) * kKeys, i, lane, qc[i]);
+#pragma unroll
+            for (int i = 0; i < 4 * KE; i++) load_frag(p.kc + (w.key_at + chunk) * kKeys, i, lane, kc[i]);
         }
     };
-#pragma unroll
-    for (int t = 0; t < 4; t++) Y[t] = Zn[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (chunks > 0) request(chunks - 1);
+    if (chunks > 0) load_in(chunks - 1), load_t(chunks - 1), load_out(chunks - 1);
     for (int chunk = chunks - 1; chunk >= 0; chunk--) {
-        const int64_t at = (int64_t)w.chain * p.chunks + chunk;
-        const int valid = min(kRows, w.len - chunk * kRows);
-        __syncthreads();
-        k_tile.template store<RB>(kp, tid);
-        q_tile.template store<RB>(qp, tid);
-        t_tile.store(tp, tid);
-        f_tile.store(fp, tid);
-        f32x4 D[4], Z[4], O[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) D[t] = Y[t], Z[t] = Zn[t], O[t] = G[t];
-        __syncthreads();
-        if (chunk > 0) request(chunk - 1);
-
-        if (mine) {
-            float *const to = p.ds + (at * p.col_blocks + block) * (ET * 256) + 4 * lane;
+        const int64_t at = (w.at + chunk) * p.col_blocks + block;
+        const int next = max(chunk - 1, 0);
+        {
+            float *const to = p.ds + at * (ET * 256) + 4 * lane;
 #pragma unroll
             for (int t = 0; t < ET; t++) *(f32x4a *)(to + 256 * t) = S[t];
         }
-        f32x4 P[4] = {};
+        f32x4 P[4] = {}, D[4], G[4];
 #pragma unroll
         for (int s = 0; s < KE; s++) {
             Frag sf[3];
             cut(S[2 * s], S[2 * s + 1], sf);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                Frag kf[PIECES];
-                rows_of<RB>(kp, t, s, c, q, kf);
-                P[t] = product(kf, sf, P[t]);
-            }
+            for (int t = 0; t < 4; t++)
+                P[t] = times<kHold>(kr[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, sf, P[t]);
         }
-        // dU, its products with Z (the gradient of beta), and diag(beta) dU
+        // diag(beta) dU
+        f32x4 written = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            D[t] += factor(fp, kFall, t, q) * factor(fp, kRk, t, q) * P[t];
-            f32x4 dot = Z[t] * D[t];
-#pragma unroll
-            for (int r = 0; r < 4; r++) dot[r] = sum16(dot[r]);
-            if (mine && c == 0) *(f32x4a *)(p.zdu + (at * p.col_blocks + block) * kRows + 16 * t + 4 * q) = dot;
-            D[t] *= factor(fp, kBeta, t, q);
+            P[t] *= write[t];
+            D[t] = beta[t] * Y[t] + P[t];
+            written += Z[t] * P[t];
             P[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
+        p.written[at * 64 + lane] = (written[0] + written[1]) + (written[2] + written[3]);
+        phase();
+        load_in(next);
+        phase();
         // dE = T^T diag(beta) dU
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag df[3];
             cut(D[2 * s], D[2 * s + 1], df);
 #pragma unroll
-            for (int t = 0; t < 2 * s + 2; t++) {
-                Frag tf[3];
-                columns_of<128>(tp, t, s, c, q, tf);
-                P[t] = product(tf, df, P[t]);
-            }
+            for (int t = 0; t < 2 * s + 2; t++) P[t] = product(tf[tt_number(t, s)], df, P[t]);
         }
-        if (mine) {
-            float *const to = p.de + (at * p.col_blocks + block) * (4 * 256) + 4 * lane;
+        store_tiles(p.de + at * (4 * 256) + 4 * lane, P);
+        if (p.gv.ptr) {  // (a buffer drops what lies outside)
+            const int64_t l0 = (int64_t)chunk * kRows;
+            const __amdgpu_buffer_rsrc_t rs = chunk_rows(Operand{p.gv.ptr, p.gv.stride_n, p.gv.stride_h, p.gv.stride_l, 0, 0},
+                                                         w.n, w.h, l0, Elem<T>::kBytes);
 #pragma unroll
-            for (int t = 0; t < 4; t++) *(f32x4a *)(to + 256 * t) = P[t];
-            if (p.gv.ptr && col < p.M)
+            for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int row = 16 * t + 4 * q + r;
-                        if (row < valid)
-                            store_from_f32(p.gv.ptr, p.gv.dtype,
-                                           w.n * p.gv.stride_n + w.h * p.gv.stride_h +
-                                               ((int64_t)chunk * kRows + row) * p.gv.stride_l + col, P[t][r]);
-                    }
+                for (int r = 0; r < 4; r++) {
+                    const int row = 16 * t + 4 * q + r;
+                    const uint32_t to = l0 + row < w.len && col < p.M
+                                            ? (uint32_t)row * gv_row + (uint32_t)(col * Elem<T>::kBytes) : kOutside;
+                    if (Elem<T>::kBytes == 4)
+                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(P[t][r]), rs, to, 0, 0);
+                    else
+                        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (__bf16)P[t][r]), rs, to, 0, 0);
+                }
         }
-        const float last = fp[kRise * kRows + kRows - 1];
+        settle();
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const f32x4 rise = factor(fp, kRise, t, q);
-            O[t] *= rise * factor(fp, kRq, t, q);
-            P[t] *= -rise * factor(fp, kRk, t, q);
-        }
+        for (int t = 0; t < 4; t++) G[t] = Gr.values(t) * read_q[t], P[t] *= -read_k[t];
 #pragma unroll
         for (int t = 0; t < ET; t++) S[t] *= last;
+        phase();
+        load_t(next);
+        phase();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag of[3], ef[3];
-            cut(O[2 * s], O[2 * s + 1], of);
+            cut(G[2 * s], G[2 * s + 1], of);
+#pragma unroll
+            for (int t = 0; t < ET; t++)
+                S[t] = times<kHold>(qc[2 * t + s], p.qc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, of, S[t]);
             cut(P[2 * s], P[2 * s + 1], ef);
 #pragma unroll
-            for (int t = 0; t < ET; t++) {
-                Frag f[PIECES];
-                columns_of<RB>(qp, t, s, c, q, f);
-                S[t] = product(f, of, S[t]);
-                columns_of<RB>(kp, t, s, c, q, f);
-                S[t] = product(f, ef, S[t]);
-            }
+            for (int t = 0; t < ET; t++)
+                S[t] = times<kHold>(kc[2 * t + s], p.kc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, ef, S[t]);
         }
+        phase();
+        load_out(next);
+        phase();
     }
-    if (!mine) return;
     if (p.grad_initial.ptr)
 #pragma unroll
         for (int t = 0; t < ET; t++)
@@ -355,8 +344,9 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_back_kernel(DeltaArgs p) {
 
 template <typename T, int KE>
 void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
-    constexpr int NW = 4;
-    const dim3 grid((uint32_t)p.N * (uint32_t)p.H * (uint32_t)((p.col_blocks + NW - 1) / NW));
+    constexpr int NW = 1;
+    const uint32_t groups = (uint32_t)((p.col_blocks + NW - 1) / NW);
+    const dim3 grid(((uint32_t)p.N * (uint32_t)p.H + 7) / 8 * 8 * groups);
     if (back) delta_scan_back_kernel<T, KE, NW><<<grid, 64 * NW, 0, stream>>>(p);
     else delta_scan_kernel<T, KE, NW><<<grid, 64 * NW, 0, stream>>>(p);
 }

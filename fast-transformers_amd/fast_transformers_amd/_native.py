@@ -169,7 +169,7 @@ def load():
                  "ftc_gated_delta_rule_backward_workspace_bytes"):
         f = getattr(lib, name)
         f.restype = ctypes.c_int64
-        f.argtypes = [ctypes.c_int64] * 6
+        f.argtypes = [ctypes.c_int64] * 6 + [ctypes.c_int32]
     scalars = [ctypes.c_void_p, ctypes.c_float, ctypes.c_int32]  # lengths, scale, normalize
     memory = [ctypes.c_void_p, ctypes.c_size_t]
     lib.ftc_gated_delta_rule.restype = ctypes.c_int

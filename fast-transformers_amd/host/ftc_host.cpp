@@ -789,8 +789,8 @@ std::tuple<Tensor, OptTensor, OptTensor> delta_rule(const Tensor &queries, const
     const Tensor out = at::empty({N, L, H, M}, t.v.options()).permute({0, 2, 1, 3});
     OptTensor s1;
     if (return_state) s1 = at::empty({N, H, E, M}, t.v.options().dtype(at::kFloat));
-    const Tensor memory = keep ? delta_memory(ftc_gated_delta_rule_kept_bytes(N, H, Hk, L, E, M), "ftc_gated_delta_rule_kept_bytes", t.q)
-                               : delta_memory(ftc_gated_delta_rule_workspace_bytes(N, H, Hk, L, E, M),
+    const Tensor memory = keep ? delta_memory(ftc_gated_delta_rule_kept_bytes(N, H, Hk, L, E, M, t.dq.dtype), "ftc_gated_delta_rule_kept_bytes", t.q)
+                               : delta_memory(ftc_gated_delta_rule_workspace_bytes(N, H, Hk, L, E, M, t.dq.dtype),
                                               "ftc_gated_delta_rule_workspace_bytes", t.q);
     const ftc_tensor4 dout = describe(out);
     const Out d1(s1, "final_state");
@@ -830,7 +830,7 @@ std::vector<OptTensor> delta_rule_backward(const Tensor &queries, const Tensor &
     const Out gq(grads[0], "grad_queries"), gk(grads[1], "grad_keys"), gv(grads[2], "grad_values"),
         gg(wide(grads[3]), "grad_log_decay"), gb(wide(grads[4]), "grad_beta"), g0(grads[5], "grad_initial_state");
     const ftc_tensor4 dgo = delta_describe(go, "grad_out");
-    const Tensor ws = delta_memory(ftc_gated_delta_rule_backward_workspace_bytes(N, H, Hk, L, E, M),
+    const Tensor ws = delta_memory(ftc_gated_delta_rule_backward_workspace_bytes(N, H, Hk, L, E, M, t.dq.dtype),
                                    "ftc_gated_delta_rule_backward_workspace_bytes", t.q);
     hipStream_t const stream = c10::hip::getCurrentHIPStream(t.q.device().index()).stream();
     const void *const held = kept.const_data_ptr();

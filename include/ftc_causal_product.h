@@ -352,8 +352,10 @@ int ftc_linear_split_normed(const void *x, const float *x_scale, int64_t tokens,
  * position among it), or NULL for a forward without one, which then needs `workspace`.  Neither needs
  * initialisation, both are 256-byte aligned.
  */
-int64_t ftc_gated_delta_rule_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M);
-int64_t ftc_gated_delta_rule_kept_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M);
+int64_t ftc_gated_delta_rule_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M,
+                                             int32_t dtype);
+int64_t ftc_gated_delta_rule_kept_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M,
+                                             int32_t dtype);
 int ftc_gated_delta_rule(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,
                          const ftc_tensor4 *log_decay, const ftc_tensor4 *beta, const int64_t *lengths, float scale,
                          int32_t normalize, const ftc_tensor4 *initial_state, const ftc_tensor4 *out,
@@ -365,7 +367,8 @@ int ftc_gated_delta_rule(const ftc_tensor4 *queries, const ftc_tensor4 *keys, co
  * those of the forward; gradients have their inputs' dtypes (grad_initial_state: FTC_F32), those of positions past
  * a sequence's end are zero, and one that is not wanted may be NULL.  L >= 1.
  */
-int64_t ftc_gated_delta_rule_backward_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M);
+int64_t ftc_gated_delta_rule_backward_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M,
+                                             int32_t dtype);
 int ftc_gated_delta_rule_backward(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,
                                   const ftc_tensor4 *log_decay, const ftc_tensor4 *beta, const int64_t *lengths,
                                   float scale, int32_t normalize, const void *kept, size_t kept_bytes,

@@ -117,10 +117,11 @@ def test_c_abi_refuses_on_the_host():
     status, message = _call()                       # no workspace
     assert status == -3 and "needs" in message
     lib = _native.load()
-    assert lib.ftc_gated_delta_rule_workspace_bytes(1, 2, 1, 8, 8, 8) == 0
-    assert lib.ftc_gated_delta_rule_workspace_bytes(1, 2, 1, 9, 8, 8) > 0
-    assert lib.ftc_gated_delta_rule_kept_bytes(1, 3, 2, 9, 8, 8) == -1
-    assert lib.ftc_gated_delta_rule_backward_workspace_bytes(1 << 20, 1 << 10, 1, 1 << 20, 128, 128) == -2
+    assert lib.ftc_gated_delta_rule_workspace_bytes(1, 2, 1, 8, 8, 8, 0) == 0
+    assert lib.ftc_gated_delta_rule_workspace_bytes(1, 2, 1, 9, 8, 8, 0) > 0
+    assert lib.ftc_gated_delta_rule_kept_bytes(1, 3, 2, 9, 8, 8, 0) == -1
+    assert lib.ftc_gated_delta_rule_backward_workspace_bytes(1 << 20, 1 << 10, 1, 1 << 20, 128, 128, 0) == -2
+    assert lib.ftc_gated_delta_rule_kept_bytes(1, 2, 1, 9, 8, 8, 2) == -1
     q, v, g, s = _t4((1, 1, 1, 8)), _t4((1, 2, 1, 8)), _t4((1, 2, 1, 1)), _t4((1, 2, 8, 8), stride=(0, 0, 8, 1))
     args = [ctypes.byref(t) for t in (q, q, v, g, g)]
     assert lib.ftc_gated_delta_step(*args, 1.0, 0, ctypes.byref(s), ctypes.byref(v), None) == -1
