@@ -31,7 +31,7 @@ HIPCC_FLAGS = [
 ]
 # Accumulators in ordinary vector registers: with up to 256 of them in the other file the
 # compiler moves the matrix products' sums back and forth in every k-step.
-FILE_FLAGS = {"ftc_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("ftc_linear.hip", "ftc_delta_scan.hip")}
 
 
 def find_hipcc():

@@ -107,7 +107,7 @@ int read_inputs(const ftc_tensor4 *q, const ftc_tensor4 *k, const ftc_tensor4 *v
     p->N = (int32_t)s->N, p->H = (int32_t)s->H, p->Hk = (int32_t)s->Hk, p->L = (int32_t)s->L;
     p->E = (int32_t)s->E, p->M = (int32_t)s->M;
     p->chunks = (int32_t)s->chunks(), p->col_blocks = (int32_t)s->col_blocks();
-    p->vec_q = reads_wide(p->q), p->vec_k = reads_wide(p->k);
+    p->vec_q = reads_wide(p->q), p->vec_k = reads_wide(p->k), p->vec_v = reads_wide(p->v);
     return FTC_OK;
 }
 void place_forward(const Sizes &s, void *at, bool keep, DeltaArgs *p) {
@@ -230,6 +230,7 @@ int ftc_gated_delta_rule_backward(const ftc_tensor4 *queries, const ftc_tensor4 
     p.qc = (uint16_t *)(p.written + s.dots());
     p.go = as_operand(grad_out), p.vec_go = reads_wide(p.go);
     p.gq = rows_out(grad_queries), p.gk = rows_out(grad_keys), p.gv = rows_out(grad_values);
+    p.vec_gv = !grad_values || reads_wide(as_operand(grad_values));
     p.gg = scalars(grad_log_decay), p.gb = scalars(grad_beta);
     p.grad_final = state(grad_final_state), p.grad_initial = state(grad_initial_state);
     const bool bf16 = queries->dtype == FTC_BF16;

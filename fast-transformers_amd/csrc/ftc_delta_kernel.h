@@ -77,7 +77,7 @@ struct DeltaArgs {
     StateRef initial, final_;
     OperandOut out;
     int32_t N, H, Hk, L, E, M, chunks, col_blocks;  // col_blocks: of 16 columns
-    int32_t vec_q, vec_k, vec_go;  // rows can be read 16 bytes at a time
+    int32_t vec_q, vec_k, vec_v, vec_go, vec_gv;  // rows can be read 16 bytes at a time
     int32_t normalize;
     float scale;
     float *factors;          // [chain][chunk][kFactors][64]
@@ -139,6 +139,20 @@ __device__ __forceinline__ f32x4 product(const Frag (&a)[NA], const Frag (&b)[NB
             if (pb >= 0 && pb < NB) acc = mfma16(a[pa], b[pb], acc);
         }
     return acc;
+}
+// ... of several tiles by one right operand, a piece product of every tile after the other: each waits for its
+// tile's last one, which has had the others' time
+template <int FROM, int TILES, int NA, int NB>
+__device__ __forceinline__ void products(const Frag (&a)[TILES][NA], const Frag (&b)[NB], f32x4 (&acc)[TILES]) {
+#pragma unroll
+    for (int order = NA > 2 || NB > 2 ? 2 : 1; order >= 0; order--)
+#pragma unroll
+        for (int pa = 0; pa < NA; pa++) {
+            const int pb = order - pa;
+            if (pb >= 0 && pb < NB)
+#pragma unroll
+                for (int t = FROM; t < TILES; t++) acc[t] = mfma16(a[t][pa], b[pb], acc[t]);
+        }
 }
 // Lets the last products' results arrive before a branch.  The compiler counts the instructions between a matrix
 // product and the first use of its result, but where a branch skips a block it counts those of the block on the path

@@ -13,11 +13,17 @@ namespace {
 // Keeps the requests of a phase where they are written
 __device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
 
-// rows 16 t + 4 q .. of a factor
-__device__ __forceinline__ void load_factor(const float *f, int which, int q, f32x4 (&x)[4]) {
-#pragma unroll
-    for (int t = 0; t < 4; t++) x[t] = *(const f32x4a *)(f + which * kRows + 16 * t + 4 * q);
-}
+// One factor of a chunk's rows: a float a lane from memory, through LDS to the rows 16 t + 4 q .. of the tiles
+struct FactorRow {
+    float x;
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int which, int lane) {
+        x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (kRows * which + lane), 0, 0));
+    }
+    __device__ __forceinline__ void put(lds_float *to, int lane) const { to[lane] = x; }
+    __device__ static __forceinline__ f32x4 rows(const lds_float *from, int t, int q) {
+        return *(const __attribute__((address_space(3))) f32x4a *)(from + 16 * t + 4 * q);
+    }
+};
 __device__ __forceinline__ void load_tiles(const float *from, f32x4 (&x)[4]) {
 #pragma unroll
     for (int t = 0; t < 4; t++) x[t] = *(const f32x4a *)(from + 256 * t);
@@ -27,16 +33,14 @@ __device__ __forceinline__ void store_tiles(float *to, const f32x4 (&x)[4]) {
     for (int t = 0; t < 4; t++) *(f32x4a *)(to + 256 * t) = x[t];
 }
 
-// acc += A B with the left operand's fragment held, or read here
-template <bool HELD, int HA, int NB>
-__device__ __forceinline__ f32x4 times(const Frag (&held)[HA], const uint16_t *from, int number, int lane, const Frag (&b)[NB],
-                                       f32x4 acc) {
+// A left operand's fragment, held or read here
+template <bool HELD, int HA, int PIECES>
+__device__ __forceinline__ void get(const Frag (&held)[HA], const uint16_t *from, int number, int lane, Frag (&a)[PIECES]) {
     if constexpr (HELD) {
-        return product(held, b, acc);
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) a[k] = held[k];
     } else {
-        Frag a[3];
         load_frag(from, number, lane, a);
-        return product(a, b, acc);
     }
 }
 
@@ -47,38 +51,100 @@ __device__ __forceinline__ bool place(const DeltaArgs &p, int groups, int &chain
     return chain < p.N * p.H;
 }
 
-// Values of rows 16 t + 4 q + r of a column, as they come from memory: what is done to them here would wait for them
-template <typename T>
-struct Column {
-    uint32_t raw[4][4];
-    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row_bytes, int col, int width, int valid, int q) {
+// 64 rows of the wavefront's 16 columns, row by row from memory and through LDS to rows 16 t + 4 q + r of column c.
+// Only what comes from memory stays in registers: whatever was done to it where it is requested would wait for it.
+template <typename T, bool VEC>
+struct ColumnTile {
+    static constexpr int kBytes = Elem<T>::kBytes, kLoads = kRows * kCols * kBytes / 1024, kAcross = kCols * kBytes / 16;
+    static constexpr int kTile = kRows * kCols * kBytes;
+    u32x4 r[VEC ? kLoads : 4];
+
+    // VEC: lane's row 64 / kAcross i + lane / kAcross, 16 bytes of it; else its values one by one
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row_bytes, int col0, int width, int valid, int lane) {
+        if constexpr (VEC) {
+            const int col = col0 + lane % kAcross * (16 / kBytes);
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                const int row = 64 / kAcross * i + lane / kAcross;
+                r[i] = __builtin_amdgcn_raw_buffer_load_b128(
+                    rs, row < valid && col < width ? (uint32_t)row * row_bytes + (uint32_t)(col * kBytes) : kOutside, 0, 0);
+            }
+        } else {
+            const int col = col0 + (lane & 15);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int row = 16 * t + 4 * (lane >> 4) + x;
+                    const uint32_t at = row < valid && col < width ? (uint32_t)row * row_bytes + (uint32_t)(col * kBytes) : kOutside;
+                    r[t][x] = kBytes == 4 ? __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0)
+                                          : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, at, 0, 0);
+                }
+        }
+    }
+    __device__ __forceinline__ void put(lds_char *to, int lane) const {
+        if constexpr (VEC)
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) *(__attribute__((address_space(3))) u32x4a *)(to + 1024 * i + 16 * lane) = r[i];
+    }
+    __device__ __forceinline__ f32x4 values(const lds_char *from, int t, int c, int q) const {
+        f32x4 x;
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = __uint_as_float(kBytes == 4 ? r[t][i] : r[t][i] << 16);
+        } else if constexpr (kBytes == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = *(const lds_float *)(from + 64 * (16 * t + 4 * q + i) + 4 * c);
+        } else {
+            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (mfma::lds_s16x4 *)(from + 32 * (16 * t + 4 * q + (c >> 2)) + 8 * (c & 3))));
+            x[0] = __uint_as_float(w.x << 16), x[1] = __uint_as_float(w.x & 0xffff0000u);
+            x[2] = __uint_as_float(w.y << 16), x[3] = __uint_as_float(w.y & 0xffff0000u);
+        }
+        return x;
+    }
+    // the way back: values of the tiles to rows in memory (a buffer drops what lies outside)
+    __device__ static __forceinline__ void store(__amdgpu_buffer_rsrc_t rs, uint32_t row_bytes, int col0, int width, int valid,
+                                                 int lane, const f32x4 (&x)[4], lds_char *through) {
+        const int c = lane & 15, q = lane >> 4;
+        auto at = [&](int row, int col) {
+            return row < valid && col < width ? (uint32_t)row * row_bytes + (uint32_t)(col * kBytes) : kOutside;
+        };
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int row = 16 * t + 4 * q + r;
-                const uint32_t at = row < valid && col < width
-                                        ? (uint32_t)row * row_bytes + (uint32_t)(col * Elem<T>::kBytes) : kOutside;
-                raw[t][r] = Elem<T>::kBytes == 4 ? __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0)
-                                                 : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, at, 0, 0);
+            for (int i = 0; i < 4; i++) {
+                const int row = 16 * t + 4 * q + i;
+                const uint16_t half = __builtin_bit_cast(uint16_t, (__bf16)x[t][i]);
+                if constexpr (VEC && kBytes == 4) *(lds_float *)(through + 64 * row + 4 * c) = x[t][i];
+                else if constexpr (VEC) *(__attribute__((address_space(3))) uint16_t *)(through + 32 * row + 2 * c) = half;
+                else if constexpr (kBytes == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[t][i]), rs, at(row, col0 + c), 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b16(half, rs, at(row, col0 + c), 0, 0);
             }
-    }
-    __device__ __forceinline__ f32x4 values(int t) const {
-        f32x4 x;
+        if constexpr (VEC) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int r = 0; r < 4; r++) x[r] = __uint_as_float(Elem<T>::kBytes == 4 ? raw[t][r] : raw[t][r] << 16);
-        return x;
+            for (int i = 0; i < kLoads; i++)
+                __builtin_amdgcn_raw_buffer_store_b128(*(__attribute__((address_space(3))) u32x4a *)(through + 1024 * i + 16 * lane), rs,
+                    at(64 / kAcross * i + lane / kAcross, col0 + lane % kAcross * (16 / kBytes)), 0, 0);
+        }
     }
 };
+// A chunk's factors
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t factor_rows(const DeltaArgs &p, int64_t at) {
+    const uint64_t from = (uint64_t)(p.factors + at * (kFactors * kRows));
+    return __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(((uint64_t)(uint32_t)scalar((int)(from >> 32)) << 32) | (uint32_t)scalar((int)(uint32_t)from)), 0,
+        4 * kFactors * kRows, mfma::kRsrcFlags);
+}
 
-template <typename T, int KE, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_kernel(DeltaArgs p) {
+template <typename T, int KE, bool VEC>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_kernel(DeltaArgs p) {
     constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512;
-    const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6), c = lane & 15, q = lane >> 4;
-    int chain, group;
-    if (!place(p, (p.col_blocks + NW - 1) / NW, chain, group)) return;
-    const int block = group * NW + wave, col = kCols * block + c;
-    if (block >= p.col_blocks) return;
+    const int lane = threadIdx.x, c = lane & 15, q = lane >> 4;
+    int chain, block;
+    if (!place(p, p.col_blocks, chain, block)) return;
+    const int col = kCols * block + c;
     const Where w = where_of(p, chain, 0);
     const int chunks = chunks_of(w.len);
 
@@ -97,34 +163,41 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1)))
     // (three pieces of wide rows would not fit: read when they are used)
     constexpr bool kHold = KE * PIECES <= 6;
     Frag kr[4 * KE][kHold ? PIECES : 1], kc[4 * KE][kHold ? PIECES : 1], tf[kTFrags][3];
-    Column<T> V;
-    f32x4 in[4], out[4];
+    using Tile = ColumnTile<T, VEC>;
+    __shared__ __align__(16) char v_mem[Tile::kTile];
+    __shared__ __align__(16) float f_mem[2][kRows];
+    lds_char *const vp = (lds_char *)v_mem;
+    lds_float *const fp = (lds_float *)f_mem;
+    Tile V;
+    FactorRow in, out;
     float last;
     auto load_in = [&](int chunk) {
         if constexpr (kHold)
 #pragma unroll
             for (int i = 0; i < 4 * KE; i++) load_frag(p.kr + (w.key_at + chunk) * kKeys, i, lane, kr[i]);
     };
-    auto load_values = [&](int chunk) {
-        V.load(chunk_rows(p.v, w.n, w.h, (int64_t)chunk * kRows, Elem<T>::kBytes), v_row, col, p.M,
-               min(kRows, w.len - chunk * kRows), q);
-        load_factor(p.factors + (w.at + chunk) * (kFactors * kRows), kReadK, q, in);
+    auto load_rows = [&](int chunk) {
+        V.load(chunk_rows(p.v, w.n, w.h, (int64_t)chunk * kRows, Elem<T>::kBytes), v_row, kCols * block, p.M,
+               min(kRows, w.len - chunk * kRows), lane);
+        const __amdgpu_buffer_rsrc_t rs = factor_rows(p, w.at + chunk);
+        in.load(rs, kReadK, lane), out.load(rs, kWrite, lane);
+        last = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (kRows * kRise + kRows - 1), 0, 0));
     };
     auto load_t = [&](int chunk) {
 #pragma unroll
         for (int i = 0; i < kTFrags; i++) load_frag(p.t + (w.at + chunk) * (kTFrags * 3 * 512), i, lane, tf[i]);
-        load_factor(p.factors + (w.at + chunk) * (kFactors * kRows), kWrite, q, out);
-        last = p.factors[(w.at + chunk) * (kFactors * kRows) + kRise * kRows + kRows - 1];
     };
     auto load_out = [&](int chunk) {
         if constexpr (kHold)
 #pragma unroll
             for (int i = 0; i < 4 * KE; i++) load_frag(p.kc + (w.key_at + chunk) * kKeys, i, lane, kc[i]);
     };
-    if (chunks > 0) load_in(0), load_values(0), load_t(0), load_out(0);
+    if (chunks > 0) load_rows(0), load_in(0), load_t(0), load_out(0);
     for (int chunk = 0; chunk < chunks; chunk++) {
         const int64_t at = (w.at + chunk) * p.col_blocks + block;
         const int next = min(chunk + 1, chunks - 1);
+        V.put(vp, lane), in.put(fp, lane), out.put(fp + kRows, lane);
+        const float fade = last;
         {
             float *const to = p.s + at * (ET * 256) + 4 * lane;
 #pragma unroll
@@ -134,40 +207,45 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1)))
         f32x4 P[4] = {}, Z[4] = {};
 #pragma unroll
         for (int s = 0; s < KE; s++) {
-            Frag sf[3];
+            Frag sf[3], a[4][PIECES];
             cut(S[2 * s], S[2 * s + 1], sf);
 #pragma unroll
-            for (int t = 0; t < 4; t++) P[t] = times<kHold>(kr[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, sf, P[t]);
+            for (int t = 0; t < 4; t++) get<kHold>(kr[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, a[t]);
+            products<0>(a, sf, P);
         }
 #pragma unroll
-        for (int t = 0; t < 4; t++) P[t] = V.values(t) - in[t] * P[t];
+        for (int t = 0; t < 4; t++) P[t] = V.values(vp, t, c, q) - FactorRow::rows(fp, t, q) * P[t];
         phase();
-        load_in(next), load_values(next);
+        load_rows(next), load_in(next);
         phase();
         // Z = T E (tiles above the diagonal are zero)
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            Frag ef[3];
+            Frag ef[3], a[4][3];
             cut(P[2 * s], P[2 * s + 1], ef);
 #pragma unroll
-            for (int t = 2 * s; t < 4; t++) Z[t] = product(tf[t_number(t, s)], ef, Z[t]);
+            for (int t = 2 * s; t < 4; t++)
+#pragma unroll
+                for (int k = 0; k < 3; k++) a[t][k] = tf[t_number(t, s)][k];
+            if (s == 0) products<0>(a, ef, Z);
+            else products<2>(a, ef, Z);
         }
         store_tiles(p.z + at * (4 * 256) + 4 * lane, Z);
         // S <- e^{G_64} S + K^T diag(rk beta e^{G_64 - G}) Z
 #pragma unroll
-        for (int t = 0; t < 4; t++) Z[t] *= out[t];
+        for (int t = 0; t < 4; t++) Z[t] *= FactorRow::rows(fp + kRows, t, q);
 #pragma unroll
-        for (int t = 0; t < ET; t++) S[t] *= last;
+        for (int t = 0; t < ET; t++) S[t] *= fade;
         phase();
         load_t(next);
         phase();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            Frag uf[3];
+            Frag uf[3], a[ET][PIECES];
             cut(Z[2 * s], Z[2 * s + 1], uf);
 #pragma unroll
-            for (int t = 0; t < ET; t++)
-                S[t] = times<kHold>(kc[2 * t + s], p.kc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, uf, S[t]);
+            for (int t = 0; t < ET; t++) get<kHold>(kc[2 * t + s], p.kc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, a[t]);
+            products<0>(a, uf, S);
         }
         phase();
         load_out(next);
@@ -188,14 +266,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1)))
 //   dU = A^T dO + diag(rk e^{G_64 - G}) K dS,   dE = T^T diag(beta) dU,
 //   dS <- e^{G_64} dS + Q^T diag(rq e^G) dO - K^T diag(rk e^G) dE
 // and what the chunk's keys write of <state, its gradient>: the sum of beta Z . diag(rk e^{G_64 - G}) K dS.
-template <typename T, int KE, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_back_kernel(DeltaArgs p) {
+template <typename T, int KE, bool VEC>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_back_kernel(DeltaArgs p) {
     constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512;
-    const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6), c = lane & 15, q = lane >> 4;
-    int chain, group;
-    if (!place(p, (p.col_blocks + NW - 1) / NW, chain, group)) return;
-    const int block = group * NW + wave, col = kCols * block + c;
-    if (block >= p.col_blocks) return;
+    const int lane = threadIdx.x, c = lane & 15, q = lane >> 4;
+    int chain, block;
+    if (!place(p, p.col_blocks, chain, block)) return;
+    const int col = kCols * block + c;
     const Where w = where_of(p, chain, 0);
     const int chunks = chunks_of(w.len);
 
@@ -212,43 +289,54 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1)))
         }
 
     const uint32_t g_row = (uint32_t)p.go.stride_l * Elem<T>::kBytes, gv_row = (uint32_t)p.gv.stride_l * Elem<T>::kBytes;
-    constexpr bool kHold = KE * PIECES <= 4;
-    Frag kr[4 * KE][kHold ? PIECES : 1], kc[4 * KE][kHold ? PIECES : 1], qc[4 * KE][kHold ? PIECES : 1], tf[kTFrags][3];
-    Column<T> Gr;
-    f32x4 Y[4], Z[4], write[4], beta[4], read_q[4], read_k[4];
+    constexpr bool kHold = KE * PIECES <= 6;
+    // (x: the rows of k, then, while T is used, the columns of q)
+    Frag x[4 * KE][kHold ? PIECES : 1], kc[4 * KE][kHold ? PIECES : 1], tf[kTFrags][3];
+    using Tile = ColumnTile<T, VEC>;
+    __shared__ __align__(16) char g_mem[Tile::kTile], through_mem[Tile::kTile];
+    __shared__ __align__(16) float f_mem[4][kRows];
+    lds_char *const gp = (lds_char *)g_mem, *const through = (lds_char *)through_mem;
+    lds_float *const fp = (lds_float *)f_mem;
+    Tile Gr;
+    FactorRow write, beta, read_q, read_k;
+    f32x4 Y[4], Z[4];
     float last;
-    auto factors = [&](int chunk) { return p.factors + (w.at + chunk) * (kFactors * kRows); };
     auto tiles = [&](int chunk) { return ((w.at + chunk) * p.col_blocks + block) * (4 * 256) + 4 * lane; };
     auto load_in = [&](int chunk) {
         if constexpr (kHold)
 #pragma unroll
-            for (int i = 0; i < 4 * KE; i++) load_frag(p.kr + (w.key_at + chunk) * kKeys, i, lane, kr[i]);
-        load_factor(factors(chunk), kWrite, q, write);
-        load_factor(factors(chunk), kBeta, q, beta);
+            for (int i = 0; i < 4 * KE; i++) load_frag(p.kr + (w.key_at + chunk) * kKeys, i, lane, x[i]);
+    };
+    auto load_rows = [&](int chunk) {
+        const __amdgpu_buffer_rsrc_t rs = factor_rows(p, w.at + chunk);
+        write.load(rs, kWrite, lane), beta.load(rs, kBeta, lane), read_q.load(rs, kReadQ, lane), read_k.load(rs, kReadK, lane);
+        last = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (kRows * kRise + kRows - 1), 0, 0));
         load_tiles(p.de + tiles(chunk), Y);
         load_tiles(p.z + tiles(chunk), Z);
     };
     auto load_t = [&](int chunk) {
 #pragma unroll
         for (int i = 0; i < kTFrags; i++) load_frag(p.tt + (w.at + chunk) * (kTFrags * 3 * 512), i, lane, tf[i]);
-        load_factor(factors(chunk), kReadQ, q, read_q);
-        load_factor(factors(chunk), kReadK, q, read_k);
-        last = factors(chunk)[kRise * kRows + kRows - 1];
-        Gr.load(chunk_rows(p.go, w.n, w.h, (int64_t)chunk * kRows, Elem<T>::kBytes), g_row, col, p.M,
-                min(kRows, w.len - chunk * kRows), q);
+        Gr.load(chunk_rows(p.go, w.n, w.h, (int64_t)chunk * kRows, Elem<T>::kBytes), g_row, kCols * block, p.M,
+                min(kRows, w.len - chunk * kRows), lane);
+    };
+    auto load_q = [&](int chunk) {
+        if constexpr (kHold)
+#pragma unroll
+            for (int i = 0; i < 4 * KE; i++) load_frag(p.qc + (w.key_at + chunk) * kKeys, i, lane, x[i]);
     };
     auto load_out = [&](int chunk) {
-        if constexpr (kHold) {
-#pragma unroll
-            for (int i = 0; i < 4 * KE; i++) load_frag(p.qc + (w.key_at + chunk) * kKeys, i, lane, qc[i]);
+        if constexpr (kHold)
 #pragma unroll
             for (int i = 0; i < 4 * KE; i++) load_frag(p.kc + (w.key_at + chunk) * kKeys, i, lane, kc[i]);
-        }
     };
-    if (chunks > 0) load_in(chunks - 1), load_t(chunks - 1), load_out(chunks - 1);
+    if (chunks > 0) load_in(chunks - 1), load_rows(chunks - 1), load_t(chunks - 1), load_out(chunks - 1);
     for (int chunk = chunks - 1; chunk >= 0; chunk--) {
         const int64_t at = (w.at + chunk) * p.col_blocks + block;
         const int next = max(chunk - 1, 0);
+        Gr.put(gp, lane), write.put(fp, lane), beta.put(fp + kRows, lane);
+        read_q.put(fp + 2 * kRows, lane), read_k.put(fp + 3 * kRows, lane);
+        const float fade = last;
         {
             float *const to = p.ds + at * (ET * 256) + 4 * lane;
 #pragma unroll
@@ -257,70 +345,72 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1)))
         f32x4 P[4] = {}, D[4], G[4];
 #pragma unroll
         for (int s = 0; s < KE; s++) {
-            Frag sf[3];
+            Frag sf[3], a[4][PIECES];
             cut(S[2 * s], S[2 * s + 1], sf);
 #pragma unroll
-            for (int t = 0; t < 4; t++)
-                P[t] = times<kHold>(kr[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, sf, P[t]);
+            for (int t = 0; t < 4; t++) get<kHold>(x[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, a[t]);
+            products<0>(a, sf, P);
         }
         // diag(beta) dU
         f32x4 written = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            P[t] *= write[t];
-            D[t] = beta[t] * Y[t] + P[t];
+            P[t] *= FactorRow::rows(fp, t, q);
+            D[t] = FactorRow::rows(fp + kRows, t, q) * Y[t] + P[t];
             written += Z[t] * P[t];
             P[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         p.written[at * 64 + lane] = (written[0] + written[1]) + (written[2] + written[3]);
         phase();
-        load_in(next);
+        load_q(chunk), load_rows(next);
         phase();
         // dE = T^T diag(beta) dU
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            Frag df[3];
+            Frag df[3], a[4][3];
+            f32x4(&head)[2] = *(f32x4(*)[2])&P[0];
             cut(D[2 * s], D[2 * s + 1], df);
 #pragma unroll
-            for (int t = 0; t < 2 * s + 2; t++) P[t] = product(tf[tt_number(t, s)], df, P[t]);
+            for (int t = 0; t < 2 * s + 2; t++)
+#pragma unroll
+                for (int k = 0; k < 3; k++) a[t][k] = tf[tt_number(t, s)][k];
+            if (s == 0) products<0>(*(Frag(*)[2][3])&a, df, head);
+            else products<0>(a, df, P);
         }
         store_tiles(p.de + at * (4 * 256) + 4 * lane, P);
-        if (p.gv.ptr) {  // (a buffer drops what lies outside)
-            const int64_t l0 = (int64_t)chunk * kRows;
-            const __amdgpu_buffer_rsrc_t rs = chunk_rows(Operand{p.gv.ptr, p.gv.stride_n, p.gv.stride_h, p.gv.stride_l, 0, 0},
-                                                         w.n, w.h, l0, Elem<T>::kBytes);
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int row = 16 * t + 4 * q + r;
-                    const uint32_t to = l0 + row < w.len && col < p.M
-                                            ? (uint32_t)row * gv_row + (uint32_t)(col * Elem<T>::kBytes) : kOutside;
-                    if (Elem<T>::kBytes == 4)
-                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(P[t][r]), rs, to, 0, 0);
-                    else
-                        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (__bf16)P[t][r]), rs, to, 0, 0);
-                }
-        }
+        if (p.gv.ptr)
+            Tile::store(chunk_rows(Operand{p.gv.ptr, p.gv.stride_n, p.gv.stride_h, p.gv.stride_l, 0, 0}, w.n, w.h,
+                                   (int64_t)chunk * kRows, Elem<T>::kBytes),
+                        gv_row, kCols * block, p.M, min(kRows, w.len - chunk * kRows), lane, P, through);
         settle();
 #pragma unroll
-        for (int t = 0; t < 4; t++) G[t] = Gr.values(t) * read_q[t], P[t] *= -read_k[t];
+        for (int t = 0; t < 4; t++) {
+            G[t] = Gr.values(gp, t, c, q) * FactorRow::rows(fp + 2 * kRows, t, q);
+            P[t] *= -FactorRow::rows(fp + 3 * kRows, t, q);
+        }
 #pragma unroll
-        for (int t = 0; t < ET; t++) S[t] *= last;
+        for (int t = 0; t < ET; t++) S[t] *= fade;
         phase();
         load_t(next);
         phase();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            Frag of[3], ef[3];
+            Frag of[3], a[ET][PIECES];
             cut(G[2 * s], G[2 * s + 1], of);
 #pragma unroll
-            for (int t = 0; t < ET; t++)
-                S[t] = times<kHold>(qc[2 * t + s], p.qc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, of, S[t]);
+            for (int t = 0; t < ET; t++) get<kHold>(x[2 * t + s], p.qc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, a[t]);
+            products<0>(a, of, S);
+        }
+        phase();
+        load_in(next);
+        phase();
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            Frag ef[3], a[ET][PIECES];
             cut(P[2 * s], P[2 * s + 1], ef);
 #pragma unroll
-            for (int t = 0; t < ET; t++)
-                S[t] = times<kHold>(kc[2 * t + s], p.kc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, ef, S[t]);
+            for (int t = 0; t < ET; t++) get<kHold>(kc[2 * t + s], p.kc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, a[t]);
+            products<0>(a, ef, S);
         }
         phase();
         load_out(next);
@@ -342,24 +432,26 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1, 1)))
             store_from_f32(p.gv.ptr, p.gv.dtype, w.n * p.gv.stride_n + w.h * p.gv.stride_h + l * p.gv.stride_l + col, 0.f);
 }
 
-template <typename T, int KE>
+template <typename T, int KE, bool VEC>
 void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
-    constexpr int NW = 1;
-    const uint32_t groups = (uint32_t)((p.col_blocks + NW - 1) / NW);
-    const dim3 grid(((uint32_t)p.N * (uint32_t)p.H + 7) / 8 * 8 * groups);
-    if (back) delta_scan_back_kernel<T, KE, NW><<<grid, 64 * NW, 0, stream>>>(p);
-    else delta_scan_kernel<T, KE, NW><<<grid, 64 * NW, 0, stream>>>(p);
+    const dim3 grid(((uint32_t)p.N * (uint32_t)p.H + 7) / 8 * 8 * (uint32_t)p.col_blocks);
+    if (back) delta_scan_back_kernel<T, KE, VEC><<<grid, 64, 0, stream>>>(p);
+    else delta_scan_kernel<T, KE, VEC><<<grid, 64, 0, stream>>>(p);
 }
-int dispatch(const DeltaArgs &p, bool bf16, bool back, hipStream_t stream) {
-    if (p.E <= 64) bf16 ? launch<bf16_t, 2>(p, back, stream) : launch<float, 2>(p, back, stream);
-    else bf16 ? launch<bf16_t, 4>(p, back, stream) : launch<float, 4>(p, back, stream);
+template <typename T, int KE>
+void launch(const DeltaArgs &p, bool vec, bool back, hipStream_t stream) {
+    vec ? launch<T, KE, true>(p, back, stream) : launch<T, KE, false>(p, back, stream);
+}
+int dispatch(const DeltaArgs &p, bool bf16, bool vec, bool back, hipStream_t stream) {
+    if (p.E <= 64) bf16 ? launch<bf16_t, 2>(p, vec, back, stream) : launch<float, 2>(p, vec, back, stream);
+    else bf16 ? launch<bf16_t, 4>(p, vec, back, stream) : launch<float, 4>(p, vec, back, stream);
     return FTC_OK;
 }
 
 }  // namespace
 
-int delta_scan(const DeltaArgs &p, bool bf16, hipStream_t stream) { return dispatch(p, bf16, false, stream); }
-int delta_scan_back(const DeltaArgs &p, bool bf16, hipStream_t stream) { return dispatch(p, bf16, true, stream); }
+int delta_scan(const DeltaArgs &p, bool bf16, hipStream_t stream) { return dispatch(p, bf16, p.vec_v, false, stream); }
+int delta_scan_back(const DeltaArgs &p, bool bf16, hipStream_t stream) { return dispatch(p, bf16, p.vec_go && p.vec_gv, true, stream); }
 
 }  // namespace delta
 }  // namespace ftc
