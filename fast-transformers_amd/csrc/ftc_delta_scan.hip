@@ -204,7 +204,13 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
             for (int t = 0; t < ET; t++) *(f32x4a *)(to + 256 * t) = S[t];
         }
         // E = V - diag(rk e^G) K S
-        f32x4 P[4] = {}, Z[4] = {};
+        f32x4 P[4] = {}, Z[4] = {}, read[4], write[4], values[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            values[t] = V.values(vp, t, c, q);
+            read[t] = FactorRow::rows(fp, t, q), write[t] = FactorRow::rows(fp + kRows, t, q);
+        }
+        phase();
 #pragma unroll
         for (int s = 0; s < KE; s++) {
             Frag sf[3], a[4][PIECES];
@@ -214,7 +220,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
             products<0>(a, sf, P);
         }
 #pragma unroll
-        for (int t = 0; t < 4; t++) P[t] = V.values(vp, t, c, q) - FactorRow::rows(fp, t, q) * P[t];
+        for (int t = 0; t < 4; t++) P[t] = values[t] - read[t] * P[t];
         phase();
         load_rows(next), load_in(next);
         phase();
@@ -233,7 +239,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         store_tiles(p.z + at * (4 * 256) + 4 * lane, Z);
         // S <- e^{G_64} S + K^T diag(rk beta e^{G_64 - G}) Z
 #pragma unroll
-        for (int t = 0; t < 4; t++) Z[t] *= FactorRow::rows(fp + kRows, t, q);
+        for (int t = 0; t < 4; t++) Z[t] *= write[t];
 #pragma unroll
         for (int t = 0; t < ET; t++) S[t] *= fade;
         phase();
@@ -290,8 +296,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 
     const uint32_t g_row = (uint32_t)p.go.stride_l * Elem<T>::kBytes, gv_row = (uint32_t)p.gv.stride_l * Elem<T>::kBytes;
     constexpr bool kHold = KE * PIECES <= 6;
-    // (x: the rows of k, then, while T is used, the columns of q)
-    Frag x[4 * KE][kHold ? PIECES : 1], kc[4 * KE][kHold ? PIECES : 1], tf[kTFrags][3];
+    // (three pieces: the columns of q where the rows of k were, requested while T is used)
+    constexpr bool kShare = KE * PIECES > 4;
+    Frag kr[4 * KE][kHold ? PIECES : 1], own_q[kShare ? 1 : 4 * KE][kHold ? PIECES : 1], kc[4 * KE][kHold ? PIECES : 1], tf[kTFrags][3];
     using Tile = ColumnTile<T, VEC>;
     __shared__ __align__(16) char g_mem[Tile::kTile], through_mem[Tile::kTile];
     __shared__ __align__(16) float f_mem[4][kRows];
@@ -305,7 +312,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     auto load_in = [&](int chunk) {
         if constexpr (kHold)
 #pragma unroll
-            for (int i = 0; i < 4 * KE; i++) load_frag(p.kr + (w.key_at + chunk) * kKeys, i, lane, x[i]);
+            for (int i = 0; i < 4 * KE; i++) load_frag(p.kr + (w.key_at + chunk) * kKeys, i, lane, kr[i]);
     };
     auto load_rows = [&](int chunk) {
         const __amdgpu_buffer_rsrc_t rs = factor_rows(p, w.at + chunk);
@@ -323,18 +330,22 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     auto load_q = [&](int chunk) {
         if constexpr (kHold)
 #pragma unroll
-            for (int i = 0; i < 4 * KE; i++) load_frag(p.qc + (w.key_at + chunk) * kKeys, i, lane, x[i]);
+            for (int i = 0; i < 4 * KE; i++) {
+                if constexpr (kShare) load_frag(p.qc + (w.key_at + chunk) * kKeys, i, lane, kr[i]);
+                else load_frag(p.qc + (w.key_at + chunk) * kKeys, i, lane, own_q[i]);
+            }
     };
     auto load_out = [&](int chunk) {
         if constexpr (kHold)
 #pragma unroll
             for (int i = 0; i < 4 * KE; i++) load_frag(p.kc + (w.key_at + chunk) * kKeys, i, lane, kc[i]);
     };
+    if (!kShare && chunks > 0) load_q(chunks - 1);
     if (chunks > 0) load_in(chunks - 1), load_rows(chunks - 1), load_t(chunks - 1), load_out(chunks - 1);
     for (int chunk = chunks - 1; chunk >= 0; chunk--) {
         const int64_t at = (w.at + chunk) * p.col_blocks + block;
         const int next = max(chunk - 1, 0);
-        Gr.put(gp, lane), write.put(fp, lane), beta.put(fp + kRows, lane);
+        write.put(fp, lane), beta.put(fp + kRows, lane);
         read_q.put(fp + 2 * kRows, lane), read_k.put(fp + 3 * kRows, lane);
         const float fade = last;
         {
@@ -342,29 +353,41 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 #pragma unroll
             for (int t = 0; t < ET; t++) *(f32x4a *)(to + 256 * t) = S[t];
         }
-        f32x4 P[4] = {}, D[4], G[4];
+        f32x4 P[4] = {}, D[4], G[4], write_rows[4], beta_rows[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) write_rows[t] = FactorRow::rows(fp, t, q), beta_rows[t] = FactorRow::rows(fp + kRows, t, q);
+        phase();
 #pragma unroll
         for (int s = 0; s < KE; s++) {
             Frag sf[3], a[4][PIECES];
             cut(S[2 * s], S[2 * s + 1], sf);
 #pragma unroll
-            for (int t = 0; t < 4; t++) get<kHold>(x[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, a[t]);
+            for (int t = 0; t < 4; t++) get<kHold>(kr[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, a[t]);
             products<0>(a, sf, P);
         }
         // diag(beta) dU
         f32x4 written = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            P[t] *= FactorRow::rows(fp, t, q);
-            D[t] = FactorRow::rows(fp + kRows, t, q) * Y[t] + P[t];
+            P[t] *= write_rows[t];
+            D[t] = beta_rows[t] * Y[t] + P[t];
             written += Z[t] * P[t];
             P[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         p.written[at * 64 + lane] = (written[0] + written[1]) + (written[2] + written[3]);
         phase();
-        load_q(chunk), load_rows(next);
+        if constexpr (kShare) load_q(chunk), load_rows(next);
+        else load_in(next), load_rows(next);
         phase();
         // dE = T^T diag(beta) dU
+        Gr.put(gp, lane);
+        f32x4 read_q_rows[4], read_k_rows[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            G[t] = Gr.values(gp, t, c, q);
+            read_q_rows[t] = FactorRow::rows(fp + 2 * kRows, t, q), read_k_rows[t] = FactorRow::rows(fp + 3 * kRows, t, q);
+        }
+        phase();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag df[3], a[4][3];
@@ -385,8 +408,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         settle();
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            G[t] = Gr.values(gp, t, c, q) * FactorRow::rows(fp + 2 * kRows, t, q);
-            P[t] *= -FactorRow::rows(fp + 3 * kRows, t, q);
+            G[t] *= read_q_rows[t];
+            P[t] *= -read_k_rows[t];
         }
 #pragma unroll
         for (int t = 0; t < ET; t++) S[t] *= fade;
@@ -398,11 +421,13 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
             Frag of[3], a[ET][PIECES];
             cut(G[2 * s], G[2 * s + 1], of);
 #pragma unroll
-            for (int t = 0; t < ET; t++) get<kHold>(x[2 * t + s], p.qc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, a[t]);
+            for (int t = 0; t < ET; t++)
+                get<kHold>(kShare ? kr[2 * t + s] : own_q[kShare ? 0 : 2 * t + s], p.qc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, a[t]);
             products<0>(a, of, S);
         }
         phase();
-        load_in(next);
+        if constexpr (kShare) load_in(next);
+        else load_q(next);
         phase();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
