@@ -28,6 +28,14 @@ namespace {
 
 constexpr int kThreads = 512;
 
+// The lane's column and row group anew: what is made of them belongs to the phase behind (all phases' addresses, held
+// through the loop over heads, would not leave registers for the products)
+__device__ __forceinline__ void renew(int &c, int &q) { asm volatile("" : "+v"(c), "+v"(q)); }
+__device__ __forceinline__ int renewed(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 template <typename T, int KE>
 __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) {
     constexpr int PIECES = Elem<T>::kPieces, NP = PIECES == 1 ? 2 : 3;
@@ -51,7 +59,8 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
     lds_char *const pp = lds + kQK, *const rp = pp + NP * kSquare;
     lds_float *const fp = (lds_float *)f_mem;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6), c = lane & 15, q = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
+    int c = lane & 15, q = lane >> 4;
     const int e0 = EW * (wave & 3), t0 = RT * (wave >> 2);  // the wavefront's tiles of key columns and of positions
     const int G = scalar(p.H / p.Hk);
     const int nk = scalar((int)(blockIdx.x / (uint32_t)p.chunks)), chunk = (int)blockIdx.x - nk * p.chunks;
@@ -79,14 +88,15 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
     uint32_t vr[4];
     auto request = [&](int h, int m0) {
         const int64_t at = ((int64_t)(n * p.H + h) * p.chunks + chunk) * p.col_blocks;
-        if (tid < 256) {
+        const int half = scalar(tid >> 8), unit = renewed(tid & 255), block = m0 + half;
+        if (half == 0) {
             Operand shifted = p.go;
             shifted.ptr = (const char *)p.go.ptr + (int64_t)m0 * kCols * Elem<T>::kBytes;
             go.load(chunk_rows(shifted, n, h, l0, Elem<T>::kBytes), (uint32_t)p.go.stride_l * Elem<T>::kBytes,
-                    p.M - m0 * kCols, valid, p.vec_go, tid);
+                    p.M - m0 * kCols, valid, p.vec_go, unit);
         }
-        const int block = m0 + (tid >> 8), unit = tid & 255, row = 4 * (unit >> 4 & 15), col = block * kCols + c;
         {
+            const int row = 4 * (unit >> 4), col = block * kCols + (unit & 15);
             const __amdgpu_buffer_rsrc_t rs = chunk_rows(p.v, n, h, l0, Elem<T>::kBytes);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
@@ -96,35 +106,35 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
                                              : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, from, 0, 0);
             }
         }
-        zr = er = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (block < p.col_blocks) {
-            zr = *(const f32x4a *)(p.z + (at + block) * (4 * 256) + 4 * unit);
-            er = *(const f32x4a *)(p.de + (at + block) * (4 * 256) + 4 * unit);
-        }
+        // (a block past the last one: zeros, from a buffer of no bytes)
+        const bool there = block < p.col_blocks;
+        auto fragments = [&](const float *from, int tiles, int number) {
+            const uint64_t base = (uint64_t)(from + (at + block) * (tiles * 256));
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)(((uint64_t)(uint32_t)scalar((int)(base >> 32)) << 32) | (uint32_t)scalar((int)(uint32_t)base)), 0,
+                there ? tiles * 1024 : 0, mfma::kRsrcFlags);
+            return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * unit + 4096 * number, 0, 0));
+        };
+        zr = fragments(p.z, 4, 0), er = fragments(p.de, 4, 0);
 #pragma unroll
-        for (int u = 0; u < ET / 4; u++) {
-            sr[u] = dr[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (block < p.col_blocks) {
-                sr[u] = *(const f32x4a *)(p.s + (at + block) * (ET * 256) + 4 * (unit + 256 * u));
-                dr[u] = *(const f32x4a *)(p.ds + (at + block) * (ET * 256) + 4 * (unit + 256 * u));
-            }
-        }
+        for (int u = 0; u < ET / 4; u++) sr[u] = fragments(p.s, ET, u), dr[u] = fragments(p.ds, ET, u);
     };
     // a fragment's place in planes with a row per column: four positions (or key columns) of column c
     auto put = [&](f32x4 &dot_z, f32x4 &dot_v) {
-        if (tid < 256) go.template store<64>(gop, tid);
-        const int row = 16 * (tid >> 8) + c, t = (tid & 255) >> 6;
+        const int half = scalar(tid >> 8), unit = renewed(tid & 255);
+        if (half == 0) go.template store<64>(gop, unit);
+        const int row = 16 * half + (unit & 15), slot = unit >> 4;
         float dot = 0.f;
-        store_pieces<NP>(zp + Plane<128>::addr(row, 4 * t + q), kSq, zr);
-        store_pieces<NP>(dep + Plane<128>::addr(row, 4 * t + q), kSq, er);
+        store_pieces<NP>(zp + Plane<128>::addr(row, slot), kSq, zr);
+        store_pieces<NP>(dep + Plane<128>::addr(row, slot), kSq, er);
         dot_z += er * zr;
 #pragma unroll
         for (int r = 0; r < 4; r++)
             dot_v[r] = fmaf(er[r], __uint_as_float(Elem<T>::kBytes == 4 ? vr[r] : vr[r] << 16), dot_v[r]);
 #pragma unroll
         for (int u = 0; u < ET / 4; u++) {
-            store_pieces<NP>(sp + Plane<RB>::addr(row, 4 * (t + 4 * u) + q), kSt, sr[u]);
-            store_pieces<NP>(dsp + Plane<RB>::addr(row, 4 * (t + 4 * u) + q), kSt, dr[u]);
+            store_pieces<NP>(sp + Plane<RB>::addr(row, slot + 16 * u), kSt, sr[u]);
+            store_pieces<NP>(dsp + Plane<RB>::addr(row, slot + 16 * u), kSt, dr[u]);
             dot += (sr[u][0] * dr[u][0] + sr[u][1] * dr[u][1]) + (sr[u][2] * dr[u][2] + sr[u][3] * dr[u][3]);
         }
         return dot;
@@ -162,8 +172,9 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
             __syncthreads();  // (what was staged before has been read)
             state_dot += put(dot_z, dot_v);
             __syncthreads();
-            if (m0 + 2 < p.col_blocks) request(h, m0 + 2);
-            else if (g + 1 < G) request(h + 1, 0);
+            const bool more = m0 + 2 < p.col_blocks;
+            if (more || g + 1 < G) request(more ? h : h + 1, more ? m0 + 2 : 0);
+            renew(c, q);
 #pragma unroll
             for (int x = 0; x < 2; x++) {
                 int ti, tj;
@@ -219,6 +230,7 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
 
         // ---- phase 2 ----
         __syncthreads();
+        renew(c, q);
         if (!kResident) stage_rows();
 #pragma unroll
         for (int x = 0; x < 2; x++) {
@@ -306,6 +318,7 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
         __syncthreads();
     }
 
+    renew(c, q);
     if (valid > 0 && p.normalize) {  // (the factors of the last head: those of q and k are alike)
         auto row_value = [&](const lds_char *planes, int row, int col) {
             float v = 0.f;
