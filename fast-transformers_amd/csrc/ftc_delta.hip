@@ -28,7 +28,7 @@ struct Sizes {
     int64_t dots() const { return units() * col_blocks() * kRows; }
     // T, keys, factors, states, Z; to be kept for the backward also the transpose of T and O
     int64_t forward(bool keep) const { return 4 * (factors() + (keep ? 2 : 1) * (t() + z()) + 2 * keys() + s()); }
-    int64_t backward() const { return 4 * (s() + z() + 2 * dots() + keys()); }
+    int64_t backward() const { return 4 * (s() + z() + 2 * dots() + units() * kSums + keys()); }
 };
 
 int check_sizes(const Sizes &s) {
@@ -227,7 +227,8 @@ int ftc_gated_delta_rule_backward(const ftc_tensor4 *queries, const ftc_tensor4 
     p.lengths = lengths, p.scale = scale, p.normalize = normalize != 0;
     place_forward(s, (void *)kept, true, &p);
     p.ds = (float *)workspace, p.de = p.ds + s.s(), p.dots = p.de + s.z(), p.written = p.dots + s.dots();
-    p.qc = (uint16_t *)(p.written + s.dots());
+    p.sums = p.written + s.dots();
+    p.qc = (uint16_t *)(p.sums + s.units() * kSums);
     p.go = as_operand(grad_out), p.vec_go = reads_wide(p.go);
     p.gq = rows_out(grad_queries), p.gk = rows_out(grad_keys), p.gv = rows_out(grad_values);
     p.vec_gv = !grad_values || reads_wide(as_operand(grad_values));

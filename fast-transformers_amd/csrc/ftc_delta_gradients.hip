@@ -14,19 +14,20 @@
 //   dG_i = dO_i . O_i - dE_i . V_i,   dg_l = sum of dG_i over i >= l in the chunk + <state after it, its gradient>
 // (the last is e^{G_64} <S, dS> + what the chunk's keys write, taken anew in every chunk: nothing adds up over chunks).
 //
-// A workgroup of eight wavefronts takes a chunk of one key head and its value heads one after the other, so that the
-// gradients of shared keys are summed in registers, in one order.  Phase 1 walks the columns of the state, 32 at a
-// time through LDS, the next 32 on their way meanwhile; a wavefront has 32 positions of a quarter of the key
-// columns, and some of the tiles of dO Z^T and dE Z^T.  Phase 2 multiplies the 64 x 64 matrices with the rows.
-// Gradients of bf16 rows are made of values in two pieces (2^-17 of them is left out, against half a step of 2^-8 that the
-// rounding of the results takes).
+// A workgroup of four wavefronts takes a chunk of one key head and 64 of its columns, two to a compute unit, and the
+// head's value heads one after the other, so that the gradients of shared keys are summed in registers, in one
+// order.  Phase 1 walks the columns of the state, 32 at a time through LDS, the next 32 on their way meanwhile; a
+// wavefront has 32 positions of 32 key columns, and a quarter of the tiles of dO Z^T and dE Z^T.  Phase 2 multiplies the
+// 64 x 64 matrices with the rows.  Gradients of bf16 rows are made of values in two pieces (2^-17 of them is left out,
+// against half a step of 2^-8 that the rounding of the results takes).
 #include "ftc_delta_kernel.h"
 
 namespace ftc {
 namespace delta {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kSlice = 64;  // key columns of a workgroup
 
 // The lane's column and row group anew: what is made of them belongs to the phase behind (all phases' addresses, held
 // through the loop over heads, would not leave registers for the products)
@@ -36,114 +37,118 @@ __device__ __forceinline__ int renewed(int x) {
     return x;
 }
 
-template <typename T, int KE>
-__global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) {
+template <typename T>
+__global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs p) {
     constexpr int PIECES = Elem<T>::kPieces, NP = PIECES == 1 ? 2 : 3;
-    constexpr int RB = 64 * KE, ET = 2 * KE, EW = ET / 4, RT = 2;
-    constexpr int kMB = 32;                                           // columns of the state at a time
-    constexpr int kGo = kRows * 64, kSq = kMB * 128, kSt = kMB * RB;  // bytes of a plane of dO, of Z or dE, of a state
-    constexpr int kRowsPlane = Plane<RB>::kBytes, kSquare = Plane<128>::kBytes;
-    constexpr int kQK = 2 * PIECES * kRowsPlane, kPhase1 = PIECES * kGo + 2 * NP * kSq + 2 * NP * kSt;
+    constexpr int RB = 2 * kSlice, EW = 2, RT = 2;
+    constexpr int kMB = 32;                                // columns of the state at a time
+    constexpr int kGo = kRows * 2 * kMB, kSq = kMB * 128;  // bytes of a plane of dO, of the others
+    constexpr int kSquare = Plane<128>::kBytes;
+    constexpr int kQK = 2 * PIECES * kSquare, kPhase1 = PIECES * kGo + 4 * NP * kSq, kPR = 2 * NP * kSquare;
     constexpr bool kResident = PIECES == 1;  // rows of q and k stay in LDS; else they come after phase 1
-    constexpr int kPR = 2 * NP * kSquare;
     constexpr int kBytes = kResident ? kQK + (kPhase1 > kPR ? kPhase1 : kPR) : (kPhase1 > kQK + kPR ? kPhase1 : kQK + kPR);
     __shared__ __align__(16) char mem[kBytes];
     __shared__ __align__(16) float f_mem[kFactors * kRows];
-    __shared__ float dot_mem[2][2][kRows];  // per half of the columns staged together: dE . Z, dE . V
-    __shared__ float total_mem[2][kRows];  // q . dq and k . dk of all value heads
-    __shared__ float state_mem[8];         // per wavefront: its share of <S, dS>
+    __shared__ float dot_mem[2][kRows];    // of a value head: dE . Z, dE . V
+    __shared__ float total_mem[2][kRows];  // q . dq and k . dk of all of them
+    __shared__ float state_mem[4];         // per wavefront: its share of <S, dS>
     lds_char *const lds = (lds_char *)mem;
-    lds_char *const qp = lds, *const kp = qp + PIECES * kRowsPlane;
+    lds_char *const qp = lds, *const kp = qp + PIECES * kSquare;
     lds_char *const gop = lds + (kResident ? kQK : 0), *const zp = gop + PIECES * kGo, *const dep = zp + NP * kSq,
-                    *const sp = dep + NP * kSq, *const dsp = sp + NP * kSt;
+                    *const sp = dep + NP * kSq, *const dsp = sp + NP * kSq;
     lds_char *const pp = lds + kQK, *const rp = pp + NP * kSquare;
     lds_float *const fp = (lds_float *)f_mem;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
     int c = lane & 15, q = lane >> 4;
-    const int e0 = EW * (wave & 3), t0 = RT * (wave >> 2);  // the wavefront's tiles of key columns and of positions
+    const int e0 = EW * (wave & 1), t0 = RT * (wave >> 1);  // the wavefront's tiles of key columns and of positions
+    // (workgroups go to the eight dies in turn: the slices of a chunk to the same)
+    const int slices = (p.E + kSlice - 1) / kSlice, tiles = p.E <= 64 ? 4 : 8;
+    const int turn = (int)(blockIdx.x >> 3), slice = scalar(turn % slices);
+    const int unit_of = scalar((turn / slices) * 8 + (int)(blockIdx.x & 7));
     const int G = scalar(p.H / p.Hk);
-    const int nk = scalar((int)(blockIdx.x / (uint32_t)p.chunks)), chunk = (int)blockIdx.x - nk * p.chunks;
+    const int nk = scalar(unit_of / p.chunks), chunk = unit_of - nk * p.chunks;
+    if (nk >= p.N * p.Hk) return;
     const int n = scalar(nk / p.Hk), hk = nk - n * p.Hk;
     const int64_t l0 = (int64_t)chunk * kRows;
     const int rows = (int)min((int64_t)kRows, p.L - l0);  // of the chunk in memory
-    auto grad_at = [&](const Scalars &x, int h, int i) { return n * x.sn + h * x.sh + (l0 + i) * x.sl; };
-    const Where first = where_of(p, n * p.H + hk * G, chunk);
-    const int valid = first.valid;  // (the same for all heads of a sequence)
+    const int valid = where_of(p, n * p.H + hk * G, chunk).valid;  // (the same for all heads of a sequence)
 
     f32x4 dQ[RT][EW] = {}, dK[RT][EW] = {};
+    auto slice_of = [&](const Operand &o) {
+        Operand s = o;
+        s.ptr = (const char *)o.ptr + slice * kSlice * Elem<T>::kBytes;
+        return s;
+    };
     auto stage_rows = [&]() {
-        RowTile<T, 32 * KE, kThreads> tile;
-        tile.load(chunk_rows(p.q, n, hk, l0, Elem<T>::kBytes), (uint32_t)p.q.stride_l * Elem<T>::kBytes, p.E, valid,
-                  p.vec_q, tid);
-        tile.template store<RB>(qp, tid);
-        tile.load(chunk_rows(p.k, n, hk, l0, Elem<T>::kBytes), (uint32_t)p.k.stride_l * Elem<T>::kBytes, p.E, valid,
-                  p.vec_k, tid);
-        tile.template store<RB>(kp, tid);
+        RowTile<T, kSlice, kThreads> tile;
+        tile.load(chunk_rows(slice_of(p.q), n, hk, l0, Elem<T>::kBytes), (uint32_t)p.q.stride_l * Elem<T>::kBytes,
+                  p.E - slice * kSlice, valid, p.vec_q, renewed(tid));
+        tile.template store<RB>(qp, renewed(tid));
+        tile.load(chunk_rows(slice_of(p.k), n, hk, l0, Elem<T>::kBytes), (uint32_t)p.k.stride_l * Elem<T>::kBytes,
+                  p.E - slice * kSlice, valid, p.vec_k, renewed(tid));
+        tile.template store<RB>(kp, renewed(tid));
     };
 
-    // ---- what phase 1 stages: dO's rows by the first 256 threads, the others' fragments by all ----
-    RowTile<T, kMB, 256> go;
-    f32x4 zr, er, sr[ET / 4], dr[ET / 4];
-    uint32_t vr[4];
+    // ---- what phase 1 stages of 32 columns: dO's rows, and the fragments' tile `wave` of either block ----
+    RowTile<T, kMB, kThreads> go;
+    f32x4 zr[2], er[2], sr[2], dr[2];
+    uint32_t vr[2][4];
     auto request = [&](int h, int m0) {
         const int64_t at = ((int64_t)(n * p.H + h) * p.chunks + chunk) * p.col_blocks;
-        const int half = scalar(tid >> 8), unit = renewed(tid & 255), block = m0 + half;
-        if (half == 0) {
-            Operand shifted = p.go;
-            shifted.ptr = (const char *)p.go.ptr + (int64_t)m0 * kCols * Elem<T>::kBytes;
-            go.load(chunk_rows(shifted, n, h, l0, Elem<T>::kBytes), (uint32_t)p.go.stride_l * Elem<T>::kBytes,
-                    p.M - m0 * kCols, valid, p.vec_go, unit);
-        }
-        {
-            const int row = 4 * (unit >> 4), col = block * kCols + (unit & 15);
-            const __amdgpu_buffer_rsrc_t rs = chunk_rows(p.v, n, h, l0, Elem<T>::kBytes);
+        const int l = renewed(lane);
+        Operand shifted = p.go;
+        shifted.ptr = (const char *)p.go.ptr + (int64_t)m0 * kCols * Elem<T>::kBytes;
+        go.load(chunk_rows(shifted, n, h, l0, Elem<T>::kBytes), (uint32_t)p.go.stride_l * Elem<T>::kBytes,
+                p.M - m0 * kCols, valid, p.vec_go, 64 * wave + l);
+        const __amdgpu_buffer_rsrc_t v_rows = chunk_rows(p.v, n, h, l0, Elem<T>::kBytes);
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int block = m0 + b, col = block * kCols + (l & 15);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const uint32_t from = row + r < valid && col < p.M
-                    ? (uint32_t)(row + r) * ((uint32_t)p.v.stride_l * Elem<T>::kBytes) + (uint32_t)(col * Elem<T>::kBytes) : kOutside;
-                vr[r] = Elem<T>::kBytes == 4 ? __builtin_amdgcn_raw_buffer_load_b32(rs, from, 0, 0)
-                                             : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, from, 0, 0);
+                const int row = 16 * wave + 4 * (l >> 4) + r;
+                const uint32_t from = row < valid && col < p.M
+                    ? (uint32_t)row * ((uint32_t)p.v.stride_l * Elem<T>::kBytes) + (uint32_t)(col * Elem<T>::kBytes) : kOutside;
+                vr[b][r] = Elem<T>::kBytes == 4 ? __builtin_amdgcn_raw_buffer_load_b32(v_rows, from, 0, 0)
+                                                : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(v_rows, from, 0, 0);
             }
+            // (a block past the last one: zeros, from a buffer of no bytes)
+            auto fragment = [&](const float *from, int count, int tile) {
+                const uint64_t base = (uint64_t)(from + ((at + block) * count + tile) * 256);
+                const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                    (void *)(((uint64_t)(uint32_t)scalar((int)(base >> 32)) << 32) | (uint32_t)scalar((int)(uint32_t)base)), 0,
+                    block < p.col_blocks ? 1024 : 0, mfma::kRsrcFlags);
+                return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * l, 0, 0));
+            };
+            zr[b] = fragment(p.z, 4, wave), er[b] = fragment(p.de, 4, wave);
+            sr[b] = fragment(p.s, tiles, 4 * slice + wave), dr[b] = fragment(p.ds, tiles, 4 * slice + wave);
         }
-        // (a block past the last one: zeros, from a buffer of no bytes)
-        const bool there = block < p.col_blocks;
-        auto fragments = [&](const float *from, int tiles, int number) {
-            const uint64_t base = (uint64_t)(from + (at + block) * (tiles * 256));
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                (void *)(((uint64_t)(uint32_t)scalar((int)(base >> 32)) << 32) | (uint32_t)scalar((int)(uint32_t)base)), 0,
-                there ? tiles * 1024 : 0, mfma::kRsrcFlags);
-            return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * unit + 4096 * number, 0, 0));
-        };
-        zr = fragments(p.z, 4, 0), er = fragments(p.de, 4, 0);
-#pragma unroll
-        for (int u = 0; u < ET / 4; u++) sr[u] = fragments(p.s, ET, u), dr[u] = fragments(p.ds, ET, u);
     };
     // a fragment's place in planes with a row per column: four positions (or key columns) of column c
     auto put = [&](f32x4 &dot_z, f32x4 &dot_v) {
-        const int half = scalar(tid >> 8), unit = renewed(tid & 255);
-        if (half == 0) go.template store<64>(gop, unit);
-        const int row = 16 * half + (unit & 15), slot = unit >> 4;
+        const int l = renewed(lane), slot = 4 * wave + (l >> 4);
+        go.template store<64>(gop, 64 * wave + l);
         float dot = 0.f;
-        store_pieces<NP>(zp + Plane<128>::addr(row, slot), kSq, zr);
-        store_pieces<NP>(dep + Plane<128>::addr(row, slot), kSq, er);
-        dot_z += er * zr;
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-            dot_v[r] = fmaf(er[r], __uint_as_float(Elem<T>::kBytes == 4 ? vr[r] : vr[r] << 16), dot_v[r]);
+        for (int b = 0; b < 2; b++) {
+            const int to = Plane<128>::addr(16 * b + (l & 15), slot);
+            store_pieces<NP>(zp + to, kSq, zr[b]);
+            store_pieces<NP>(dep + to, kSq, er[b]);
+            store_pieces<NP>(sp + to, kSq, sr[b]);
+            store_pieces<NP>(dsp + to, kSq, dr[b]);
+            dot_z += er[b] * zr[b];
 #pragma unroll
-        for (int u = 0; u < ET / 4; u++) {
-            store_pieces<NP>(sp + Plane<RB>::addr(row, slot + 16 * u), kSt, sr[u]);
-            store_pieces<NP>(dsp + Plane<RB>::addr(row, slot + 16 * u), kSt, dr[u]);
-            dot += (sr[u][0] * dr[u][0] + sr[u][1] * dr[u][1]) + (sr[u][2] * dr[u][2] + sr[u][3] * dr[u][3]);
+            for (int r = 0; r < 4; r++)
+                dot_v[r] = fmaf(er[b][r], __uint_as_float(Elem<T>::kBytes == 4 ? vr[b][r] : vr[b][r] << 16), dot_v[r]);
+            dot += (sr[b][0] * dr[b][0] + sr[b][1] * dr[b][1]) + (sr[b][2] * dr[b][2] + sr[b][3] * dr[b][3]);
         }
         return dot;
     };
     // the tiles of the square matrices, transposed: rows j of tile tj, columns i of tile ti
     auto tile_of = [&](int x, int &ti, int &tj) {
-        const int id = wave + 8 * x;
+        const int id = wave + 4 * x;
         ti = id < 2 ? 0 : id < 4 ? 1 : id < 8 ? 2 : 3, tj = id < 4 ? id & 1 : id & 3;
-        return id < 12;
     };
 
     if (valid > 0) {
@@ -151,20 +156,16 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
         if (kResident) stage_rows();
     }
     if (tid < kRows) total_mem[0][tid] = total_mem[1][tid] = 0.f;
-    for (int g = 0; g < G; g++) {
+    for (int g = 0; g < G && valid > 0; g++) {
         const int h = hk * G + g;
-        if (valid == 0) {
-            if (tid < rows) {
-                if (p.gg.ptr) store_from_f32(p.gg.ptr, p.gg.dtype, grad_at(p.gg, h, tid), 0.f);
-                if (p.gb.ptr) store_from_f32(p.gb.ptr, p.gb.dtype, grad_at(p.gb, h, tid), 0.f);
-            }
-            continue;
-        }
         const int64_t at = (int64_t)(n * p.H + h) * p.chunks + chunk;
+        float o = 0.f;  // (dO . O of a row, for the normalisation)
+        if (p.normalize && wave == 3)
+            for (int b = 0; b < p.col_blocks; b++) o += p.dots[(at * p.col_blocks + b) * kRows + lane];
         for (int i = tid; i < kFactors * kRows; i += kThreads) fp[i] = p.factors[at * (kFactors * kRows) + i];
 
         // ---- phase 1 ----
-        f32x4 F[2] = {}, N[2] = {};                                    // (dO Z^T)^T, (dE Z^T)^T
+        f32x4 F[3] = {}, N[3] = {};                                    // (dO Z^T)^T, (dE Z^T)^T
         f32x4 aQ[RT][EW] = {}, aP[RT][EW] = {}, aM[RT][EW] = {};       // S dO, S dE, dS Z
         f32x4 dot_z = {0.f, 0.f, 0.f, 0.f}, dot_v = {0.f, 0.f, 0.f, 0.f};
         float state_dot = 0.f;
@@ -176,9 +177,9 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
             if (more || g + 1 < G) request(more ? h : h + 1, more ? m0 + 2 : 0);
             renew(c, q);
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
+            for (int x = 0; x < 3; x++) {
                 int ti, tj;
-                if (!tile_of(x, ti, tj)) continue;
+                tile_of(x, ti, tj);
                 Frag zf[NP], of[PIECES], ef[NP];
                 columns_of<128>(zp, tj, 0, c, q, zf, kSq);
 #pragma unroll
@@ -190,8 +191,8 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
             Frag sf[EW][NP], df[EW][NP];
 #pragma unroll
             for (int e = 0; e < EW; e++) {
-                columns_of<RB>(sp, e0 + e, 0, c, q, sf[e], kSt);
-                columns_of<RB>(dsp, e0 + e, 0, c, q, df[e], kSt);
+                columns_of<RB>(sp, e0 + e, 0, c, q, sf[e], kSq);
+                columns_of<RB>(dsp, e0 + e, 0, c, q, df[e], kSq);
             }
 #pragma unroll
             for (int t = 0; t < RT; t++) {
@@ -217,15 +218,8 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
         if (c == 0)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                dot_mem[wave >> 2][0][16 * (wave & 3) + 4 * q + r] = dot_z[r];
-                dot_mem[wave >> 2][1][16 * (wave & 3) + 4 * q + r] = dot_v[r];
-            }
-        // (by the wavefront that sums the decays: on its way during phase 2)
-        float o = 0.f, written = 0.f;
-        if (wave == 0)
-            for (int b = 0; b < p.col_blocks; b++) {
-                o += p.dots[(at * p.col_blocks + b) * kRows + lane];
-                written += p.written[(at * p.col_blocks + b) * 64 + lane];
+                dot_mem[0][16 * wave + 4 * q + r] = dot_z[r];
+                dot_mem[1][16 * wave + 4 * q + r] = dot_v[r];
             }
 
         // ---- phase 2 ----
@@ -233,9 +227,9 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
         renew(c, q);
         if (!kResident) stage_rows();
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
+        for (int x = 0; x < 3; x++) {
             int ti, tj;
-            if (!tile_of(x, ti, tj)) continue;
+            tile_of(x, ti, tj);
             const int i = 16 * ti + c, j0 = 16 * tj + 4 * q;
             const float rk_i = fp[kRk * kRows + i], rq_i = fp[kRq * kRows + i];
             f32x4 pt, rt;
@@ -263,6 +257,14 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
                     dK[t][e][r] += write * aM[t][e][r] - read_k * aP[t][e][r];
                 }
             }
+        // what the decays' and beta's gradients are made of, for the kernel behind
+        if (wave < 2) {
+            if (slice == 0) p.sums[at * kSums + kRows * wave + lane] = dot_mem[wave][lane];
+        } else if (wave == 2) {
+            if (lane == 0) p.sums[at * kSums + 2 * kRows + slice] = (state_mem[0] + state_mem[1]) + (state_mem[2] + state_mem[3]);
+        } else if (p.normalize) {
+            total_mem[0][lane] += o, total_mem[1][lane] += 2.f * dot_mem[0][lane] - dot_mem[1][lane];
+        }
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
@@ -293,28 +295,7 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
                 }
             }
         }
-        if (wave == 0) {
-            const float z = dot_mem[0][0][lane] + dot_mem[1][0][lane], v = dot_mem[0][1][lane] + dot_mem[1][1][lane];
-            total_mem[0][lane] += o, total_mem[1][lane] += 2.f * z - v;
-            double sum = (double)o - (double)v, all = written, state = 0.0;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-#pragma unroll
-            for (int i = 0; i < 8; i++) state += state_mem[i];
-            all += (double)fp[kRise * kRows + kRows - 1] * state;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {  // sums from here to the end
-                const double other = __shfl_down(sum, d);
-                if (lane + d < 64) sum += other;
-            }
-            if (lane < rows) {
-                if (p.gg.ptr)
-                    store_from_f32(p.gg.ptr, p.gg.dtype, grad_at(p.gg, h, lane), lane < valid ? (float)(sum + all) : 0.f);
-                if (p.gb.ptr)
-                    store_from_f32(p.gb.ptr, p.gb.dtype, grad_at(p.gb, h, lane),
-                                   lane < valid ? z / fp[kBeta * kRows + lane] : 0.f);
-            }
-        }
+        settle();
         __syncthreads();
     }
 
@@ -325,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
 #pragma unroll
             for (int k = PIECES - 1; k >= 0; k--)
                 v += bf16_to_f32(*(const __attribute__((address_space(3))) uint16_t *)(
-                    planes + k * kRowsPlane + Plane<RB>::addr(row, col >> 2) + 2 * (col & 3)));
+                    planes + k * kSquare + Plane<RB>::addr(row, col >> 2) + 2 * (col & 3)));
             return v;
         };
 #pragma unroll
@@ -343,37 +324,74 @@ __global__ __launch_bounds__(kThreads) void delta_gradients_kernel(DeltaArgs p) 
                 }
             }
     }
+    // (a buffer drops what lies outside)
+    auto leave = [&](const OperandOut &out, const f32x4 (&x)[RT][EW]) {
+        if (!out.ptr) return;
+        const __amdgpu_buffer_rsrc_t rs = chunk_rows(Operand{out.ptr, out.stride_n, out.stride_h, out.stride_l, 0, 0}, n, hk, l0,
+                                                     Elem<T>::kBytes);
 #pragma unroll
-    for (int t = 0; t < RT; t++)
+        for (int t = 0; t < RT; t++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int row = 16 * (t0 + t) + 4 * q + r;
-            if (row >= rows) continue;
+            for (int r = 0; r < 4; r++)
 #pragma unroll
-            for (int e = 0; e < EW; e++) {
-                const int col = 16 * (e0 + e) + c;
-                if (col >= p.E) continue;
-                if (p.gq.ptr)
-                    store_from_f32(p.gq.ptr, p.gq.dtype,
-                                   n * p.gq.stride_n + hk * p.gq.stride_h + (l0 + row) * p.gq.stride_l + col, dQ[t][e][r]);
-                if (p.gk.ptr)
-                    store_from_f32(p.gk.ptr, p.gk.dtype,
-                                   n * p.gk.stride_n + hk * p.gk.stride_h + (l0 + row) * p.gk.stride_l + col, dK[t][e][r]);
-            }
-        }
+                for (int e = 0; e < EW; e++) {
+                    const int row = 16 * (t0 + t) + 4 * q + r, col = slice * kSlice + 16 * (e0 + e) + c;
+                    const uint32_t to = row < rows && col < p.E
+                        ? (uint32_t)row * ((uint32_t)out.stride_l * Elem<T>::kBytes) + (uint32_t)(col * Elem<T>::kBytes) : kOutside;
+                    if (Elem<T>::kBytes == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[t][e][r]), rs, to, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (__bf16)x[t][e][r]), rs, to, 0, 0);
+                }
+    };
+    leave(p.gq, dQ);
+    leave(p.gk, dK);
 }
 
-template <typename T, int KE>
-void launch(const DeltaArgs &p, hipStream_t stream) {
-    const dim3 grid((uint32_t)p.N * (uint32_t)p.Hk * (uint32_t)p.chunks);
-    delta_gradients_kernel<T, KE><<<grid, kThreads, 0, stream>>>(p);
+// The gradients of the decays and of beta: a wavefront per chunk and chain, a lane per position
+__global__ __launch_bounds__(256) void delta_decays_kernel(DeltaArgs p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + scalar(threadIdx.x >> 6);
+    if (unit >= (int64_t)p.N * p.H * p.chunks) return;
+    const int chain = scalar((int)(unit / p.chunks));
+    const Where w = where_of(p, chain, (int)(unit - (int64_t)chain * p.chunks));
+    const int64_t l = (int64_t)w.chunk * kRows + lane;
+    float dg = 0.f, db = 0.f;
+    if (w.valid > 0) {
+        const float *const sums = p.sums + w.at * kSums, *const factors = p.factors + w.at * (kFactors * kRows);
+        const float z = sums[lane], v = sums[kRows + lane], beta = factors[kBeta * kRows + lane];
+        const float state = p.E <= kSlice ? sums[2 * kRows] : sums[2 * kRows] + sums[2 * kRows + 1];
+        float o = 0.f, written = 0.f;
+#pragma unroll 4
+        for (int b = 0; b < p.col_blocks; b++) {
+            o += p.dots[(w.at * p.col_blocks + b) * kRows + lane];
+            written += p.written[(w.at * p.col_blocks + b) * 64 + lane];
+        }
+        double sum = (double)o - (double)v, all = written;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+        all += (double)factors[kRise * kRows + kRows - 1] * (double)state;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {  // sums from here to the end
+            const double other = __shfl_down(sum, d);
+            if (lane + d < 64) sum += other;
+        }
+        if (lane < w.valid) dg = (float)(sum + all), db = z / beta;
+    }
+    if (l >= p.L) return;
+    if (p.gg.ptr) store_from_f32(p.gg.ptr, p.gg.dtype, w.n * p.gg.sn + w.h * p.gg.sh + l * p.gg.sl, dg);
+    if (p.gb.ptr) store_from_f32(p.gb.ptr, p.gb.dtype, w.n * p.gb.sn + w.h * p.gb.sh + l * p.gb.sl, db);
 }
 
 }  // namespace
 
 int delta_gradients(const DeltaArgs &p, bool bf16, hipStream_t stream) {
-    if (p.E <= 64) bf16 ? launch<bf16_t, 2>(p, stream) : launch<float, 2>(p, stream);
-    else bf16 ? launch<bf16_t, 4>(p, stream) : launch<float, 4>(p, stream);
+    const uint32_t slices = (uint32_t)((p.E + kSlice - 1) / kSlice);
+    const dim3 grid(((uint32_t)p.N * (uint32_t)p.Hk * (uint32_t)p.chunks + 7) / 8 * 8 * slices);
+    if (bf16) delta_gradients_kernel<bf16_t><<<grid, kThreads, 0, stream>>>(p);
+    else delta_gradients_kernel<float><<<grid, kThreads, 0, stream>>>(p);
+    if (p.gg.ptr || p.gb.ptr) {
+        const int64_t units = (int64_t)p.N * p.H * p.chunks;
+        delta_decays_kernel<<<dim3((uint32_t)((units + 3) / 4)), 256, 0, stream>>>(p);
+    }
     return FTC_OK;
 }
 

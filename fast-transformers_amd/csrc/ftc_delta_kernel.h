@@ -64,6 +64,8 @@ enum Factor {
     kWrite,  // ... times beta_i
     kFactors
 };
+constexpr int kSums = 3 * kRows;
+
 struct Scalars {  // one value per position: log decays, beta and their gradients
     void *ptr;
     int64_t sn, sh, sl;
@@ -95,6 +97,7 @@ struct DeltaArgs {
     float *ds;               // the gradient of the state after each chunk, as s
     float *de;               // A^T dO, then dE, as z
     float *dots;             // dO . O of every position, column block by column block: [chain][chunk][col block][64]
+    float *sums;             // dE . Z and dE . V of every position, two shares of <S, dS>: [chain][chunk][kSums]
     float *written;          // shares of what a chunk's keys write of <state, its gradient>: the same, [64 lanes]
 };
 
