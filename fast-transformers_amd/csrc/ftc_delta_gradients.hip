@@ -20,6 +20,8 @@
 // wavefront has 32 positions of 32 key columns, and a quarter of the tiles of dO Z^T and dE Z^T.  Phase 2 multiplies the
 // 64 x 64 matrices with the rows.  Gradients of bf16 rows are made of values in two pieces (2^-17 of them is left out,
 // against half a step of 2^-8 that the rounding of the results takes).
+#include <type_traits>
+
 #include "ftc_delta_kernel.h"
 
 namespace ftc {
@@ -93,14 +95,18 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
     // ---- what phase 1 stages of 32 columns: dO's rows, and the fragments' tile `wave` of either block ----
     RowTile<T, kMB, kThreads> go;
     f32x4 zr[2], er[2], sr[2], dr[2];
-    uint32_t vr[2][4];
-    auto request = [&](int h, int m0) {
+    // (of v in its own type: widening it here would wait for it)
+    using Raw = typename std::conditional<Elem<T>::kBytes == 4, uint32_t, uint16_t>::type;
+    Raw vr[2][4];
+    auto request = [&](int h, int m0, bool any) {
         const int64_t at = ((int64_t)(n * p.H + h) * p.chunks + chunk) * p.col_blocks;
         const int l = renewed(lane);
         Operand shifted = p.go;
         shifted.ptr = (const char *)p.go.ptr + (int64_t)m0 * kCols * Elem<T>::kBytes;
+        // (a block past the last one: zeros, from a buffer of no bytes or rows of no values)
+        const int live = any ? valid : 0;
         go.load(chunk_rows(shifted, n, h, l0, Elem<T>::kBytes), (uint32_t)p.go.stride_l * Elem<T>::kBytes,
-                p.M - m0 * kCols, valid, p.vec_go, 64 * wave + l);
+                p.M - m0 * kCols, live, p.vec_go, 64 * wave + l);
         const __amdgpu_buffer_rsrc_t v_rows = chunk_rows(p.v, n, h, l0, Elem<T>::kBytes);
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -108,17 +114,17 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int row = 16 * wave + 4 * (l >> 4) + r;
-                const uint32_t from = row < valid && col < p.M
-                    ? (uint32_t)row * ((uint32_t)p.v.stride_l * Elem<T>::kBytes) + (uint32_t)(col * Elem<T>::kBytes) : kOutside;
-                vr[b][r] = Elem<T>::kBytes == 4 ? __builtin_amdgcn_raw_buffer_load_b32(v_rows, from, 0, 0)
-                                                : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(v_rows, from, 0, 0);
+                const bool in = (row < live) & (col < p.M);
+                const uint32_t at = (uint32_t)row * ((uint32_t)p.v.stride_l * Elem<T>::kBytes) + (uint32_t)(col * Elem<T>::kBytes);
+                const uint32_t from = in ? at : kOutside;
+                if constexpr (Elem<T>::kBytes == 4) vr[b][r] = __builtin_amdgcn_raw_buffer_load_b32(v_rows, from, 0, 0);
+                else vr[b][r] = __builtin_amdgcn_raw_buffer_load_b16(v_rows, from, 0, 0);
             }
-            // (a block past the last one: zeros, from a buffer of no bytes)
             auto fragment = [&](const float *from, int count, int tile) {
                 const uint64_t base = (uint64_t)(from + ((at + block) * count + tile) * 256);
                 const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
                     (void *)(((uint64_t)(uint32_t)scalar((int)(base >> 32)) << 32) | (uint32_t)scalar((int)(uint32_t)base)), 0,
-                    block < p.col_blocks ? 1024 : 0, mfma::kRsrcFlags);
+                    any && block < p.col_blocks ? 1024 : 0, mfma::kRsrcFlags);
                 return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * l, 0, 0));
             };
             zr[b] = fragment(p.z, 4, wave), er[b] = fragment(p.de, 4, wave);
@@ -140,7 +146,7 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
             dot_z += er[b] * zr[b];
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                dot_v[r] = fmaf(er[b][r], __uint_as_float(Elem<T>::kBytes == 4 ? vr[b][r] : vr[b][r] << 16), dot_v[r]);
+                dot_v[r] = fmaf(er[b][r], __uint_as_float(Elem<T>::kBytes == 4 ? (uint32_t)vr[b][r] : (uint32_t)vr[b][r] << 16), dot_v[r]);
             dot += (sr[b][0] * dr[b][0] + sr[b][1] * dr[b][1]) + (sr[b][2] * dr[b][2] + sr[b][3] * dr[b][3]);
         }
         return dot;
@@ -152,7 +158,7 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
     };
 
     if (valid > 0) {
-        request(hk * G, 0);
+        request(hk * G, 0, true);
         if (kResident) stage_rows();
     }
     if (tid < kRows) total_mem[0][tid] = total_mem[1][tid] = 0.f;
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
             state_dot += put(dot_z, dot_v);
             __syncthreads();
             const bool more = m0 + 2 < p.col_blocks;
-            if (more || g + 1 < G) request(more ? h : h + 1, more ? m0 + 2 : 0);
+            request(more || g + 1 == G ? h : h + 1, more ? m0 + 2 : 0, more || g + 1 < G);
             renew(c, q);
 #pragma unroll
             for (int x = 0; x < 3; x++) {

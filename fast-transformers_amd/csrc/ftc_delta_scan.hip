@@ -58,6 +58,7 @@ struct ColumnTile {
     static constexpr int kBytes = Elem<T>::kBytes, kLoads = kRows * kCols * kBytes / 1024, kAcross = kCols * kBytes / 16;
     static constexpr int kTile = kRows * kCols * kBytes;
     u32x4 r[VEC ? kLoads : 4];
+    uint16_t half[VEC || kBytes == 4 ? 1 : 16];
 
     // VEC: lane's row 64 / kAcross i + lane / kAcross, 16 bytes of it; else its values one by one
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row_bytes, int col0, int width, int valid, int lane) {
@@ -77,8 +78,8 @@ struct ColumnTile {
                 for (int x = 0; x < 4; x++) {
                     const int row = 16 * t + 4 * (lane >> 4) + x;
                     const uint32_t at = row < valid && col < width ? (uint32_t)row * row_bytes + (uint32_t)(col * kBytes) : kOutside;
-                    r[t][x] = kBytes == 4 ? __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0)
-                                          : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, at, 0, 0);
+                    if constexpr (kBytes == 4) r[t][x] = __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0);
+                    else half[4 * t + x] = __builtin_amdgcn_raw_buffer_load_b16(rs, at, 0, 0);
                 }
         }
     }
@@ -91,7 +92,7 @@ struct ColumnTile {
         f32x4 x;
         if constexpr (!VEC) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = __uint_as_float(kBytes == 4 ? r[t][i] : r[t][i] << 16);
+            for (int i = 0; i < 4; i++) x[i] = __uint_as_float(kBytes == 4 ? r[t][i] : (uint32_t)half[kBytes == 4 ? 0 : 4 * t + i] << 16);
         } else if constexpr (kBytes == 4) {
 #pragma unroll
             for (int i = 0; i < 4; i++) x[i] = *(const lds_float *)(from + 64 * (16 * t + 4 * q + i) + 4 * c);
