@@ -76,10 +76,12 @@ __device__ __forceinline__ void store_lot(void *base, int dtype, int64_t at, int
             *(float4 *)((float *)base + at) = make_float4(r.x[0], r.x[1], r.x[2], r.x[3]);
             *(float4 *)((float *)base + at + 4) = make_float4(r.x[4], r.x[5], r.x[6], r.x[7]);
         } else {
+            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+            typedef float f32x2 __attribute__((ext_vector_type(2)));
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                w[i] = (uint32_t)f32_to_bf16(r.x[2 * i]) | ((uint32_t)f32_to_bf16(r.x[2 * i + 1]) << 16);
+                w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{r.x[2 * i], r.x[2 * i + 1]}, bf16x2));
             *(uint4 *)((uint16_t *)base + at) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     } else {
@@ -107,14 +109,23 @@ __device__ __forceinline__ void team_sum(float &a, float &b, float (*mem)[2][16]
     }
 }
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + expf(-g)); }
-__device__ __forceinline__ float activate(float g, int activation) {
-    return activation == FTC_GATE_PLAIN ? g : activation == FTC_GATE_SIGMOID ? sigmoid(g) : g * sigmoid(g);
+// 1 / (1 + exp(-g)), from the hardware's 2^x of the exponent's whole product (its rounding made good, since it is
+// multiplied by the exponent) and its reciprocal: within 3 half steps
+__device__ __forceinline__ float sigmoid(float g) {
+    constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // log2(e) in two floats
+    const float x = fmaxf(-g, -126.f), t = x * kLog2e, rest = fmaf(x, kRest, fmaf(x, kLog2e, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_amdgcn_rcpf(1.f + fmaf(e, rest * 0.693147181f, e));
 }
-__device__ __forceinline__ float activate_slope(float g, int activation) {
-    if (activation == FTC_GATE_PLAIN) return 1.f;
-    const float s = sigmoid(g);
-    return activation == FTC_GATE_SIGMOID ? s * (1.f - s) : s * (1.f + g * (1.f - s));
+// The gate's factor and its slope
+__device__ __forceinline__ void activate(float g, int activation, float &value, float &slope) {
+    if (activation == FTC_GATE_PLAIN) {
+        value = g, slope = 1.f;
+    } else {
+        const float s = sigmoid(g);
+        value = activation == FTC_GATE_SIGMOID ? s : g * s;
+        slope = activation == FTC_GATE_SIGMOID ? s * (1.f - s) : s * fmaf(g, 1.f - s, 1.f);
+    }
 }
 
 // One lot of a norm's weight and bias
@@ -190,7 +201,11 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
             if (p.gate.ptr) {
                 const Lot g = load_lot<VEC>(p.gate.ptr, p.gate.dtype, gate_row * p.gate.stride + col, p.D - col);
 #pragma unroll
-                for (int i = 0; i < kLot; i++) r[v].x[i] *= activate(g.x[i], p.activation);
+                for (int i = 0; i < kLot; i++) {
+                    float value, slope;
+                    activate(g.x[i], p.activation, value, slope);
+                    r[v].x[i] *= value;
+                }
             }
             if (p.residual.ptr) {
                 const Lot d = load_lot<VEC>(p.residual.ptr, p.residual.dtype, row * p.residual.stride + col, p.D - col);
@@ -222,7 +237,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
     }
 }
 
-template <int LPR, int NV, bool VEC>
+// BIAS: a norm has a bias; SHARED: several rows have one gate row
+template <int LPR, int NV, bool VEC, bool BIAS, bool SHARED>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_kernel(Args p) {
     constexpr int kThreads = LPR > 256 ? LPR : 256, kTeams = kThreads / LPR;
     __shared__ float mem[2][2][16];
@@ -232,7 +248,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
     const float per = 1.f / (float)p.D;
     auto column = [&](int v) { return kLot * (lane + LPR * v); };
     // the teams' sums to one row of floats
-    auto leave = [&](Lot (&sum)[NV], float *to) {
+    auto leave = [&](auto &sum, float *to) {
         if (kTeams > 1) {
             __syncthreads();
 #pragma unroll
@@ -256,14 +272,14 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
             if (column(v) < p.D) store_lot<VEC>(to, FTC_F32, column(v), p.D - column(v), sum[v]);
     };
 
-    Lot dwa[NV] = {}, dba[NV] = {}, dwb[NV] = {}, dbb[NV] = {};
+    Lot dwa[NV] = {}, dba[BIAS ? NV : 1] = {}, dwb[NV] = {}, dbb[BIAS ? NV : 1] = {};
     // segments of rows (one per gate row), the part of them that is this workgroup's
     const int part = blockIdx.x % p.parts;
     for (int64_t seg = blockIdx.x / p.parts; seg * p.segment < p.rows; seg += gridDim.x / p.parts) {
         const int64_t first = seg * p.segment, end = min(p.rows, first + p.segment);
-        Lot dgate[NV] = {};
+        Lot dgate[SHARED ? NV : 1] = {};
         for (int64_t base = first + (int64_t)part * kTeams; base < end; base += (int64_t)p.parts * kTeams) {
-            const int64_t row = base + team, gate_row = p.shared ? seg : row;
+            const int64_t row = base + team, gate_row = SHARED ? seg : row;
             const bool live = row < end;
             float mean_a = 0.f, rstd_a = 1.f, mean_b = 0.f, rstd_b = 1.f;
             if (live && p.stats) {
@@ -297,14 +313,16 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
 #pragma unroll
                 for (int i = 0; i < kLot; i++) {
                     const float y = fmaf(n[v].x[i], w.x[i], b.x[i]);
-                    const float a = p.gate.ptr ? activate(gate[v].x[i], p.activation) * y : y;
+                    float value = 1.f, slope;
+                    if (p.gate.ptr) activate(gate[v].x[i], p.activation, value, slope);
+                    const float a = value * y;
                     xh[v].x[i] = VEC || i < left ? (fmaf(p.scale, a, xh[v].x[i]) - mean_b) * rstd_b : 0.f;
                 }
                 params_lot<VEC>(p.before, col, left, w, b);
 #pragma unroll
                 for (int i = 0; i < kLot; i++) {
                     dwb[v].x[i] = fmaf(dx[v].x[i], xh[v].x[i], dwb[v].x[i]);
-                    dbb[v].x[i] += dx[v].x[i];
+                    if (BIAS) dbb[BIAS ? v : 0].x[i] += dx[v].x[i];
                     dx[v].x[i] *= w.x[i];
                     s0 += dx[v].x[i];
                     s1 = fmaf(dx[v].x[i], xh[v].x[i], s1);
@@ -339,12 +357,14 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
                     Lot d;
 #pragma unroll
                     for (int i = 0; i < kLot; i++) {
-                        const float y = fmaf(n[v].x[i], w.x[i], b.x[i]), g = gate[v].x[i];
-                        d.x[i] = p.scale * activate_slope(g, p.activation) * y * dx[v].x[i];
-                        dx[v].x[i] *= p.scale * activate(g, p.activation);
-                        dgate[v].x[i] += d.x[i];
+                        const float y = fmaf(n[v].x[i], w.x[i], b.x[i]);
+                        float value, slope;
+                        activate(gate[v].x[i], p.activation, value, slope);
+                        d.x[i] = p.scale * slope * y * dx[v].x[i];
+                        dx[v].x[i] *= p.scale * value;
+                        if (SHARED) dgate[SHARED ? v : 0].x[i] += d.x[i];
                     }
-                    if (p.grad_gate.ptr && !p.shared)
+                    if (p.grad_gate.ptr && !SHARED)
                         store_lot<VEC>(p.grad_gate.ptr, p.grad_gate.dtype, row * p.grad_gate.stride + col, left, d);
                 } else {
 #pragma unroll
@@ -354,7 +374,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
 #pragma unroll
                 for (int i = 0; i < kLot; i++) {
                     dwa[v].x[i] = fmaf(dx[v].x[i], n[v].x[i], dwa[v].x[i]);
-                    dba[v].x[i] += dx[v].x[i];
+                    if (BIAS) dba[BIAS ? v : 0].x[i] += dx[v].x[i];
                     dx[v].x[i] *= w.x[i];
                     t0 += dx[v].x[i];
                     t1 = fmaf(dx[v].x[i], n[v].x[i], t1);
@@ -375,16 +395,19 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
                         store_lot<VEC>(p.grad_block.ptr, p.grad_block.dtype, row * p.grad_block.stride + column(v),
                                        p.D - column(v), dx[v]);
         }
-        if (p.shared && p.gate_sums) leave(dgate, p.gate_sums + (seg * p.parts + part) * p.D);
+        if constexpr (SHARED)
+            if (p.gate_sums) leave(dgate, p.gate_sums + (seg * p.parts + part) * p.D);
     }
     float *const to = p.sums + (int64_t)blockIdx.x * kSums * p.D;
     if (p.sums && p.after.weight) leave(dwa, to + kAfterWeight * p.D);
-    if (p.sums && p.after.bias) leave(dba, to + kAfterBias * p.D);
+    if constexpr (BIAS)
+        if (p.sums && p.after.bias) leave(dba, to + kAfterBias * p.D);
     if (p.sums && p.before.weight) leave(dwb, to + kBeforeWeight * p.D);
-    if (p.sums && p.before.bias) leave(dbb, to + kBeforeBias * p.D);
+    if constexpr (BIAS)
+        if (p.sums && p.before.bias) leave(dbb, to + kBeforeBias * p.D);
 }
 
-// out[row][col] = sum over `count` rows of floats, `stride` apart, in a fixed order: 8 lots of them by 32 columns
+// out[row][col] = sum over `count` rows of floats, `stride` apart, in a fixed order: 32 lots of them by 32 columns
 struct Fold {
     const float *from;
     void *to;
@@ -395,23 +418,29 @@ struct FoldArgs {
     Fold fold[kSums + 1];
     int32_t D, folds;
 };
-__global__ __launch_bounds__(256) void fold_rows_kernel(FoldArgs p) {
-    __shared__ float mem[8][32];
+__global__ __launch_bounds__(1024) void fold_rows_kernel(FoldArgs p) {
+    __shared__ float mem[32][33];
     const int x = threadIdx.x % 32, lot = threadIdx.x / 32, col = blockIdx.x * 32 + x;
     const Fold f = p.fold[blockIdx.y];
     for (int r = blockIdx.z; r < f.results; r += gridDim.z) {
-        float sum = 0.f;
-        if (col < p.D)
-            for (int i = lot; i < f.count; i += 8) sum += f.from[r * f.from_stride + (int64_t)i * f.stride + col];
-        __syncthreads();
-        mem[lot][x] = sum;
-        __syncthreads();
-        if (lot == 0 && col < p.D) {
-            float all = 0.f;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if (col < p.D) {
+            const float *const from = f.from + r * f.from_stride + col;
+            int i = lot;
+            for (; i + 96 < f.count; i += 128)
 #pragma unroll
-            for (int k = 0; k < 8; k++) all += mem[k][x];
-            store_from_f32(f.to, f.dtype, r * f.to_stride + col, all);
+                for (int k = 0; k < 4; k++) sum[k] += from[(int64_t)(i + 32 * k) * f.stride];
+            for (; i < f.count; i += 32) sum[0] += from[(int64_t)i * f.stride];
         }
+        __syncthreads();
+        mem[lot][x] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        __syncthreads();
+        // the lots' sums of a column, by the 32 lanes of one of them
+        float all = mem[x][lot];
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) all += __shfl_xor(all, d);
+        const int own = blockIdx.x * 32 + lot;
+        if (x == 0 && own < p.D) store_from_f32(f.to, f.dtype, r * f.to_stride + own, all);
     }
 }
 
@@ -437,12 +466,19 @@ Plan plan_of(int64_t D, int64_t rows, int64_t segment, bool backward) {
 template <int LPR, int NV>
 void launch(const Args &p, const Plan &q, bool vec, bool backward, hipStream_t stream) {
     const dim3 grid((uint32_t)q.groups), block(LPR > 256 ? LPR : 256);
-    if (backward) {
-        if (vec) residual_norm_backward_kernel<LPR, NV, true><<<grid, block, 0, stream>>>(p);
-        else residual_norm_backward_kernel<LPR, NV, false><<<grid, block, 0, stream>>>(p);
-    } else {
+    const bool bias = p.after.bias || p.before.bias;
+    if (!backward) {
         if (vec) residual_norm_kernel<LPR, NV, true><<<grid, block, 0, stream>>>(p);
         else residual_norm_kernel<LPR, NV, false><<<grid, block, 0, stream>>>(p);
+    } else if (!vec) {
+        if (p.shared) residual_norm_backward_kernel<LPR, NV, false, true, true><<<grid, block, 0, stream>>>(p);
+        else residual_norm_backward_kernel<LPR, NV, false, true, false><<<grid, block, 0, stream>>>(p);
+    } else if (bias) {
+        if (p.shared) residual_norm_backward_kernel<LPR, NV, true, true, true><<<grid, block, 0, stream>>>(p);
+        else residual_norm_backward_kernel<LPR, NV, true, true, false><<<grid, block, 0, stream>>>(p);
+    } else {
+        if (p.shared) residual_norm_backward_kernel<LPR, NV, true, false, true><<<grid, block, 0, stream>>>(p);
+        else residual_norm_backward_kernel<LPR, NV, true, false, false><<<grid, block, 0, stream>>>(p);
     }
 }
 void dispatch(const Args &p, const Plan &q, bool vec, bool backward, hipStream_t stream) {
@@ -597,7 +633,7 @@ int ftc_residual_norm_backward(const ftc_residual_norm_call *call, const float *
     }
     dispatch(p, q, wide(p), true, (hipStream_t)stream);
     if (f.folds)
-        fold_rows_kernel<<<dim3((uint32_t)((p.D + 31) / 32), (uint32_t)f.folds, (uint32_t)results), 256, 0, (hipStream_t)stream>>>(f);
+        fold_rows_kernel<<<dim3((uint32_t)((p.D + 31) / 32), (uint32_t)f.folds, (uint32_t)results), 1024, 0, (hipStream_t)stream>>>(f);
     return launched("residual_norm_backward_kernel");
 }
 
