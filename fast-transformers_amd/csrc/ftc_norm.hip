@@ -15,6 +15,7 @@
 // order.  A gate that several rows share is summed the same way: a workgroup's rows all belong to one of its rows.
 // All arithmetic is fp32; results are rounded once.
 #include <algorithm>
+#include <initializer_list>
 
 #include "ftc_common.h"
 
@@ -49,25 +50,38 @@ enum { kAfterWeight, kAfterBias, kBeforeWeight, kBeforeBias, kSums };
 struct Lot {
     float x[kLot];
 };
+// A lot as it comes from memory: widening it where it is requested would wait for it
+struct Raw {
+    uint4 a, b;
+};
 template <bool VEC>
-__device__ __forceinline__ Lot load_lot(const void *base, int dtype, int64_t at, int left) {
-    Lot r;
+__device__ __forceinline__ Raw request(const void *base, int dtype, int64_t at, int left) {
+    Raw r;
     if (VEC) {
-        if (dtype == FTC_F32) {
-            const float4 a = *(const float4 *)((const float *)base + at), b = *(const float4 *)((const float *)base + at + 4);
-            r.x[0] = a.x, r.x[1] = a.y, r.x[2] = a.z, r.x[3] = a.w, r.x[4] = b.x, r.x[5] = b.y, r.x[6] = b.z, r.x[7] = b.w;
-        } else {
-            const uint4 a = *(const uint4 *)((const uint16_t *)base + at);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                r.x[2 * i] = __uint_as_float(w[i] << 16), r.x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+        const char *const from = (const char *)base + at * (dtype == FTC_F32 ? 4 : 2);
+        r.a = *(const uint4 *)from;
+        if (dtype == FTC_F32) r.b = *(const uint4 *)(from + 16);
     } else {
+        uint32_t x[kLot];
 #pragma unroll
-        for (int i = 0; i < kLot; i++) r.x[i] = i < left ? load_as_f32(base, dtype, at + i) : 0.f;
+        for (int i = 0; i < kLot; i++) x[i] = i < left ? __float_as_uint(load_as_f32(base, dtype, at + i)) : 0u;
+        r.a = make_uint4(x[0], x[1], x[2], x[3]), r.b = make_uint4(x[4], x[5], x[6], x[7]);
     }
     return r;
+}
+template <bool VEC>
+__device__ __forceinline__ Lot widen(const Raw &r, int dtype) {
+    const uint32_t a[4] = {r.a.x, r.a.y, r.a.z, r.a.w}, b[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+    Lot x;
+    if (!VEC || dtype == FTC_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x.x[i] = __uint_as_float(a[i]), x.x[4 + i] = __uint_as_float(b[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            x.x[2 * i] = __uint_as_float(a[i] << 16), x.x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+    }
+    return x;
 }
 template <bool VEC>
 __device__ __forceinline__ void store_lot(void *base, int dtype, int64_t at, int left, const Lot &r) {
@@ -99,12 +113,12 @@ __device__ __forceinline__ void team_sum(float &a, float &b, float (*mem)[2][16]
     for (int d = 1; d < (LPR < 64 ? LPR : 64); d *= 2) a += __shfl_xor(a, d), b += __shfl_xor(b, d);
     if (LPR > 64) {
         constexpr int kWaves = LPR / 64;
-        const int wave = threadIdx.x >> 6;
+        const int wave = threadIdx.x >> 6, first = wave / kWaves * kWaves;
         if ((threadIdx.x & 63) == 0) mem[turn][0][wave] = a, mem[turn][1][wave] = b;
         __syncthreads();
         a = 0.f, b = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) a += mem[turn][0][w], b += mem[turn][1][w];
+        for (int w = 0; w < kWaves; w++) a += mem[turn][0][first + w], b += mem[turn][1][first + w];
         turn ^= 1;
     }
 }
@@ -128,21 +142,27 @@ __device__ __forceinline__ void activate(float g, int activation, float &value, 
     }
 }
 
-// One lot of a norm's weight and bias
+// One lot of a norm's weight and bias (from the caches: where they are used)
 template <bool VEC>
 __device__ __forceinline__ void params_lot(const Params &p, int col, int left, Lot &w, Lot &b) {
-    if (p.weight) w = load_lot<VEC>(p.weight, p.weight_dtype, col, left);
+    if (p.weight) w = widen<VEC>(request<VEC>(p.weight, p.weight_dtype, col, left), p.weight_dtype);
     else
 #pragma unroll
         for (int i = 0; i < kLot; i++) w.x[i] = 1.f;
-    if (p.bias) b = load_lot<VEC>(p.bias, p.bias_dtype, col, left);
+    if (p.bias) b = widen<VEC>(request<VEC>(p.bias, p.bias_dtype, col, left), p.bias_dtype);
     else
 #pragma unroll
         for (int i = 0; i < kLot; i++) b.x[i] = 0.f;
 }
+// The type of rows that the kernel is made for, or any
+template <int DTYPE>
+__device__ __forceinline__ int type_of(const Rows &r) {
+    return DTYPE >= 0 ? DTYPE : r.dtype;
+}
 
 // LPR lanes take a row, NV lots each; THREADS / LPR rows at a time
-template <int LPR, int NV, bool VEC>
+// DB, DS: types of the block's rows (gate and h too) and of the stream's
+template <int LPR, int NV, bool VEC, int DB, int DS>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Args p) {
     constexpr int kThreads = LPR > 256 ? LPR : 256, kTeams = kThreads / LPR;
     __shared__ float mem[2][2][16];
@@ -177,11 +197,20 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
     for (int64_t base = (int64_t)blockIdx.x * kTeams; base < p.rows; base += (int64_t)gridDim.x * kTeams) {
         const int64_t row = base + team, gate_row = p.every == 1 ? row : row / p.every;
         const bool live = row < p.rows;
+        Raw block[NV], gate[NV], residual[NV];
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int col = column(v), left = p.D - col;
+            if (!live || left <= 0) continue;
+            block[v] = request<VEC>(p.block.ptr, type_of<DB>(p.block), row * p.block.stride + col, left);
+            if (p.gate.ptr) gate[v] = request<VEC>(p.gate.ptr, type_of<DB>(p.gate), gate_row * p.gate.stride + col, left);
+            if (p.residual.ptr)
+                residual[v] = request<VEC>(p.residual.ptr, type_of<DS>(p.residual), row * p.residual.stride + col, left);
+        }
         Lot r[NV];
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-            const int col = column(v);
-            if (live && col < p.D) r[v] = load_lot<VEC>(p.block.ptr, p.block.dtype, row * p.block.stride + col, p.D - col);
+            if (live && column(v) < p.D) r[v] = widen<VEC>(block[v], type_of<DB>(p.block));
             else
 #pragma unroll
                 for (int i = 0; i < kLot; i++) r[v].x[i] = 0.f;
@@ -199,7 +228,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
                 for (int i = 0; i < kLot; i++) r[v].x[i] = fmaf((r[v].x[i] - mean_a) * rstd_a, w.x[i], b.x[i]);
             }
             if (p.gate.ptr) {
-                const Lot g = load_lot<VEC>(p.gate.ptr, p.gate.dtype, gate_row * p.gate.stride + col, p.D - col);
+                const Lot g = widen<VEC>(gate[v], type_of<DB>(p.gate));
 #pragma unroll
                 for (int i = 0; i < kLot; i++) {
                     float value, slope;
@@ -208,7 +237,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
                 }
             }
             if (p.residual.ptr) {
-                const Lot d = load_lot<VEC>(p.residual.ptr, p.residual.dtype, row * p.residual.stride + col, p.D - col);
+                const Lot d = widen<VEC>(residual[v], type_of<DS>(p.residual));
 #pragma unroll
                 for (int i = 0; i < kLot; i++) r[v].x[i] = fmaf(p.scale, r[v].x[i], d.x[i]);
             } else {
@@ -218,7 +247,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
             if (!VEC)
 #pragma unroll
                 for (int i = 0; i < kLot; i++) r[v].x[i] = col + i < p.D ? r[v].x[i] : 0.f;
-            store_lot<VEC>(p.x.ptr, p.x.dtype, row * p.x.stride + col, p.D - col, r[v]);
+            store_lot<VEC>(p.x.ptr, type_of<DS>(p.x), row * p.x.stride + col, p.D - col, r[v]);
         }
         statistics(r, p.before, mean_b, rstd_b);
         if (p.h.ptr && live)
@@ -230,15 +259,15 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
                 params_lot<VEC>(p.before, col, p.D - col, w, b);
 #pragma unroll
                 for (int i = 0; i < kLot; i++) r[v].x[i] = fmaf((r[v].x[i] - mean_b) * rstd_b, w.x[i], b.x[i]);
-                store_lot<VEC>(p.h.ptr, p.h.dtype, row * p.h.stride + col, p.D - col, r[v]);
+                store_lot<VEC>(p.h.ptr, type_of<DB>(p.h), row * p.h.stride + col, p.D - col, r[v]);
             }
         if (p.stats && live && lane == 0)
             *(float4 *)(p.stats + 4 * row) = make_float4(mean_a, rstd_a, mean_b, rstd_b);
     }
 }
 
-// BIAS: a norm has a bias; SHARED: several rows have one gate row
-template <int LPR, int NV, bool VEC, bool BIAS, bool SHARED>
+// FULL: a norm has a bias, or several rows have one gate row
+template <int LPR, int NV, bool VEC, int DB, int DS, bool FULL>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_kernel(Args p) {
     constexpr int kThreads = LPR > 256 ? LPR : 256, kTeams = kThreads / LPR;
     __shared__ float mem[2][2][16];
@@ -272,19 +301,33 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
             if (column(v) < p.D) store_lot<VEC>(to, FTC_F32, column(v), p.D - column(v), sum[v]);
     };
 
-    Lot dwa[NV] = {}, dba[BIAS ? NV : 1] = {}, dwb[NV] = {}, dbb[BIAS ? NV : 1] = {};
+    Lot dwa[NV] = {}, dba[FULL ? NV : 1] = {}, dwb[NV] = {}, dbb[FULL ? NV : 1] = {};
     // segments of rows (one per gate row), the part of them that is this workgroup's
     const int part = blockIdx.x % p.parts;
     for (int64_t seg = blockIdx.x / p.parts; seg * p.segment < p.rows; seg += gridDim.x / p.parts) {
         const int64_t first = seg * p.segment, end = min(p.rows, first + p.segment);
-        Lot dgate[SHARED ? NV : 1] = {};
+        Lot dgate[FULL ? NV : 1] = {};
         for (int64_t base = first + (int64_t)part * kTeams; base < end; base += (int64_t)p.parts * kTeams) {
-            const int64_t row = base + team, gate_row = SHARED ? seg : row;
+            const int64_t row = base + team, gate_row = FULL && p.shared ? seg : row;
             const bool live = row < end;
             float mean_a = 0.f, rstd_a = 1.f, mean_b = 0.f, rstd_b = 1.f;
             if (live && p.stats) {
                 const float4 s = *(const float4 *)(p.stats + 4 * row);
                 mean_a = s.x, rstd_a = s.y, mean_b = s.z, rstd_b = s.w;
+            }
+            Raw block_raw[NV], gate_raw[NV], residual_raw[NV], gh_raw[NV], gx_raw[NV];
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int col = column(v), left = p.D - col;
+                if (!live || left <= 0) continue;
+                block_raw[v] = request<VEC>(p.block.ptr, type_of<DB>(p.block), row * p.block.stride + col, left);
+                if (p.gate.ptr) gate_raw[v] = request<VEC>(p.gate.ptr, type_of<DB>(p.gate), gate_row * p.gate.stride + col, left);
+                if (p.before.kind != FTC_NORM_NONE) {
+                    if (p.residual.ptr)
+                        residual_raw[v] = request<VEC>(p.residual.ptr, type_of<DS>(p.residual), row * p.residual.stride + col, left);
+                    if (p.grad_h.ptr) gh_raw[v] = request<VEC>(p.grad_h.ptr, type_of<DB>(p.grad_h), row * p.grad_h.stride + col, left);
+                }
+                if (p.grad_x.ptr) gx_raw[v] = request<VEC>(p.grad_x.ptr, type_of<DS>(p.grad_x), row * p.grad_x.stride + col, left);
             }
             Lot n[NV], dx[NV], gate[NV], xh[NV];
             float s0 = 0.f, s1 = 0.f;
@@ -294,20 +337,13 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
 #pragma unroll
                 for (int i = 0; i < kLot; i++) n[v].x[i] = dx[v].x[i] = xh[v].x[i] = gate[v].x[i] = 0.f;
                 if (!live || col >= p.D) continue;
-                n[v] = load_lot<VEC>(p.block.ptr, p.block.dtype, row * p.block.stride + col, left);
-                if (p.gate.ptr) gate[v] = load_lot<VEC>(p.gate.ptr, p.gate.dtype, gate_row * p.gate.stride + col, left);
-                if (p.before.kind != FTC_NORM_NONE) {
-                    if (p.residual.ptr) xh[v] = load_lot<VEC>(p.residual.ptr, p.residual.dtype, row * p.residual.stride + col, left);
-                    if (p.grad_h.ptr) dx[v] = load_lot<VEC>(p.grad_h.ptr, p.grad_h.dtype, row * p.grad_h.stride + col, left);
-                }
-            }
-#pragma unroll
-            for (int v = 0; v < NV; v++) {
-                const int col = column(v), left = p.D - col;
-                if (!live || col >= p.D) continue;
+                n[v] = widen<VEC>(block_raw[v], type_of<DB>(p.block));
+                if (p.gate.ptr) gate[v] = widen<VEC>(gate_raw[v], type_of<DB>(p.gate));
 #pragma unroll
                 for (int i = 0; i < kLot; i++) n[v].x[i] = VEC || i < left ? (n[v].x[i] - mean_a) * rstd_a : 0.f;
                 if (p.before.kind == FTC_NORM_NONE) continue;
+                if (p.residual.ptr) xh[v] = widen<VEC>(residual_raw[v], type_of<DS>(p.residual));
+                if (p.grad_h.ptr) dx[v] = widen<VEC>(gh_raw[v], type_of<DB>(p.grad_h));
                 Lot w, b;
                 params_lot<VEC>(p.after, col, left, w, b);
 #pragma unroll
@@ -322,7 +358,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
 #pragma unroll
                 for (int i = 0; i < kLot; i++) {
                     dwb[v].x[i] = fmaf(dx[v].x[i], xh[v].x[i], dwb[v].x[i]);
-                    if (BIAS) dbb[BIAS ? v : 0].x[i] += dx[v].x[i];
+                    if (FULL) dbb[FULL ? v : 0].x[i] += dx[v].x[i];
                     dx[v].x[i] *= w.x[i];
                     s0 += dx[v].x[i];
                     s1 = fmaf(dx[v].x[i], xh[v].x[i], s1);
@@ -342,7 +378,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
                 const int col = column(v), left = p.D - col;
                 if (!live || col >= p.D) continue;
                 if (p.grad_x.ptr) {
-                    const Lot g = load_lot<VEC>(p.grad_x.ptr, p.grad_x.dtype, row * p.grad_x.stride + col, left);
+                    const Lot g = widen<VEC>(gx_raw[v], type_of<DS>(p.grad_x));
 #pragma unroll
                     for (int i = 0; i < kLot; i++) dx[v].x[i] += g.x[i];
                 }
@@ -350,7 +386,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
 #pragma unroll
                     for (int i = 0; i < kLot; i++) dx[v].x[i] = i < left ? dx[v].x[i] : 0.f;
                 if (p.grad_residual.ptr)
-                    store_lot<VEC>(p.grad_residual.ptr, p.grad_residual.dtype, row * p.grad_residual.stride + col, left, dx[v]);
+                    store_lot<VEC>(p.grad_residual.ptr, type_of<DS>(p.grad_residual), row * p.grad_residual.stride + col, left, dx[v]);
                 Lot w, b;
                 params_lot<VEC>(p.after, col, left, w, b);
                 if (p.gate.ptr) {
@@ -362,10 +398,10 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
                         activate(gate[v].x[i], p.activation, value, slope);
                         d.x[i] = p.scale * slope * y * dx[v].x[i];
                         dx[v].x[i] *= p.scale * value;
-                        if (SHARED) dgate[SHARED ? v : 0].x[i] += d.x[i];
+                        if (FULL) dgate[FULL ? v : 0].x[i] += d.x[i];
                     }
-                    if (p.grad_gate.ptr && !SHARED)
-                        store_lot<VEC>(p.grad_gate.ptr, p.grad_gate.dtype, row * p.grad_gate.stride + col, left, d);
+                    if (p.grad_gate.ptr && !(FULL && p.shared))
+                        store_lot<VEC>(p.grad_gate.ptr, type_of<DB>(p.grad_gate), row * p.grad_gate.stride + col, left, d);
                 } else {
 #pragma unroll
                     for (int i = 0; i < kLot; i++) dx[v].x[i] *= p.scale;
@@ -374,7 +410,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
 #pragma unroll
                 for (int i = 0; i < kLot; i++) {
                     dwa[v].x[i] = fmaf(dx[v].x[i], n[v].x[i], dwa[v].x[i]);
-                    if (BIAS) dba[BIAS ? v : 0].x[i] += dx[v].x[i];
+                    if (FULL) dba[FULL ? v : 0].x[i] += dx[v].x[i];
                     dx[v].x[i] *= w.x[i];
                     t0 += dx[v].x[i];
                     t1 = fmaf(dx[v].x[i], n[v].x[i], t1);
@@ -392,18 +428,18 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
 #pragma unroll
                 for (int v = 0; v < NV; v++)
                     if (column(v) < p.D)
-                        store_lot<VEC>(p.grad_block.ptr, p.grad_block.dtype, row * p.grad_block.stride + column(v),
+                        store_lot<VEC>(p.grad_block.ptr, type_of<DB>(p.grad_block), row * p.grad_block.stride + column(v),
                                        p.D - column(v), dx[v]);
         }
-        if constexpr (SHARED)
+        if constexpr (FULL)
             if (p.gate_sums) leave(dgate, p.gate_sums + (seg * p.parts + part) * p.D);
     }
     float *const to = p.sums + (int64_t)blockIdx.x * kSums * p.D;
     if (p.sums && p.after.weight) leave(dwa, to + kAfterWeight * p.D);
-    if constexpr (BIAS)
+    if constexpr (FULL)
         if (p.sums && p.after.bias) leave(dba, to + kAfterBias * p.D);
     if (p.sums && p.before.weight) leave(dwb, to + kBeforeWeight * p.D);
-    if constexpr (BIAS)
+    if constexpr (FULL)
         if (p.sums && p.before.bias) leave(dbb, to + kBeforeBias * p.D);
 }
 
@@ -448,46 +484,60 @@ __global__ __launch_bounds__(1024) void fold_rows_kernel(FoldArgs p) {
 constexpr int64_t kMostWidth = 16384;
 constexpr int kLeastNormed = 3;
 
+// Whether the backward needs the kernel that sums biases and shared gates as well
+bool full(const Args &p) { return p.after.bias || p.before.bias || p.shared; }
+
 struct Plan {
     int lpr, teams;
     int64_t groups, parts;  // workgroups, workgroups per segment
 };
-Plan plan_of(int64_t D, int64_t rows, int64_t segment, bool backward) {
+Plan plan_of(int64_t D, int64_t rows, int64_t segment, bool backward, bool full) {
     Plan q;
-    q.lpr = D <= 128 ? 16 : D <= 1024 ? 64 : D <= 8192 ? 256 : 1024;
+    q.lpr = D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 8192 ? 512 : 1024;
     q.teams = q.lpr > 256 ? 1 : 256 / q.lpr;
-    // four workgroups a compute unit; the backward leaves sums with each of them: two
-    const int64_t most = backward ? 512 : 1024, segments = (rows + segment - 1) / segment;
+    // As many as the GPU holds at a time, by their registers (more would wait, and the backward leaves sums with each of
+    // them).  Backward of 524288 x 128 with 768 of the lean kernel 143 us, with 512 179; of 40960 x 512 with 512 of the full
+    // one 115, with 768 138; forward of either with 1024 95 and 78, with 2048 104 and 82.
+    const int64_t most = q.lpr > 512 ? 256 : q.lpr > 256 ? 512 : !backward ? 1024 : full ? 512 : 768;
+    const int64_t segments = (rows + segment - 1) / segment;
     q.parts = std::min((segment + q.teams - 1) / q.teams, std::max<int64_t>(1, most / segments));
     q.groups = std::min(segments, std::max<int64_t>(1, most / q.parts)) * q.parts;
     return q;
 }
 
+template <int LPR, int NV, bool VEC, int DB, int DS>
+void launch(const Args &p, const Plan &q, bool backward, hipStream_t stream) {
+    const dim3 grid((uint32_t)q.groups), block(LPR > 256 ? LPR : 256);
+    if (!backward) residual_norm_kernel<LPR, NV, VEC, DB, DS><<<grid, block, 0, stream>>>(p);
+    else if (full(p))
+        residual_norm_backward_kernel<LPR, NV, VEC, DB, DS, true><<<grid, block, 0, stream>>>(p);
+    else residual_norm_backward_kernel<LPR, NV, VEC, DB, DS, false><<<grid, block, 0, stream>>>(p);
+}
 template <int LPR, int NV>
 void launch(const Args &p, const Plan &q, bool vec, bool backward, hipStream_t stream) {
-    const dim3 grid((uint32_t)q.groups), block(LPR > 256 ? LPR : 256);
-    const bool bias = p.after.bias || p.before.bias;
-    if (!backward) {
-        if (vec) residual_norm_kernel<LPR, NV, true><<<grid, block, 0, stream>>>(p);
-        else residual_norm_kernel<LPR, NV, false><<<grid, block, 0, stream>>>(p);
-    } else if (!vec) {
-        if (p.shared) residual_norm_backward_kernel<LPR, NV, false, true, true><<<grid, block, 0, stream>>>(p);
-        else residual_norm_backward_kernel<LPR, NV, false, true, false><<<grid, block, 0, stream>>>(p);
-    } else if (bias) {
-        if (p.shared) residual_norm_backward_kernel<LPR, NV, true, true, true><<<grid, block, 0, stream>>>(p);
-        else residual_norm_backward_kernel<LPR, NV, true, true, false><<<grid, block, 0, stream>>>(p);
-    } else {
-        if (p.shared) residual_norm_backward_kernel<LPR, NV, true, false, true><<<grid, block, 0, stream>>>(p);
-        else residual_norm_backward_kernel<LPR, NV, true, false, false><<<grid, block, 0, stream>>>(p);
-    }
+    // the type that all the rows of a side have, or -1
+    auto common = [](std::initializer_list<const Rows *> rows, int otherwise) {
+        int type = otherwise;
+        for (const Rows *r : rows)
+            if (r->ptr) type = type == otherwise || type == r->dtype ? r->dtype : -2;
+        return type;
+    };
+    const int b = common({&p.block, &p.gate, &p.h, &p.grad_h, &p.grad_block, &p.grad_gate}, -1);
+    const int s = common({&p.residual, &p.x, &p.grad_x, &p.grad_residual}, -1);
+    const int stream_type = s == -1 ? b : s;  // (no rows of that side at all: any will do)
+    if (!vec) launch<LPR, NV, false, -1, -1>(p, q, backward, stream);
+    else if (b == FTC_F32 && stream_type == FTC_F32) launch<LPR, NV, true, FTC_F32, FTC_F32>(p, q, backward, stream);
+    else if (b == FTC_BF16 && stream_type == FTC_BF16) launch<LPR, NV, true, FTC_BF16, FTC_BF16>(p, q, backward, stream);
+    else if (b == FTC_BF16 && stream_type == FTC_F32) launch<LPR, NV, true, FTC_BF16, FTC_F32>(p, q, backward, stream);
+    else launch<LPR, NV, true, -1, -1>(p, q, backward, stream);
 }
 void dispatch(const Args &p, const Plan &q, bool vec, bool backward, hipStream_t stream) {
     if (p.D <= 128) launch<16, 1>(p, q, vec, backward, stream);
     else if (p.D <= 512) launch<64, 1>(p, q, vec, backward, stream);
-    else if (p.D <= 1024) launch<64, 2>(p, q, vec, backward, stream);
+    else if (p.D <= 1024) launch<128, 1>(p, q, vec, backward, stream);
     else if (p.D <= 2048) launch<256, 1>(p, q, vec, backward, stream);
-    else if (p.D <= 4096) launch<256, 2>(p, q, vec, backward, stream);
-    else if (p.D <= 8192) launch<256, 4>(p, q, vec, backward, stream);
+    else if (p.D <= 4096) launch<512, 1>(p, q, vec, backward, stream);
+    else if (p.D <= 8192) launch<512, 2>(p, q, vec, backward, stream);
     else launch<1024, 2>(p, q, vec, backward, stream);
 }
 
@@ -545,7 +595,7 @@ bool wide(const Args &p) {
         if (q && ((uintptr_t)q & 15)) return false;
     return true;
 }
-Plan backward_plan(const Args &p) { return plan_of(p.D, p.rows, p.segment, true); }
+Plan backward_plan(const Args &p) { return plan_of(p.D, p.rows, p.segment, true, full(p)); }
 int64_t sums_floats(const Args &p, const Plan &q) { return q.groups * kSums * p.D; }
 int64_t gate_floats(const Args &p, const Plan &q) { return p.shared ? p.gate_rows * q.parts * p.D : 0; }
 int launched(const char *name) {
@@ -572,7 +622,7 @@ int ftc_residual_norm(const ftc_residual_norm_call *call, const ftc_rows *x, con
     if (p.rows == 0) return FTC_OK;
     p.stats = stats;
     set_segments(&p);
-    const Plan q = plan_of(p.D, p.rows, p.rows, false);
+    const Plan q = plan_of(p.D, p.rows, p.rows, false, false);
     dispatch(p, q, wide(p), false, (hipStream_t)stream);
     return launched("residual_norm_kernel");
 }
