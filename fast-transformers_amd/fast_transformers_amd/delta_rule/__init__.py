@@ -21,7 +21,7 @@ _CPU_CHUNK = 32
 
 
 def _check(queries, keys, values, log_decay, beta, state, what):
-    """Shapes and types, for either device, before anything is launched."""
+    """Shapes and types of a call on CPU tensors."""
     if queries.dim() != values.dim() or keys.shape != queries.shape or \
             queries.shape[0] != values.shape[0] or queries.shape[2:-1] != values.shape[2:-1]:
         raise RuntimeError("%s: expected queries and keys of one shape and values that fit them, got %s, %s and %s"
@@ -51,7 +51,9 @@ def _check(queries, keys, values, log_decay, beta, state, what):
 
 
 class GatedDeltaRule(torch.autograd.Function):
-    """``(out, final_state)`` on the GPU and their gradients, tensors in the ``(N, H, L, X)`` layout."""
+    """``(out, final_state)`` on the GPU and their gradients, tensors in the ``(N, H, L, X)`` layout.  Plain calls run as
+    the same function of the C++ engine (``host/ftc_host.cpp``), which costs the host less; calls that are watched or
+    transformed run this one."""
 
     @staticmethod
     def forward(ctx, queries, keys, values, log_decay, beta, initial_state, lengths, scale, normalize):
@@ -140,20 +142,22 @@ def gated_delta_rule(queries, keys, values, log_decay, beta, initial_state=None,
     before every 64th position (``4 E M / 64`` bytes a position and head)."""
     if queries.dim() != 4:
         raise RuntimeError("gated_delta_rule: expected queries (N, Hk, L, E), got %s" % (tuple(queries.shape),))
-    _check(queries, keys, values, log_decay, beta, initial_state, "gated_delta_rule")
+    if queries.device.type != "cuda":  # (the native code checks for itself)
+        _check(queries, keys, values, log_decay, beta, initial_state, "gated_delta_rule")
     if scale is None:
-        scale = queries.shape[3] ** -0.5
+        scale = max(1, queries.shape[3]) ** -0.5
     if lengths is not None:
         if lengths.shape != values.shape[:1]:
             raise RuntimeError("gated_delta_rule: expected %d lengths, got shape %s"
                                % (values.shape[0], tuple(lengths.shape)))
         lengths = lengths.to(device=queries.device, dtype=torch.int64).contiguous()
-    if queries.device.type == "cpu":
+    if queries.device.type != "cuda":
         out, state = _cpu_rule(queries, keys, values, log_decay, beta, initial_state, lengths, scale, normalize)
     elif torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (queries, keys, values, log_decay, beta, initial_state)):
-        out, state = GatedDeltaRule.apply(queries, keys, values, log_decay, beta, initial_state, lengths, scale,
-                                          normalize)
+        args = (queries, keys, values, log_decay, beta, initial_state, lengths, scale, normalize)
+        out, state = (None if torch.compiler.is_compiling() else _native.host().delta_rule_plain(*args)) or \
+            GatedDeltaRule.apply(*args)
     else:
         out, state, _ = _native.host().delta_rule(queries, keys, values, log_decay, beta, initial_state, lengths, scale,
                                                   normalize, return_state, False)
@@ -166,12 +170,14 @@ def gated_delta_step(queries, keys, values, log_decay, beta, state, *, scale=Non
     along M contiguous).  Returns the outputs ``(N, H, M)`` in the values' type.  Not differentiable; one launch."""
     if queries.dim() != 3:
         raise RuntimeError("gated_delta_step: expected queries (N, Hk, E), got %s" % (tuple(queries.shape),))
-    _check(queries, keys, values, log_decay, beta, state, "gated_delta_step")
+    on_gpu = queries.device.type == "cuda"
+    if not on_gpu:  # (the native code checks for itself)
+        _check(queries, keys, values, log_decay, beta, state, "gated_delta_step")
     if state.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("gated_delta_step: the state is updated in place and cannot be differentiated")
     if scale is None:
-        scale = queries.shape[2] ** -0.5
-    if queries.device.type == "cpu":
+        scale = max(1, queries.shape[2]) ** -0.5
+    if not on_gpu:
         with torch.no_grad():
             out, after = _cpu_rule(*(t.unsqueeze(2) for t in (queries, keys, values, log_decay, beta)), state, None,
                                    scale, normalize)

@@ -48,7 +48,8 @@ def _gate_rows(gate, shape):
 
 
 class ResidualNorm(torch.autograd.Function):
-    """``(x, h)`` on the GPU and their gradients; ``h`` is None without a norm before the next block."""
+    """``(x, h)`` on the GPU and their gradients; ``h`` is None without a norm before the next block.  Plain calls run as
+    the same function of the C++ engine (``host/ftc_host.cpp``); calls that are watched or transformed run this one."""
 
     @staticmethod
     def forward(ctx, block, residual, gate, after_weight, after_bias, before_weight, before_bias, options):
@@ -125,6 +126,10 @@ def residual_norm(block, residual=None, gate=None, *, after=None, before=None, s
     if block.device.type == "cpu":
         return _cpu_residual_norm(block, residual, gate, after, before, activation, scale, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        if not torch.compiler.is_compiling():
+            pair = _native.host().residual_norm_plain(block, residual, gate, *after, *before, activation, scale, eps)
+            if pair is not None:
+                return pair
         return ResidualNorm.apply(block, residual, gate, after[1], after[2], before[1], before[2],
                                   (after[0], before[0], activation, scale, eps))
     x, h, _ = _native.host().residual_norm(block, residual, gate, *after, *before, activation, scale, eps, False)

@@ -844,26 +844,106 @@ std::vector<OptTensor> delta_rule_backward(const Tensor &queries, const Tensor &
     return grads;
 }
 
+// The tensors of one token as the library takes them, a dimension of one position more: (N, H, X) or (N, H)
+ftc_tensor4 delta_token(const Tensor &t, int64_t dims, const char *name, const Tensor &like) {
+    if (t.dim() != dims || t.device() != like.device())
+        error(std::string("gated_delta_step: ") + name + " must be " + std::to_string(dims) +
+              "-dimensional, on the device of the queries");
+    ftc_tensor4 d;
+    d.ptr = t.numel() == 0 ? nullptr : t.data_ptr();
+    if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16) return delta_describe(t, name);  // (which says so)
+    d.dtype = t.scalar_type() == at::kFloat ? FTC_F32 : FTC_BF16;
+    d.size[0] = t.size(0), d.size[1] = t.size(1), d.size[2] = 1, d.size[3] = dims == 3 ? t.size(2) : 1;
+    d.stride[0] = t.stride(0), d.stride[1] = t.stride(1), d.stride[2] = 0, d.stride[3] = dims == 3 ? t.stride(2) : 1;
+    return d;
+}
 // One token: queries, keys (N, Hk, E), values (N, H, M), log_decay, beta (N, H), state (N, H, E, M) in place
 Tensor delta_step(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &log_decay,
                   const Tensor &beta, const Tensor &state, double scale, bool normalize) {
     const at::NoGradGuard no_grad;
-    if (queries.dim() != 3 || keys.dim() != 3 || values.dim() != 3 || log_decay.dim() != 2 || beta.dim() != 2)
-        error("gated_delta_step: expected queries and keys (N, Hk, E), values (N, H, M), log_decay and beta (N, H)");
-    const DeltaTensors t = delta_tensors(queries.unsqueeze(2), keys.unsqueeze(2), values.unsqueeze(2),
-                                         log_decay.unsqueeze(2), beta.unsqueeze(2));
-    const c10::DeviceGuard guard(t.q.device());
-    if (state.size(-1) > 1 && state.stride(-1) != 1)
-        error("gated_delta_step: state is updated in place and must be contiguous in its last dimension");
-    const DeltaState s(state, "state", t.q);
-    const Tensor out = at::empty(values.sizes(), values.options());
-    const ftc_tensor4 dout = describe(out.unsqueeze(2));
-    hipStream_t const stream = c10::hip::getCurrentHIPStream(t.q.device().index()).stream();
+    if (!queries.is_cuda()) error("gated_delta_step: queries are on " + queries.device().str() + ", expected a GPU tensor");
+    // (rows whose values lie apart are copied)
+    auto rows = [](const Tensor &t) { return t.dim() == 3 && t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; };
+    const Tensor q = rows(queries), k = rows(keys), v = rows(values);
+    const ftc_tensor4 dq = delta_token(q, 3, "queries", q), dk = delta_token(k, 3, "keys", q), dv = delta_token(v, 3, "values", q),
+                      dg = delta_token(log_decay, 2, "log_decay", q), db = delta_token(beta, 2, "beta", q);
+    const c10::DeviceGuard guard(q.device());
+    if (state.dim() != 4 || (state.size(3) > 1 && state.stride(3) != 1))
+        error("gated_delta_step: state (N, H, E, M) is updated in place and must be contiguous in its last dimension");
+    const DeltaState s(state, "state", q);
+    const Tensor out = at::empty(v.sizes(), v.options());
+    const ftc_tensor4 dout = delta_token(out, 3, "out", q);
+    hipStream_t const stream = c10::hip::getCurrentHIPStream(q.device().index()).stream();
     const int rc = native([&] {
-        return ftc_gated_delta_step(&t.dq, &t.dk, &t.dv, &t.dg, &t.db, (float)scale, normalize, s.p, &dout, stream);
+        return ftc_gated_delta_step(&dq, &dk, &dv, &dg, &db, (float)scale, normalize, s.p, &dout, stream);
     });
     check(rc, "ftc_gated_delta_step");
     return out;
+}
+
+// The differentiable rule as a function of the C++ engine, as above for the attention: a step of a few short sequences
+// is bound by the host.
+bool plain_or_none(py::handle h, OptTensor &to) {
+    if (h.is_none()) return true;
+    if (!THPVariable_CheckExact(h.ptr()) && !py::isinstance(h, py::module_::import("torch.nn").attr("Parameter"))) return false;
+    const Tensor &t = THPVariable_Unpack(h.ptr());
+    using K = c10::DispatchKey;
+    constexpr c10::DispatchKeySet usual =
+        c10::DispatchKeySet({K::CUDA, K::AutogradCUDA, K::ADInplaceOrView, K::AutocastCUDA});
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.is_inference() || !only(t.key_set(), usual) ||
+        t._fw_grad(0).defined())
+        return false;
+    to = t;
+    return true;
+}
+
+struct DeltaRule : torch::autograd::Function<DeltaRule> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
+                                 const Tensor &b, const OptTensor &s0, const OptTensor &lengths, double scale, bool normalize) {
+        auto [out, state, kept] = delta_rule(q, k, v, g, b, s0, lengths, scale, normalize, true, true);
+        ctx->save_for_backward({q, k, v, g, b, *kept, lengths ? *lengths : Tensor()});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["normalize"] = normalize;
+        ctx->saved_data["state"] = s0.has_value();
+        ctx->set_materialize_grads(false);
+        return {out, *state};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        RECORD_FUNCTION("GatedDeltaRuleBackward", std::vector<c10::IValue>());
+        const variable_list saved = ctx->get_saved_variables();
+        const bool state = ctx->saved_data["state"].toBool();
+        std::vector<bool> needed(6, false);
+        for (int i = 0; i < 5 + state; i++) needed[i] = ctx->needs_input_grad(i);
+        variable_list out(9);
+        if (saved[2].size(2) == 0) {  // (no positions: the state's gradient goes through)
+            for (int i = 0; i < 5; i++)
+                if (needed[i]) out[i] = at::zeros_like(saved[i]);
+            if (needed[5]) out[5] = grads[1];
+            return out;
+        }
+        from_engine([&] {
+            const OptTensor lengths = saved[6].defined() ? OptTensor(saved[6]) : OptTensor();
+            const std::vector<OptTensor> got = delta_rule_backward(
+                saved[0], saved[1], saved[2], saved[3], saved[4], lengths, ctx->saved_data["scale"].toDouble(),
+                ctx->saved_data["normalize"].toBool(), saved[5], grads[0].defined() ? grads[0] : at::zeros_like(saved[2]),
+                grads[1].defined() ? OptTensor(grads[1]) : OptTensor(), needed);
+            for (int i = 0; i < 6; i++)
+                if (got[i]) out[i] = *got[i];
+        });
+        return out;
+    }
+};
+// gated_delta_rule on plain tensors, (out, state); None: not such a call
+py::object delta_rule_plain(py::handle queries, py::handle keys, py::handle values, py::handle log_decay, py::handle beta,
+                            py::handle initial_state, py::handle lengths, double scale, bool normalize) {
+    OptTensor t[7];
+    const py::handle handles[] = {queries, keys, values, log_decay, beta, initial_state, lengths};
+    for (int i = 0; i < 7; i++)
+        if (!plain_or_none(handles[i], t[i]) || (i < 5 && !t[i])) return py::none();
+    if (!nothing_watches()) return py::none();
+    RECORD_FUNCTION("GatedDeltaRule", std::vector<c10::IValue>({*t[0], *t[1], *t[2], *t[3], *t[4]}));
+    const variable_list got = DeltaRule::apply(*t[0], *t[1], *t[2], *t[3], *t[4], t[5], t[6], scale, normalize);
+    return py::make_tuple(got[0], got[1]);
 }
 
 // ---- the norms around a block (norms/__init__.py) ----
@@ -972,6 +1052,54 @@ std::vector<OptTensor> residual_norm_backward(const Tensor &block, const OptTens
     return grads;
 }
 
+struct ResidualNormFunction : torch::autograd::Function<ResidualNormFunction> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &block, const OptTensor &residual, const OptTensor &gate,
+                                 const OptTensor &aw, const OptTensor &ab, const OptTensor &bw, const OptTensor &bb, int64_t after,
+                                 int64_t before, int64_t activation, double scale, double eps) {
+        auto [x, h, stats] = residual_norm(block, residual, gate, (int)after, aw, ab, (int)before, bw, bb, (int)activation, scale,
+                                           eps, true);
+        auto kept = [](const OptTensor &t) { return t ? *t : Tensor(); };
+        ctx->save_for_backward({block, kept(residual), kept(gate), kept(aw), kept(ab), kept(bw), kept(bb), kept(stats)});
+        ctx->saved_data["after"] = after, ctx->saved_data["before"] = before, ctx->saved_data["activation"] = activation;
+        ctx->saved_data["scale"] = scale, ctx->saved_data["eps"] = eps;
+        ctx->set_materialize_grads(false);
+        return h ? variable_list{x, *h} : variable_list{x};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        RECORD_FUNCTION("ResidualNormBackward", std::vector<c10::IValue>());
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list out(12);
+        std::vector<bool> needed(7, false);
+        auto given = [&](int i) { return saved[i].defined() ? OptTensor(saved[i]) : OptTensor(); };
+        for (int i = 0, edge = 0; i < 7; i++)
+            if (saved[i].defined()) needed[i] = ctx->needs_input_grad(edge++);
+        from_engine([&] {
+            auto number = [&](const char *name) { return (int)ctx->saved_data[name].toInt(); };
+            const std::vector<OptTensor> got = residual_norm_backward(
+                saved[0], given(1), given(2), number("after"), given(3), given(4), number("before"), given(5), given(6),
+                number("activation"), ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), given(7),
+                grads[0].defined() ? OptTensor(grads[0]) : OptTensor(),
+                grads.size() > 1 && grads[1].defined() ? OptTensor(grads[1]) : OptTensor(), needed);
+            for (int i = 0; i < 7; i++)
+                if (got[i]) out[i] = *got[i];
+        });
+        return out;
+    }
+};
+// residual_norm on plain tensors that are to be differentiated, (x, h or None); None: not such a call
+py::object residual_norm_plain(py::handle block, py::handle residual, py::handle gate, int64_t after, py::handle aw, py::handle ab,
+                               int64_t before, py::handle bw, py::handle bb, int64_t activation, double scale, double eps) {
+    OptTensor t[7];
+    const py::handle handles[] = {block, residual, gate, aw, ab, bw, bb};
+    for (int i = 0; i < 7; i++)
+        if (!plain_or_none(handles[i], t[i]) || (i < 1 && !t[i])) return py::none();
+    if (!nothing_watches()) return py::none();
+    RECORD_FUNCTION("ResidualNorm", std::vector<c10::IValue>({*t[0]}));
+    const variable_list got = ResidualNormFunction::apply(*t[0], t[1], t[2], t[3], t[4], t[5], t[6], after, before, activation,
+                                                          scale, eps);
+    return py::make_tuple(got[0], got.size() > 1 ? py::cast(got[1]) : py::none());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ftc_host, m) {
@@ -992,6 +1120,8 @@ PYBIND11_MODULE(_ftc_host, m) {
     m.def("delta_rule", &delta_rule);
     m.def("delta_rule_backward", &delta_rule_backward);
     m.def("delta_step", &delta_step);
+    m.def("delta_rule_plain", &delta_rule_plain);
     m.def("residual_norm", &residual_norm);
+    m.def("residual_norm_plain", &residual_norm_plain);
     m.def("residual_norm_backward", &residual_norm_backward);
 }
