@@ -1,0 +1,38 @@
+"""Backward passes of operators that are differentiated once."""
+import functools
+
+import torch
+
+
+class _Again(torch.autograd.Function):
+    """The gradients as they are, as functions of all that they were made of, whose own gradient is an error."""
+
+    @staticmethod
+    def forward(ctx, what, count, *tensors):
+        ctx.what = what
+        return tuple(t.clone() for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(ctx.what + ": the gradients cannot be differentiated again")
+
+
+def differentiated_once(what):
+    """Decorator of a Function's backward: where the gradients are to be differentiated again (``create_graph``), their
+    own gradient is an error, also with respect to saved tensors (which torch's ``once_differentiable`` passes over)."""
+    def wrap(backward):
+        @functools.wraps(backward)
+        def run(ctx, *grads):
+            with torch.no_grad():
+                out = list(backward(ctx, *grads))
+            if torch.is_grad_enabled():
+                there = [i for i, t in enumerate(out) if t is not None]
+                made_of = [t for t in (*ctx.saved_tensors, *grads) if t is not None]
+                for i, t in zip(there, _Again.apply(what, len(there), *(out[i] for i in there), *made_of)):
+                    out[i] = t
+            return tuple(out)
+        return run
+    return wrap
+
+
+__all__ = ["differentiated_once"]

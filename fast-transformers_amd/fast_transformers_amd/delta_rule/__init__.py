@@ -15,6 +15,7 @@ take an implementation of their own in torch operations, which shares nothing wi
 import torch
 
 from .. import _native
+from .._once import differentiated_once
 
 _EPS = 1e-6
 _CPU_CHUNK = 32
@@ -65,7 +66,7 @@ class GatedDeltaRule(torch.autograd.Function):
         return out, state
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @differentiated_once("gated_delta_rule")
     def backward(ctx, grad_out, grad_state):
         queries, keys, values, log_decay, beta, kept, lengths = ctx.saved_tensors
         if values.shape[2] == 0:

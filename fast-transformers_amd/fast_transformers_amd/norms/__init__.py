@@ -9,6 +9,7 @@
 import torch
 
 from .. import _native
+from .._once import differentiated_once
 
 _KINDS = {"rms": 1, "layer": 2}
 _ACTIVATIONS = {None: 0, "sigmoid": 1, "silu": 2}
@@ -62,7 +63,7 @@ class ResidualNorm(torch.autograd.Function):
         return x, h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @differentiated_once("residual_norm")
     def backward(ctx, grad_x, grad_h):
         block, residual, gate, aw, ab, bw, bb, stats = ctx.saved_tensors
         after, before, activation, scale, eps = ctx.options

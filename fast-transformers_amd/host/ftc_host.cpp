@@ -878,6 +878,7 @@ Tensor delta_step(const Tensor &queries, const Tensor &keys, const Tensor &value
         return ftc_gated_delta_step(&dq, &dk, &dv, &dg, &db, (float)scale, normalize, s.p, &dout, stream);
     });
     check(rc, "ftc_gated_delta_step");
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
     return out;
 }
 
@@ -895,6 +896,34 @@ bool plain_or_none(py::handle h, OptTensor &to) {
         return false;
     to = t;
     return true;
+}
+
+// Gradients of an operator that is differentiated once: where the caller will differentiate them again
+// (create_graph) they are functions of all that they were made of, whose own gradient is an error.
+struct Again : torch::autograd::Function<Again> {
+    static variable_list forward(AutogradContext *ctx, const char *what, at::TensorList grads, at::TensorList) {
+        ctx->saved_data["what"] = std::string(what);
+        variable_list same;
+        for (const Tensor &t : grads) same.push_back(t.variable_data());
+        return same;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list) {
+        const std::string what = ctx->saved_data["what"].toStringRef();
+        TORCH_CHECK(false, what, ": the gradients cannot be differentiated again");
+    }
+};
+void once(variable_list &grads, const char *what, const variable_list &saved, const variable_list &above) {
+    if (!at::GradMode::is_enabled()) return;
+    variable_list there, made_of;
+    for (const Tensor &t : grads)
+        if (t.defined()) there.push_back(t);
+    for (const variable_list *list : {&saved, &above})
+        for (const Tensor &t : *list)
+            if (t.defined()) made_of.push_back(t);
+    const variable_list marked = Again::apply(what, at::TensorList(there), at::TensorList(made_of));
+    size_t next = 0;
+    for (Tensor &t : grads)
+        if (t.defined()) t = marked[next++];
 }
 
 struct DeltaRule : torch::autograd::Function<DeltaRule> {
@@ -919,6 +948,7 @@ struct DeltaRule : torch::autograd::Function<DeltaRule> {
             for (int i = 0; i < 5; i++)
                 if (needed[i]) out[i] = at::zeros_like(saved[i]);
             if (needed[5]) out[5] = grads[1];
+            once(out, "gated_delta_rule", saved, grads);
             return out;
         }
         from_engine([&] {
@@ -930,6 +960,7 @@ struct DeltaRule : torch::autograd::Function<DeltaRule> {
             for (int i = 0; i < 6; i++)
                 if (got[i]) out[i] = *got[i];
         });
+        once(out, "gated_delta_rule", saved, grads);
         return out;
     }
 };
@@ -1083,6 +1114,7 @@ struct ResidualNormFunction : torch::autograd::Function<ResidualNormFunction> {
             for (int i = 0; i < 7; i++)
                 if (got[i]) out[i] = *got[i];
         });
+        once(out, "residual_norm", saved, grads);
         return out;
     }
 };
