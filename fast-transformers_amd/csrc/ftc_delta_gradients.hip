@@ -352,37 +352,205 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
     leave(p.gk, dK);
 }
 
-// The gradients of the decays and of beta: a wavefront per chunk and chain, a lane per position
-__global__ __launch_bounds__(256) void delta_decays_kernel(DeltaArgs p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + scalar(threadIdx.x >> 6);
-    if (unit >= (int64_t)p.N * p.H * p.chunks) return;
-    const int chain = scalar((int)(unit / p.chunks));
-    const Where w = where_of(p, chain, (int)(unit - (int64_t)chain * p.chunks));
-    const int64_t l = (int64_t)w.chunk * kRows + lane;
+// The gradients of the decays and of beta: a workgroup per chunk and chain, a lane per position.
+//
+// The sums of dG take back what each pair of positions added to it except where the pair lies astride l; what is left over of the
+// rest is rounding, 2^-22 or so of a position's dO . O.  That is nothing beside what lies astride, unless there are only
+// a few positions or all decays are strong.  Such chunks add up what lies astride itself: pairs up to kBand positions
+// apart, reads of the state by the first 16 positions and writes to it by the last; what is further off has faded
+// by e^{kStrong (kBand + 1)} = 2^-28.  Products on the fp32 matrix instruction, whose operands are values as they are.
+constexpr int kFew = 4;            // positions
+constexpr int kBand = 9;
+constexpr float kStrong = -2.f;    // the weakest log decay (the rounding is then below 2^-19 of what lies astride)
+constexpr int kPairs = kRows * 33;  // pairs (i, j) in LDS, at 33 i + j - 16 (i / 16) + 16
+constexpr int kAstride = kPairs + 4 * (16 + kRows);  // ... and each wavefront's sums of reads and of writes
+
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma4(const f32x4 &a, const f32x4 &b, f32x4 acc) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) acc = mfma4(a[r], b[r], acc);
+    return acc;
+}
+// By the four wavefronts of a workgroup: 16 positions' pairs each, and every fourth block of columns.  Measured (E = M = 128, bf16): a
+// chunk of 1 to 4 positions 26 us, of 64 strong ones 27, 8192 of them 650 (of others the whole kernel takes 4, 4 and 26).
+// VEC: rows can be read 16 bytes at a time (here 8, or 16).
+template <typename T, bool VEC>
+__device__ __forceinline__ void find_astride(const DeltaArgs &p, const Where &w, int wave, int lane, lds_float *mem) {
+    constexpr uint32_t B = Elem<T>::kBytes;
+    const int c = lane & 15, q4 = lane / 16 * 4, valid = scalar(w.valid), tiles = p.E <= 64 ? 4 : 8;
+    const int64_t l0 = (int64_t)w.chunk * kRows;
+    const float *const factors = p.factors + w.at * (kFactors * kRows);
+    const float *const Z = p.z + w.at * p.col_blocks * 1024, *const dE = p.de + w.at * p.col_blocks * 1024;
+    const auto rq = chunk_rows(p.q, w.n, w.hk, l0, B), rk = chunk_rows(p.k, w.n, w.hk, l0, B), ro = chunk_rows(p.go, w.n, w.h, l0, B);
+    const uint32_t sq = (uint32_t)p.q.stride_l * B, sk = (uint32_t)p.k.stride_l * B, so = (uint32_t)p.go.stride_l * B;
+    // four values of a row from column `col`; four rows' values of one column; a result's tile with its rows in the lanes
+    auto along = [&](__amdgpu_buffer_rsrc_t rs, uint32_t stride, int width, int row, int col) {
+        f32x4 x;
+        if (VEC) {
+            const uint32_t at = row < valid && col < width ? (uint32_t)row * stride + (uint32_t)col * B : kOutside;
+            if (B == 4) return __builtin_bit_cast(f32x4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0));
+            const u32x2 two = __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0);
+            return f32x4{__uint_as_float(two.x << 16), __uint_as_float(two.x & 0xffff0000u), __uint_as_float(two.y << 16),
+                         __uint_as_float(two.y & 0xffff0000u)};
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            x[r] = load_one<T>(rs, row < valid && col + r < width ? (uint32_t)row * stride + (uint32_t)(col + r) * B : kOutside);
+        return x;
+    };
+    auto down = [&](int row, int col) {
+        f32x4 x;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            x[r] = load_one<T>(ro, row + r < valid && col < p.M ? (uint32_t)(row + r) * so + (uint32_t)col * B : kOutside);
+        return x;
+    };
+    auto turned = [&](const float *of, int b, int t) {  // row 16 t + c, columns 16 b + q4 ..
+        f32x4 x;
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = of[b * 1024 + t * 256 + c / 4 * 64 + (q4 + r) * 4 + c % 4];
+        return x;
+    };
+    lds_float *const pairs = mem, *const reads = mem + kPairs + wave * (16 + kRows), *const writes = reads + 16;
+
+    if (16 * wave < valid) {
+        const int ti = wave;
+        f32x4 P[2] = {}, R[2] = {}, A[2] = {}, K[2] = {};  // pairs of a position with those of its tile and of the tile before
+        const int before = ti > 0 ? ti - 1 : 0;
+#pragma unroll 4
+        for (int b = 0; b < p.col_blocks; b++) {
+            const f32x4 o = along(ro, so, p.M, 16 * ti + c, 16 * b + q4), e = turned(dE, b, ti);
+            const f32x4 z0 = turned(Z, b, ti), z1 = turned(Z, b, before);
+            P[0] = mfma4(o, z0, P[0]), R[0] = mfma4(e, z0, R[0]), P[1] = mfma4(o, z1, P[1]), R[1] = mfma4(e, z1, R[1]);
+        }
+#pragma unroll 4
+        for (int t = 0; t < tiles; t++) {
+            const f32x4 q = along(rq, sq, p.E, 16 * ti + c, 16 * t + q4), k0 = along(rk, sk, p.E, 16 * ti + c, 16 * t + q4);
+            const f32x4 k1 = along(rk, sk, p.E, 16 * before + c, 16 * t + q4);
+            A[0] = mfma4(q, k0, A[0]), K[0] = mfma4(k0, k0, K[0]), A[1] = mfma4(q, k1, A[1]), K[1] = mfma4(k0, k1, K[1]);
+        }
+        settle();
+#pragma unroll
+        for (int back = 0; back < 2; back++) {
+            const int j = 16 * (ti - back) + c, from = j < 0 ? 0 : j;
+            const float beta = factors[kBeta * kRows + from] * factors[kRk * kRows + from];
+            const float high = factors[kHigh * kRows + from], low = factors[kLow * kRows + from];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int i = 16 * ti + q4 + r;
+                const float fade = expf((factors[kHigh * kRows + i] - high) + (factors[kLow * kRows + i] - low));
+                const float x = factors[kRq * kRows + i] * A[back][r] * P[back][r] - factors[kRk * kRows + i] * K[back][r] * R[back][r];
+                pairs[33 * i + c + 16 - 16 * back] = j >= 0 && j < i && i < valid ? fade * beta * x : 0.f;
+            }
+        }
+    }
+    // what positions 0 to 15 read of the state before the chunk, and what the last ones' two tiles write to the one after
+    const int last = (valid - 1) / 16, but_one = last > 0 ? last - 1 : 0;
+    const f32x4 by_q = *(const f32x4a *)(factors + kReadQ * kRows + q4), by_k = *(const f32x4a *)(factors + kReadK * kRows + q4);
+    const f32x4 by0 = *(const f32x4a *)(factors + kWrite * kRows + 16 * last + q4);
+    const f32x4 by1 = *(const f32x4a *)(factors + kWrite * kRows + 16 * but_one + q4);
+    f32x4 read = {0.f, 0.f, 0.f, 0.f}, write0 = read, write1 = read;
+    for (int b = wave; b < p.col_blocks; b += 4) {
+        const float *const S = p.s + ((w.at * p.col_blocks + b) * tiles * 64 + lane) * 4;
+        const float *const dS = p.ds + ((w.at * p.col_blocks + b) * tiles * 64 + lane) * 4;
+        const f32x4 o = down(q4, 16 * b + c), e = *(const f32x4a *)(dE + b * 1024 + lane * 4);
+        const f32x4 z0 = *(const f32x4a *)(Z + b * 1024 + last * 256 + lane * 4);
+        const f32x4 z1 = *(const f32x4a *)(Z + b * 1024 + but_one * 256 + lane * 4);
+        f32x4 yq = {0.f, 0.f, 0.f, 0.f}, yk = yq, y0 = yq, y1 = yq;
+#pragma unroll 4
+        for (int t = 0; t < tiles; t++) {
+            const f32x4 s = *(const f32x4a *)(S + 256 * t), ds = *(const f32x4a *)(dS + 256 * t);
+            const f32x4 q = along(rq, sq, p.E, c, 16 * t + q4), k = along(rk, sk, p.E, c, 16 * t + q4);
+            const f32x4 k0 = along(rk, sk, p.E, 16 * last + c, 16 * t + q4), k1 = along(rk, sk, p.E, 16 * but_one + c, 16 * t + q4);
+            yq = mfma4(q, s, yq), yk = mfma4(k, s, yk), y0 = mfma4(k0, ds, y0), y1 = mfma4(k1, ds, y1);
+        }
+        settle();
+        read += by_q * yq * o - by_k * yk * e, write0 += by0 * y0 * z0, write1 += by1 * y1 * z1;
+    }
+    auto leave = [&](lds_float *to, int row, const f32x4 &sum) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            float x = row + r < valid ? sum[r] : 0.f;
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) x += __shfl_xor(x, d);
+            if (c == 0) to[row + r] = x;
+        }
+    };
+    writes[lane] = 0.f;
+    leave(reads, q4, read);
+    if (last > 0) leave(writes, 16 * but_one + q4, write1);
+    leave(writes, 16 * last + q4, write0);
+}
+// the lane's position of what find_astride left
+__device__ __forceinline__ float add_astride(const lds_float *mem, int valid, int lane) {
+    const lds_float *const reads = mem + kPairs, *const writes = reads + 16;
+    constexpr int kNext = 16 + kRows;
+    float dg = 0.f, wrote = writes[lane] + writes[kNext + lane] + writes[2 * kNext + lane] + writes[3 * kNext + lane];
+    float read = lane < 16 ? reads[lane] + reads[kNext + lane] + reads[2 * kNext + lane] + reads[3 * kNext + lane] : 0.f;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {  // (reads from here on, writes up to here)
+        const float later = __shfl_down(read, d), earlier = __shfl_up(wrote, d);
+        if (lane + d < 64) read += later;
+        if (lane >= d) wrote += earlier;
+    }
+    wrote = __shfl_up(wrote, 1);
+    dg = read + (lane > 0 ? wrote : 0.f);
+#pragma unroll
+    for (int s = kBand - 1; s >= 0; s--) {
+        const int i = lane + s, at = 33 * i - i / 16 * 16 + 16;
+#pragma unroll
+        for (int back = s + 1; back <= kBand; back++)
+            if (i < valid && i >= back) dg += mem[at + i - back];
+    }
+    return dg;
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256, 4) void delta_decays_kernel(DeltaArgs p) {
+    __shared__ float astride_mem[kAstride], sums_mem[2][4][kRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6);
+    const int chain = scalar((int)(blockIdx.x / (uint32_t)p.chunks));
+    const Where w = where_of(p, chain, (int)(blockIdx.x - (uint32_t)chain * (uint32_t)p.chunks));
     float dg = 0.f, db = 0.f;
     if (w.valid > 0) {
         const float *const sums = p.sums + w.at * kSums, *const factors = p.factors + w.at * (kFactors * kRows);
-        const float z = sums[lane], v = sums[kRows + lane], beta = factors[kBeta * kRows + lane];
-        const float state = p.E <= kSlice ? sums[2 * kRows] : sums[2 * kRows] + sums[2 * kRows + 1];
         float o = 0.f, written = 0.f;
-#pragma unroll 4
-        for (int b = 0; b < p.col_blocks; b++) {
+#pragma unroll 2
+        for (int b = wave; b < p.col_blocks; b += 4) {
             o += p.dots[(w.at * p.col_blocks + b) * kRows + lane];
             written += p.written[(w.at * p.col_blocks + b) * 64 + lane];
         }
-        double sum = (double)o - (double)v, all = written;
+        const float z = sums[lane], v = sums[kRows + lane], beta = factors[kBeta * kRows + lane];
+        const float high = factors[kHigh * kRows + lane], before = __shfl_up(high, 1);
+        const bool apart = w.valid <= kFew || __all(lane == 0 || lane >= w.valid || high - before <= kStrong);
+        sums_mem[0][wave][lane] = o, sums_mem[1][wave][lane] = written;
+        if (apart) find_astride<T, VEC>(p, w, wave, lane, (lds_float *)astride_mem);
+        __syncthreads();
+        if (wave > 0) return;
+        const float state = p.E <= kSlice ? sums[2 * kRows] : sums[2 * kRows] + sums[2 * kRows + 1];
+        const float through = factors[kRise * kRows + kRows - 1] * state;
+        if (apart) {
+            dg = through + add_astride((const lds_float *)astride_mem, w.valid, lane);
+        } else {
+            auto all_of = [&](int i) { return (sums_mem[i][0][lane] + sums_mem[i][1][lane]) + (sums_mem[i][2][lane] + sums_mem[i][3][lane]); };
+            double sum = (double)all_of(0) - (double)v, all = all_of(1);
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-        all += (double)factors[kRise * kRows + kRows - 1] * (double)state;
+            for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+            all += (double)through;
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {  // sums from here to the end
-            const double other = __shfl_down(sum, d);
-            if (lane + d < 64) sum += other;
+            for (int d = 1; d < 64; d *= 2) {  // sums from here to the end
+                const double other = __shfl_down(sum, d);
+                if (lane + d < 64) sum += other;
+            }
+            dg = (float)(sum + all);
         }
-        if (lane < w.valid) dg = (float)(sum + all), db = z / beta;
+        db = z / beta;
     }
-    if (l >= p.L) return;
+    const int64_t l = (int64_t)w.chunk * kRows + lane;
+    if (wave > 0 || l >= p.L) return;
+    if (lane >= w.valid) dg = db = 0.f;
     if (p.gg.ptr) store_from_f32(p.gg.ptr, p.gg.dtype, w.n * p.gg.sn + w.h * p.gg.sh + l * p.gg.sl, dg);
     if (p.gb.ptr) store_from_f32(p.gb.ptr, p.gb.dtype, w.n * p.gb.sn + w.h * p.gb.sh + l * p.gb.sl, db);
 }
@@ -395,8 +563,10 @@ int delta_gradients(const DeltaArgs &p, bool bf16, hipStream_t stream) {
     if (bf16) delta_gradients_kernel<bf16_t><<<grid, kThreads, 0, stream>>>(p);
     else delta_gradients_kernel<float><<<grid, kThreads, 0, stream>>>(p);
     if (p.gg.ptr || p.gb.ptr) {
-        const int64_t units = (int64_t)p.N * p.H * p.chunks;
-        delta_decays_kernel<<<dim3((uint32_t)((units + 3) / 4)), 256, 0, stream>>>(p);
+        const dim3 units((uint32_t)p.N * (uint32_t)p.H * (uint32_t)p.chunks);
+        const bool vec = p.vec_q && p.vec_k && p.vec_go;
+        (bf16 ? vec ? delta_decays_kernel<bf16_t, true> : delta_decays_kernel<bf16_t, false>
+              : vec ? delta_decays_kernel<float, true> : delta_decays_kernel<float, false>)<<<units, 256, 0, stream>>>(p);
     }
     return FTC_OK;
 }

@@ -309,3 +309,25 @@ def test_pieces_of_a_sequence_carry_the_state():
         outs.append(out)
     assert ref.far(state, last) <= ref.FP32
     assert ref.far(torch.cat(outs, 2), whole) <= 2 * ref.BF16
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("L", [1, 2, 4, 5, 66, 130])
+@pytest.mark.parametrize("strength", [None, -2.0, -4.0, -12.0])
+def test_gradients_of_few_or_strong_decays(dtype, L, strength):
+    """They are small beside what the positions pass to and fro: found from what crosses a position, not as a difference."""
+    for E, M, state in ((64, 64, True), (100, 80, False), (37, 51, True)):
+        args = ref.inputs(2, 4, 2, L, E, M, dtype=dtype, device="cuda", seed=L)
+        if strength is not None:
+            args[3].copy_(strength - args[3].abs())
+        if not state:
+            args[5].zero_()
+        go, gs = seeds(args)
+        got, want = results(args, go, gs, normalize=True), wanted(args, go, gs, normalize=True)
+        check(got, want)
+        if not state:  # nothing decays at the first position
+            leaves = [t.detach().requires_grad_(True) for t in args[:5]]
+            o, s = gated_delta_rule(*leaves, normalize=True, return_state=True)
+            (dg,) = torch.autograd.grad([o, s], [leaves[3]], [go, gs])
+            if L <= 4 or strength is not None:
+                assert not dg[:, :, 0].any()
