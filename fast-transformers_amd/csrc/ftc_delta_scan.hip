@@ -1,9 +1,11 @@
 // The gated delta rule's state from chunk to chunk, forward (Z of every position, the state before every chunk and
 // after the last) and backward (the gradient of the state, dE = dV).  Formulas and layouts: ftc_delta_kernel.h.
 //
-// A wavefront owns 16 columns of one chain's state in registers and walks the chunks, alone: what it multiplies with
-// it reads as fragments, straight into the registers of the operands, each one's next chunk requested as soon as this
-// chunk's is used.  A chunk is a chain of dependent products, so what bounds few chains is its latency.
+// A wavefront owns 16 columns of one chain's state in registers and walks the chunks.  What it multiplies with it reads
+// as fragments, each one's next chunk requested as soon as this chunk's is used: where there are few wavefronts straight
+// into the registers of the operands, without a barrier; where there are many, four wavefronts share them in LDS.  A
+// chunk is a chain of dependent products, so what bounds few chains is its latency (1.5 us forward, 2.3 back at
+// 64 x 64, 2.3 and 3.3 at 128 x 128); many are bound by what a compute unit gets from its caches.
 #include "ftc_delta_kernel.h"
 
 namespace ftc {
@@ -33,15 +35,56 @@ __device__ __forceinline__ void store_tiles(float *to, const f32x4 (&x)[4]) {
     for (int t = 0; t < 4; t++) *(f32x4a *)(to + 256 * t) = x[t];
 }
 
-// A left operand's fragment, held or read here
-template <bool HELD, int HA, int PIECES>
-__device__ __forceinline__ void get(const Frag (&held)[HA], const uint16_t *from, int number, int lane, Frag (&a)[PIECES]) {
-    if constexpr (HELD) {
+// A left operand of N fragments: a wavefront that works alone holds it in registers; four that share it keep it in LDS, and
+// each carries every fourth piece of the next chunk's on its way there.
+constexpr int kWaves = 4;
+// Up to two wavefronts a compute unit work alone.  Each of them fetches all its operands, 34 to 64 KB a chunk, and what a
+// compute unit gets from the L2 beside latency is some 20 bytes a clock: more of them wait for each other.  Measured (forward and
+// back, us, alone | shared), bf16, 64 chunks of 128 x 128: 256 wavefronts 165, 227 | 213, 326; 512: 248, 311 | 241, 354; 640:
+// 297, 424 | 245, 359; 1024: 400, 561 | 287, 422.  fp32, 32 chunks of 64 x 64: 256: 85, 115 | 114, 189; 512: 146, 191 | 132, 206;
+// 1024: 259, 380 | 224, 327.  (Three pieces of 128 key columns do not fit the registers: always shared.)
+constexpr int64_t kAlone = 512;
+template <bool SHARE, int N, int PIECES>
+struct Left {
+    static constexpr int kCount = N * PIECES, kPer = SHARE ? (kCount + kWaves - 1) / kWaves : 1;
+    Frag held[SHARE ? 1 : N][SHARE ? 1 : PIECES];
+    u32x4 carried[kPer];
+    __device__ __forceinline__ void load(const uint16_t *from, int wave, int lane) {
+        if constexpr (SHARE) {
 #pragma unroll
-        for (int k = 0; k < PIECES; k++) a[k] = held[k];
-    } else {
-        load_frag(from, number, lane, a);
+            for (int i = 0; i < kPer; i++)
+                if (kCount % kWaves == 0 || i + 1 < kPer || wave + kWaves * i < kCount)
+                    carried[i] = *(const u32x4a *)(from + (wave + kWaves * i) * 512 + 8 * lane);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) load_frag(from, i, lane, held[i]);
+        }
     }
+    __device__ __forceinline__ void put(lds_char *to, int wave, int lane) const {
+        if constexpr (SHARE)
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+                if (kCount % kWaves == 0 || i + 1 < kPer || wave + kWaves * i < kCount)
+                    *(__attribute__((address_space(3))) u32x4a *)(to + (wave + kWaves * i) * 1024 + 16 * lane) = carried[i];
+    }
+    __device__ __forceinline__ void get(const lds_char *from, int number, int lane, Frag (&a)[PIECES]) const {
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) {
+            if constexpr (SHARE) {
+                const u32x4 x = *(const __attribute__((address_space(3))) u32x4a *)(from + (number * PIECES + k) * 1024 + 16 * lane);
+                a[k] = Frag{{x.x, x.y, x.z, x.w}};
+            } else {
+                a[k] = held[number][k];
+            }
+        }
+    }
+};
+// What was written to LDS is there for all four, and what was read may be overwritten
+template <bool SHARE>
+__device__ __forceinline__ void meet() {
+    phase();
+    if (SHARE) mfma::wg_barrier();
+    phase();
 }
 
 // Workgroups go to the eight dies in turn: those of one chain to the same, whose cache they share
@@ -139,13 +182,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t factor_rows(const DeltaArgs &p
         4 * kFactors * kRows, mfma::kRsrcFlags);
 }
 
-template <typename T, int KE, bool VEC>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_kernel(DeltaArgs p) {
-    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512;
-    const int lane = threadIdx.x, c = lane & 15, q = lane >> 4;
-    int chain, block;
-    if (!place(p, p.col_blocks, chain, block)) return;
-    const int col = kCols * block + c;
+template <typename T, int KE, bool VEC, bool SHARE>
+__global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_kernel(DeltaArgs p) {
+    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512, W = SHARE ? kWaves : 1;
+    const int lane = threadIdx.x & 63, wave = SHARE ? scalar(threadIdx.x >> 6) : 0, c = lane & 15, q = lane >> 4;
+    int chain, group;
+    if (!place(p, (p.col_blocks + W - 1) / W, chain, group)) return;
+    const int block = scalar(group * W + wave), col = kCols * block + c;
+    const bool here = !SHARE || block < p.col_blocks;  // (the others carry operands, and compute with zeros)
     const Where w = where_of(p, chain, 0);
     const int chunks = chunks_of(w.len);
 
@@ -161,22 +205,18 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         }
 
     const uint32_t v_row = (uint32_t)p.v.stride_l * Elem<T>::kBytes;
-    // (three pieces of wide rows would not fit: read when they are used)
-    constexpr bool kHold = KE * PIECES <= 6;
-    Frag kr[4 * KE][kHold ? PIECES : 1], kc[4 * KE][kHold ? PIECES : 1], tf[kTFrags][3];
     using Tile = ColumnTile<T, VEC>;
-    __shared__ __align__(16) char v_mem[Tile::kTile];
-    __shared__ __align__(16) float f_mem[2][kRows];
-    lds_char *const vp = (lds_char *)v_mem;
-    lds_float *const fp = (lds_float *)f_mem;
+    __shared__ __align__(16) char v_mem[W][Tile::kTile];
+    __shared__ __align__(16) float f_mem[W][2][kRows];
+    __shared__ __align__(16) char kr_mem[SHARE ? 2 * kKeys : 16], kc_mem[SHARE ? 2 * kKeys : 16], t_mem[SHARE ? kTFrags * 3072 : 16];
+    lds_char *const vp = (lds_char *)v_mem[wave], *const krp = (lds_char *)kr_mem, *const kcp = (lds_char *)kc_mem, *const tp = (lds_char *)t_mem;
+    lds_float *const fp = (lds_float *)f_mem[wave];
+    Left<SHARE, 4 * KE, PIECES> kr, kc;
+    Left<SHARE, kTFrags, 3> tf;
     Tile V;
     FactorRow in, out;
     float last;
-    auto load_in = [&](int chunk) {
-        if constexpr (kHold)
-#pragma unroll
-            for (int i = 0; i < 4 * KE; i++) load_frag(p.kr + (w.key_at + chunk) * kKeys, i, lane, kr[i]);
-    };
+    auto load_in = [&](int chunk) { kr.load(p.kr + (w.key_at + chunk) * kKeys, wave, lane); };
     auto load_rows = [&](int chunk) {
         V.load(chunk_rows(p.v, w.n, w.h, (int64_t)chunk * kRows, Elem<T>::kBytes), v_row, kCols * block, p.M,
                min(kRows, w.len - chunk * kRows), lane);
@@ -184,22 +224,19 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         in.load(rs, kReadK, lane), out.load(rs, kWrite, lane);
         last = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (kRows * kRise + kRows - 1), 0, 0));
     };
-    auto load_t = [&](int chunk) {
-#pragma unroll
-        for (int i = 0; i < kTFrags; i++) load_frag(p.t + (w.at + chunk) * (kTFrags * 3 * 512), i, lane, tf[i]);
-    };
-    auto load_out = [&](int chunk) {
-        if constexpr (kHold)
-#pragma unroll
-            for (int i = 0; i < 4 * KE; i++) load_frag(p.kc + (w.key_at + chunk) * kKeys, i, lane, kc[i]);
-    };
-    if (chunks > 0) load_rows(0), load_in(0), load_t(0), load_out(0);
+    auto load_t = [&](int chunk) { tf.load(p.t + (w.at + chunk) * (kTFrags * 3 * 512), wave, lane); };
+    auto load_out = [&](int chunk) { kc.load(p.kc + (w.key_at + chunk) * kKeys, wave, lane); };
+    if (chunks > 0) {
+        load_rows(0), load_in(0), load_t(0), load_out(0);
+        if (SHARE) kr.put(krp, wave, lane), load_in(min(1, chunks - 1));
+    }
     for (int chunk = 0; chunk < chunks; chunk++) {
         const int64_t at = (w.at + chunk) * p.col_blocks + block;
         const int next = min(chunk + 1, chunks - 1);
         V.put(vp, lane), in.put(fp, lane), out.put(fp + kRows, lane);
         const float fade = last;
-        {
+        if (SHARE) meet<SHARE>();
+        if (here) {
             float *const to = p.s + at * (ET * 256) + 4 * lane;
 #pragma unroll
             for (int t = 0; t < ET; t++) *(f32x4a *)(to + 256 * t) = S[t];
@@ -211,51 +248,55 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
             values[t] = V.values(vp, t, c, q);
             read[t] = FactorRow::rows(fp, t, q), write[t] = FactorRow::rows(fp + kRows, t, q);
         }
-        phase();
+        if (!SHARE) phase();
 #pragma unroll
         for (int s = 0; s < KE; s++) {
             Frag sf[3], a[4][PIECES];
-            cut(S[2 * s], S[2 * s + 1], sf);
 #pragma unroll
-            for (int t = 0; t < 4; t++) get<kHold>(kr[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, a[t]);
+            for (int t = 0; t < 4; t++) kr.get(krp, t * KE + s, lane, a[t]);
+            cut(S[2 * s], S[2 * s + 1], sf);
             products<0>(a, sf, P);
         }
 #pragma unroll
         for (int t = 0; t < 4; t++) P[t] = values[t] - read[t] * P[t];
         phase();
-        load_rows(next), load_in(next);
-        phase();
+        tf.put(tp, wave, lane);
+        if (SHARE) load_t(next), load_rows(next);
+        else load_rows(next), load_in(next);
+        meet<SHARE>();
         // Z = T E (tiles above the diagonal are zero)
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag ef[3], a[4][3];
+#pragma unroll
+            for (int t = 2 * s; t < 4; t++) tf.get(tp, t_number(t, s), lane, a[t]);
             cut(P[2 * s], P[2 * s + 1], ef);
-#pragma unroll
-            for (int t = 2 * s; t < 4; t++)
-#pragma unroll
-                for (int k = 0; k < 3; k++) a[t][k] = tf[t_number(t, s)][k];
             if (s == 0) products<0>(a, ef, Z);
             else products<2>(a, ef, Z);
         }
-        store_tiles(p.z + at * (4 * 256) + 4 * lane, Z);
+        if (SHARE) settle();
+        if (here) store_tiles(p.z + at * (4 * 256) + 4 * lane, Z);
         // S <- e^{G_64} S + K^T diag(rk beta e^{G_64 - G}) Z
 #pragma unroll
         for (int t = 0; t < 4; t++) Z[t] *= write[t];
 #pragma unroll
         for (int t = 0; t < ET; t++) S[t] *= fade;
         phase();
-        load_t(next);
-        phase();
+        kc.put(kcp, wave, lane);
+        if (SHARE) load_out(next);
+        else load_t(next);
+        meet<SHARE>();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag uf[3], a[ET][PIECES];
-            cut(Z[2 * s], Z[2 * s + 1], uf);
 #pragma unroll
-            for (int t = 0; t < ET; t++) get<kHold>(kc[2 * t + s], p.kc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, a[t]);
+            for (int t = 0; t < ET; t++) kc.get(kcp, 2 * t + s, lane, a[t]);
+            cut(Z[2 * s], Z[2 * s + 1], uf);
             products<0>(a, uf, S);
         }
         phase();
-        load_out(next);
+        if (SHARE) kr.put(krp, wave, lane), load_in(min(chunk + 2, chunks - 1));
+        else load_out(next);
         phase();
     }
     if (p.final_.ptr)
@@ -273,13 +314,14 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 //   dU = A^T dO + diag(rk e^{G_64 - G}) K dS,   dE = T^T diag(beta) dU,
 //   dS <- e^{G_64} dS + Q^T diag(rq e^G) dO - K^T diag(rk e^G) dE
 // and what the chunk's keys write of <state, its gradient>: the sum of beta Z . diag(rk e^{G_64 - G}) K dS.
-template <typename T, int KE, bool VEC>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_back_kernel(DeltaArgs p) {
-    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512;
-    const int lane = threadIdx.x, c = lane & 15, q = lane >> 4;
-    int chain, block;
-    if (!place(p, p.col_blocks, chain, block)) return;
-    const int col = kCols * block + c;
+template <typename T, int KE, bool VEC, bool SHARE>
+__global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_back_kernel(DeltaArgs p) {
+    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512, W = SHARE ? kWaves : 1;
+    const int lane = threadIdx.x & 63, wave = SHARE ? scalar(threadIdx.x >> 6) : 0, c = lane & 15, q = lane >> 4;
+    int chain, group;
+    if (!place(p, (p.col_blocks + W - 1) / W, chain, group)) return;
+    const int block = scalar(group * W + wave), col = kCols * block + c;
+    const bool here = !SHARE || block < p.col_blocks;
     const Where w = where_of(p, chain, 0);
     const int chunks = chunks_of(w.len);
 
@@ -296,25 +338,26 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         }
 
     const uint32_t g_row = (uint32_t)p.go.stride_l * Elem<T>::kBytes, gv_row = (uint32_t)p.gv.stride_l * Elem<T>::kBytes;
-    constexpr bool kHold = KE * PIECES <= 6;
-    // (three pieces: the columns of q where the rows of k were, requested while T is used)
-    constexpr bool kShare = KE * PIECES > 4;
-    Frag kr[4 * KE][kHold ? PIECES : 1], own_q[kShare ? 1 : 4 * KE][kHold ? PIECES : 1], kc[4 * KE][kHold ? PIECES : 1], tf[kTFrags][3];
+    // (three pieces of two k-steps held: the columns of q where the rows of k were, requested while T is used)
+    constexpr bool kTurns = !SHARE && KE * PIECES > 4;
     using Tile = ColumnTile<T, VEC>;
-    __shared__ __align__(16) char g_mem[Tile::kTile], through_mem[Tile::kTile];
-    __shared__ __align__(16) float f_mem[4][kRows];
-    lds_char *const gp = (lds_char *)g_mem, *const through = (lds_char *)through_mem;
-    lds_float *const fp = (lds_float *)f_mem;
+    __shared__ __align__(16) char g_mem[W][Tile::kTile], through_mem[W][SHARE ? 16 : Tile::kTile];
+    __shared__ __align__(16) float f_mem[W][4][kRows];
+    // (shared: the rows of k and the columns of q take turns in one place)
+    __shared__ __align__(16) char in_mem[SHARE ? 2 * kKeys : 16], kc_mem[SHARE ? 2 * kKeys : 16], t_mem[SHARE ? kTFrags * 3072 : 16];
+    lds_char *const inp = (lds_char *)in_mem, *const kcp = (lds_char *)kc_mem, *const tp = (lds_char *)t_mem;
+    lds_char *const gp = (lds_char *)g_mem[wave], *const through = SHARE ? gp : (lds_char *)through_mem[wave];
+    lds_float *const fp = (lds_float *)f_mem[wave];
+    using Keys = Left<SHARE, 4 * KE, PIECES>;
+    Keys kr, own_q, kc;
+    Keys &qc = kTurns ? kr : own_q;
+    Left<SHARE, kTFrags, 3> tf;
     Tile Gr;
     FactorRow write, beta, read_q, read_k;
     f32x4 Y[4], Z[4];
     float last;
-    auto tiles = [&](int chunk) { return ((w.at + chunk) * p.col_blocks + block) * (4 * 256) + 4 * lane; };
-    auto load_in = [&](int chunk) {
-        if constexpr (kHold)
-#pragma unroll
-            for (int i = 0; i < 4 * KE; i++) load_frag(p.kr + (w.key_at + chunk) * kKeys, i, lane, kr[i]);
-    };
+    auto tiles = [&](int chunk) { return ((w.at + chunk) * p.col_blocks + (here ? block : 0)) * (4 * 256) + 4 * lane; };
+    auto load_in = [&](int chunk) { kr.load(p.kr + (w.key_at + chunk) * kKeys, wave, lane); };
     auto load_rows = [&](int chunk) {
         const __amdgpu_buffer_rsrc_t rs = factor_rows(p, w.at + chunk);
         write.load(rs, kWrite, lane), beta.load(rs, kBeta, lane), read_q.load(rs, kReadQ, lane), read_k.load(rs, kReadK, lane);
@@ -322,34 +365,27 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         load_tiles(p.de + tiles(chunk), Y);
         load_tiles(p.z + tiles(chunk), Z);
     };
-    auto load_t = [&](int chunk) {
-#pragma unroll
-        for (int i = 0; i < kTFrags; i++) load_frag(p.tt + (w.at + chunk) * (kTFrags * 3 * 512), i, lane, tf[i]);
+    auto load_t = [&](int chunk) { tf.load(p.tt + (w.at + chunk) * (kTFrags * 3 * 512), wave, lane); };
+    auto load_g = [&](int chunk) {
         Gr.load(chunk_rows(p.go, w.n, w.h, (int64_t)chunk * kRows, Elem<T>::kBytes), g_row, kCols * block, p.M,
                 min(kRows, w.len - chunk * kRows), lane);
     };
-    auto load_q = [&](int chunk) {
-        if constexpr (kHold)
-#pragma unroll
-            for (int i = 0; i < 4 * KE; i++) {
-                if constexpr (kShare) load_frag(p.qc + (w.key_at + chunk) * kKeys, i, lane, kr[i]);
-                else load_frag(p.qc + (w.key_at + chunk) * kKeys, i, lane, own_q[i]);
-            }
-    };
-    auto load_out = [&](int chunk) {
-        if constexpr (kHold)
-#pragma unroll
-            for (int i = 0; i < 4 * KE; i++) load_frag(p.kc + (w.key_at + chunk) * kKeys, i, lane, kc[i]);
-    };
-    if (!kShare && chunks > 0) load_q(chunks - 1);
-    if (chunks > 0) load_in(chunks - 1), load_rows(chunks - 1), load_t(chunks - 1), load_out(chunks - 1);
+    auto load_q = [&](int chunk) { qc.load(p.qc + (w.key_at + chunk) * kKeys, wave, lane); };
+    auto load_out = [&](int chunk) { kc.load(p.kc + (w.key_at + chunk) * kKeys, wave, lane); };
+    if (chunks > 0) {
+        const int first = chunks - 1;
+        if (!kTurns) load_q(first);
+        load_in(first), load_rows(first), load_t(first), load_g(first), load_out(first);
+        if (SHARE) kr.put(inp, wave, lane), load_in(max(first - 1, 0));
+    }
     for (int chunk = chunks - 1; chunk >= 0; chunk--) {
         const int64_t at = (w.at + chunk) * p.col_blocks + block;
         const int next = max(chunk - 1, 0);
         write.put(fp, lane), beta.put(fp + kRows, lane);
         read_q.put(fp + 2 * kRows, lane), read_k.put(fp + 3 * kRows, lane);
         const float fade = last;
-        {
+        if (SHARE) meet<SHARE>();
+        if (here) {
             float *const to = p.ds + at * (ET * 256) + 4 * lane;
 #pragma unroll
             for (int t = 0; t < ET; t++) *(f32x4a *)(to + 256 * t) = S[t];
@@ -357,13 +393,13 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         f32x4 P[4] = {}, D[4], G[4], write_rows[4], beta_rows[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) write_rows[t] = FactorRow::rows(fp, t, q), beta_rows[t] = FactorRow::rows(fp + kRows, t, q);
-        phase();
+        if (!SHARE) phase();
 #pragma unroll
         for (int s = 0; s < KE; s++) {
             Frag sf[3], a[4][PIECES];
-            cut(S[2 * s], S[2 * s + 1], sf);
 #pragma unroll
-            for (int t = 0; t < 4; t++) get<kHold>(kr[t * KE + s], p.kr + (w.key_at + chunk) * kKeys, t * KE + s, lane, a[t]);
+            for (int t = 0; t < 4; t++) kr.get(inp, t * KE + s, lane, a[t]);
+            cut(S[2 * s], S[2 * s + 1], sf);
             products<0>(a, sf, P);
         }
         // diag(beta) dU
@@ -375,34 +411,37 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
             written += Z[t] * P[t];
             P[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        p.written[at * 64 + lane] = (written[0] + written[1]) + (written[2] + written[3]);
+        if (SHARE) settle();
+        if (here) p.written[at * 64 + lane] = (written[0] + written[1]) + (written[2] + written[3]);
         phase();
-        if constexpr (kShare) load_q(chunk), load_rows(next);
+        tf.put(tp, wave, lane);
+        if (SHARE) load_t(next), load_rows(next);
+        else if (kTurns) load_q(chunk), load_rows(next);
         else load_in(next), load_rows(next);
-        phase();
-        // dE = T^T diag(beta) dU
+        if (!SHARE) phase();
         Gr.put(gp, lane);
+        if (SHARE) meet<SHARE>();
+        // dE = T^T diag(beta) dU
         f32x4 read_q_rows[4], read_k_rows[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             G[t] = Gr.values(gp, t, c, q);
             read_q_rows[t] = FactorRow::rows(fp + 2 * kRows, t, q), read_k_rows[t] = FactorRow::rows(fp + 3 * kRows, t, q);
         }
-        phase();
+        if (!SHARE) phase();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag df[3], a[4][3];
             f32x4(&head)[2] = *(f32x4(*)[2])&P[0];
+#pragma unroll
+            for (int t = 0; t < 2 * s + 2; t++) tf.get(tp, tt_number(t, s), lane, a[t]);
             cut(D[2 * s], D[2 * s + 1], df);
-#pragma unroll
-            for (int t = 0; t < 2 * s + 2; t++)
-#pragma unroll
-                for (int k = 0; k < 3; k++) a[t][k] = tf[tt_number(t, s)][k];
             if (s == 0) products<0>(*(Frag(*)[2][3])&a, df, head);
             else products<0>(a, df, P);
         }
-        store_tiles(p.de + at * (4 * 256) + 4 * lane, P);
-        if (p.gv.ptr)
+        if (SHARE) phase(), qc.put(inp, wave, lane), load_q(next), load_g(next), settle();
+        if (here) store_tiles(p.de + at * (4 * 256) + 4 * lane, P);
+        if (here && p.gv.ptr)
             Tile::store(chunk_rows(Operand{p.gv.ptr, p.gv.stride_n, p.gv.stride_h, p.gv.stride_l, 0, 0}, w.n, w.h,
                                    (int64_t)chunk * kRows, Elem<T>::kBytes),
                         gv_row, kCols * block, p.M, min(kRows, w.len - chunk * kRows), lane, P, through);
@@ -415,31 +454,33 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 #pragma unroll
         for (int t = 0; t < ET; t++) S[t] *= fade;
         phase();
-        load_t(next);
-        phase();
+        if (!SHARE) load_t(next), load_g(next);
+        meet<SHARE>();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag of[3], a[ET][PIECES];
-            cut(G[2 * s], G[2 * s + 1], of);
 #pragma unroll
-            for (int t = 0; t < ET; t++)
-                get<kHold>(kShare ? kr[2 * t + s] : own_q[kShare ? 0 : 2 * t + s], p.qc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, a[t]);
+            for (int t = 0; t < ET; t++) qc.get(inp, 2 * t + s, lane, a[t]);
+            cut(G[2 * s], G[2 * s + 1], of);
             products<0>(a, of, S);
         }
         phase();
-        if constexpr (kShare) load_in(next);
+        kc.put(kcp, wave, lane);
+        if (SHARE) load_out(next);
+        else if (kTurns) load_in(next);
         else load_q(next);
-        phase();
+        meet<SHARE>();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag ef[3], a[ET][PIECES];
-            cut(P[2 * s], P[2 * s + 1], ef);
 #pragma unroll
-            for (int t = 0; t < ET; t++) get<kHold>(kc[2 * t + s], p.kc + (w.key_at + chunk) * kKeys, 2 * t + s, lane, a[t]);
+            for (int t = 0; t < ET; t++) kc.get(kcp, 2 * t + s, lane, a[t]);
+            cut(P[2 * s], P[2 * s + 1], ef);
             products<0>(a, ef, S);
         }
         phase();
-        load_out(next);
+        if (SHARE) kr.put(inp, wave, lane), load_in(max(chunk - 2, 0));
+        else load_out(next);
         phase();
     }
     if (p.grad_initial.ptr)
@@ -458,11 +499,18 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
             store_from_f32(p.gv.ptr, p.gv.dtype, w.n * p.gv.stride_n + w.h * p.gv.stride_h + l * p.gv.stride_l + col, 0.f);
 }
 
+template <typename T, int KE, bool VEC, bool SHARE>
+void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
+    constexpr uint32_t W = SHARE ? kWaves : 1;
+    const dim3 grid(((uint32_t)p.N * (uint32_t)p.H + 7) / 8 * 8 * (((uint32_t)p.col_blocks + W - 1) / W));
+    if (back) delta_scan_back_kernel<T, KE, VEC, SHARE><<<grid, 64 * W, 0, stream>>>(p);
+    else delta_scan_kernel<T, KE, VEC, SHARE><<<grid, 64 * W, 0, stream>>>(p);
+}
 template <typename T, int KE, bool VEC>
 void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
-    const dim3 grid(((uint32_t)p.N * (uint32_t)p.H + 7) / 8 * 8 * (uint32_t)p.col_blocks);
-    if (back) delta_scan_back_kernel<T, KE, VEC><<<grid, 64, 0, stream>>>(p);
-    else delta_scan_kernel<T, KE, VEC><<<grid, 64, 0, stream>>>(p);
+    const bool share = (int64_t)p.N * p.H * p.col_blocks > kAlone;
+    if (Elem<T>::kPieces * KE > 6 || share) launch<T, KE, VEC, true>(p, back, stream);
+    else if constexpr (Elem<T>::kPieces * KE <= 6) launch<T, KE, VEC, false>(p, back, stream);
 }
 template <typename T, int KE>
 void launch(const DeltaArgs &p, bool vec, bool back, hipStream_t stream) {
