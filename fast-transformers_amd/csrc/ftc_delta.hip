@@ -25,10 +25,26 @@ struct Sizes {
     int64_t keys() const { return N * Hk * chunks() * 2 * tiles() * pieces() * 256; }
     int64_t s() const { return units() * col_blocks() * tiles() * 256; }
     int64_t z() const { return units() * col_blocks() * 4 * 256; }
+    // Few chains are walked in segments, side by side: first what each makes of its first state (a linear map and what
+    // it adds), then the walk itself.  Twice the products, so three segments at least; more while there are up to two
+    // wavefronts a compute unit and the maps of the segments before (1.2 us each at 64 key columns, 4.5 at 128) are
+    // applied in less time than it saves.
+    int64_t segments() const {
+        const int64_t waves = N * H * col_blocks(), most = waves > 0 ? 512 / waves : 1;
+        int64_t n = 1;
+        while (n < most && 4 * (n + 1) <= chunks() && (n + 1) * (n + 1) <= chunks() * (tiles() == 4 ? 3 : 1)) n++;
+        if (n < 3) return 1;
+        return (chunks() + segment_chunks(n) - 1) / segment_chunks(n);
+    }
+    int64_t segment_chunks(int64_t n) const { return (chunks() + n - 1) / n; }
+    int64_t segment_states() const {
+        const int64_t n = segments();
+        return n == 1 ? 0 : N * H * n * (col_blocks() + (E + kCols - 1) / kCols) * tiles() * 256;
+    }
     int64_t dots() const { return units() * col_blocks() * kRows; }
-    // T, keys, factors, states, Z; to be kept for the backward also the transpose of T and O
-    int64_t forward(bool keep) const { return 4 * (factors() + (keep ? 2 : 1) * (t() + z()) + 2 * keys() + s()); }
-    int64_t backward() const { return 4 * (s() + z() + 2 * dots() + units() * kSums + keys()); }
+    // T, keys, factors, states, Z, segments; to be kept for the backward also the transpose of T and O
+    int64_t forward(bool keep) const { return 4 * (factors() + (keep ? 2 : 1) * (t() + z()) + 2 * keys() + s() + segment_states()); }
+    int64_t backward() const { return 4 * (s() + z() + 2 * dots() + units() * kSums + keys() + segment_states()); }
 };
 
 int check_sizes(const Sizes &s) {
@@ -107,6 +123,7 @@ int read_inputs(const ftc_tensor4 *q, const ftc_tensor4 *k, const ftc_tensor4 *v
     p->N = (int32_t)s->N, p->H = (int32_t)s->H, p->Hk = (int32_t)s->Hk, p->L = (int32_t)s->L;
     p->E = (int32_t)s->E, p->M = (int32_t)s->M;
     p->chunks = (int32_t)s->chunks(), p->col_blocks = (int32_t)s->col_blocks();
+    p->segments = (int32_t)s->segments(), p->seg_chunks = (int32_t)s->segment_chunks(p->segments);
     p->vec_q = reads_wide(p->q), p->vec_k = reads_wide(p->k), p->vec_v = reads_wide(p->v);
     return FTC_OK;
 }
@@ -119,6 +136,7 @@ void place_forward(const Sizes &s, void *at, bool keep, DeltaArgs *p) {
     };
     p->factors = take(s.factors()), p->s = take(s.s()), p->z = take(s.z());
     p->t = (uint16_t *)take(s.t()), p->kr = (uint16_t *)take(s.keys()), p->kc = (uint16_t *)take(s.keys());
+    p->seg = take(s.segment_states());
     if (keep) p->o = take(s.z()), p->tt = (uint16_t *)take(s.t());
 }
 int launched(const char *name) {
@@ -228,7 +246,8 @@ int ftc_gated_delta_rule_backward(const ftc_tensor4 *queries, const ftc_tensor4 
     place_forward(s, (void *)kept, true, &p);
     p.ds = (float *)workspace, p.de = p.ds + s.s(), p.dots = p.de + s.z(), p.written = p.dots + s.dots();
     p.sums = p.written + s.dots();
-    p.qc = (uint16_t *)(p.sums + s.units() * kSums);
+    p.seg = p.sums + s.units() * kSums;
+    p.qc = (uint16_t *)(p.seg + s.segment_states());
     p.go = as_operand(grad_out), p.vec_go = reads_wide(p.go);
     p.gq = rows_out(grad_queries), p.gk = rows_out(grad_keys), p.gv = rows_out(grad_values);
     p.vec_gv = !grad_values || reads_wide(as_operand(grad_values));

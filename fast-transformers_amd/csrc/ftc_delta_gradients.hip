@@ -365,14 +365,6 @@ constexpr float kStrong = -2.f;    // the weakest log decay (the rounding is the
 constexpr int kPairs = kRows * 33;  // pairs (i, j) in LDS, at 33 i + j - 16 (i / 16) + 16
 constexpr int kAstride = kPairs + 4 * (16 + kRows);  // ... and each wavefront's sums of reads and of writes
 
-__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 acc) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma4(const f32x4 &a, const f32x4 &b, f32x4 acc) {
-#pragma unroll
-    for (int r = 0; r < 4; r++) acc = mfma4(a[r], b[r], acc);
-    return acc;
-}
 // By the four wavefronts of a workgroup: 16 positions' pairs each, and every fourth block of columns.  Measured (E = M = 128, bf16): a
 // chunk of 1 to 4 positions 26 us, of 64 strong ones 27, 8192 of them 650 (of others the whole kernel takes 4, 4 and 26).
 // VEC: rows can be read 16 bytes at a time (here 8, or 16).

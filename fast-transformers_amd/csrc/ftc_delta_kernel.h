@@ -98,6 +98,9 @@ struct DeltaArgs {
     float *de;               // A^T dO, then dE, as z
     float *dots;             // dO . O of every position, column block by column block: [chain][chunk][col block][64]
     float *sums;             // dE . Z and dE . V of every position, two shares of <S, dS>: [chain][chunk][kSums]
+    // few chains: their chunks in segments of seg_chunks (ftc_delta_scan.hip)
+    int32_t segments, seg_chunks;
+    float *seg;              // what a segment makes of its first state: [chain][segment][col blocks + key blocks][2 KE][64][4]
     float *written;          // shares of what a chunk's keys write of <state, its gradient>: the same, [64 lanes]
 };
 
@@ -130,6 +133,15 @@ struct Plane {
 __device__ __forceinline__ f32x4 mfma16(const Frag &a, const Frag &b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mfma::bf16x8, a),
                                                    __builtin_bit_cast(mfma::bf16x8, b), c, 0, 0, 0);
+}
+// fp32 values as they are: lane's a is row c of column q, b row q of column c
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma4(const f32x4 &a, const f32x4 &b, f32x4 acc) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) acc = mfma4(a[r], b[r], acc);
+    return acc;
 }
 // acc += A B over the piece products of order <= 2 (two pieces at most: <= 1), smallest first
 template <int NA, int NB>

@@ -94,6 +94,106 @@ __device__ __forceinline__ bool place(const DeltaArgs &p, int groups, int &chain
     return chain < p.N * p.H;
 }
 
+// ---- segments ----
+// Few chains are walked in segments.  A first launch (MAP) walks all but the last: the first one as it is, the others from
+// a state of zeros and, as further columns without rows of their own, from the identity: what they add, and the
+// linear map that they are.  The second launch makes its segment's first state of those before it, and walks it.  (In
+// reverse the same from the other end.)
+template <bool MAP>
+__host__ __device__ __forceinline__ int blocks_of(const DeltaArgs &p) {
+    return p.col_blocks + (MAP ? (p.E + kCols - 1) / kCols : 0);
+}
+struct Part {
+    int chain, segment, block, first, end;
+    bool none, here, map, last;  // here: its tiles are stored; map: columns of the identity; last: of the segments, on the way
+};
+template <int W, bool MAP, bool BACK>
+__device__ __forceinline__ Part part_of(const DeltaArgs &p, int wave) {
+    Part a;
+    int group;
+    const int per = (blocks_of<MAP>(p) + W - 1) / W, count = p.segments > 1 ? p.segments - 1 : 1;
+    a.none = !place(p, per * count, a.chain, group);
+    const int turn = group / per + (!MAP && p.segments > 1 ? 1 : 0);  // on the way
+    const int block0 = (group - group / per * per) * W;
+    a.segment = scalar(BACK ? p.segments - 1 - turn : turn), a.block = scalar(block0 + wave);
+    a.last = turn == p.segments - 1;
+    a.none = a.none || (MAP && turn == 0 && block0 >= p.col_blocks);
+    a.here = a.block < p.col_blocks && (!MAP || turn == 0), a.map = MAP && a.block >= p.col_blocks;
+    a.first = scalar(a.segment * p.seg_chunks), a.end = scalar((a.segment + 1) * p.seg_chunks);
+    return a;
+}
+// What a segment's first launch leaves: states of col_blocks blocks, then the map, tile by tile as a left operand of mfma4
+__device__ __forceinline__ float *segment_of(const DeltaArgs &p, int chain, int segment, int tiles) {
+    return p.seg + ((int64_t)chain * p.segments + segment) * blocks_of<true>(p) * tiles * 256;
+}
+template <int KE, bool MAP, bool BACK>
+__device__ __forceinline__ void first_state(const DeltaArgs &p, const Part &a, const Where &w, const StateRef &from, int lane,
+                                            f32x4 (&S)[2 * KE]) {
+    constexpr int ET = 2 * KE;
+    const int c = lane & 15, q = lane >> 4, col = kCols * a.block + c, home = BACK ? p.segments - 1 : 0;
+    const bool given = from.ptr && a.segment == home && !a.map;
+#pragma unroll
+    for (int t = 0; t < ET; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int e = 16 * t + 4 * q + r;
+            S[t][r] = given && e < p.E && col < p.M ? from.ptr[w.n * from.stride_n + w.h * from.stride_h + e * from.stride_d + col]
+                      : MAP && a.map && e == col - kCols * p.col_blocks && a.segment != home ? 1.f : 0.f;
+        }
+    if (MAP || p.segments == 1 || a.block >= p.col_blocks) return;
+    const float *const start = segment_of(p, w.chain, home, ET) + (a.block * ET * 64 + lane) * 4;
+#pragma unroll
+    for (int t = 0; t < ET; t++) S[t] = *(const f32x4a *)(start + 256 * t);
+    const int keys = (p.E + kCols - 1) / kCols, step = BACK ? -1 : 1;
+    for (int g = home + step; g != a.segment; g += step) {
+        const float *const there = segment_of(p, w.chain, g, ET);
+        const float *const add = there + (a.block * ET * 64 + lane) * 4, *const map = there + (p.col_blocks * ET * 64 + lane) * 4;
+        f32x4 N[ET];
+#pragma unroll
+        for (int t = 0; t < ET; t++) N[t] = *(const f32x4a *)(add + 256 * t);
+#pragma unroll
+        for (int b = 0; b < ET; b++) {  // (rows of S behind the last key column are zero)
+            f32x4 left[ET];
+#pragma unroll
+            for (int t = 0; t < ET; t++) left[t] = *(const f32x4a *)(map + 256 * (min(b, keys - 1) * ET + t));
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int t = 0; t < ET; t++) N[t] = mfma4(left[t][r], S[b][r], N[t]);
+        }
+        settle();
+#pragma unroll
+        for (int t = 0; t < ET; t++) S[t] = N[t];
+    }
+}
+template <int KE, bool MAP, bool BACK>
+__device__ __forceinline__ void last_state(const DeltaArgs &p, const Part &a, const Where &w, const StateRef &to, int lane,
+                                           const f32x4 (&S)[2 * KE]) {
+    constexpr int ET = 2 * KE;
+    const int c = lane & 15, q = lane >> 4, col = kCols * a.block + c;
+    settle();
+    if (MAP) {
+        if (a.block >= blocks_of<true>(p)) return;
+        float *const there = segment_of(p, w.chain, a.segment, ET) + a.block * ET * 256;
+#pragma unroll
+        for (int t = 0; t < ET; t++) {
+            if (!a.map) *(f32x4a *)(there + 256 * t + 4 * lane) = S[t];
+            else  // row 4 q + r, column c of its block: to the row's lane
+#pragma unroll
+                for (int r = 0; r < 4; r++) there[256 * t + (4 * q + r + 16 * (c / 4)) * 4 + c % 4] = S[t][r];
+        }
+        return;
+    }
+    if (!a.last || !to.ptr) return;
+#pragma unroll
+    for (int t = 0; t < ET; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int e = 16 * t + 4 * q + r;
+            if (e < p.E && col < p.M) to.ptr[w.n * to.stride_n + w.h * to.stride_h + e * to.stride_d + col] = S[t][r];
+        }
+}
+
 // 64 rows of the wavefront's 16 columns, row by row from memory and through LDS to rows 16 t + 4 q + r of column c.
 // Only what comes from memory stays in registers: whatever was done to it where it is requested would wait for it.
 template <typename T, bool VEC>
@@ -182,27 +282,19 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t factor_rows(const DeltaArgs &p
         4 * kFactors * kRows, mfma::kRsrcFlags);
 }
 
-template <typename T, int KE, bool VEC, bool SHARE>
+template <typename T, int KE, bool VEC, bool SHARE, bool MAP>
 __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_kernel(DeltaArgs p) {
     constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512, W = SHARE ? kWaves : 1;
     const int lane = threadIdx.x & 63, wave = SHARE ? scalar(threadIdx.x >> 6) : 0, c = lane & 15, q = lane >> 4;
-    int chain, group;
-    if (!place(p, (p.col_blocks + W - 1) / W, chain, group)) return;
-    const int block = scalar(group * W + wave), col = kCols * block + c;
-    const bool here = !SHARE || block < p.col_blocks;  // (the others carry operands, and compute with zeros)
-    const Where w = where_of(p, chain, 0);
-    const int chunks = chunks_of(w.len);
+    const Part part = part_of<W, MAP, false>(p, wave);
+    if (part.none) return;
+    const int block = part.block, col = kCols * block + c;
+    const bool here = SHARE || MAP ? part.here : true;  // (the others carry operands, and compute with zeros)
+    const Where w = where_of(p, part.chain, 0);
+    const int first = part.first, last = min(part.end, chunks_of(w.len));  // (of its chunks, past the last)
 
     f32x4 S[ET];
-#pragma unroll
-    for (int t = 0; t < ET; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int e = 16 * t + 4 * q + r;
-            S[t][r] = p.initial.ptr && e < p.E && col < p.M
-                          ? p.initial.ptr[w.n * p.initial.stride_n + w.h * p.initial.stride_h + e * p.initial.stride_d + col]
-                          : 0.f;
-        }
+    first_state<KE, MAP, false>(p, part, w, p.initial, lane, S);
 
     const uint32_t v_row = (uint32_t)p.v.stride_l * Elem<T>::kBytes;
     using Tile = ColumnTile<T, VEC>;
@@ -215,26 +307,26 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
     Left<SHARE, kTFrags, 3> tf;
     Tile V;
     FactorRow in, out;
-    float last;
+    float decay;
     auto load_in = [&](int chunk) { kr.load(p.kr + (w.key_at + chunk) * kKeys, wave, lane); };
     auto load_rows = [&](int chunk) {
         V.load(chunk_rows(p.v, w.n, w.h, (int64_t)chunk * kRows, Elem<T>::kBytes), v_row, kCols * block, p.M,
                min(kRows, w.len - chunk * kRows), lane);
         const __amdgpu_buffer_rsrc_t rs = factor_rows(p, w.at + chunk);
         in.load(rs, kReadK, lane), out.load(rs, kWrite, lane);
-        last = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (kRows * kRise + kRows - 1), 0, 0));
+        decay = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (kRows * kRise + kRows - 1), 0, 0));
     };
     auto load_t = [&](int chunk) { tf.load(p.t + (w.at + chunk) * (kTFrags * 3 * 512), wave, lane); };
     auto load_out = [&](int chunk) { kc.load(p.kc + (w.key_at + chunk) * kKeys, wave, lane); };
-    if (chunks > 0) {
-        load_rows(0), load_in(0), load_t(0), load_out(0);
-        if (SHARE) kr.put(krp, wave, lane), load_in(min(1, chunks - 1));
+    if (first < last) {
+        load_rows(first), load_in(first), load_t(first), load_out(first);
+        if (SHARE) kr.put(krp, wave, lane), load_in(min(first + 1, last - 1));
     }
-    for (int chunk = 0; chunk < chunks; chunk++) {
+    for (int chunk = first; chunk < last; chunk++) {
         const int64_t at = (w.at + chunk) * p.col_blocks + block;
-        const int next = min(chunk + 1, chunks - 1);
+        const int next = min(chunk + 1, last - 1);
         V.put(vp, lane), in.put(fp, lane), out.put(fp + kRows, lane);
-        const float fade = last;
+        const float fade = decay;
         if (SHARE) meet<SHARE>();
         if (here) {
             float *const to = p.s + at * (ET * 256) + 4 * lane;
@@ -274,7 +366,7 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
             if (s == 0) products<0>(a, ef, Z);
             else products<2>(a, ef, Z);
         }
-        if (SHARE) settle();
+        if (SHARE || MAP) settle();
         if (here) store_tiles(p.z + at * (4 * 256) + 4 * lane, Z);
         // S <- e^{G_64} S + K^T diag(rk beta e^{G_64 - G}) Z
 #pragma unroll
@@ -295,47 +387,30 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
             products<0>(a, uf, S);
         }
         phase();
-        if (SHARE) kr.put(krp, wave, lane), load_in(min(chunk + 2, chunks - 1));
+        if (SHARE) kr.put(krp, wave, lane), load_in(min(chunk + 2, last - 1));
         else load_out(next);
         phase();
     }
-    if (p.final_.ptr)
-#pragma unroll
-        for (int t = 0; t < ET; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int e = 16 * t + 4 * q + r;
-                if (e < p.E && col < p.M)
-                    p.final_.ptr[w.n * p.final_.stride_n + w.h * p.final_.stride_h + e * p.final_.stride_d + col] = S[t][r];
-            }
+    last_state<KE, MAP, false>(p, part, w, p.final_, lane, S);
 }
 
 // The same walk from the last chunk to the first, on the gradient of the state:
 //   dU = A^T dO + diag(rk e^{G_64 - G}) K dS,   dE = T^T diag(beta) dU,
 //   dS <- e^{G_64} dS + Q^T diag(rq e^G) dO - K^T diag(rk e^G) dE
 // and what the chunk's keys write of <state, its gradient>: the sum of beta Z . diag(rk e^{G_64 - G}) K dS.
-template <typename T, int KE, bool VEC, bool SHARE>
+template <typename T, int KE, bool VEC, bool SHARE, bool MAP>
 __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_back_kernel(DeltaArgs p) {
     constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512, W = SHARE ? kWaves : 1;
     const int lane = threadIdx.x & 63, wave = SHARE ? scalar(threadIdx.x >> 6) : 0, c = lane & 15, q = lane >> 4;
-    int chain, group;
-    if (!place(p, (p.col_blocks + W - 1) / W, chain, group)) return;
-    const int block = scalar(group * W + wave), col = kCols * block + c;
-    const bool here = !SHARE || block < p.col_blocks;
-    const Where w = where_of(p, chain, 0);
-    const int chunks = chunks_of(w.len);
+    const Part part = part_of<W, MAP, true>(p, wave);
+    if (part.none) return;
+    const int block = part.block, col = kCols * block + c;
+    const bool here = SHARE || MAP ? part.here : true;  // (the others carry operands, and compute with zeros)
+    const Where w = where_of(p, part.chain, 0);
+    const int first = part.first, last = min(part.end, chunks_of(w.len));  // (of its chunks, past the last)
 
     f32x4 S[ET];
-#pragma unroll
-    for (int t = 0; t < ET; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int e = 16 * t + 4 * q + r;
-            S[t][r] = p.grad_final.ptr && e < p.E && col < p.M
-                          ? p.grad_final.ptr[w.n * p.grad_final.stride_n + w.h * p.grad_final.stride_h +
-                                             e * p.grad_final.stride_d + col]
-                          : 0.f;
-        }
+    first_state<KE, MAP, true>(p, part, w, p.grad_final, lane, S);
 
     const uint32_t g_row = (uint32_t)p.go.stride_l * Elem<T>::kBytes, gv_row = (uint32_t)p.gv.stride_l * Elem<T>::kBytes;
     // (three pieces of two k-steps held: the columns of q where the rows of k were, requested while T is used)
@@ -355,13 +430,13 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
     Tile Gr;
     FactorRow write, beta, read_q, read_k;
     f32x4 Y[4], Z[4];
-    float last;
-    auto tiles = [&](int chunk) { return ((w.at + chunk) * p.col_blocks + (here ? block : 0)) * (4 * 256) + 4 * lane; };
+    float decay;
+    auto tiles = [&](int chunk) { return ((w.at + chunk) * p.col_blocks + (SHARE || MAP ? min(block, p.col_blocks - 1) : block)) * (4 * 256) + 4 * lane; };
     auto load_in = [&](int chunk) { kr.load(p.kr + (w.key_at + chunk) * kKeys, wave, lane); };
     auto load_rows = [&](int chunk) {
         const __amdgpu_buffer_rsrc_t rs = factor_rows(p, w.at + chunk);
         write.load(rs, kWrite, lane), beta.load(rs, kBeta, lane), read_q.load(rs, kReadQ, lane), read_k.load(rs, kReadK, lane);
-        last = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (kRows * kRise + kRows - 1), 0, 0));
+        decay = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (kRows * kRise + kRows - 1), 0, 0));
         load_tiles(p.de + tiles(chunk), Y);
         load_tiles(p.z + tiles(chunk), Z);
     };
@@ -372,18 +447,18 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
     };
     auto load_q = [&](int chunk) { qc.load(p.qc + (w.key_at + chunk) * kKeys, wave, lane); };
     auto load_out = [&](int chunk) { kc.load(p.kc + (w.key_at + chunk) * kKeys, wave, lane); };
-    if (chunks > 0) {
-        const int first = chunks - 1;
-        if (!kTurns) load_q(first);
-        load_in(first), load_rows(first), load_t(first), load_g(first), load_out(first);
-        if (SHARE) kr.put(inp, wave, lane), load_in(max(first - 1, 0));
+    if (first < last) {
+        const int from = last - 1;
+        if (!kTurns) load_q(from);
+        load_in(from), load_rows(from), load_t(from), load_g(from), load_out(from);
+        if (SHARE) kr.put(inp, wave, lane), load_in(max(from - 1, first));
     }
-    for (int chunk = chunks - 1; chunk >= 0; chunk--) {
+    for (int chunk = last - 1; chunk >= first; chunk--) {
         const int64_t at = (w.at + chunk) * p.col_blocks + block;
-        const int next = max(chunk - 1, 0);
+        const int next = max(chunk - 1, first);
         write.put(fp, lane), beta.put(fp + kRows, lane);
         read_q.put(fp + 2 * kRows, lane), read_k.put(fp + 3 * kRows, lane);
-        const float fade = last;
+        const float fade = decay;
         if (SHARE) meet<SHARE>();
         if (here) {
             float *const to = p.ds + at * (ET * 256) + 4 * lane;
@@ -407,11 +482,11 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             P[t] *= write_rows[t];
-            D[t] = beta_rows[t] * Y[t] + P[t];
+            D[t] = MAP && part.map ? P[t] : beta_rows[t] * Y[t] + P[t];
             written += Z[t] * P[t];
             P[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        if (SHARE) settle();
+        if (SHARE || MAP) settle();
         if (here) p.written[at * 64 + lane] = (written[0] + written[1]) + (written[2] + written[3]);
         phase();
         tf.put(tp, wave, lane);
@@ -440,6 +515,7 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
             else products<0>(a, df, P);
         }
         if (SHARE) phase(), qc.put(inp, wave, lane), load_q(next), load_g(next), settle();
+        if (MAP) settle();
         if (here) store_tiles(p.de + at * (4 * 256) + 4 * lane, P);
         if (here && p.gv.ptr)
             Tile::store(chunk_rows(Operand{p.gv.ptr, p.gv.stride_n, p.gv.stride_h, p.gv.stride_l, 0, 0}, w.n, w.h,
@@ -479,38 +555,35 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
             products<0>(a, ef, S);
         }
         phase();
-        if (SHARE) kr.put(inp, wave, lane), load_in(max(chunk - 2, 0));
+        if (SHARE) kr.put(inp, wave, lane), load_in(max(chunk - 2, first));
         else load_out(next);
         phase();
     }
-    if (p.grad_initial.ptr)
-#pragma unroll
-        for (int t = 0; t < ET; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int e = 16 * t + 4 * q + r;
-                if (e < p.E && col < p.M)
-                    p.grad_initial.ptr[w.n * p.grad_initial.stride_n + w.h * p.grad_initial.stride_h +
-                                       e * p.grad_initial.stride_d + col] = S[t][r];
-            }
+    last_state<KE, MAP, true>(p, part, w, p.grad_initial, lane, S);
     // positions past the end of the sequence
-    if (p.gv.ptr && col < p.M)
+    if (!MAP && part.last && p.gv.ptr && col < p.M)
         for (int l = w.len + q; l < p.L; l += 4)
             store_from_f32(p.gv.ptr, p.gv.dtype, w.n * p.gv.stride_n + w.h * p.gv.stride_h + l * p.gv.stride_l + col, 0.f);
 }
 
-template <typename T, int KE, bool VEC, bool SHARE>
-void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
+template <typename T, int KE, bool VEC, bool SHARE, bool MAP>
+void launch(const DeltaArgs &p, bool back, int64_t groups, hipStream_t stream) {
     constexpr uint32_t W = SHARE ? kWaves : 1;
-    const dim3 grid(((uint32_t)p.N * (uint32_t)p.H + 7) / 8 * 8 * (((uint32_t)p.col_blocks + W - 1) / W));
-    if (back) delta_scan_back_kernel<T, KE, VEC, SHARE><<<grid, 64 * W, 0, stream>>>(p);
-    else delta_scan_kernel<T, KE, VEC, SHARE><<<grid, 64 * W, 0, stream>>>(p);
+    const dim3 grid(((uint32_t)p.N * (uint32_t)p.H + 7) / 8 * 8 * (uint32_t)groups);
+    if (back) delta_scan_back_kernel<T, KE, VEC, SHARE, MAP><<<grid, 64 * W, 0, stream>>>(p);
+    else delta_scan_kernel<T, KE, VEC, SHARE, MAP><<<grid, 64 * W, 0, stream>>>(p);
+}
+template <typename T, int KE, bool VEC, bool MAP>
+void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
+    const int64_t segments = p.segments > 1 ? p.segments - 1 : 1, blocks = blocks_of<MAP>(p);
+    const bool share = (int64_t)p.N * p.H * blocks * segments > kAlone;
+    if (Elem<T>::kPieces * KE > 6 || share) launch<T, KE, VEC, true, MAP>(p, back, (blocks + kWaves - 1) / kWaves * segments, stream);
+    else if constexpr (Elem<T>::kPieces * KE <= 6) launch<T, KE, VEC, false, MAP>(p, back, blocks * segments, stream);
 }
 template <typename T, int KE, bool VEC>
 void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
-    const bool share = (int64_t)p.N * p.H * p.col_blocks > kAlone;
-    if (Elem<T>::kPieces * KE > 6 || share) launch<T, KE, VEC, true>(p, back, stream);
-    else if constexpr (Elem<T>::kPieces * KE <= 6) launch<T, KE, VEC, false>(p, back, stream);
+    if (p.segments > 1) launch<T, KE, VEC, true>(p, back, stream);
+    launch<T, KE, VEC, false>(p, back, stream);
 }
 template <typename T, int KE>
 void launch(const DeltaArgs &p, bool vec, bool back, hipStream_t stream) {

@@ -331,3 +331,23 @@ def test_gradients_of_few_or_strong_decays(dtype, L, strength):
             (dg,) = torch.autograd.grad([o, s], [leaves[3]], [go, gs])
             if L <= 4 or strength is not None:
                 assert not dg[:, :, 0].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N, H, Hk, L, E, M", [(1, 2, 1, 1000, 64, 64), (3, 1, 1, 1100, 37, 21), (2, 2, 2, 1290, 128, 128), (2, 1, 1, 800, 70, 130),
+                                               (1, 1, 1, 3100, 16, 16)])
+def test_few_long_chains_are_walked_in_segments(dtype, N, H, Hk, L, E, M):
+    args = ref.inputs(N, H, Hk, L, E, M, dtype=dtype, device="cuda", seed=L)
+    args[3][:, :1].mul_(0.02)                                            # (a head that remembers over segments)
+    go, gs = seeds(args)
+    for lengths in (None, [L] + [L // 2, 5][:N - 1]):
+        got = results(args, go, gs, normalize=True, lengths=None if lengths is None else torch.tensor(lengths, device="cuda"))
+        want = wanted(args, go, gs, normalize=True, lengths=None if lengths is None else torch.tensor(lengths))
+        check(got, want)
+        out, state = gated_delta_rule(*args, normalize=True, return_state=True,
+                                      lengths=None if lengths is None else torch.tensor(lengths, device="cuda"))
+        assert torch.equal(out, got[0]) and torch.equal(state, got[1])
+    zero = args[:5] + [torch.zeros_like(args[5])]
+    out, state = gated_delta_rule(*args[:5], return_state=True)          # without a state
+    again, last = gated_delta_rule(*zero, return_state=True)
+    assert torch.equal(out, again) and torch.equal(state, last)
