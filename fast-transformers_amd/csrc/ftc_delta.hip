@@ -26,14 +26,17 @@ struct Sizes {
     int64_t s() const { return units() * col_blocks() * tiles() * 256; }
     int64_t z() const { return units() * col_blocks() * 4 * 256; }
     // Few chains are walked in segments, side by side: first what each makes of its first state (a linear map and what
-    // it adds), then the walk itself.  Twice the products, so three segments at least; more while there are up to two
-    // wavefronts a compute unit and the maps of the segments before (1.2 us each at 64 key columns, 4.5 at 128) are
-    // applied in less time than it saves.
+    // it adds), then the walk itself.  That is twice the products, so it takes room for four, up to two wavefronts a
+    // compute unit; and the maps of the segments before take 1.2 us each at 64 key columns, 4.5 at 128, which n segments
+    // of chunks / n chunks pay back while n^2 is below the chunks, or half of them (bf16).  Measured (forward and back, us,
+    // whole | in segments): 16 chains of 64 x 64, bf16, 12 chunks 25, 34 | 25, 32; 64: 98, 153 | 53, 71 (8); 256: 370, 587 | 172, 256 (8;
+    // 4: 225, 330); 32 chains, 64 chunks: 100, 154 | 81, 129 (4); 40: 105, 160 | 109, 173 (3: not done).  128 x 128: 16
+    // chains, 16 chunks 44, 59 | 46, 61 (3: not done); 64: 148, 210 | 116, 167 (4); 4 chains, 128 chunks 276, 400 | 124, 162 (8; 11: 157, 207).
     int64_t segments() const {
-        const int64_t waves = N * H * col_blocks(), most = waves > 0 ? 512 / waves : 1;
+        const int64_t waves = N * H * col_blocks(), most = waves > 0 ? 512 / waves : 1, gain = tiles() == 4 || dtype == FTC_F32 ? chunks() : chunks() / 2;
         int64_t n = 1;
-        while (n < most && 4 * (n + 1) <= chunks() && (n + 1) * (n + 1) <= chunks() * (tiles() == 4 ? 3 : 1)) n++;
-        if (n < 3) return 1;
+        while (n < most && (n + 1) * (n + 1) <= gain) n++;
+        if (most < 4 || n < 3) return 1;
         return (chunks() + segment_chunks(n) - 1) / segment_chunks(n);
     }
     int64_t segment_chunks(int64_t n) const { return (chunks() + n - 1) / n; }
