@@ -188,6 +188,7 @@ int ftc_gated_delta_rule(const ftc_tensor4 *queries, const ftc_tensor4 *keys, co
     if (int rc = check_state(final_state, "final_state", s)) return rc;
     if (s.N * s.H == 0) return FTC_OK;
     p.out = rows_out(out), p.initial = state(initial_state), p.final_ = state(final_state);
+    p.vec_out = reads_wide(as_operand(out));
     p.lengths = lengths, p.scale = scale, p.normalize = normalize != 0;
     if (s.L == 0 && !final_state) return FTC_OK;
     if (!kept && s.L <= kStepMost) {

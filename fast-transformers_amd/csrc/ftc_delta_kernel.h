@@ -79,7 +79,7 @@ struct DeltaArgs {
     StateRef initial, final_;
     OperandOut out;
     int32_t N, H, Hk, L, E, M, chunks, col_blocks;  // col_blocks: of 16 columns
-    int32_t vec_q, vec_k, vec_v, vec_go, vec_gv;  // rows can be read 16 bytes at a time
+    int32_t vec_q, vec_k, vec_v, vec_out, vec_go, vec_gv;  // rows can be read 16 bytes at a time
     int32_t normalize;
     float scale;
     float *factors;          // [chain][chunk][kFactors][64]

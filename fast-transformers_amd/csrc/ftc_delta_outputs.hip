@@ -5,6 +5,7 @@
 // A workgroup of four wavefronts takes one chunk and 16 CT columns per wavefront: A once for all of them, in LDS in
 // three pieces, then a wavefront's columns of the products.
 #include "ftc_delta_kernel.h"
+#include <type_traits>
 
 namespace ftc {
 namespace delta {
@@ -13,39 +14,46 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kAPlane = Plane<128>::kBytes;
 
-// A to three planes (row i, column j).  Its transpose is what is multiplied, so that a lane has four
-// consecutive columns.  The tiles above the diagonal that share a k-step with it are zero.
-template <int RB, int KE, int PIECES>
-__device__ __forceinline__ void make_a(const lds_char *qp, const lds_char *kp, lds_char *ap, const float *factors,
-                                       int wave, int c, int q) {
+// A wavefront's three tiles of A.  Its transpose is what is multiplied, so that a lane has four consecutive
+// columns.  The tiles above the diagonal that share a k-step with it are zero.
+struct TilesOfA {
+    f32x4 x[3];
+    __device__ static __forceinline__ int row_tile(int id) { return id < 2 ? 0 : id < 4 ? 1 : id < 8 ? 2 : 3; }
+    __device__ static __forceinline__ int column_tile(int id) { return id < 4 ? id & 1 : id & 3; }
+    template <int RB, int KE, int PIECES>
+    __device__ __forceinline__ void make(const lds_char *qp, const lds_char *kp, const float *factors, int wave, int c, int q) {
 #pragma unroll
-    for (int x = 0; x < 3; x++) {
-        const int id = wave + 4 * x, ti = id < 2 ? 0 : id < 4 ? 1 : id < 8 ? 2 : 3,
-                  tj = id < 4 ? id & 1 : id & 3;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < 3; n++) {
+            const int ti = row_tile(wave + 4 * n), tj = column_tile(wave + 4 * n);
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < KE; s++) {
-            Frag a[PIECES], b[PIECES];
-            rows_of<RB>(kp, tj, s, c, q, a);
-            rows_of<RB>(qp, ti, s, c, q, b);
-            acc = product(a, b, acc);
+            for (int s = 0; s < KE; s++) {
+                Frag a[PIECES], b[PIECES];
+                rows_of<RB>(kp, tj, s, c, q, a);
+                rows_of<RB>(qp, ti, s, c, q, b);
+                acc = product(a, b, acc);
+            }
+            const int i = 16 * ti + c, j0 = 16 * tj + 4 * q;
+            const f32x4 high = *(const f32x4a *)(factors + kHigh * kRows + j0), low = *(const f32x4a *)(factors + kLow * kRows + j0),
+                        rk = *(const f32x4a *)(factors + kRk * kRows + j0);
+            const float high_i = factors[kHigh * kRows + i], low_i = factors[kLow * kRows + i], rq = factors[kRq * kRows + i];
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                x[n][r] = j0 + r <= i ? acc[r] * expf((high_i - high[r]) + (low_i - low[r])) * (rq * rk[r]) : 0.f;
         }
-        const int i = 16 * ti + c, j0 = 16 * tj + 4 * q;
-        const f32x4 high = *(const f32x4a *)(factors + kHigh * kRows + j0), low = *(const f32x4a *)(factors + kLow * kRows + j0),
-                    rk = *(const f32x4a *)(factors + kRk * kRows + j0);
-        const float high_i = factors[kHigh * kRows + i], low_i = factors[kLow * kRows + i], rq = factors[kRq * kRows + i];
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            acc[r] = j0 + r <= i ? acc[r] * expf((high_i - high[r]) + (low_i - low[r])) * (rq * rk[r]) : 0.f;
-        store_pieces(ap + Plane<128>::addr(i, 4 * tj + q), kAPlane, acc);
     }
-}
+    // to three planes, row i, column j
+    __device__ __forceinline__ void put(lds_char *ap, int wave, int c, int q) const {
+#pragma unroll
+        for (int n = 0; n < 3; n++)
+            store_pieces(ap + Plane<128>::addr(16 * row_tile(wave + 4 * n) + c, 4 * column_tile(wave + 4 * n) + q), kAPlane, x[n]);
+    }
+};
 
-// Rows of q and k into LDS, and A from them
+// Rows of q and k into LDS
 template <typename T, int KE>
-__device__ __forceinline__ void stage(const DeltaArgs &p, const Where &w, const float *factors, lds_char *qp, lds_char *kp,
-                                      lds_char *ap, int tid) {
-    constexpr int RB = 64 * KE, PIECES = Elem<T>::kPieces;
+__device__ __forceinline__ void stage(const DeltaArgs &p, const Where &w, lds_char *qp, lds_char *kp, int tid) {
+    constexpr int RB = 64 * KE;
     RowTile<T, 32 * KE, kThreads> q_tile, k_tile;
     const int64_t l0 = (int64_t)w.chunk * kRows;
     q_tile.load(chunk_rows(p.q, w.n, w.hk, l0, Elem<T>::kBytes), (uint32_t)p.q.stride_l * Elem<T>::kBytes, p.E, w.valid,
@@ -55,15 +63,32 @@ __device__ __forceinline__ void stage(const DeltaArgs &p, const Where &w, const 
     q_tile.template store<RB>(qp, tid);
     k_tile.template store<RB>(kp, tid);
     __syncthreads();
-    make_a<RB, KE, PIECES>(qp, kp, ap, factors, tid >> 6, tid & 15, (tid & 63) >> 4);
-    __syncthreads();
+}
+// Four lanes side by side exchange: lane j of them has value j of all four
+__device__ __forceinline__ void exchange(f32x4 &x, int lane) {
+    auto beside = [](float v, auto control) {
+        return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(control)::value, 0xf, 0xf, false));
+    };
+    const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const float there = beside(odd ? x[i] : x[i + 1], std::integral_constant<int, 0xb1>());  // lanes 1 0 3 2
+        x[i] = odd ? there : x[i], x[i + 1] = odd ? x[i + 1] : there;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float there = beside(high ? x[i] : x[i + 2], std::integral_constant<int, 0x4e>());  // lanes 2 3 0 1
+        x[i] = high ? there : x[i], x[i + 2] = high ? x[i + 2] : there;
+    }
 }
 
 template <typename T, int KE, int CT>
 __global__ __launch_bounds__(kThreads) void delta_outputs_kernel(DeltaArgs p) {
     constexpr int RB = 64 * KE, PIECES = Elem<T>::kPieces, ET = 2 * KE;
-    __shared__ __align__(16) char q_mem[PIECES * Plane<RB>::kBytes], k_mem[PIECES * Plane<RB>::kBytes], a_mem[3 * kAPlane];
-    lds_char *const qp = (lds_char *)q_mem, *const kp = (lds_char *)k_mem, *const ap = (lds_char *)a_mem;
+    constexpr int kPlanes = PIECES * Plane<RB>::kBytes;
+    // (A where k was)
+    __shared__ __align__(16) char q_mem[kPlanes], k_mem[kPlanes > 3 * kAPlane ? kPlanes : 3 * kAPlane];
+    lds_char *const qp = (lds_char *)q_mem, *const kp = (lds_char *)k_mem, *const ap = kp;
     const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6), c = lane & 15, q = lane >> 4;
     const int groups = (p.col_blocks + 4 * CT - 1) / (4 * CT);
     const uint32_t id = blockIdx.x / (uint32_t)groups;
@@ -73,7 +98,14 @@ __global__ __launch_bounds__(kThreads) void delta_outputs_kernel(DeltaArgs p) {
     const int64_t l0 = (int64_t)w.chunk * kRows;
     const int rows = min((int64_t)kRows, p.L - l0);
     const int64_t out0 = w.n * p.out.stride_n + w.h * p.out.stride_h + l0 * p.out.stride_l;
-    if (w.valid > 0) stage<T, KE>(p, w, factors, qp, kp, ap, tid);
+    if (w.valid > 0) {
+        TilesOfA A;
+        stage<T, KE>(p, w, qp, kp, tid);
+        A.make<RB, KE, PIECES>(qp, kp, factors, wave, c, q);
+        __syncthreads();
+        A.put(ap, wave, c, q);
+        __syncthreads();
+    }
 
 #pragma unroll
     for (int x = 0; x < CT; x++) {
@@ -123,7 +155,23 @@ __global__ __launch_bounds__(kThreads) void delta_outputs_kernel(DeltaArgs p) {
                 for (int t = 0; t < 4; t++) *(f32x4a *)(to + 256 * t) = O[t];
             }
         }
-        if (col < p.M)
+        if (p.vec_out) {  // four columns of a row a lane
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                exchange(O[t], lane);
+                const int row = 16 * t + 4 * q + (c & 3), at = kCols * block + (c & ~3);
+                if (row >= rows || at >= p.M) continue;
+                T *const to = (T *)p.out.ptr + out0 + row * p.out.stride_l + at;
+                if constexpr (Elem<T>::kBytes == 4) {
+                    *(f32x4a *)to = O[t];
+                } else {
+                    uint32_t two[2][1];
+                    pieces_of<1>(O[t][0], O[t][1], two[0]);
+                    pieces_of<1>(O[t][2], O[t][3], two[1]);
+                    *(u32x2a *)to = u32x2{two[0][0], two[1][0]};
+                }
+            }
+        } else if (col < p.M)
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -137,8 +185,10 @@ __global__ __launch_bounds__(kThreads) void delta_outputs_kernel(DeltaArgs p) {
 template <typename T, int KE, int CT>
 __global__ __launch_bounds__(kThreads) void delta_pull_kernel(DeltaArgs p) {
     constexpr int RB = 64 * KE, PIECES = Elem<T>::kPieces;
-    __shared__ __align__(16) char q_mem[PIECES * Plane<RB>::kBytes], k_mem[PIECES * Plane<RB>::kBytes], a_mem[3 * kAPlane];
-    lds_char *const qp = (lds_char *)q_mem, *const kp = (lds_char *)k_mem, *const ap = (lds_char *)a_mem;
+    constexpr int kPlanes = PIECES * Plane<RB>::kBytes;
+    // (A where q and k were)
+    __shared__ __align__(16) char mem[2 * kPlanes > 3 * kAPlane ? 2 * kPlanes : 3 * kAPlane];
+    lds_char *const qp = (lds_char *)mem, *const kp = qp + kPlanes, *const ap = qp;
     const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6), c = lane & 15, q = lane >> 4;
     const int groups = (p.col_blocks + 4 * CT - 1) / (4 * CT);
     const uint32_t id = blockIdx.x / (uint32_t)groups;
@@ -146,7 +196,9 @@ __global__ __launch_bounds__(kThreads) void delta_pull_kernel(DeltaArgs p) {
     const Where w = where_of(p, (int)(id / (uint32_t)p.chunks), (int)(id % (uint32_t)p.chunks));
     const float *const factors = p.factors + w.at * (kFactors * kRows);
     if (w.valid == 0) return;
-    stage<T, KE>(p, w, factors, qp, kp, ap, tid);
+    stage<T, KE>(p, w, qp, kp, tid);
+    TilesOfA A;
+    A.make<RB, KE, PIECES>(qp, kp, factors, wave, c, q);
     // the queries' fragments, by the first workgroup of the first value head
     if (w.h % (p.H / p.Hk) == 0 && blockIdx.x % (uint32_t)groups == 0)
         for (int i = wave; i < 4 * KE; i += 4) {
@@ -154,6 +206,9 @@ __global__ __launch_bounds__(kThreads) void delta_pull_kernel(DeltaArgs p) {
             columns_of<RB>(qp, i / 2, i % 2, c, q, f);
             store_frag(p.qc + w.key_at * (4 * KE * PIECES * 512), i, lane, f);
         }
+    __syncthreads();
+    A.put(ap, wave, c, q);
+    __syncthreads();
 
     const __amdgpu_buffer_rsrc_t rows = chunk_rows(p.go, w.n, w.h, (int64_t)w.chunk * kRows, Elem<T>::kBytes);
     const uint32_t row_bytes = (uint32_t)p.go.stride_l * Elem<T>::kBytes;

@@ -38,12 +38,12 @@ template <typename T, int KE>
 __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
     constexpr int RB = 64 * KE, PIECES = Elem<T>::kPieces;
     using Tile = RowTile<T, 32 * KE, kThreads>;
-    __shared__ __align__(16) char k_mem[PIECES * Plane<RB>::kBytes];
-    // (M; at the end T's three planes)
-    __shared__ __align__(16) float m_mem[3 * Plane<128>::kBytes / 4], t_mem[kRows * kStride], x_mem[32 * kStride];
+    // k, and T where it was; M and what is made of it, and at the end T's three planes there
+    constexpr int kPlanes = PIECES * Plane<RB>::kBytes, kT = 4 * kRows * kStride, kM = kT + 4 * 32 * kStride;
+    __shared__ __align__(16) char k_mem[kPlanes > kT ? kPlanes : kT], m_mem[kM > 3 * Plane<128>::kBytes ? kM : 3 * Plane<128>::kBytes];
     __shared__ float k2_mem[kRows], q2_mem[kRows], high_mem[kRows], low_mem[kRows], beta_mem[kRows], rk_mem[kRows];
     lds_char *const kp = (lds_char *)k_mem;
-    lds_float *const Mx = (lds_float *)m_mem, *const Tm = (lds_float *)t_mem, *const X = (lds_float *)x_mem;
+    lds_float *const Mx = (lds_float *)m_mem, *const Tm = (lds_float *)k_mem, *const X = Mx + kRows * kStride;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = scalar(tid >> 6), c = lane & 15, q = lane >> 4;
     const Where w = where_of(p, (int)(blockIdx.x / (uint32_t)p.chunks), (int)(blockIdx.x % (uint32_t)p.chunks));
@@ -60,7 +60,6 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
               p.vec_k, tid);
     if (p.normalize) squares(tile, (lds_float *)k2_mem, tid);
     tile.template store<RB>(kp, tid);
-    for (int i = tid; i < kRows * kStride; i += kThreads) Tm[i] = 0.f;
     __syncthreads();
 
     float *const factors = p.factors + w.at * (kFactors * kRows);
@@ -134,6 +133,8 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
             Mx[i * kStride + j] = j < i ? acc[r] * d * (rk_mem[i] * rk_mem[j]) * beta_mem[j] : 0.f;
         }
     }
+    __syncthreads();
+    for (int i = tid; i < kRows * kStride; i += kThreads) Tm[i] = 0.f;
     __syncthreads();
 
     // diagonal blocks: column c of block `wave`
