@@ -4,6 +4,11 @@
 //
 // A workgroup of four wavefronts takes one chunk and 16 CT columns per wavefront: A once for all of them, in LDS in
 // three pieces, then a wavefront's columns of the products.
+//
+// What bounds it: memory where there are many chunks.  A lies where k was (and q, in A^T dO), so that four and five workgroups
+// fit a compute unit (bf16); results are stored four columns a lane.  Measured: 8192 chunks of 128 x 128, bf16: outputs 320 us, 4.2 TB/s
+// of states, Z, rows, out and O (two workgroups a compute unit, and a value a store: 410); A^T dO 181 us, 4.9 TB/s
+// (243).  1280 chunks of 64 x 64, fp32: 32 and 35 us.
 #include "ftc_delta_kernel.h"
 #include <type_traits>
 

@@ -7,6 +7,7 @@
 // What bounds it is the state, read and written once per call (8 E M bytes a chain), and on few chains latency.  A
 // workgroup of 256 lanes owns 64 columns of one chain's state in registers: 64 / VEC lanes side by side (VEC = 4:
 // 16-byte accesses), the others take every kGroups-th row.  Sums are in a fixed order, everything is fp32.
+// Measured: 4096 chains of 128 x 128 107 us, 5.0 TB/s of states; 8 chains of 64 x 64 6 us, of which a launch is 4.
 #include "ftc_delta_kernel.h"
 
 namespace ftc {
