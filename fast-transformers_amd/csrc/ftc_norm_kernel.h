@@ -135,23 +135,22 @@ __device__ __forceinline__ void team_sum(float &a, float &b, float (*mem)[2][16]
     }
 }
 
-// 1 / (1 + exp(-g)), from the hardware's 2^x of the exponent's whole product (its rounding made good, since it is
-// multiplied by the exponent) and its reciprocal: within 3 half steps
-__device__ __forceinline__ float sigmoid(float g) {
-    constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // log2(e) in two floats
-    const float x = fmaxf(-g, -126.f), t = x * kLog2e, rest = fmaf(x, kRest, fmaf(x, kLog2e, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __builtin_amdgcn_rcpf(1.f + fmaf(e, rest * 0.693147181f, e));
-}
-// The gate's factor and its slope
+// The gate's factor and its slope.  s = 1 / (1 + exp(-g)) and 1 - s from the hardware's 2^x of the exponent's whole product
+// (its rounding made good, since it is multiplied by the exponent) and its reciprocal: within 3 half steps, and 7.  Gates
+// below -88.5 count as that (2^x would be infinite a little further): s is then under 2^-127, which the reciprocal gives as
+// zero.  A NaN stays one.
 __device__ __forceinline__ void activate(float g, int activation, float &value, float &slope) {
     if (activation == FTC_GATE_PLAIN) {
         value = g, slope = 1.f;
-    } else {
-        const float s = sigmoid(g);
-        value = activation == FTC_GATE_SIGMOID ? s : g * s;
-        slope = activation == FTC_GATE_SIGMOID ? s * (1.f - s) : s * fmaf(g, 1.f - s, 1.f);
+        return;
     }
+    constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // log2(e) in two floats
+    const float low = __builtin_elementwise_maximum(g, -88.5f), x = __builtin_elementwise_minimum(low, 126.f);
+    const float t = x * -kLog2e, lost = fmaf(x, -kRest, fmaf(x, -kLog2e, -t));
+    const float two = __builtin_amdgcn_exp2f(t), e = fmaf(two, lost * 0.693147181f, two);
+    const float s = __builtin_amdgcn_rcpf(1.f + e), rest = e * s;
+    if (activation == FTC_GATE_SIGMOID) value = s, slope = s * rest;
+    else value = low * s, slope = s * fmaf(x, rest, 1.f);
 }
 
 // One lot of a norm's weight and bias (from the caches: where they are used)

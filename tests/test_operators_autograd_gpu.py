@@ -205,3 +205,34 @@ def test_refusals_of_the_norms_on_the_gpu():
                                  ((torch.zeros(2, 0, device="cuda"),), {}, "1 to 16384")):
         with pytest.raises(RuntimeError, match=match):
             residual_norm(*args, **options)
+
+
+@pytest.mark.parametrize("activation", ["sigmoid", "silu"])
+@pytest.mark.parametrize("dtype", [F, B])
+def test_gates_far_out(activation, dtype):
+    """Gates that close or open entirely: factors and slopes are what they tend to, also at the type's lowest value."""
+    ends = [torch.finfo(dtype).min, -1e4, -200.0, -100.0, -95.0, -90.0, -89.0, -88.0, -87.0, -60.0, -20.0, 0.0, 20.0, 87.0, 89.0, 100.0,
+            1e4]
+    gen = torch.Generator().manual_seed(1)
+    block = (1 + torch.rand(8, 64 * len(ends), generator=gen)).to(dtype)
+    gate = (torch.tensor(ends).repeat_interleave(64)[None] * (1 + 0.004 * torch.rand(8, 64 * len(ends), generator=gen))).to(dtype)
+    gate = gate.clamp_min(torch.finfo(dtype).min)
+    b, g = block.cuda().requires_grad_(True), gate.cuda().requires_grad_(True)
+    x, _ = residual_norm(b, gate=g, activation=activation)
+    got = torch.autograd.grad(x, [b, g], torch.ones_like(x))
+    wb, wg = block.double().requires_grad_(True), gate.double().requires_grad_(True)
+    s = 1 / (1 + torch.exp(-wg.clamp_min(-700.0)))
+    want = wb * (s if activation == "sigmoid" else wg.clamp_min(-700.0) * s)
+    exact = torch.autograd.grad(want, [wb, wg], torch.ones_like(want))
+    for a, e in zip((x, *got), (want, *exact)):
+        a = a.detach().double().cpu()
+        assert torch.isfinite(a).all()
+        # (element by element: twelve half steps at most, 2^-24 each, of the factors and their products; and what is below 2^-118
+        # may be zero: 88 x 2^-125)
+        assert ((a - e.detach()).abs() <= (2.0 ** -20 + torch.finfo(dtype).eps / 2) * e.detach().abs() + 2.0 ** -118).all()
+    ends = torch.tensor([[-float("inf"), float("inf"), float("nan")]], device="cuda", dtype=dtype).requires_grad_(True)
+    x, _ = residual_norm(torch.ones(1, 3, device="cuda", dtype=dtype), gate=ends, activation=activation)
+    (slope,) = torch.autograd.grad(x, ends, torch.ones_like(x))
+    top = 1.0 if activation == "sigmoid" else float("inf")
+    assert x[0, 0] == 0 and x[0, 1] == top and x[0, 2].isnan()
+    assert slope[0, 0] == 0 and slope[0, 1] == (0 if activation == "sigmoid" else 1) and slope[0, 2].isnan()
