@@ -58,8 +58,11 @@ int check_sizes(const Sizes &s) {
     if (s.E < 1 || s.E > kMaxE || s.M < 1 || s.M > 512)
         return fail(FTC_ERR_UNSUPPORTED, "the gated delta rule takes key rows of 1 to 128 values and value rows of 1 to "
                     "512, got %lld and %lld", (long long)s.E, (long long)s.M);
-    if (s.N > 0x7fffffff || s.H > 0x7fffffff || s.L > 0x7fffff00 ||
-        (s.N * s.H > 0 && (s.N * s.H > 0x7fffffff || s.N * s.H * s.col_blocks() > 0x7fffffff / (s.chunks() + 1))))
+    // (a launch has fewer than 2^32 lanes: 2^24 workgroups of 256, of one chunk and 64 columns or less)
+    constexpr int64_t kMost = 0xffffff;
+    const int64_t groups = (s.col_blocks() + 3) / 4;
+    if (s.N > kMost || s.H > kMost || s.L > 0x7fffff00 ||
+        (s.N * s.H > 0 && (s.N * s.H > kMost || s.N * s.H * groups > kMost / (s.chunks() + 1))))
         return fail(FTC_ERR_UNSUPPORTED, "too many chains, positions and columns for one call");
     return FTC_OK;
 }

@@ -122,7 +122,7 @@ def _cpu_rule(queries, keys, values, log_decay, beta, state, lengths, scale, nor
         outs.append(scale * (rise * torch.matmul(qc, S) + torch.matmul(A, u)))
         S = rise[:, :, -1:] * S + torch.matmul((fall * kc).transpose(-1, -2), u)
     out = torch.cat(outs, 2) if outs else v.new_zeros((N, H, 0, M))
-    return out.to(values.dtype), S
+    return out.to(values.dtype), S if outs or state is None else S.clone()
 
 
 def gated_delta_rule(queries, keys, values, log_decay, beta, initial_state=None, *, scale=None, normalize=False,

@@ -127,3 +127,11 @@ def test_c_abi_refuses_on_the_host():
     assert lib.ftc_gated_delta_step(*args, 1.0, 0, ctypes.byref(s), ctypes.byref(v), None) == -1
     assert "overlap" in _native.last_error()
     assert lib.ftc_gated_delta_step(*args, 1.0, 0, None, ctypes.byref(v), None) == -1
+
+
+def test_a_state_that_no_position_changed_is_the_callers_no_more():
+    q, k, v, g, b, s0 = ref.inputs(1, 2, 2, 1, 8, 8)
+    before = s0.clone()
+    _, state = gated_delta_rule(*(t[:, :, :0] for t in (q, k, v, g, b)), s0, return_state=True)
+    gated_delta_step(*(t[:, :, 0] for t in (q, k, v, g, b)), state)
+    assert torch.equal(s0, before) and not torch.equal(state, before)
