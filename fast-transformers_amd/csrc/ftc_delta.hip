@@ -62,7 +62,7 @@ int check_sizes(const Sizes &s) {
     constexpr int64_t kMost = 0xffffff;
     const int64_t groups = (s.col_blocks() + 3) / 4;
     if (s.N > kMost || s.H > kMost || s.L > 0x7fffff00 ||
-        (s.N * s.H > 0 && (s.N * s.H > kMost || s.N * s.H * groups > kMost / (s.chunks() + 1))))
+        (s.N * s.H > 0 && (s.N * s.H > kMost || s.N * s.H * groups > kMost / (s.chunks() > 1 ? s.chunks() : 1))))
         return fail(FTC_ERR_UNSUPPORTED, "too many chains, positions and columns for one call");
     return FTC_OK;
 }

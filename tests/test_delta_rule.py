@@ -135,3 +135,11 @@ def test_a_state_that_no_position_changed_is_the_callers_no_more():
     _, state = gated_delta_rule(*(t[:, :, :0] for t in (q, k, v, g, b)), s0, return_state=True)
     gated_delta_step(*(t[:, :, 0] for t in (q, k, v, g, b)), state)
     assert torch.equal(s0, before) and not torch.equal(state, before)
+
+
+def test_calls_of_more_workgroups_than_a_launch_has_are_refused():
+    lib = _native.load()
+    assert lib.ftc_gated_delta_rule_workspace_bytes(1 << 23, 1, 1, 1, 1, 1, _native.FTC_F32) >= 0
+    for N, L, M in ((1 << 24, 1, 1), (1 << 22, 1, 512), (1 << 12, 1 << 19, 64)):
+        assert lib.ftc_gated_delta_rule_workspace_bytes(N, 1, 1, L, 1, M, _native.FTC_F32) == -2, (N, L, M)
+        assert "too many" in _native.last_error()
