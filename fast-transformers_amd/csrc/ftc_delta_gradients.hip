@@ -14,16 +14,16 @@
 //   dG_i = dO_i . O_i - dE_i . V_i,   dg_l = sum of dG_i over i >= l in the chunk + <state after it, its gradient>
 // (the last is e^{G_64} <S, dS> + what the chunk's keys write, taken anew in every chunk: nothing adds up over chunks).
 //
-// A workgroup of four wavefronts takes a chunk of one key head and 64 of its columns, two to a compute unit, and the
+// A workgroup of four or eight wavefronts takes a chunk of one key head and 64 of its columns, two to a compute unit, and the
 // head's value heads one after the other, so that the gradients of shared keys are summed in registers, in one
 // order.  Phase 1 walks the columns of the state, 32 at a time through LDS, the next 32 on their way meanwhile; a
-// wavefront has 32 positions of 32 key columns, and a quarter of the tiles of dO Z^T and dE Z^T.  Phase 2 multiplies the
+// wavefront has 32 positions (of eight: 16) of 32 key columns, and its share of the tiles of dO Z^T and dE Z^T.  Phase 2 multiplies the
 // 64 x 64 matrices with the rows.  Gradients of bf16 rows are made of values in two pieces (2^-17 of them is left out,
 // against half a step of 2^-8 that the rounding of the results takes).
 //
 // What bounds it: the instructions that cut values into pieces and LDS, each about a third of the time with two workgroups a compute
 // unit, beside 2.2 GB of states, their gradients, Z, dE and rows.  Measured: 8192 chunks of 128 x 128 on 4096 of
-// key heads, bf16, 740 to 780 us (2.9 TB/s); 1280 of 64 x 64, fp32, 111.
+// key heads, bf16, 740 to 780 us (2.9 TB/s); 1280 of 64 x 64, fp32, 94.
 #include <type_traits>
 
 #include "ftc_delta_kernel.h"
@@ -32,8 +32,11 @@ namespace ftc {
 namespace delta {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kSlice = 64;  // key columns of a workgroup
+// Wavefronts of a workgroup: four, two workgroups to a compute unit; three pieces leave LDS for one workgroup, of eight.  (1280 chunks
+// of 64 x 64, fp32: 94 us, with four 111.  8192 of 128 x 128, bf16: 817, with four 780: as many wavefronts read operands twice.)
+template <typename T>
+constexpr int kWaves = Elem<T>::kPieces == 1 ? 4 : 8;
 
 // The lane's column and row group anew: what is made of them belongs to the phase behind (all phases' addresses, held
 // through the loop over heads, would not leave registers for the products)
@@ -44,9 +47,10 @@ __device__ __forceinline__ int renewed(int x) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs p) {
+__global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(DeltaArgs p) {
     constexpr int PIECES = Elem<T>::kPieces, NP = PIECES == 1 ? 2 : 3;
-    constexpr int RB = 2 * kSlice, EW = 2, RT = 2;
+    constexpr int RB = 2 * kSlice, EW = 2;
+    constexpr int WAVES = kWaves<T>, kThreads = 64 * WAVES, RT = 8 / WAVES, XT = 12 / WAVES + (12 % WAVES != 0), BLOCKS = 8 / WAVES;
     constexpr int kMB = 32;                                // columns of the state at a time
     constexpr int kGo = kRows * 2 * kMB, kSq = kMB * 128;  // bytes of a plane of dO, of the others
     constexpr int kSquare = Plane<128>::kBytes;
@@ -55,9 +59,9 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
     constexpr int kBytes = kResident ? kQK + (kPhase1 > kPR ? kPhase1 : kPR) : (kPhase1 > kQK + kPR ? kPhase1 : kQK + kPR);
     __shared__ __align__(16) char mem[kBytes];
     __shared__ __align__(16) float f_mem[kFactors * kRows];
-    __shared__ float dot_mem[2][kRows];    // of a value head: dE . Z, dE . V
+    __shared__ float dot_mem[2][WAVES / 4][kRows]; // of a value head: dE . Z, dE . V, by every other block of columns
     __shared__ float total_mem[2][kRows];  // q . dq and k . dk of all of them
-    __shared__ float state_mem[4];         // per wavefront: its share of <S, dS>
+    __shared__ float state_mem[WAVES];         // per wavefront: its share of <S, dS>
     lds_char *const lds = (lds_char *)mem;
     lds_char *const qp = lds, *const kp = qp + PIECES * kSquare;
     lds_char *const gop = lds + (kResident ? kQK : 0), *const zp = gop + PIECES * kGo, *const dep = zp + NP * kSq,
@@ -96,12 +100,13 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
         tile.template store<RB>(kp, renewed(tid));
     };
 
-    // ---- what phase 1 stages of 32 columns: dO's rows, and the fragments' tile `wave` of either block ----
-    RowTile<T, kMB, kThreads> go;
-    f32x4 zr[2], er[2], sr[2], dr[2];
+    // ---- what phase 1 stages of 32 columns: dO's rows (the first four wavefronts), and a tile of the fragments of either block ----
+    RowTile<T, kMB, 256> go;
+    const int tile = wave & 3, half = WAVES == 8 ? wave >> 2 : 0;  // (half: eight wavefronts have a block each)
+    f32x4 zr[BLOCKS], er[BLOCKS], sr[BLOCKS], dr[BLOCKS];
     // (of v in its own type: widening it here would wait for it)
     using Raw = typename std::conditional<Elem<T>::kBytes == 4, uint32_t, uint16_t>::type;
-    Raw vr[2][4];
+    Raw vr[BLOCKS][4];
     auto request = [&](int h, int m0, bool any) {
         const int64_t at = ((int64_t)(n * p.H + h) * p.chunks + chunk) * p.col_blocks;
         const int l = renewed(lane);
@@ -109,40 +114,41 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
         shifted.ptr = (const char *)p.go.ptr + (int64_t)m0 * kCols * Elem<T>::kBytes;
         // (a block past the last one: zeros, from a buffer of no bytes or rows of no values)
         const int live = any ? valid : 0;
-        go.load(chunk_rows(shifted, n, h, l0, Elem<T>::kBytes), (uint32_t)p.go.stride_l * Elem<T>::kBytes,
-                p.M - m0 * kCols, live, p.vec_go, 64 * wave + l);
+        if (wave < 4)
+            go.load(chunk_rows(shifted, n, h, l0, Elem<T>::kBytes), (uint32_t)p.go.stride_l * Elem<T>::kBytes,
+                    p.M - m0 * kCols, live, p.vec_go, 64 * wave + l);
         const __amdgpu_buffer_rsrc_t v_rows = chunk_rows(p.v, n, h, l0, Elem<T>::kBytes);
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-            const int block = m0 + b, col = block * kCols + (l & 15);
+        for (int b = 0; b < BLOCKS; b++) {
+            const int block = m0 + half + b, col = block * kCols + (l & 15);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int row = 16 * wave + 4 * (l >> 4) + r;
+                const int row = 16 * tile + 4 * (l >> 4) + r;
                 const bool in = (row < live) & (col < p.M);
                 const uint32_t at = (uint32_t)row * ((uint32_t)p.v.stride_l * Elem<T>::kBytes) + (uint32_t)(col * Elem<T>::kBytes);
                 const uint32_t from = in ? at : kOutside;
                 if constexpr (Elem<T>::kBytes == 4) vr[b][r] = __builtin_amdgcn_raw_buffer_load_b32(v_rows, from, 0, 0);
                 else vr[b][r] = __builtin_amdgcn_raw_buffer_load_b16(v_rows, from, 0, 0);
             }
-            auto fragment = [&](const float *from, int count, int tile) {
-                const uint64_t base = (uint64_t)(from + ((at + block) * count + tile) * 256);
+            auto fragment = [&](const float *from, int count, int number) {
+                const uint64_t base = (uint64_t)(from + ((at + block) * count + number) * 256);
                 const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
                     (void *)(((uint64_t)(uint32_t)scalar((int)(base >> 32)) << 32) | (uint32_t)scalar((int)(uint32_t)base)), 0,
                     any && block < p.col_blocks ? 1024 : 0, mfma::kRsrcFlags);
                 return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * l, 0, 0));
             };
-            zr[b] = fragment(p.z, 4, wave), er[b] = fragment(p.de, 4, wave);
-            sr[b] = fragment(p.s, tiles, 4 * slice + wave), dr[b] = fragment(p.ds, tiles, 4 * slice + wave);
+            zr[b] = fragment(p.z, 4, tile), er[b] = fragment(p.de, 4, tile);
+            sr[b] = fragment(p.s, tiles, 4 * slice + tile), dr[b] = fragment(p.ds, tiles, 4 * slice + tile);
         }
     };
     // a fragment's place in planes with a row per column: four positions (or key columns) of column c
     auto put = [&](f32x4 &dot_z, f32x4 &dot_v) {
-        const int l = renewed(lane), slot = 4 * wave + (l >> 4);
-        go.template store<64>(gop, 64 * wave + l);
+        const int l = renewed(lane), slot = 4 * tile + (l >> 4);
+        if (wave < 4) go.template store<64>(gop, 64 * wave + l);
         float dot = 0.f;
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-            const int to = Plane<128>::addr(16 * b + (l & 15), slot);
+        for (int b = 0; b < BLOCKS; b++) {
+            const int to = Plane<128>::addr(16 * (half + b) + (l & 15), slot);
             store_pieces<NP>(zp + to, kSq, zr[b]);
             store_pieces<NP>(dep + to, kSq, er[b]);
             store_pieces<NP>(sp + to, kSq, sr[b]);
@@ -157,7 +163,7 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
     };
     // the tiles of the square matrices, transposed: rows j of tile tj, columns i of tile ti
     auto tile_of = [&](int x, int &ti, int &tj) {
-        const int id = wave + 4 * x;
+        const int id = min(wave + WAVES * x, 11);  // (twelve: four of eight wavefronts make the last one once more)
         ti = id < 2 ? 0 : id < 4 ? 1 : id < 8 ? 2 : 3, tj = id < 4 ? id & 1 : id & 3;
     };
 
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
         for (int i = tid; i < kFactors * kRows; i += kThreads) fp[i] = p.factors[at * (kFactors * kRows) + i];
 
         // ---- phase 1 ----
-        f32x4 F[3] = {}, N[3] = {};                                    // (dO Z^T)^T, (dE Z^T)^T
+        f32x4 F[XT] = {}, N[XT] = {};                                    // (dO Z^T)^T, (dE Z^T)^T
         f32x4 aQ[RT][EW] = {}, aP[RT][EW] = {}, aM[RT][EW] = {};       // S dO, S dE, dS Z
         f32x4 dot_z = {0.f, 0.f, 0.f, 0.f}, dot_v = {0.f, 0.f, 0.f, 0.f};
         float state_dot = 0.f;
@@ -187,7 +193,7 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
             request(more || g + 1 == G ? h : h + 1, more ? m0 + 2 : 0, more || g + 1 < G);
             renew(c, q);
 #pragma unroll
-            for (int x = 0; x < 3; x++) {
+            for (int x = 0; x < XT; x++) {
                 int ti, tj;
                 tile_of(x, ti, tj);
                 Frag zf[NP], of[PIECES], ef[NP];
@@ -228,8 +234,8 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
         if (c == 0)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                dot_mem[0][16 * wave + 4 * q + r] = dot_z[r];
-                dot_mem[1][16 * wave + 4 * q + r] = dot_v[r];
+                dot_mem[0][half][16 * tile + 4 * q + r] = dot_z[r];
+                dot_mem[1][half][16 * tile + 4 * q + r] = dot_v[r];
             }
 
         // ---- phase 2 ----
@@ -237,7 +243,7 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
         renew(c, q);
         if (!kResident) stage_rows();
 #pragma unroll
-        for (int x = 0; x < 3; x++) {
+        for (int x = 0; x < XT; x++) {
             int ti, tj;
             tile_of(x, ti, tj);
             const int i = 16 * ti + c, j0 = 16 * tj + 4 * q;
@@ -268,12 +274,18 @@ __global__ __launch_bounds__(kThreads, 2) void delta_gradients_kernel(DeltaArgs 
                 }
             }
         // what the decays' and beta's gradients are made of, for the kernel behind
+        auto dots_of = [&](int which) {
+            return WAVES == 8 ? dot_mem[which][0][lane] + dot_mem[which][WAVES / 4 - 1][lane] : dot_mem[which][0][lane];
+        };
         if (wave < 2) {
-            if (slice == 0) p.sums[at * kSums + kRows * wave + lane] = dot_mem[wave][lane];
+            if (slice == 0) p.sums[at * kSums + kRows * wave + lane] = dots_of(wave);
         } else if (wave == 2) {
-            if (lane == 0) p.sums[at * kSums + 2 * kRows + slice] = (state_mem[0] + state_mem[1]) + (state_mem[2] + state_mem[3]);
-        } else if (p.normalize) {
-            total_mem[0][lane] += o, total_mem[1][lane] += 2.f * dot_mem[0][lane] - dot_mem[1][lane];
+            float state = (state_mem[0] + state_mem[1]) + (state_mem[2] + state_mem[3]);
+            if (WAVES == 8)
+                state += (state_mem[WAVES - 4] + state_mem[WAVES - 3]) + (state_mem[WAVES - 2] + state_mem[WAVES - 1]);
+            if (lane == 0) p.sums[at * kSums + 2 * kRows + slice] = state;
+        } else if (p.normalize && wave == 3) {
+            total_mem[0][lane] += o, total_mem[1][lane] += 2.f * dots_of(0) - dots_of(1);
         }
         __syncthreads();
 #pragma unroll
@@ -556,8 +568,8 @@ __global__ __launch_bounds__(256, 4) void delta_decays_kernel(DeltaArgs p) {
 int delta_gradients(const DeltaArgs &p, bool bf16, hipStream_t stream) {
     const uint32_t slices = (uint32_t)((p.E + kSlice - 1) / kSlice);
     const dim3 grid(((uint32_t)p.N * (uint32_t)p.Hk * (uint32_t)p.chunks + 7) / 8 * 8 * slices);
-    if (bf16) delta_gradients_kernel<bf16_t><<<grid, kThreads, 0, stream>>>(p);
-    else delta_gradients_kernel<float><<<grid, kThreads, 0, stream>>>(p);
+    if (bf16) delta_gradients_kernel<bf16_t><<<grid, 64 * kWaves<bf16_t>, 0, stream>>>(p);
+    else delta_gradients_kernel<float><<<grid, 64 * kWaves<float>, 0, stream>>>(p);
     if (p.gg.ptr || p.gb.ptr) {
         const dim3 units((uint32_t)p.N * (uint32_t)p.H * (uint32_t)p.chunks);
         const bool vec = p.vec_q && p.vec_k && p.vec_go;
