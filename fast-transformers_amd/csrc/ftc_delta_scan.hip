@@ -3,7 +3,7 @@
 //
 // A wavefront owns 16 columns of one chain's state in registers and walks the chunks.  What it multiplies with it reads
 // as fragments, each one's next chunk requested as soon as this chunk's is used: where there are few wavefronts straight
-// into the registers of the operands, without a barrier; where there are many, four wavefronts share them in LDS.  A
+// into the registers of the operands, without a barrier; where there are many, two or four wavefronts share them in LDS.  A
 // chunk is a chain of dependent products, so what bounds few chains is its latency (1.5 us forward, 2.3 back at
 // 64 x 64, 2.3 and 3.3 at 128 x 128); many are bound by what a compute unit gets from its caches.
 #include "ftc_delta_kernel.h"
@@ -35,27 +35,27 @@ __device__ __forceinline__ void store_tiles(float *to, const f32x4 (&x)[4]) {
     for (int t = 0; t < 4; t++) *(f32x4a *)(to + 256 * t) = x[t];
 }
 
-// A left operand of N fragments: a wavefront that works alone holds it in registers; four that share it keep it in LDS, and
-// each carries every fourth piece of the next chunk's on its way there.
-constexpr int kWaves = 4;
-// Up to two wavefronts a compute unit work alone.  Each of them fetches all its operands, 34 to 64 KB a chunk, and what a
-// compute unit gets from the L2 beside latency is some 20 bytes a clock: more of them wait for each other.  Measured (forward and
-// back, us, alone | shared), bf16, 64 chunks of 128 x 128: 256 wavefronts 165, 227 | 213, 326; 512: 248, 311 | 241, 354; 640:
-// 297, 424 | 245, 359; 1024: 400, 561 | 287, 422.  fp32, 32 chunks of 64 x 64: 256: 85, 115 | 114, 189; 512: 146, 191 | 132, 206;
-// 1024: 259, 380 | 224, 327.  (Three pieces of 128 key columns do not fit the registers: always shared.)
-// Shared, 1024 wavefronts of 128 x 128 move 1.2 GB in 290 us and 2.0 in 425: 4.3 and 4.7 TB/s, states and results of fp32 for the most.
-constexpr int64_t kAlone = 512;
-template <bool SHARE, int N, int PIECES>
+// A left operand of N fragments: a wavefront that works alone holds it in registers; W that share it keep it in LDS, and
+// each carries every W-th piece of the next chunk's on its way there.
+// Up to one wavefront a compute unit they work alone, up to two in pairs, above four together.  Each alone fetches all its
+// operands, 34 to 64 KB a chunk, and what a compute unit gets from the L2 beside latency is some 20 bytes a clock: more of them
+// wait for each other.  Measured (forward and back, us, alone | pairs | four), bf16, 64 chunks of 128 x 128: 256 wavefronts
+// 166, 229 | 187, 270 | 213, 327; 512: 261, 326 | 216, 305 | 243, 355; 768: 322, 464 | 295, 413 | 249, 380; 1024: 400, 561 | 340, 490 | 287, 422.
+// fp32, 32 chunks of 64 x 64: 256: 86, 119 | 100, 155 | 109, 187; 512: 150, 193 | 121, 172 | 135, 205; 1024: 263, 386 | 226, 327 | 225, 321.
+// (Three pieces of 128 key columns do not fit the registers alone, nor in pairs without spills: always four.)
+// Four, 1024 wavefronts of 128 x 128 move 1.2 GB in 290 us and 2.0 in 425: 4.3 and 4.7 TB/s, states and results of fp32 for the most.
+template <int W, int N, int PIECES>
 struct Left {
-    static constexpr int kCount = N * PIECES, kPer = SHARE ? (kCount + kWaves - 1) / kWaves : 1;
+    static constexpr bool SHARE = W > 1;
+    static constexpr int kCount = N * PIECES, kPer = SHARE ? (kCount + W - 1) / W : 1;
     Frag held[SHARE ? 1 : N][SHARE ? 1 : PIECES];
     u32x4 carried[kPer];
     __device__ __forceinline__ void load(const uint16_t *from, int wave, int lane) {
         if constexpr (SHARE) {
 #pragma unroll
             for (int i = 0; i < kPer; i++)
-                if (kCount % kWaves == 0 || i + 1 < kPer || wave + kWaves * i < kCount)
-                    carried[i] = *(const u32x4a *)(from + (wave + kWaves * i) * 512 + 8 * lane);
+                if (kCount % W == 0 || i + 1 < kPer || wave + W * i < kCount)
+                    carried[i] = *(const u32x4a *)(from + (wave + W * i) * 512 + 8 * lane);
         } else {
 #pragma unroll
             for (int i = 0; i < N; i++) load_frag(from, i, lane, held[i]);
@@ -65,8 +65,8 @@ struct Left {
         if constexpr (SHARE)
 #pragma unroll
             for (int i = 0; i < kPer; i++)
-                if (kCount % kWaves == 0 || i + 1 < kPer || wave + kWaves * i < kCount)
-                    *(__attribute__((address_space(3))) u32x4a *)(to + (wave + kWaves * i) * 1024 + 16 * lane) = carried[i];
+                if (kCount % W == 0 || i + 1 < kPer || wave + W * i < kCount)
+                    *(__attribute__((address_space(3))) u32x4a *)(to + (wave + W * i) * 1024 + 16 * lane) = carried[i];
     }
     __device__ __forceinline__ void get(const lds_char *from, int number, int lane, Frag (&a)[PIECES]) const {
 #pragma unroll
@@ -80,11 +80,11 @@ struct Left {
         }
     }
 };
-// What was written to LDS is there for all four, and what was read may be overwritten
-template <bool SHARE>
+// What was written to LDS is there for all, and what was read may be overwritten
+template <int W>
 __device__ __forceinline__ void meet() {
     phase();
-    if (SHARE) mfma::wg_barrier();
+    if (W > 1) mfma::wg_barrier();
     phase();
 }
 
@@ -283,9 +283,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t factor_rows(const DeltaArgs &p
         4 * kFactors * kRows, mfma::kRsrcFlags);
 }
 
-template <typename T, int KE, bool VEC, bool SHARE, bool MAP>
-__global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_kernel(DeltaArgs p) {
-    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512, W = SHARE ? kWaves : 1;
+template <typename T, int KE, bool VEC, int W, bool MAP>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_kernel(DeltaArgs p) {
+    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512;
+    constexpr bool SHARE = W > 1;
     const int lane = threadIdx.x & 63, wave = SHARE ? scalar(threadIdx.x >> 6) : 0, c = lane & 15, q = lane >> 4;
     const Part part = part_of<W, MAP, false>(p, wave);
     if (part.none) return;
@@ -304,8 +305,8 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
     __shared__ __align__(16) char kr_mem[SHARE ? 2 * kKeys : 16], kc_mem[SHARE ? 2 * kKeys : 16], t_mem[SHARE ? kTFrags * 3072 : 16];
     lds_char *const vp = (lds_char *)v_mem[wave], *const krp = (lds_char *)kr_mem, *const kcp = (lds_char *)kc_mem, *const tp = (lds_char *)t_mem;
     lds_float *const fp = (lds_float *)f_mem[wave];
-    Left<SHARE, 4 * KE, PIECES> kr, kc;
-    Left<SHARE, kTFrags, 3> tf;
+    Left<W, 4 * KE, PIECES> kr, kc;
+    Left<W, kTFrags, 3> tf;
     Tile V;
     FactorRow in, out;
     float decay;
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
         const int next = min(chunk + 1, last - 1);
         V.put(vp, lane), in.put(fp, lane), out.put(fp + kRows, lane);
         const float fade = decay;
-        if (SHARE) meet<SHARE>();
+        if (SHARE) meet<W>();
         if (here) {
             float *const to = p.s + at * (ET * 256) + 4 * lane;
 #pragma unroll
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
         tf.put(tp, wave, lane);
         if (SHARE) load_t(next), load_rows(next);
         else load_rows(next), load_in(next);
-        meet<SHARE>();
+        meet<W>();
         // Z = T E (tiles above the diagonal are zero)
 #pragma unroll
         for (int s = 0; s < 2; s++) {
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
         kc.put(kcp, wave, lane);
         if (SHARE) load_out(next);
         else load_t(next);
-        meet<SHARE>();
+        meet<W>();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag uf[3], a[ET][PIECES];
@@ -399,9 +400,10 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
 //   dU = A^T dO + diag(rk e^{G_64 - G}) K dS,   dE = T^T diag(beta) dU,
 //   dS <- e^{G_64} dS + Q^T diag(rq e^G) dO - K^T diag(rk e^G) dE
 // and what the chunk's keys write of <state, its gradient>: the sum of beta Z . diag(rk e^{G_64 - G}) K dS.
-template <typename T, int KE, bool VEC, bool SHARE, bool MAP>
-__global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_back_kernel(DeltaArgs p) {
-    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512, W = SHARE ? kWaves : 1;
+template <typename T, int KE, bool VEC, int W, bool MAP>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_scan_back_kernel(DeltaArgs p) {
+    constexpr int PIECES = Elem<T>::kPieces, ET = 2 * KE, kKeys = 4 * KE * PIECES * 512;
+    constexpr bool SHARE = W > 1;
     const int lane = threadIdx.x & 63, wave = SHARE ? scalar(threadIdx.x >> 6) : 0, c = lane & 15, q = lane >> 4;
     const Part part = part_of<W, MAP, true>(p, wave);
     if (part.none) return;
@@ -424,10 +426,10 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
     lds_char *const inp = (lds_char *)in_mem, *const kcp = (lds_char *)kc_mem, *const tp = (lds_char *)t_mem;
     lds_char *const gp = (lds_char *)g_mem[wave], *const through = SHARE ? gp : (lds_char *)through_mem[wave];
     lds_float *const fp = (lds_float *)f_mem[wave];
-    using Keys = Left<SHARE, 4 * KE, PIECES>;
+    using Keys = Left<W, 4 * KE, PIECES>;
     Keys kr, own_q, kc;
     Keys &qc = kTurns ? kr : own_q;
-    Left<SHARE, kTFrags, 3> tf;
+    Left<W, kTFrags, 3> tf;
     Tile Gr;
     FactorRow write, beta, read_q, read_k;
     f32x4 Y[4], Z[4];
@@ -460,7 +462,7 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
         write.put(fp, lane), beta.put(fp + kRows, lane);
         read_q.put(fp + 2 * kRows, lane), read_k.put(fp + 3 * kRows, lane);
         const float fade = decay;
-        if (SHARE) meet<SHARE>();
+        if (SHARE) meet<W>();
         if (here) {
             float *const to = p.ds + at * (ET * 256) + 4 * lane;
 #pragma unroll
@@ -496,7 +498,7 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
         else load_in(next), load_rows(next);
         if (!SHARE) phase();
         Gr.put(gp, lane);
-        if (SHARE) meet<SHARE>();
+        if (SHARE) meet<W>();
         // dE = T^T diag(beta) dU
         f32x4 read_q_rows[4], read_k_rows[4];
 #pragma unroll
@@ -532,7 +534,7 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
         for (int t = 0; t < ET; t++) S[t] *= fade;
         phase();
         if (!SHARE) load_t(next), load_g(next);
-        meet<SHARE>();
+        meet<W>();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag of[3], a[ET][PIECES];
@@ -546,7 +548,7 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
         if (SHARE) load_out(next);
         else if (kTurns) load_in(next);
         else load_q(next);
-        meet<SHARE>();
+        meet<W>();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             Frag ef[3], a[ET][PIECES];
@@ -567,19 +569,21 @@ __global__ __launch_bounds__(SHARE ? 64 * kWaves : 64) __attribute__((amdgpu_wav
             store_from_f32(p.gv.ptr, p.gv.dtype, w.n * p.gv.stride_n + w.h * p.gv.stride_h + l * p.gv.stride_l + col, 0.f);
 }
 
-template <typename T, int KE, bool VEC, bool SHARE, bool MAP>
-void launch(const DeltaArgs &p, bool back, int64_t groups, hipStream_t stream) {
-    constexpr uint32_t W = SHARE ? kWaves : 1;
+template <typename T, int KE, bool VEC, int W, bool MAP>
+void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
+    const int64_t segments = p.segments > 1 ? p.segments - 1 : 1, groups = (blocks_of<MAP>(p) + W - 1) / W * segments;
     const dim3 grid(((uint32_t)p.N * (uint32_t)p.H + 7) / 8 * 8 * (uint32_t)groups);
-    if (back) delta_scan_back_kernel<T, KE, VEC, SHARE, MAP><<<grid, 64 * W, 0, stream>>>(p);
-    else delta_scan_kernel<T, KE, VEC, SHARE, MAP><<<grid, 64 * W, 0, stream>>>(p);
+    if (back) delta_scan_back_kernel<T, KE, VEC, W, MAP><<<grid, 64 * W, 0, stream>>>(p);
+    else delta_scan_kernel<T, KE, VEC, W, MAP><<<grid, 64 * W, 0, stream>>>(p);
 }
 template <typename T, int KE, bool VEC, bool MAP>
 void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
-    const int64_t segments = p.segments > 1 ? p.segments - 1 : 1, blocks = blocks_of<MAP>(p);
-    const bool share = (int64_t)p.N * p.H * blocks * segments > kAlone;
-    if (Elem<T>::kPieces * KE > 6 || share) launch<T, KE, VEC, true, MAP>(p, back, (blocks + kWaves - 1) / kWaves * segments, stream);
-    else if constexpr (Elem<T>::kPieces * KE <= 6) launch<T, KE, VEC, false, MAP>(p, back, blocks * segments, stream);
+    const int64_t waves = (int64_t)p.N * p.H * blocks_of<MAP>(p) * (p.segments > 1 ? p.segments - 1 : 1);
+    if (Elem<T>::kPieces * KE > 6 || waves > 512) launch<T, KE, VEC, 4, MAP>(p, back, stream);
+    else if constexpr (Elem<T>::kPieces * KE <= 6) {
+        if (waves > 256 && blocks_of<MAP>(p) % 2 == 0) launch<T, KE, VEC, 2, MAP>(p, back, stream);
+        else launch<T, KE, VEC, 1, MAP>(p, back, stream);
+    }
 }
 template <typename T, int KE, bool VEC>
 void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
