@@ -50,7 +50,8 @@ def _gate_rows(gate, shape):
 
 class ResidualNorm(torch.autograd.Function):
     """``(x, h)`` on the GPU and their gradients; ``h`` is None without a norm before the next block.  Plain calls run as
-    the same function of the C++ engine (``host/ftc_host.cpp``); calls that are watched or transformed run this one."""
+    the same function of the C++ engine (``host/ftc_host.cpp``); calls that are watched or transformed, and those whose gate lies
+    across the rows, run this one."""
 
     @staticmethod
     def forward(ctx, block, residual, gate, after_weight, after_bias, before_weight, before_bias, options):
@@ -104,6 +105,10 @@ def residual_norm(block, residual=None, gate=None, *, after=None, before=None, s
     dimension.  ``after``, ``before``: None, or ``("rms" or "layer", weight, bias)`` with weight and bias optional.
     ``activation`` of the gate: None, ``"sigmoid"`` or ``"silu"``.  ``h`` is the norm of ``x`` before ``x`` is rounded to its type.
     Differentiable once, with respect to all tensors."""
+    if block.is_cuda and not torch.compiler.is_compiling():  # (calls as they mostly are, checked by the native code)
+        pair = _native.host().residual_norm_plain(block, residual, gate, after, before, scale, activation, eps)
+        if pair is not None:
+            return pair
     if block.dim() < 1 or not 1 <= block.shape[-1] <= 16384:
         raise RuntimeError("residual_norm: takes rows of 1 to 16384 values, got shape %s" % (tuple(block.shape),))
     if activation not in _ACTIVATIONS:
@@ -127,10 +132,6 @@ def residual_norm(block, residual=None, gate=None, *, after=None, before=None, s
     if block.device.type == "cpu":
         return _cpu_residual_norm(block, residual, gate, after, before, activation, scale, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        if not torch.compiler.is_compiling():
-            pair = _native.host().residual_norm_plain(block, residual, gate, *after, *before, activation, scale, eps)
-            if pair is not None:
-                return pair
         return ResidualNorm.apply(block, residual, gate, after[1], after[2], before[1], before[2],
                                   (after[0], before[0], activation, scale, eps))
     x, h, _ = _native.host().residual_norm(block, residual, gate, *after, *before, activation, scale, eps, False)

@@ -236,3 +236,32 @@ def test_gates_far_out(activation, dtype):
     top = 1.0 if activation == "sigmoid" else float("inf")
     assert x[0, 0] == 0 and x[0, 1] == top and x[0, 2].isnan()
     assert slope[0, 0] == 0 and slope[0, 1] == (0 if activation == "sigmoid" else 1) and slope[0, 2].isnan()
+
+
+@pytest.mark.parametrize("gate", [(5, 7, 64), (5, 1, 64), (1, 1, 64), (64,), (7, 64), (1, 7, 64), (5, 7, 1), (2, 7, 64), (3, 5, 7, 64)])
+def test_plain_and_watched_calls_agree_on_gates(gate):
+    """Gates of every broadcast, on rows with one and two strides, through both ways of a call."""
+    gen = torch.Generator().manual_seed(3)
+    wide = torch.randn(5, 7, 2 * 64, generator=gen).cuda()
+    w = torch.rand(64, generator=gen).cuda().add_(0.5).requires_grad_(True)
+    g = torch.randn(*gate, generator=gen).cuda().requires_grad_(True)
+    bad = gate in ((5, 7, 1), (2, 7, 64), (3, 5, 7, 64))
+    for block in (wide[..., 64:], wide[..., :64].contiguous(), wide.transpose(0, 1).contiguous().transpose(0, 1)[..., :64]):
+        block = block.detach().requires_grad_(True)
+        call = lambda: residual_norm(block, block, g, after=("rms", w), before="layer", activation="silu")  # noqa: E731
+        if bad:
+            with pytest.raises(RuntimeError, match="gate of shape"):
+                call()
+            continue
+        plain = call()
+        go = [torch.ones_like(t) for t in plain]
+        first = [*plain, *torch.autograd.grad(plain, [block, g, w], go)]
+        with watched():
+            seen = call()
+        second = [*seen, *torch.autograd.grad(seen, [block, g, w], go)]
+        with torch.no_grad():
+            third = call()
+        assert all(torch.equal(a, b) for a, b in zip(first, second)) and all(torch.equal(a, b) for a, b in zip(first, third))
+        b, gg = (t.detach().double().cpu() for t in (block, g))
+        want = norm.residual_norm(b, b, gg, ("rms", w.detach().double().cpu()), ("layer",), 1.0, "silu")
+        assert norm.far(plain[0].detach(), want[0]) <= norm.FP32 and norm.far(plain[1].detach(), want[1]) <= norm.FP32
