@@ -56,7 +56,10 @@ Plan plan_of(int64_t D, int64_t rows, int64_t segment, bool backward, bool full)
     // As many as the GPU holds at a time, by their registers (more would wait, and the backward leaves sums with each of
     // them).  Backward of 524288 x 128 with 768 of the lean kernel 143 us, with 512 179; of 40960 x 512 with 512 of the full
     // one 115, with 768 138; forward of either with 1024 95 and 78, with 2048 104 and 82.
-    const int64_t most = q.lpr > 512 ? 256 : q.lpr > 256 ? 512 : !backward ? 1024 : full ? 512 : 768;
+    // (forward, teams of 128 lanes and more: rows waiting fill the gaps between a row's loads, sums and stores.  60000 x 1024, bf16, 95 with
+    // 4096, with 1024 117; 32768 x 2048 147 and 156; 37735 x 3160 198 with 1536, with 512 242.)
+    const int64_t most = q.lpr > 512 ? 256 : !backward ? (q.lpr > 256 ? 1536 : q.lpr > 64 ? 4096 : 1024)
+                                              : q.lpr > 256 ? 512 : full ? 512 : 768;
     const int64_t segments = (rows + segment - 1) / segment;
     q.parts = std::min((segment + q.teams - 1) / q.teams, std::max<int64_t>(1, most / segments));
     q.groups = std::min(segments, std::max<int64_t>(1, most / q.parts)) * q.parts;

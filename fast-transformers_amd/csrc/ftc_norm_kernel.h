@@ -59,18 +59,24 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(2), may_alias));
 
 // A lot as it comes from memory: widening it where it is requested would wait for it.  TAIL: a row may end inside it
-// (`left` values of it are there), and what lies behind reads as zero.
+// (`left` values of it are there).  Then it is the row's last eight values that are read, in one access as well, and they are
+// moved to their places when they are widened, with zeros behind: read one by one, which has to wait for them, rows of 1023
+// bf16 values took 256 us forward and 735 back instead of 152 and 352 (60000 of them).  Rows of fewer than eight
+// are read so all the same, and tails of those that leave no registers for the moves (MOVE; two lots a lane: 8190 values,
+// 194 forward and 436 back, with the moves 235 and 532).
 struct Raw {
     u32x4 a, b;
 };
-template <bool TAIL>
-__device__ __forceinline__ Raw request(const void *base, int dtype, int64_t at, int left) {
+template <bool TAIL, bool MOVE>
+__device__ __forceinline__ Raw request(const void *base, int dtype, int64_t at, int left, bool is_short) {
     Raw r;
-    const char *const from = (const char *)base + at * (dtype == FTC_F32 ? 4 : 2);
-    if (!TAIL || left >= kLot) {
+    if (!TAIL || (MOVE ? !is_short : left >= kLot)) {
+        if (TAIL && MOVE && left < kLot) at -= kLot - left;
+        const char *const from = (const char *)base + at * (dtype == FTC_F32 ? 4 : 2);
         r.a = *(const any_u32x4 *)from;
         if (dtype == FTC_F32) r.b = *(const any_u32x4 *)(from + 16);
     } else {
+        const char *const from = (const char *)base + at * (dtype == FTC_F32 ? 4 : 2);
         uint32_t x[kLot];
 #pragma unroll
         for (int i = 0; i < kLot; i++)
@@ -80,7 +86,8 @@ __device__ __forceinline__ Raw request(const void *base, int dtype, int64_t at, 
     }
     return r;
 }
-__device__ __forceinline__ Lot widen(const Raw &r, int dtype) {
+template <bool TAIL, bool MOVE>
+__device__ __forceinline__ Lot widen(const Raw &r, int dtype, int left, bool is_short) {
     Lot x;
     if (dtype == FTC_F32) {
 #pragma unroll
@@ -89,6 +96,14 @@ __device__ __forceinline__ Lot widen(const Raw &r, int dtype) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             x.x[2 * i] = __uint_as_float(r.a[i] << 16), x.x[2 * i + 1] = __uint_as_float(r.a[i] & 0xffff0000u);
+    }
+    if (TAIL && MOVE && left < kLot && !is_short) {
+        const int by = kLot - left;
+#pragma unroll
+        for (int bit = 4; bit >= 1; bit /= 2)
+            if (by & bit)
+#pragma unroll
+                for (int i = 0; i < kLot; i++) x.x[i] = i + bit < kLot ? x.x[(i + bit) % kLot] : 0.f;
     }
     return x;
 }
@@ -154,13 +169,13 @@ __device__ __forceinline__ void activate(float g, int activation, float &value, 
 }
 
 // One lot of a norm's weight and bias (from the caches: where they are used)
-template <bool TAIL>
-__device__ __forceinline__ void params_lot(const Params &p, int col, int left, Lot &w, Lot &b) {
-    if (p.weight) w = widen(request<TAIL>(p.weight, p.weight_dtype, col, left), p.weight_dtype);
+template <bool TAIL, bool MOVE>
+__device__ __forceinline__ void params_lot(const Params &p, int col, int left, bool is_short, Lot &w, Lot &b) {
+    if (p.weight) w = widen<TAIL, MOVE>(request<TAIL, MOVE>(p.weight, p.weight_dtype, col, left, is_short), p.weight_dtype, left, is_short);
     else
 #pragma unroll
         for (int i = 0; i < kLot; i++) w.x[i] = 1.f;
-    if (p.bias) b = widen(request<TAIL>(p.bias, p.bias_dtype, col, left), p.bias_dtype);
+    if (p.bias) b = widen<TAIL, MOVE>(request<TAIL, MOVE>(p.bias, p.bias_dtype, col, left, is_short), p.bias_dtype, left, is_short);
     else
 #pragma unroll
         for (int i = 0; i < kLot; i++) b.x[i] = 0.f;
@@ -180,6 +195,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
     const int team = threadIdx.x / LPR, lane = threadIdx.x % LPR;
     int turn = 0;
     const float per = 1.f / (float)p.D;
+    constexpr bool MOVE = NV == 1;
+    const bool is_short = p.D < kLot;
     auto column = [&](int v) { return kLot * (lane + LPR * v); };
 
     // Mean (layer norm) and 1 / deviation of the row in r
@@ -213,15 +230,15 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
         for (int v = 0; v < NV; v++) {
             const int col = column(v), left = p.D - col;
             if (!live || left <= 0) continue;
-            block[v] = request<TAIL>(p.block.ptr, type_of<DB>(p.block), row * p.block.stride + col, left);
-            if (p.gate.ptr) gate[v] = request<TAIL>(p.gate.ptr, type_of<DB>(p.gate), gate_row * p.gate.stride + col, left);
+            block[v] = request<TAIL, MOVE>(p.block.ptr, type_of<DB>(p.block), row * p.block.stride + col, left, is_short);
+            if (p.gate.ptr) gate[v] = request<TAIL, MOVE>(p.gate.ptr, type_of<DB>(p.gate), gate_row * p.gate.stride + col, left, is_short);
             if (p.residual.ptr)
-                residual[v] = request<TAIL>(p.residual.ptr, type_of<DS>(p.residual), row * p.residual.stride + col, left);
+                residual[v] = request<TAIL, MOVE>(p.residual.ptr, type_of<DS>(p.residual), row * p.residual.stride + col, left, is_short);
         }
         Lot r[NV];
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-            if (live && column(v) < p.D) r[v] = widen(block[v], type_of<DB>(p.block));
+            if (live && column(v) < p.D) r[v] = widen<TAIL, MOVE>(block[v], type_of<DB>(p.block), p.D - column(v), is_short);
             else
 #pragma unroll
                 for (int i = 0; i < kLot; i++) r[v].x[i] = 0.f;
@@ -234,12 +251,12 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
             if (!live || col >= p.D) continue;
             if (p.after.kind != FTC_NORM_NONE) {
                 Lot w, b;
-                params_lot<TAIL>(p.after, col, p.D - col, w, b);
+                params_lot<TAIL, MOVE>(p.after, col, p.D - col, is_short, w, b);
 #pragma unroll
                 for (int i = 0; i < kLot; i++) r[v].x[i] = fmaf((r[v].x[i] - mean_a) * rstd_a, w.x[i], b.x[i]);
             }
             if (p.gate.ptr) {
-                const Lot g = widen(gate[v], type_of<DB>(p.gate));
+                const Lot g = widen<TAIL, MOVE>(gate[v], type_of<DB>(p.gate), p.D - column(v), is_short);
 #pragma unroll
                 for (int i = 0; i < kLot; i++) {
                     float value, slope;
@@ -248,7 +265,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
                 }
             }
             if (p.residual.ptr) {
-                const Lot d = widen(residual[v], type_of<DS>(p.residual));
+                const Lot d = widen<TAIL, MOVE>(residual[v], type_of<DS>(p.residual), p.D - column(v), is_short);
 #pragma unroll
                 for (int i = 0; i < kLot; i++) r[v].x[i] = fmaf(p.scale, r[v].x[i], d.x[i]);
             } else {
@@ -267,7 +284,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
                 const int col = column(v);
                 if (col >= p.D) continue;
                 Lot w, b;
-                params_lot<TAIL>(p.before, col, p.D - col, w, b);
+                params_lot<TAIL, MOVE>(p.before, col, p.D - col, is_short, w, b);
 #pragma unroll
                 for (int i = 0; i < kLot; i++) r[v].x[i] = fmaf((r[v].x[i] - mean_b) * rstd_b, w.x[i], b.x[i]);
                 store_lot<TAIL>(p.h.ptr, type_of<DB>(p.h), row * p.h.stride + col, p.D - col, r[v]);
@@ -286,6 +303,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
     const int team = threadIdx.x / LPR, lane = threadIdx.x % LPR;
     int turn = 0;
     const float per = 1.f / (float)p.D;
+    constexpr bool MOVE = NV == 1;
+    const bool is_short = p.D < kLot;
     auto column = [&](int v) { return kLot * (lane + LPR * v); };
     // the teams' sums to one row of floats
     auto leave = [&](auto &sum, float *to) {
@@ -331,14 +350,14 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
             for (int v = 0; v < NV; v++) {
                 const int col = column(v), left = p.D - col;
                 if (!live || left <= 0) continue;
-                block_raw[v] = request<TAIL>(p.block.ptr, type_of<DB>(p.block), row * p.block.stride + col, left);
-                if (p.gate.ptr) gate_raw[v] = request<TAIL>(p.gate.ptr, type_of<DB>(p.gate), gate_row * p.gate.stride + col, left);
+                block_raw[v] = request<TAIL, MOVE>(p.block.ptr, type_of<DB>(p.block), row * p.block.stride + col, left, is_short);
+                if (p.gate.ptr) gate_raw[v] = request<TAIL, MOVE>(p.gate.ptr, type_of<DB>(p.gate), gate_row * p.gate.stride + col, left, is_short);
                 if (p.before.kind != FTC_NORM_NONE) {
                     if (p.residual.ptr)
-                        residual_raw[v] = request<TAIL>(p.residual.ptr, type_of<DS>(p.residual), row * p.residual.stride + col, left);
-                    if (p.grad_h.ptr) gh_raw[v] = request<TAIL>(p.grad_h.ptr, type_of<DB>(p.grad_h), row * p.grad_h.stride + col, left);
+                        residual_raw[v] = request<TAIL, MOVE>(p.residual.ptr, type_of<DS>(p.residual), row * p.residual.stride + col, left, is_short);
+                    if (p.grad_h.ptr) gh_raw[v] = request<TAIL, MOVE>(p.grad_h.ptr, type_of<DB>(p.grad_h), row * p.grad_h.stride + col, left, is_short);
                 }
-                if (p.grad_x.ptr) gx_raw[v] = request<TAIL>(p.grad_x.ptr, type_of<DS>(p.grad_x), row * p.grad_x.stride + col, left);
+                if (p.grad_x.ptr) gx_raw[v] = request<TAIL, MOVE>(p.grad_x.ptr, type_of<DS>(p.grad_x), row * p.grad_x.stride + col, left, is_short);
             }
             Lot n[NV], dx[NV], gate[NV], xh[NV];
             float s0 = 0.f, s1 = 0.f;
@@ -348,15 +367,15 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
 #pragma unroll
                 for (int i = 0; i < kLot; i++) n[v].x[i] = dx[v].x[i] = xh[v].x[i] = gate[v].x[i] = 0.f;
                 if (!live || col >= p.D) continue;
-                n[v] = widen(block_raw[v], type_of<DB>(p.block));
-                if (p.gate.ptr) gate[v] = widen(gate_raw[v], type_of<DB>(p.gate));
+                n[v] = widen<TAIL, MOVE>(block_raw[v], type_of<DB>(p.block), p.D - column(v), is_short);
+                if (p.gate.ptr) gate[v] = widen<TAIL, MOVE>(gate_raw[v], type_of<DB>(p.gate), p.D - column(v), is_short);
 #pragma unroll
                 for (int i = 0; i < kLot; i++) n[v].x[i] = !TAIL || i < left ? (n[v].x[i] - mean_a) * rstd_a : 0.f;
                 if (p.before.kind == FTC_NORM_NONE) continue;
-                if (p.residual.ptr) xh[v] = widen(residual_raw[v], type_of<DS>(p.residual));
-                if (p.grad_h.ptr) dx[v] = widen(gh_raw[v], type_of<DB>(p.grad_h));
+                if (p.residual.ptr) xh[v] = widen<TAIL, MOVE>(residual_raw[v], type_of<DS>(p.residual), p.D - column(v), is_short);
+                if (p.grad_h.ptr) dx[v] = widen<TAIL, MOVE>(gh_raw[v], type_of<DB>(p.grad_h), p.D - column(v), is_short);
                 Lot w, b;
-                params_lot<TAIL>(p.after, col, left, w, b);
+                params_lot<TAIL, MOVE>(p.after, col, left, is_short, w, b);
 #pragma unroll
                 for (int i = 0; i < kLot; i++) {
                     const float y = fmaf(n[v].x[i], w.x[i], b.x[i]);
@@ -365,7 +384,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
                     const float a = value * y;
                     xh[v].x[i] = !TAIL || i < left ? (fmaf(p.scale, a, xh[v].x[i]) - mean_b) * rstd_b : 0.f;
                 }
-                params_lot<TAIL>(p.before, col, left, w, b);
+                params_lot<TAIL, MOVE>(p.before, col, left, is_short, w, b);
 #pragma unroll
                 for (int i = 0; i < kLot; i++) {
                     dwb[v].x[i] = fmaf(dx[v].x[i], xh[v].x[i], dwb[v].x[i]);
@@ -389,7 +408,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
                 const int col = column(v), left = p.D - col;
                 if (!live || col >= p.D) continue;
                 if (p.grad_x.ptr) {
-                    const Lot g = widen(gx_raw[v], type_of<DS>(p.grad_x));
+                    const Lot g = widen<TAIL, MOVE>(gx_raw[v], type_of<DS>(p.grad_x), p.D - column(v), is_short);
 #pragma unroll
                     for (int i = 0; i < kLot; i++) dx[v].x[i] += g.x[i];
                 }
@@ -399,7 +418,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_backward_
                 if (p.grad_residual.ptr)
                     store_lot<TAIL>(p.grad_residual.ptr, type_of<DS>(p.grad_residual), row * p.grad_residual.stride + col, left, dx[v]);
                 Lot w, b;
-                params_lot<TAIL>(p.after, col, left, w, b);
+                params_lot<TAIL, MOVE>(p.after, col, left, is_short, w, b);
                 if (p.gate.ptr) {
                     Lot d;
 #pragma unroll

@@ -265,3 +265,21 @@ def test_plain_and_watched_calls_agree_on_gates(gate):
         b, gg = (t.detach().double().cpu() for t in (block, g))
         want = norm.residual_norm(b, b, gg, ("rms", w.detach().double().cpu()), ("layer",), 1.0, "silu")
         assert norm.far(plain[0].detach(), want[0]) <= norm.FP32 and norm.far(plain[1].detach(), want[1]) <= norm.FP32
+
+
+@pytest.mark.parametrize("width", [3, 5, 9, 15, 37, 101, 1023, 4093, 8195])
+@pytest.mark.parametrize("dtype", [F, B])
+def test_tails_of_rows_keep_to_themselves(width, dtype):
+    """Rows that end inside a lane's eight values, with NaN before and behind them."""
+    gen = torch.Generator().manual_seed(width)
+    names = ("block", "residual", "gate")
+    t = {n: torch.randn(9, width, generator=gen).to(dtype) for n in names}
+    inside = {}
+    for n in names:
+        buffer = torch.full((9, width + 13), float("nan"), device="cuda", dtype=dtype)
+        view = buffer[:, 7:7 + width]
+        view.copy_(t[n])
+        inside[n] = view
+    go = [torch.ones(9, width, device="cuda", dtype=dtype)] * 2
+    for a, b in zip(gradients(inside, "layer", "rms", go), gradients({n: x.cuda() for n, x in t.items()}, "layer", "rms", go)):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
