@@ -16,7 +16,7 @@
 // All arithmetic is fp32; results are rounded once.
 //
 // Measured, forward | backward, of all bytes read and written: 40960 x 512, fp32, 76 us | 119 us, 4.4 | 4.2 TB/s; 16384 x 4096, bf16 beside
-// an fp32 stream, 188 | 390, 5.0 | 3.8; 524288 x 128, bf16, 97 | 147, 4.1 | 4.6 (a copy: 5.1).  The backward of rows above
+// an fp32 stream, 180 | 390, 5.2 | 3.8; 524288 x 128, bf16, 97 | 147, 4.1 | 4.6 (a copy: 5.1).  The backward of rows above
 // 2048 has one workgroup a compute unit, by its registers: held to 128 of them it spills (440 us), and with the next
 // row requested ahead it takes 430.
 #pragma once
