@@ -302,7 +302,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     using Tile = ColumnTile<T, VEC>;
     __shared__ __align__(16) char v_mem[W][Tile::kTile];
     __shared__ __align__(16) float f_mem[W][2][kRows];
-    __shared__ __align__(16) char kr_mem[SHARE ? 2 * kKeys : 16], kc_mem[SHARE ? 2 * kKeys : 16], t_mem[SHARE ? kTFrags * 3072 : 16];
+    __shared__ __align__(16) char kr_mem[SHARE ? 2 * kKeys : 16], kc_mem[SHARE ? 2 * kKeys : 16], t_mem[SHARE ? kTFrags * 3 * 1024 : 16];
     lds_char *const vp = (lds_char *)v_mem[wave], *const krp = (lds_char *)kr_mem, *const kcp = (lds_char *)kc_mem, *const tp = (lds_char *)t_mem;
     lds_float *const fp = (lds_float *)f_mem[wave];
     Left<W, 4 * KE, PIECES> kr, kc;
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     __shared__ __align__(16) char g_mem[W][Tile::kTile], through_mem[W][SHARE ? 16 : Tile::kTile];
     __shared__ __align__(16) float f_mem[W][4][kRows];
     // (shared: the rows of k and the columns of q take turns in one place)
-    __shared__ __align__(16) char in_mem[SHARE ? 2 * kKeys : 16], kc_mem[SHARE ? 2 * kKeys : 16], t_mem[SHARE ? kTFrags * 3072 : 16];
+    __shared__ __align__(16) char in_mem[SHARE ? 2 * kKeys : 16], kc_mem[SHARE ? 2 * kKeys : 16], t_mem[SHARE ? kTFrags * 3 * 1024 : 16];
     lds_char *const inp = (lds_char *)in_mem, *const kcp = (lds_char *)kc_mem, *const tp = (lds_char *)t_mem;
     lds_char *const gp = (lds_char *)g_mem[wave], *const through = SHARE ? gp : (lds_char *)through_mem[wave];
     lds_float *const fp = (lds_float *)f_mem[wave];

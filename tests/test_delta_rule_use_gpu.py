@@ -351,3 +351,25 @@ def test_few_long_chains_are_walked_in_segments(dtype, N, H, Hk, L, E, M):
     out, state = gated_delta_rule(*args[:5], return_state=True)          # without a state
     again, last = gated_delta_rule(*zero, return_state=True)
     assert torch.equal(out, again) and torch.equal(state, last)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_drawn_shapes(seed):
+    """Sizes, heads, lengths, layouts and options as they come, on every route of the kernels."""
+    import random
+    rng = random.Random(seed)
+    Hk = rng.choice([1, 2, 3])
+    N, H, L = rng.choice([1, 2, 5]), Hk * rng.choice([1, 2, 3]), rng.choice([1, 7, 9, 63, 64, 65, 200, 777, 1300])
+    E, M = rng.choice([1, 3, 16, 33, 64, 65, 96, 128]), rng.choice([1, 5, 16, 48, 64, 100, 128, 512])
+    dtype = rng.choice([torch.float32, torch.bfloat16])
+    if M == 512:
+        N, H, Hk = 1, 2, 1
+    normalize = E > 3 and rng.random() < 0.5      # (the gradient of a row's direction is all cancellation where it has one value)
+    args = ref.inputs(N, H, Hk, L, E, M, dtype=dtype, scalars=rng.choice([torch.float32, dtype]), device="cuda", seed=seed)
+    if rng.random() < 0.5:
+        args = [t.contiguous() for t in args]
+    go, gs = seeds(args)
+    lengths = rng.choice([None, [rng.randint(0, L) for _ in range(N)]])
+    print(N, H, Hk, L, E, M, dtype, normalize, lengths, flush=True)
+    got = results(args, go, gs, normalize=normalize, lengths=None if lengths is None else torch.tensor(lengths, device="cuda"))
+    check(got, wanted(args, go, gs, normalize=normalize, lengths=None if lengths is None else torch.tensor(lengths)))
