@@ -223,7 +223,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void residual_norm_kernel(Ar
     };
 
     for (int64_t base = (int64_t)blockIdx.x * kTeams; base < p.rows; base += (int64_t)gridDim.x * kTeams) {
-        const int64_t row = base + team, gate_row = p.every == 1 ? row : row / p.every;
+        const int64_t row = base + team, gate_row = p.every == 1 ? row : (uint32_t)row / (uint32_t)p.every;  // (fewer than 2^31)
         const bool live = row < p.rows;
         Raw block[NV], gate[NV], residual[NV];
 #pragma unroll
