@@ -18,8 +18,8 @@
 // head's value heads one after the other, so that the gradients of shared keys are summed in registers, in one
 // order.  Phase 1 walks the columns of the state, 32 at a time through LDS, the next 32 on their way meanwhile; a
 // wavefront has 32 positions (of eight: 16) of 32 key columns, and its share of the tiles of dO Z^T and dE Z^T.  Phase 2 multiplies the
-// 64 x 64 matrices with the rows.  Gradients of bf16 rows are made of values in two pieces (2^-17 of them is left out,
-// against half a step of 2^-8 that the rounding of the results takes).
+// 64 x 64 matrices with the rows.  What is not rows is in three pieces for bf16
+// rows too: of a normalised row's gradient what lies along the row is taken away again, and may be nearly all of it.
 //
 // What bounds it: the instructions that cut values into pieces and LDS, each about a third of the time with two workgroups a compute
 // unit, beside 2.2 GB of states, their gradients, Z, dE and rows.  Measured: 8192 chunks of 128 x 128 on 4096 of
@@ -48,7 +48,7 @@ __device__ __forceinline__ int renewed(int x) {
 
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(DeltaArgs p) {
-    constexpr int PIECES = Elem<T>::kPieces, NP = PIECES == 1 ? 2 : 3;
+    constexpr int PIECES = Elem<T>::kPieces, NP = 3;
     constexpr int RB = 2 * kSlice, EW = 2;
     constexpr int WAVES = kWaves<T>, kThreads = 64 * WAVES, RT = 8 / WAVES, XT = 12 / WAVES + (12 % WAVES != 0), BLOCKS = 8 / WAVES;
     constexpr int kMB = 32;                                // columns of the state at a time
@@ -149,10 +149,10 @@ __global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(Delt
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
             const int to = Plane<128>::addr(16 * (half + b) + (l & 15), slot);
-            store_pieces<NP>(zp + to, kSq, zr[b]);
-            store_pieces<NP>(dep + to, kSq, er[b]);
-            store_pieces<NP>(sp + to, kSq, sr[b]);
-            store_pieces<NP>(dsp + to, kSq, dr[b]);
+            store_pieces(zp + to, kSq, zr[b]);
+            store_pieces(dep + to, kSq, er[b]);
+            store_pieces(sp + to, kSq, sr[b]);
+            store_pieces(dsp + to, kSq, dr[b]);
             dot_z += er[b] * zr[b];
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -258,8 +258,8 @@ __global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(Delt
                 pt[r] = j <= i ? F[x][r] * d * rq_i : 0.f;
                 rt[r] = j < i ? -N[x][r] * d * rk_i : 0.f;
             }
-            store_pieces<NP>(pp + Plane<128>::addr(i, 4 * tj + q), kSquare, pt);
-            store_pieces<NP>(rp + Plane<128>::addr(i, 4 * tj + q), kSquare, rt);
+            store_pieces(pp + Plane<128>::addr(i, 4 * tj + q), kSquare, pt);
+            store_pieces(rp + Plane<128>::addr(i, 4 * tj + q), kSquare, rt);
         }
 #pragma unroll
         for (int t = 0; t < RT; t++)

@@ -143,11 +143,11 @@ __device__ __forceinline__ f32x4 mfma4(const f32x4 &a, const f32x4 &b, f32x4 acc
     for (int r = 0; r < 4; r++) acc = mfma4(a[r], b[r], acc);
     return acc;
 }
-// acc += A B over the piece products of order <= 2 (two pieces at most: <= 1), smallest first
+// acc += A B over the piece products of order <= 2, smallest first
 template <int NA, int NB>
 __device__ __forceinline__ f32x4 product(const Frag (&a)[NA], const Frag (&b)[NB], f32x4 acc) {
 #pragma unroll
-    for (int order = NA > 2 || NB > 2 ? 2 : 1; order >= 0; order--)
+    for (int order = 2; order >= 0; order--)
 #pragma unroll
         for (int pa = 0; pa < NA; pa++) {
             const int pb = order - pa;
@@ -160,7 +160,7 @@ __device__ __forceinline__ f32x4 product(const Frag (&a)[NA], const Frag (&b)[NB
 template <int FROM, int TILES, int NA, int NB>
 __device__ __forceinline__ void products(const Frag (&a)[TILES][NA], const Frag (&b)[NB], f32x4 (&acc)[TILES]) {
 #pragma unroll
-    for (int order = NA > 2 || NB > 2 ? 2 : 1; order >= 0; order--)
+    for (int order = 2; order >= 0; order--)
 #pragma unroll
         for (int pa = 0; pa < NA; pa++) {
             const int pb = order - pa;
@@ -299,29 +299,19 @@ __device__ __forceinline__ void columns_of(const lds_char *planes, int t, int s,
     for (int p = 0; p < PIECES; p++) f[p] = Plane<RB>::columns(planes + p * plane_bytes, t, s, c, q);
 }
 
-// Two values -> NP pieces.  Three add up to the value exactly; two leave 2^-17 of it (both rounded to nearest).
-template <int NP>
-__device__ __forceinline__ void pieces_of(float x0, float x1, uint32_t (&o)[NP]) {
-    if constexpr (NP == 3) {
-        mfma::split_pair_under_mfma(x0, x1, o);
-    } else {
-        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-        typedef float f32x2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-        for (int p = 0; p < NP; p++) {
-            o[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x0, x1}, bf16x2));
-            x0 -= __uint_as_float(o[p] << 16), x1 -= __uint_as_float(o[p] & 0xffff0000u);
-        }
-    }
+// Two values -> two bf16, rounded to nearest
+__device__ __forceinline__ uint32_t to_bf16(float x0, float x1) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x0, x1}, bf16x2));
 }
-// Four values of consecutive columns of a row -> the planes
-template <int NP = 3>
+// Four values of consecutive columns of a row -> the planes of their three pieces
 __device__ __forceinline__ void store_pieces(lds_char *to, int plane_bytes, const f32x4 &x) {
-    uint32_t a[NP], b[NP];
-    pieces_of<NP>(x[0], x[1], a);
-    pieces_of<NP>(x[2], x[3], b);
+    uint32_t a[3], b[3];
+    mfma::split_pair_under_mfma(x[0], x[1], a);
+    mfma::split_pair_under_mfma(x[2], x[3], b);
 #pragma unroll
-    for (int p = 0; p < NP; p++)
+    for (int p = 0; p < 3; p++)
         *(__attribute__((address_space(3))) u32x2a *)(to + p * plane_bytes) = u32x2{a[p], b[p]};
 }
 

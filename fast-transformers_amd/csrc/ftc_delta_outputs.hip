@@ -170,10 +170,7 @@ __global__ __launch_bounds__(kThreads) void delta_outputs_kernel(DeltaArgs p) {
                 if constexpr (Elem<T>::kBytes == 4) {
                     *(f32x4a *)to = O[t];
                 } else {
-                    uint32_t two[2][1];
-                    pieces_of<1>(O[t][0], O[t][1], two[0]);
-                    pieces_of<1>(O[t][2], O[t][3], two[1]);
-                    *(u32x2a *)to = u32x2{two[0][0], two[1][0]};
+                    *(u32x2a *)to = u32x2{to_bf16(O[t][0], O[t][1]), to_bf16(O[t][2], O[t][3])};
                 }
             }
         } else if (col < p.M)
