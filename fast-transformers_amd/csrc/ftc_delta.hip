@@ -1,5 +1,7 @@
 // C ABI entry points of the gated delta rule (include/ftc_causal_product.h): argument checking, workspaces and the
 // sequence of launches.  The kernels: ftc_delta_{prepare,scan,outputs,gradients,step}.hip.
+#include <cstdio>
+
 #include "ftc_delta_kernel.h"
 
 namespace ftc {
@@ -113,6 +115,12 @@ StateRef state(const ftc_tensor4 *t) {
 }
 OperandOut rows_out(const ftc_tensor4 *t) { return t ? as_operand_out(t) : OperandOut{}; }
 
+void place_sizes(const Sizes &s, DeltaArgs *p) {
+    p->N = (int32_t)s.N, p->H = (int32_t)s.H, p->Hk = (int32_t)s.Hk, p->L = (int32_t)s.L;
+    p->E = (int32_t)s.E, p->M = (int32_t)s.M;
+    p->chunks = (int32_t)s.chunks(), p->col_blocks = (int32_t)s.col_blocks();
+    p->segments = (int32_t)s.segments(), p->seg_chunks = (int32_t)s.segment_chunks(p->segments);
+}
 // The inputs that both directions have
 int read_inputs(const ftc_tensor4 *q, const ftc_tensor4 *k, const ftc_tensor4 *v, const ftc_tensor4 *g, const ftc_tensor4 *b,
                 Sizes *s, DeltaArgs *p) {
@@ -126,10 +134,7 @@ int read_inputs(const ftc_tensor4 *q, const ftc_tensor4 *k, const ftc_tensor4 *v
     if (int rc = check_rows(b, "beta", s->N, s->H, s->L, 1, -1)) return rc;
     p->q = as_operand(q), p->k = as_operand(k), p->v = as_operand(v);
     p->g = scalars(g), p->b = scalars(b);
-    p->N = (int32_t)s->N, p->H = (int32_t)s->H, p->Hk = (int32_t)s->Hk, p->L = (int32_t)s->L;
-    p->E = (int32_t)s->E, p->M = (int32_t)s->M;
-    p->chunks = (int32_t)s->chunks(), p->col_blocks = (int32_t)s->col_blocks();
-    p->segments = (int32_t)s->segments(), p->seg_chunks = (int32_t)s->segment_chunks(p->segments);
+    place_sizes(*s, p);
     p->vec_q = reads_wide(p->q), p->vec_k = reads_wide(p->k), p->vec_v = reads_wide(p->v);
     return FTC_OK;
 }
@@ -176,6 +181,29 @@ int64_t ftc_gated_delta_rule_kept_bytes(int64_t N, int64_t H, int64_t Hk, int64_
 int64_t ftc_gated_delta_rule_backward_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M,
                                                       int32_t dtype) {
     return delta_bytes(N, H, Hk, L, E, M, dtype, 2);
+}
+
+int ftc_gated_delta_plan(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M, int32_t dtype, int32_t keep, char *text,
+                         size_t text_bytes) {
+    if (!text || text_bytes == 0) return fail(FTC_ERR_INVALID, "null argument");
+    text[0] = 0;
+    const Sizes s{N, H, Hk, L, E, M, dtype};
+    if (dtype != FTC_F32 && dtype != FTC_BF16) return fail(FTC_ERR_INVALID, "unknown dtype code %d", (int)dtype);
+    if (int rc = check_sizes(s)) return rc;
+    if (s.N * s.H == 0) return FTC_OK;
+    if (s.L == 0 || (!keep && s.L <= kStepMost)) {
+        snprintf(text, text_bytes, "steps");
+        return FTC_OK;
+    }
+    DeltaArgs p = {};
+    place_sizes(s, &p);
+    const bool bf16 = dtype == FTC_BF16;
+    if (p.segments == 1)
+        snprintf(text, text_bytes, "chunks %d, scan %d", (int)p.chunks, delta_scan_shared_by(p, bf16, false));
+    else
+        snprintf(text, text_bytes, "chunks %d, segments %d, maps %d, scan %d", (int)p.chunks, (int)p.segments,
+                 delta_scan_shared_by(p, bf16, true), delta_scan_shared_by(p, bf16, false));
+    return FTC_OK;
 }
 
 int ftc_gated_delta_rule(const ftc_tensor4 *queries, const ftc_tensor4 *keys, const ftc_tensor4 *values,

@@ -376,5 +376,8 @@ int delta_scan_back(const DeltaArgs &p, bool bf16, hipStream_t stream);
 int delta_gradients(const DeltaArgs &p, bool bf16, hipStream_t stream);
 int delta_steps(const DeltaArgs &p, hipStream_t stream);                        // position by position
 
+// How many wavefronts of a scan share its operands (first: in the launch that makes the segments' maps)
+int delta_scan_shared_by(const DeltaArgs &p, bool bf16, bool first);
+
 }  // namespace delta
 }  // namespace ftc

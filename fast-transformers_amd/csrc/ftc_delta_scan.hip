@@ -576,14 +576,13 @@ void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
     if (back) delta_scan_back_kernel<T, KE, VEC, W, MAP><<<grid, 64 * W, 0, stream>>>(p);
     else delta_scan_kernel<T, KE, VEC, W, MAP><<<grid, 64 * W, 0, stream>>>(p);
 }
+constexpr bool fits_registers(int pieces, int ke) { return pieces * ke <= 6; }
 template <typename T, int KE, bool VEC, bool MAP>
 void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
-    const int64_t waves = (int64_t)p.N * p.H * blocks_of<MAP>(p) * (p.segments > 1 ? p.segments - 1 : 1);
-    if (Elem<T>::kPieces * KE > 6 || waves > 512) launch<T, KE, VEC, 4, MAP>(p, back, stream);
-    else if constexpr (Elem<T>::kPieces * KE <= 6) {
-        if (waves > 256 && blocks_of<MAP>(p) % 2 == 0) launch<T, KE, VEC, 2, MAP>(p, back, stream);
-        else launch<T, KE, VEC, 1, MAP>(p, back, stream);
-    }
+    const int shared_by = delta_scan_shared_by(p, Elem<T>::kPieces == 1, MAP);
+    if (shared_by == 4) launch<T, KE, VEC, 4, MAP>(p, back, stream);
+    else if constexpr (fits_registers(Elem<T>::kPieces, KE))
+        shared_by == 2 ? launch<T, KE, VEC, 2, MAP>(p, back, stream) : launch<T, KE, VEC, 1, MAP>(p, back, stream);
 }
 template <typename T, int KE, bool VEC>
 void launch(const DeltaArgs &p, bool back, hipStream_t stream) {
@@ -602,6 +601,12 @@ int dispatch(const DeltaArgs &p, bool bf16, bool vec, bool back, hipStream_t str
 
 }  // namespace
 
+int delta_scan_shared_by(const DeltaArgs &p, bool bf16, bool first) {
+    const int blocks = first ? blocks_of<true>(p) : blocks_of<false>(p);
+    const int64_t waves = (int64_t)p.N * p.H * blocks * (p.segments > 1 ? p.segments - 1 : 1);
+    if (!fits_registers(bf16 ? 1 : 3, p.E <= 64 ? 2 : 4) || waves > 512) return 4;
+    return waves > 256 && blocks % 2 == 0 ? 2 : 1;
+}
 int delta_scan(const DeltaArgs &p, bool bf16, hipStream_t stream) { return dispatch(p, bf16, p.vec_v, false, stream); }
 int delta_scan_back(const DeltaArgs &p, bool bf16, hipStream_t stream) { return dispatch(p, bf16, p.vec_go && p.vec_gv, true, stream); }
 

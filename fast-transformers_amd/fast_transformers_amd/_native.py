@@ -46,6 +46,7 @@ EXPORTED_SYMBOLS = (
     "ftc_layer_norm_stats_split",
     "ftc_linear_split",
     "ftc_linear_split_normed",
+    "ftc_gated_delta_plan",
     "ftc_gated_delta_rule_workspace_bytes",
     "ftc_gated_delta_rule_kept_bytes",
     "ftc_gated_delta_rule",
@@ -170,6 +171,8 @@ def load():
         f = getattr(lib, name)
         f.restype = ctypes.c_int64
         f.argtypes = [ctypes.c_int64] * 6 + [ctypes.c_int32]
+    lib.ftc_gated_delta_plan.restype = ctypes.c_int
+    lib.ftc_gated_delta_plan.argtypes = [ctypes.c_int64] * 6 + [ctypes.c_int32] * 2 + [ctypes.c_char_p, ctypes.c_size_t]
     scalars = [ctypes.c_void_p, ctypes.c_float, ctypes.c_int32]  # lengths, scale, normalize
     memory = [ctypes.c_void_p, ctypes.c_size_t]
     lib.ftc_gated_delta_rule.restype = ctypes.c_int
@@ -210,6 +213,13 @@ def plan(shape_q, shape_v, dtype=FTC_F32, backward=False, strides=None):
     rc = load().ftc_causal_dot_plan(ctypes.byref(q), ctypes.byref(k), ctypes.byref(v),
                                     1 if backward else 0, buf, len(buf))
     check(rc, "ftc_causal_dot_plan")
+    return buf.value.decode()
+
+
+def delta_plan(N, H, Hk, L, E, M, dtype=FTC_F32, keep=True):
+    """Text of ``ftc_gated_delta_plan``: how the gated delta rule walks a call of these sizes.  Needs no GPU."""
+    buf = ctypes.create_string_buffer(256)
+    check(load().ftc_gated_delta_plan(N, H, Hk, L, E, M, dtype, 1 if keep else 0, buf, len(buf)), "ftc_gated_delta_plan")
     return buf.value.decode()
 
 

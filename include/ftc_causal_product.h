@@ -363,6 +363,14 @@ int ftc_gated_delta_rule(const ftc_tensor4 *queries, const ftc_tensor4 *keys, co
                          size_t workspace_bytes, void *stream);
 
 /*
+ * How ftc_gated_delta_rule (keep != 0: with `kept`, and its backward) walks a call of these sizes, written to `text`: "steps"
+ * (position by position), or "chunks C, scan W", or "chunks C, segments S, maps W, scan W", where W wavefronts
+ * share a scan's operands.  Nothing is launched and no GPU is needed.  For tests that mean to reach a route.
+ */
+int ftc_gated_delta_plan(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M, int32_t dtype, int32_t keep, char *text,
+                         size_t text_bytes);
+
+/*
  * Its gradients, given grad_out and grad_final_state (NULL: zeros) and what the forward kept.  The inputs are
  * those of the forward; gradients have their inputs' dtypes (grad_initial_state: FTC_F32), those of positions past
  * a sequence's end are zero, and one that is not wanted may be NULL.  L >= 1.
