@@ -178,7 +178,9 @@ __global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(Delt
         float o = 0.f;  // (dO . O of a row, for the normalisation)
         if (p.normalize && wave == 3)
             for (int b = 0; b < p.col_blocks; b++) o += p.dots[(at * p.col_blocks + b) * kRows + lane];
-        for (int i = tid; i < kFactors * kRows; i += kThreads) fp[i] = p.factors[at * (kFactors * kRows) + i];
+        static_assert(kFactors * kRows == 4 * 256, "four floats a lane");
+        if (tid < 256)
+            *(__attribute__((address_space(3))) f32x4a *)(fp + 4 * tid) = *(const f32x4a *)(p.factors + at * (kFactors * kRows) + 4 * tid);
 
         // ---- phase 1 ----
         f32x4 F[XT] = {}, N[XT] = {};                                    // (dO Z^T)^T, (dE Z^T)^T
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(Delt
             int ti, tj;
             tile_of(x, ti, tj);
             const int i = 16 * ti + c, j0 = 16 * tj + 4 * q;
-            const float rk_i = fp[kRk * kRows + i], rq_i = fp[kRq * kRows + i];
+            const float rk_i = fp[kRkBack * kRows + i], rq_i = fp[kRq * kRows + i];
             f32x4 pt, rt;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
@@ -266,7 +268,7 @@ __global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(Delt
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int row = 16 * (t0 + t) + 4 * q + r;
-                const float read_q = fp[kReadQ * kRows + row], read_k = fp[kReadK * kRows + row], write = fp[kWrite * kRows + row];
+                const float read_q = fp[kReadQ * kRows + row], read_k = fp[kReadBack * kRows + row], write = fp[kWrite * kRows + row];
 #pragma unroll
                 for (int e = 0; e < EW; e++) {
                     dQ[t][e][r] = fmaf(read_q, aQ[t][e][r], dQ[t][e][r]);
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(Delt
                 state += (state_mem[WAVES - 4] + state_mem[WAVES - 3]) + (state_mem[WAVES - 2] + state_mem[WAVES - 1]);
             if (lane == 0) p.sums[at * kSums + 2 * kRows + slice] = state;
         } else if (p.normalize && wave == 3) {
-            total_mem[0][lane] += o, total_mem[1][lane] += 2.f * dots_of(0) - dots_of(1);
+            total_mem[0][lane] += o, total_mem[1][lane] += fp[kRkBack * kRows + lane] == 0.f ? 0.f : 2.f * dots_of(0) - dots_of(1);
         }
         __syncthreads();
 #pragma unroll
@@ -449,14 +451,14 @@ __device__ __forceinline__ void find_astride(const DeltaArgs &p, const Where &w,
             for (int r = 0; r < 4; r++) {
                 const int i = 16 * ti + q4 + r;
                 const float fade = expf((factors[kHigh * kRows + i] - high) + (factors[kLow * kRows + i] - low));
-                const float x = factors[kRq * kRows + i] * A[back][r] * P[back][r] - factors[kRk * kRows + i] * K[back][r] * R[back][r];
+                const float x = factors[kRq * kRows + i] * A[back][r] * P[back][r] - factors[kRkBack * kRows + i] * K[back][r] * R[back][r];
                 pairs[33 * i + c + 16 - 16 * back] = j >= 0 && j < i && i < valid ? fade * beta * x : 0.f;
             }
         }
     }
     // what positions 0 to 15 read of the state before the chunk, and what the last ones' two tiles write to the one after
     const int last = (valid - 1) / 16, but_one = last > 0 ? last - 1 : 0;
-    const f32x4 by_q = *(const f32x4a *)(factors + kReadQ * kRows + q4), by_k = *(const f32x4a *)(factors + kReadK * kRows + q4);
+    const f32x4 by_q = *(const f32x4a *)(factors + kReadQ * kRows + q4), by_k = *(const f32x4a *)(factors + kReadBack * kRows + q4);
     const f32x4 by0 = *(const f32x4a *)(factors + kWrite * kRows + 16 * last + q4);
     const f32x4 by1 = *(const f32x4a *)(factors + kWrite * kRows + 16 * but_one + q4);
     f32x4 read = {0.f, 0.f, 0.f, 0.f}, write0 = read, write1 = read;
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(256, 4) void delta_decays_kernel(DeltaArgs p) {
             o += p.dots[(w.at * p.col_blocks + b) * kRows + lane];
             written += p.written[(w.at * p.col_blocks + b) * 64 + lane];
         }
-        const float z = sums[lane], v = sums[kRows + lane], beta = factors[kBeta * kRows + lane];
+        const float z = sums[lane], v = sums[kRows + lane], beta = factors[kBetaBack * kRows + lane];
         const float high = factors[kHigh * kRows + lane], before = __shfl_up(high, 1);
         const bool apart = w.valid <= kFew || __all(lane == 0 || lane >= w.valid || high - before <= kStrong);
         sums_mem[0][wave][lane] = o, sums_mem[1][wave][lane] = written;
@@ -543,7 +545,9 @@ __global__ __launch_bounds__(256, 4) void delta_decays_kernel(DeltaArgs p) {
             dg = through + add_astride((const lds_float *)astride_mem, w.valid, lane);
         } else {
             auto all_of = [&](int i) { return (sums_mem[i][0][lane] + sums_mem[i][1][lane]) + (sums_mem[i][2][lane] + sums_mem[i][3][lane]); };
-            double sum = (double)all_of(0) - (double)v, all = all_of(1);
+            // (a beta that the backward has for zero: neither read nor written)
+            const bool shut = beta == kLeastBeta;
+            double sum = (double)all_of(0) - (double)(shut ? 0.f : v), all = __all(shut || lane >= w.valid) ? 0.f : all_of(1);
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
             all += (double)through;

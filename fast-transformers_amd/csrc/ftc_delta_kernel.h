@@ -52,7 +52,7 @@ constexpr float kNormEps = 1e-6f;
 enum Factor {
     kRise,   // e^{G_i}
     kFall,   // e^{G_64 - G_i}
-    kBeta,   // beta_i (0 past the sequence's end, at least 2^-64 in size before it)
+    kBeta,   // beta_i (0 past the sequence's end)
     kRk,     // 1 / |k_i|, or 1
     kRq,     // scale / |q_i|, or scale
     kRq0,    // 1 / |q_i|, or 1
@@ -62,8 +62,15 @@ enum Factor {
     kReadQ,  // rq e^{G_i}
     kWriteK, // rk e^{G_64 - G_i}: as it is written
     kWrite,  // ... times beta_i
+    // for the backward, with betas that it can divide by: dbeta is found as dE . Z / beta (all terms of dE have that factor).  Up
+    // to 2^-64 in size they count as that there, and such rows of dE for nothing else: their other factors are zero.
+    kBetaBack,
+    kWriteBack,
+    kReadBack,  // kReadK, or 0
+    kRkBack,    // kRk, or 0
     kFactors
 };
+constexpr float kLeastBeta = 0x1p-64f;
 constexpr int kSums = 3 * kRows;
 
 struct Scalars {  // one value per position: log decays, beta and their gradients

@@ -438,7 +438,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     auto load_in = [&](int chunk) { kr.load(p.kr + (w.key_at + chunk) * kKeys, wave, lane); };
     auto load_rows = [&](int chunk) {
         const __amdgpu_buffer_rsrc_t rs = factor_rows(p, w.at + chunk);
-        write.load(rs, kWrite, lane), beta.load(rs, kBeta, lane), read_q.load(rs, kReadQ, lane), read_k.load(rs, kReadK, lane);
+        write.load(rs, kWriteBack, lane), beta.load(rs, kBetaBack, lane), read_q.load(rs, kReadQ, lane), read_k.load(rs, kReadBack, lane);
         decay = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (kRows * kRise + kRows - 1), 0, 0));
         load_tiles(p.de + tiles(chunk), Y);
         load_tiles(p.z + tiles(chunk), Z);
@@ -462,6 +462,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
         write.put(fp, lane), beta.put(fp + kRows, lane);
         read_q.put(fp + 2 * kRows, lane), read_k.put(fp + 3 * kRows, lane);
         const float fade = decay;
+        const bool shut = !MAP && __any(beta.x == kLeastBeta);
         if (SHARE) meet<W>();
         if (here) {
             float *const to = p.ds + at * (ET * 256) + 4 * lane;
@@ -481,16 +482,20 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
             products<0>(a, sf, P);
         }
         // diag(beta) dU
-        f32x4 written = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             P[t] *= write_rows[t];
             D[t] = MAP && part.map ? P[t] : beta_rows[t] * Y[t] + P[t];
-            written += Z[t] * P[t];
-            P[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         if (SHARE || MAP) settle();
-        if (here) p.written[at * 64 + lane] = (written[0] + written[1]) + (written[2] + written[3]);
+        if (here) {
+            f32x4 written = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < 4; t++) written += Z[t] * P[t];
+            p.written[at * 64 + lane] = (written[0] + written[1]) + (written[2] + written[3]);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) P[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         phase();
         tf.put(tp, wave, lane);
         if (SHARE) load_t(next), load_rows(next);
@@ -517,14 +522,24 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
             if (s == 0) products<0>(*(Frag(*)[2][3])&a, df, head);
             else products<0>(a, df, P);
         }
-        if (SHARE) phase(), qc.put(inp, wave, lane), load_q(next), load_g(next), settle();
-        if (MAP) settle();
+        if (SHARE) phase(), qc.put(inp, wave, lane), load_q(next), load_g(next);
+        settle();
         if (here) store_tiles(p.de + at * (4 * 256) + 4 * lane, P);
-        if (here && p.gv.ptr)
+        if (here && p.gv.ptr) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) D[t] = P[t];
+            // rows of dE that are there for dbeta alone (a branch costs the launch of the maps 10 %, the others 6 % without it)
+            if (MAP || shut)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const f32x4 b = FactorRow::rows(fp + kRows, t, q);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) D[t][r] = b[r] == kLeastBeta ? 0.f : P[t][r];
+                }
             Tile::store(chunk_rows(Operand{p.gv.ptr, p.gv.stride_n, p.gv.stride_h, p.gv.stride_l, 0, 0}, w.n, w.h,
                                    (int64_t)chunk * kRows, Elem<T>::kBytes),
-                        gv_row, kCols * block, p.M, min(kRows, w.len - chunk * kRows), lane, P, through);
-        settle();
+                        gv_row, kCols * block, p.M, min(kRows, w.len - chunk * kRows), lane, D, through);
+        }
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             G[t] *= read_q_rows[t];

@@ -141,7 +141,8 @@ def gated_delta_rule(queries, keys, values, log_decay, beta, initial_state=None,
     last position, float32.  E is at most 128, M at most 512.  Differentiable once, with respect to everything
     but ``lengths``, ``scale`` and ``normalize``; a call that will be differentiated keeps the states
     before every 64th position and what the chunks were solved with: 3 KB a position and value head at E = M = 128 in
-    bfloat16, 2 KB at 64 in float32.  Log decays are meant to be at most zero."""
+    bfloat16, 2 KB at 64 in float32.  Log decays are meant to be at most zero.  A ``beta`` of zero writes nothing (in
+    gradients, nor does one of up to ``2 ** -64`` in size)."""
     if queries.dim() != 4:
         raise RuntimeError("gated_delta_rule: expected queries (N, Hk, L, E), got %s" % (tuple(queries.shape),))
     if queries.device.type != "cuda":  # (the native code checks for itself)

@@ -373,7 +373,8 @@ int ftc_gated_delta_plan(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E,
 /*
  * Its gradients, given grad_out and grad_final_state (NULL: zeros) and what the forward kept.  The inputs are
  * those of the forward; gradients have their inputs' dtypes (grad_initial_state: FTC_F32), those of positions past
- * a sequence's end are zero, and one that is not wanted may be NULL.  L >= 1.
+ * a sequence's end are zero, and one that is not wanted may be NULL.  L >= 1.  A beta of up to 2^-64 in size counts
+ * as zero here, but for its own gradient.
  */
 int64_t ftc_gated_delta_rule_backward_workspace_bytes(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t M,
                                              int32_t dtype);

@@ -1,5 +1,5 @@
-"""The gated delta rule where a result is much smaller than what it is made of: gradients of normalised rows that nearly
-cancel."""
+"""The gated delta rule where a result is much smaller than what it is made of, or exactly nothing: gradients of normalised
+rows that nearly cancel, positions that write nothing."""
 import pytest
 import torch
 
@@ -67,3 +67,57 @@ def test_gradients_along_normalised_rows(made_of, L, dtype):
     error, limit = (got - want).norm().item(), 16 * 2.0 ** -24 * whole.norm().item()
     print("error %.3g of the whole, limit %.3g" % (error / whole.norm().item(), 16 * 2.0 ** -24), flush=True)
     assert error <= limit + (2.0 ** -8 * want.norm().item() if dtype == B else 0.0)
+
+
+@pytest.mark.parametrize("keep", [False, True], ids=["inference", "training"])
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("L", [5, 20, 200, 1100])
+def test_a_beta_of_zero_writes_nothing(L, dtype, keep):
+    q, k, v, g, b, s0 = ref.inputs(1, 2, 1, L, 40, 24, dtype=dtype, device="cuda", seed=L)
+    if keep:
+        v.requires_grad_(True)
+    out, state = gated_delta_rule(q, k, v, g, torch.zeros_like(b), return_state=True)
+    assert not out.any() and not state.any()                             # nothing was there, nothing has come
+    b = torch.where(torch.arange(L, device="cuda") % 3 == 1, 0.0, b)
+    first = gated_delta_rule(q, k, v, g, b, s0, return_state=True)
+    with torch.no_grad():
+        v[:, :, 1::3] = 1e30 * torch.sign(v[:, :, 1::3])                 # what such a position would write is not looked at
+    for x, y in zip(first, gated_delta_rule(q, k, v, g, b, s0, return_state=True)):
+        assert torch.equal(x, y)
+    tiny = torch.full_like(b, 2.0 ** -100)                               # a write of next to nothing is what it is
+    out, state = gated_delta_rule(q, k, v, g, tiny, return_state=True)
+    with torch.no_grad():
+        full, whole = gated_delta_rule(*(t.double().cpu().float() for t in (q, k, v.sign(), g, tiny)), return_state=True)
+    assert state.abs().max() <= 2.0 ** -80 * v.detach().abs().max()      # (at most 1100 writes of 2^-100 v)
+    assert whole.abs().max() > 0
+
+
+@pytest.mark.parametrize("normalize", [False, True])
+@pytest.mark.parametrize("L", [1, 64, 130])
+def test_gradients_where_beta_is_zero(L, normalize):
+    args = ref.inputs(2, 4, 2, L, 24, 40, device="cuda", seed=L)
+    args[4][:, :, ::2] = 0.0
+    args[4][0, 1] = 0.0
+    gen = torch.Generator().manual_seed(L)
+    go = torch.randn(args[2].shape, generator=gen).cuda()
+    gs = 0.3 * torch.randn(args[5].shape, generator=gen).cuda()
+    got, want = gradients(args, go, gs, normalize=normalize), wanted(args, go, gs, normalize=normalize)
+    errors = [ref.far(a, b) for a, b in zip(got, want)]
+    print(["%.2g" % e for e in errors], flush=True)
+    assert max(errors) <= ref.FP32, errors
+    assert not got[4][:, :, ::2].any()                                   # (values there are not written)
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("shape", [(2, 4, 2, 70, 24, 40), (1, 2, 1, 1000, 40, 24), (4, 16, 8, 70, 64, 96), (8, 15, 5, 70, 100, 77)])
+def test_nothing_comes_of_betas_of_zero(shape, dtype):
+    """From no state, and with gradients of the outputs alone, everything but the gradient of beta is exactly zero."""
+    args = ref.inputs(*shape, dtype=dtype, device="cuda", seed=1)
+    args[4].zero_()
+    args[5].zero_()
+    go = torch.randn(args[2].shape, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    out, state, gq, gk, gv, gg, gb, gs = gradients(args, go, torch.zeros_like(args[5]), normalize=True)
+    for name, t in dict(out=out, state=state, gq=gq, gk=gk, gv=gv, gg=gg).items():
+        assert not t.any(), name
+    want = wanted(args, go, torch.zeros_like(args[5]), normalize=True)
+    assert ref.far(gb, want[6]) <= ref.FP32 and ref.far(gs, want[7]) <= ref.FP32
