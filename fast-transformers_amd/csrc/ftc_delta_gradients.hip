@@ -325,6 +325,7 @@ __global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(Delt
 
     renew(c, q);
     if (valid > 0 && p.normalize) {  // (the factors of the last head: those of q and k are alike)
+        const bool one = p.E == 1;
         auto row_value = [&](const lds_char *planes, int row, int col) {
             float v = 0.f;
 #pragma unroll
@@ -339,12 +340,14 @@ __global__ __launch_bounds__(64 * kWaves<T>, 2) void delta_gradients_kernel(Delt
             for (int r = 0; r < 4; r++) {
                 const int row = 16 * (t0 + t) + 4 * q + r;
                 const float rq = fp[kRq0 * kRows + row], rk = fp[kRk * kRows + row];
-                const float fq = total_mem[0][row] * rq * rq, fk = total_mem[1][row] * rk * rk;
+                // (of a row of one value eps / (x^2 + eps) is left, which the difference would lose)
+                const float fq = one ? 0.f : total_mem[0][row] * rq * rq, fk = one ? 0.f : total_mem[1][row] * rk * rk;
+                const float left_q = one ? kNormEps * rq * rq : 1.f, left_k = one ? kNormEps * rk * rk : 1.f;
 #pragma unroll
                 for (int e = 0; e < EW; e++) {
                     const int col = 16 * (e0 + e) + c;
-                    dQ[t][e][r] = fmaf(-fq, row_value(qp, row, col), dQ[t][e][r]);
-                    dK[t][e][r] = fmaf(-fk, row_value(kp, row, col), dK[t][e][r]);
+                    dQ[t][e][r] = fmaf(-fq, row_value(qp, row, col), left_q * dQ[t][e][r]);
+                    dK[t][e][r] = fmaf(-fk, row_value(kp, row, col), left_k * dK[t][e][r]);
                 }
             }
     }

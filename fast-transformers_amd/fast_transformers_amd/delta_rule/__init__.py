@@ -82,7 +82,10 @@ class GatedDeltaRule(torch.autograd.Function):
 
 
 def _unit(x, normalize):
-    return x * torch.rsqrt((x * x).sum(-1, keepdim=True) + _EPS) if normalize else x
+    if not normalize:
+        return x
+    x = x.double()  # (of a row of one value the gradient leaves eps / (x^2 + eps) of what it is a difference of)
+    return (x * torch.rsqrt((x * x).sum(-1, keepdim=True) + _EPS)).float()
 
 
 def _solve_lower(strict, rows):

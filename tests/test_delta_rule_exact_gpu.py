@@ -1,5 +1,5 @@
 """The gated delta rule where a result is much smaller than what it is made of, or exactly nothing: gradients of normalised
-rows that nearly cancel, positions that write nothing."""
+rows that nearly cancel, rows of few values, positions that write nothing."""
 import pytest
 import torch
 
@@ -67,6 +67,22 @@ def test_gradients_along_normalised_rows(made_of, L, dtype):
     error, limit = (got - want).norm().item(), 16 * 2.0 ** -24 * whole.norm().item()
     print("error %.3g of the whole, limit %.3g" % (error / whole.norm().item(), 16 * 2.0 ** -24), flush=True)
     assert error <= limit + (2.0 ** -8 * want.norm().item() if dtype == B else 0.0)
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("L", [1, 70, 200])
+@pytest.mark.parametrize("E", [1, 2, 3, 4, 5, 8, 12, 15])
+def test_normalised_rows_of_few_values(E, L, dtype):
+    """Of one value nothing but its sign matters: the gradient is 1e-6 / (x^2 + 1e-6) of the whole, not its rounding."""
+    args = ref.inputs(2, 4, 2, L, E, 24, dtype=dtype, device="cuda", seed=E, unit=False)
+    gen = torch.Generator().manual_seed(E)
+    go = torch.randn(args[2].shape, generator=gen).to(dtype).cuda()
+    gs = 0.3 * torch.randn(args[5].shape, generator=gen).cuda()
+    got, want = gradients(args, go, gs, normalize=True), wanted(args, go, gs, normalize=True)
+    errors = [ref.far(a, b) for a, b in zip(got, want)]
+    print(["%.2g" % e for e in errors], flush=True)
+    for a, e in zip(got, errors):
+        assert e <= ref.tolerance(a.dtype), errors
 
 
 @pytest.mark.parametrize("keep", [False, True], ids=["inference", "training"])
