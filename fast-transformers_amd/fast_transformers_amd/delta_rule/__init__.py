@@ -103,12 +103,12 @@ def _cpu_rule(queries, keys, values, log_decay, beta, state, lengths, scale, nor
     """CPU tensors: chunks of positions, each solved for its writes, in float32; autograd differentiates it."""
     N, H, L, M = values.shape
     group = H // queries.shape[1] if H else 1
+    if lengths is not None:  # (before anything is made of them: gradients of what is masked afterwards may be 0 x NaN)
+        valid = (torch.arange(L, device=values.device) < lengths[:, None])[:, None]
+        queries, keys, values = (torch.where(valid[..., None], t, 0.0) for t in (queries, keys, values))
+        log_decay, beta = (torch.where(valid, t, 0.0) for t in (log_decay, beta))
     q, k = (_unit(t.float(), normalize).repeat_interleave(group, 1) for t in (queries, keys))
     v, g, b = values.float(), log_decay.float().clamp_min(-1000.0), beta.float()
-    if lengths is not None:
-        valid = (torch.arange(L, device=v.device) < lengths[:, None])[:, None]
-        q, k, v = (torch.where(valid[..., None], t, 0.0) for t in (q, k, v))
-        g, b = (torch.where(valid, t, 0.0) for t in (g, b))
     S = v.new_zeros((N, H, q.shape[3], M)) if state is None else state
     outs = []
     for lo in range(0, L, _CPU_CHUNK):
@@ -125,6 +125,8 @@ def _cpu_rule(queries, keys, values, log_decay, beta, state, lengths, scale, nor
         outs.append(scale * (rise * torch.matmul(qc, S) + torch.matmul(A, u)))
         S = rise[:, :, -1:] * S + torch.matmul((fall * kc).transpose(-1, -2), u)
     out = torch.cat(outs, 2) if outs else v.new_zeros((N, H, 0, M))
+    if lengths is not None:
+        out = torch.where(valid[..., None], out, 0.0)
     return out.to(values.dtype), S if outs or state is None else S.clone()
 
 

@@ -23,3 +23,21 @@ def test_normalised_rows_of_few_values(E, L):
     want = gradients([t.double() for t in args], go.double(), gs.double(), ref.rule, scale=E ** -0.5, normalize=True)
     errors = [ref.far(a, b) for a, b in zip(got, want)]
     assert max(errors) <= ref.FP32, errors
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("normalize", [False, True])
+def test_gradients_do_not_look_at_masked_rows(normalize, dtype):
+    args = ref.inputs(3, 4, 2, 20, 8, 6, dtype=dtype, scalars=dtype, seed=4)
+    gen = torch.Generator().manual_seed(1)
+    go, gs = torch.randn(args[2].shape, generator=gen).to(dtype), torch.randn(args[5].shape, generator=gen)
+    options = dict(normalize=normalize, lengths=torch.tensor([13, 0, 1]), return_state=True)
+    clean = gradients(args, go, gs, **options)
+    dirty, spoiled = [t.clone() for t in args], go.clone()
+    for t in dirty[:5] + [spoiled]:
+        t[0, :, 13:], t[1], t[2, :, 1:] = float("nan"), float("inf"), torch.finfo(dtype).min
+    got = gradients(dirty, spoiled, gs, **options)
+    for a, b in zip(got, clean):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    for grad in got[2:7]:
+        assert not grad[0, :, 13:].any() and not grad[1].any() and not grad[2, :, 1:].any()
