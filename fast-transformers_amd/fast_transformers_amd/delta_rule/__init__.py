@@ -102,7 +102,7 @@ def _solve_lower(strict, rows):
 def _cpu_rule(queries, keys, values, log_decay, beta, state, lengths, scale, normalize):
     """CPU tensors: chunks of positions, each solved for its writes, in float32; autograd differentiates it."""
     N, H, L, M = values.shape
-    group = H // queries.shape[1] if H else 1
+    group = H // max(1, queries.shape[1])
     if lengths is not None:  # (before anything is made of them: gradients of what is masked afterwards may be 0 x NaN)
         valid = (torch.arange(L, device=values.device) < lengths[:, None])[:, None]
         queries, keys, values = (torch.where(valid[..., None], t, 0.0) for t in (queries, keys, values))

@@ -826,6 +826,9 @@ std::vector<OptTensor> delta_rule_backward(const Tensor &queries, const Tensor &
                                     : at::empty({x.size(0), x.size(2), x.size(1)}, x.options()).permute({0, 2, 1});
         }
     if (needed[5]) grads[5] = at::empty({N, H, E, M}, t.q.options().dtype(at::kFloat));
+    if (N * H == 0)  // (key heads that no value head reads: nothing is launched)
+        for (const OptTensor &grad : grads)
+            if (grad) grad->zero_();
     auto wide = [](const OptTensor &x) { return x ? OptTensor(x->unsqueeze(3)) : OptTensor(); };
     const Out gq(grads[0], "grad_queries"), gk(grads[1], "grad_keys"), gv(grads[2], "grad_values"),
         gg(wide(grads[3]), "grad_log_decay"), gb(wide(grads[4]), "grad_beta"), g0(grads[5], "grad_initial_state");

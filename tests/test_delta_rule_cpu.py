@@ -41,3 +41,14 @@ def test_gradients_do_not_look_at_masked_rows(normalize, dtype):
         assert a.dtype == b.dtype and torch.equal(a, b)
     for grad in got[2:7]:
         assert not grad[0, :, 13:].any() and not grad[1].any() and not grad[2, :, 1:].any()
+
+
+@pytest.mark.parametrize("L", [5, 70])
+def test_no_value_heads(L):
+    q, k = (torch.randn(2, 2, L, 8, requires_grad=True) for _ in range(2))
+    v = torch.randn(2, 0, L, 4, requires_grad=True)
+    g = torch.zeros(2, 0, L, requires_grad=True)
+    out, state = gated_delta_rule(q, k, v, g, g, return_state=True)
+    assert out.shape == (2, 0, L, 4) and state.shape == (2, 0, 8, 4)
+    grads = torch.autograd.grad(out.sum() + state.sum(), [q, k], allow_unused=True)
+    assert all(grad is None or not grad.any() for grad in grads)

@@ -1,5 +1,5 @@
 """The gated delta rule where a result is much smaller than what it is made of, or exactly nothing: gradients of normalised
-rows that nearly cancel, rows of few values, positions that write nothing."""
+rows that nearly cancel, rows of few values, positions that write nothing, calls without value heads."""
 import pytest
 import torch
 
@@ -137,3 +137,18 @@ def test_nothing_comes_of_betas_of_zero(shape, dtype):
         assert not t.any(), name
     want = wanted(args, go, torch.zeros_like(args[5]), normalize=True)
     assert ref.far(gb, want[6]) <= ref.FP32 and ref.far(gs, want[7]) <= ref.FP32
+
+
+@pytest.mark.parametrize("L", [0, 5, 70])
+def test_no_value_heads(L):
+    """Key heads without value heads: empty outputs, gradients of zero."""
+    held = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]
+    del held                                                             # (what the allocator hands out next)
+    q, k = (torch.randn(2, 2, L, 8, device="cuda", requires_grad=True) for _ in range(2))
+    v = torch.randn(2, 0, L, 4, device="cuda", requires_grad=True)
+    g = torch.zeros(2, 0, L, device="cuda", requires_grad=True)
+    out, state = gated_delta_rule(q, k, v, g, g, return_state=True)
+    assert out.shape == (2, 0, L, 4) and state.shape == (2, 0, 8, 4)
+    grads = torch.autograd.grad(out.sum() + state.sum(), [q, k, v, g])
+    for t, grad in zip((q, k, v, g), grads):
+        assert grad.shape == t.shape and not grad.any()
