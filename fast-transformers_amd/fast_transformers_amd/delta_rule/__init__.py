@@ -143,7 +143,7 @@ def gated_delta_rule(queries, keys, values, log_decay, beta, initial_state=None,
     at, and have outputs and gradients of zero.
 
     Returns the outputs, ``(N, H, L, M)`` in the values' type, and with ``return_state`` also the state after the
-    last position, float32.  E is at most 128, M at most 512.  Differentiable once, with respect to everything
+    last position, float32.  E is at most 128, M at most 512.  Differentiable once, in reverse, with respect to everything
     but ``lengths``, ``scale`` and ``normalize``; a call that will be differentiated keeps the states
     before every 64th position and what the chunks were solved with: 3 KB a position and value head at E = M = 128 in
     bfloat16, 2 KB at 64 in float32.  Log decays are meant to be at most zero.  A ``beta`` of zero writes nothing (in

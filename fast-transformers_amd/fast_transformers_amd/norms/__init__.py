@@ -104,7 +104,7 @@ def residual_norm(block, residual=None, gate=None, *, after=None, before=None, s
     block's); ``gate``: None, or of either type in a shape that broadcasts to the block's over all but the last
     dimension.  ``after``, ``before``: None, or ``("rms" or "layer", weight, bias)`` with weight and bias optional.
     ``activation`` of the gate: None, ``"sigmoid"`` or ``"silu"``.  ``h`` is the norm of ``x`` before ``x`` is rounded to its type.
-    Differentiable once, with respect to all tensors."""
+    Differentiable once, in reverse, with respect to all tensors."""
     if block.is_cuda and not torch.compiler.is_compiling():  # (calls as they mostly are, checked by the native code)
         pair = _native.host().residual_norm_plain(block, residual, gate, after, before, scale, activation, eps)
         if pair is not None:

@@ -712,6 +712,14 @@ Tensor encoder(const Tensor &x, const std::vector<Layer> &layers, const std::opt
     return out;
 }
 
+// A call whose inputs carry derivatives forward would lose them
+void no_tangents(const char *what, std::initializer_list<const Tensor *> inputs) {
+    for (const Tensor *t : inputs)
+        if (t && t->defined() && t->_fw_grad(0).defined())
+            error(std::string(what) + ": derivatives are not carried forward (forward-mode differentiation)");
+}
+const Tensor *given(const OptTensor &t) { return t ? &*t : nullptr; }
+
 // ---- the gated delta rule (delta_rule/__init__.py) ----
 // Its memory comes from torch's allocator with every call (in a captured graph from the graph's own pool), so
 // calls on different streams and replays of different graphs never share any.
@@ -780,6 +788,7 @@ std::tuple<Tensor, OptTensor, OptTensor> delta_rule(const Tensor &queries, const
                                                     const OptTensor &initial_state, const OptTensor &lengths, double scale,
                                                     bool normalize, bool return_state, bool keep) {
     const at::NoGradGuard no_grad;
+    no_tangents("gated_delta_rule", {&queries, &keys, &values, &log_decay, &beta, given(initial_state)});
     const DeltaTensors t = delta_tensors(queries, keys, values, log_decay, beta);
     const c10::DeviceGuard guard(t.q.device());
     const int64_t N = t.v.size(0), H = t.v.size(1), Hk = t.q.size(1), L = t.v.size(2), E = t.q.size(3), M = t.v.size(3);
@@ -811,6 +820,7 @@ std::vector<OptTensor> delta_rule_backward(const Tensor &queries, const Tensor &
                                            double scale, bool normalize, const Tensor &kept, const Tensor &grad_out,
                                            const OptTensor &grad_final_state, const std::vector<bool> &needed) {
     const at::NoGradGuard no_grad;
+    no_tangents("gated_delta_rule", {&queries, &keys, &values, &log_decay, &beta, &grad_out, given(grad_final_state)});
     const DeltaTensors t = delta_tensors(queries, keys, values, log_decay, beta);
     const c10::DeviceGuard guard(t.q.device());
     const int64_t N = t.v.size(0), H = t.v.size(1), Hk = t.q.size(1), L = t.v.size(2), E = t.q.size(3), M = t.v.size(3);
@@ -864,6 +874,7 @@ ftc_tensor4 delta_token(const Tensor &t, int64_t dims, const char *name, const T
 Tensor delta_step(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &log_decay,
                   const Tensor &beta, const Tensor &state, double scale, bool normalize) {
     const at::NoGradGuard no_grad;
+    no_tangents("gated_delta_step", {&queries, &keys, &values, &log_decay, &beta, &state});
     if (!queries.is_cuda()) error("gated_delta_step: queries are on " + queries.device().str() + ", expected a GPU tensor");
     // (rows whose values lie apart are copied)
     auto rows = [](const Tensor &t) { return t.dim() == 3 && t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; };
@@ -1044,6 +1055,7 @@ std::tuple<Tensor, OptTensor, OptTensor> residual_norm(const Tensor &block, cons
                                                        const OptTensor &bw, const OptTensor &bb, int activation,
                                                        double scale, double eps, bool keep) {
     const at::NoGradGuard no_grad;
+    no_tangents("residual_norm", {&block, given(residual), given(gate), given(aw), given(ab), given(bw), given(bb)});
     const NormCall c(block, residual, gate, after, aw, ab, before, bw, bb, activation, scale, eps);
     const c10::DeviceGuard guard(block.device());
     const Tensor x = at::empty(block.sizes(), residual ? residual->options() : block.options());
@@ -1066,6 +1078,8 @@ std::vector<OptTensor> residual_norm_backward(const Tensor &block, const OptTens
                                               const OptTensor &stats, const OptTensor &grad_x, const OptTensor &grad_h,
                                               const std::vector<bool> &needed) {
     const at::NoGradGuard no_grad;
+    no_tangents("residual_norm", {&block, given(residual), given(gate), given(aw), given(ab), given(bw), given(bb), given(grad_x),
+                                  given(grad_h)});
     const NormCall c(block, residual, gate, after, aw, ab, before, bw, bb, activation, scale, eps);
     const c10::DeviceGuard guard(block.device());
     const NormRows gx(grad_x, "grad_x"), gh(grad_h, "grad_h");
