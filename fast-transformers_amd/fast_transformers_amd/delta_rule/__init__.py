@@ -161,8 +161,9 @@ def gated_delta_rule(queries, keys, values, log_decay, beta, initial_state=None,
         lengths = lengths.to(device=queries.device, dtype=torch.int64).contiguous()
     if queries.device.type != "cuda":
         out, state = _cpu_rule(queries, keys, values, log_decay, beta, initial_state, lengths, scale, normalize)
-    elif torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (queries, keys, values, log_decay, beta, initial_state)):
+    elif (torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (queries, keys, values, log_decay, beta, initial_state))
+            or torch.jit.is_tracing()):  # (a tracer sees the function)
         args = (queries, keys, values, log_decay, beta, initial_state, lengths, scale, normalize)
         out, state = (None if torch.compiler.is_compiling() else _native.host().delta_rule_plain(*args)) or \
             GatedDeltaRule.apply(*args)

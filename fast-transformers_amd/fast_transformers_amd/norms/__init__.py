@@ -131,7 +131,8 @@ def residual_norm(block, residual=None, gate=None, *, after=None, before=None, s
     activation = _ACTIVATIONS[activation]
     if block.device.type == "cpu":
         return _cpu_residual_norm(block, residual, gate, after, before, activation, scale, eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+            or torch.jit.is_tracing()):  # (a tracer sees the function)
         return ResidualNorm.apply(block, residual, gate, after[1], after[2], before[1], before[2],
                                   (after[0], before[0], activation, scale, eps))
     x, h, _ = _native.host().residual_norm(block, residual, gate, *after, *before, activation, scale, eps, False)

@@ -874,6 +874,7 @@ ftc_tensor4 delta_token(const Tensor &t, int64_t dims, const char *name, const T
 Tensor delta_step(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &log_decay,
                   const Tensor &beta, const Tensor &state, double scale, bool normalize) {
     const at::NoGradGuard no_grad;
+    if (torch::jit::tracer::isTracing()) error("gated_delta_step: a trace would not see the state change");
     no_tangents("gated_delta_step", {&queries, &keys, &values, &log_decay, &beta, &state});
     if (!queries.is_cuda()) error("gated_delta_step: queries are on " + queries.device().str() + ", expected a GPU tensor");
     // (rows whose values lie apart are copied)

@@ -1,5 +1,5 @@
-"""The gated delta rule, its step and the norms around a block where a derivative is carried forward or a call is
-transformed: an error, never a derivative of zero."""
+"""The gated delta rule, its step and the norms around a block where a derivative is carried forward, or a call is
+traced or transformed: an error or the right answer, never a derivative of zero or a constant."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -75,3 +75,18 @@ def test_forward_over_backward_is_refused():
             seed = fwd.make_dual(torch.ones_like(result), torch.ones_like(result))
             with pytest.raises(RuntimeError, match="forward"):
                 torch.autograd.grad(result, leaves, seed, retain_graph=True)
+
+
+def test_traces_see_the_calls():
+    args, other = rule_inputs(), delta.inputs(1, 2, 1, 20, 16, 16, device="cuda", seed=3)
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda *a: gated_delta_rule(*a, normalize=True), tuple(args), check_trace=False)
+        assert torch.equal(traced(*other), gated_delta_rule(*other, normalize=True))
+        x, y = (torch.randn(2, 6, 32, device="cuda") for _ in range(2))
+        traced = torch.jit.trace(lambda a, r: residual_norm(a, r, after="rms", before="layer"), (x[0], x[1]), check_trace=False)
+        for a, b in zip(traced(y[0], y[1]), residual_norm(y[0], y[1], after="rms", before="layer")):
+            assert torch.equal(a, b)
+        q, k, v, g, b, s = rule_inputs(1)
+        one = (q[:, :, 0], k[:, :, 0], v[:, :, 0], g[:, :, 0], b[:, :, 0], s)
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(lambda *a: gated_delta_step(*a), one, check_trace=False)
