@@ -1,20 +1,27 @@
-"""Backward passes of operators that are differentiated once."""
+"""Operators that are differentiated once, or not at all."""
 import functools
 
 import torch
 
 
-class _Again(torch.autograd.Function):
-    """The gradients as they are, as functions of all that they were made of, whose own gradient is an error."""
+class _NotDifferentiated(torch.autograd.Function):
+    """The first tensors as they are, as functions of all that they were made of, whose own gradient is an error."""
 
     @staticmethod
-    def forward(ctx, what, count, *tensors):
-        ctx.what = what
+    def forward(ctx, error, count, *tensors):
+        ctx.error = error
         return tuple(t.clone() for t in tensors[:count])
 
     @staticmethod
     def backward(ctx, *grads):
-        raise RuntimeError(ctx.what + ": the gradients cannot be differentiated again")
+        raise RuntimeError(ctx.error)
+
+
+def not_differentiated(error, result, made_of):
+    """``result`` where nothing that it was made of requires a gradient, else one whose gradient is an error."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in made_of):
+        return _NotDifferentiated.apply(error, 1, result, *made_of)[0]
+    return result
 
 
 def differentiated_once(what):
@@ -28,11 +35,12 @@ def differentiated_once(what):
             if torch.is_grad_enabled():
                 there = [i for i, t in enumerate(out) if t is not None]
                 made_of = [t for t in (*ctx.saved_tensors, *grads) if t is not None]
-                for i, t in zip(there, _Again.apply(what, len(there), *(out[i] for i in there), *made_of)):
+                for i, t in zip(there, _NotDifferentiated.apply(what + ": the gradients cannot be differentiated again", len(there),
+                                                     *(out[i] for i in there), *made_of)):
                     out[i] = t
             return tuple(out)
         return run
     return wrap
 
 
-__all__ = ["differentiated_once"]
+__all__ = ["differentiated_once", "not_differentiated"]

@@ -15,7 +15,7 @@ take an implementation of their own in torch operations, which shares nothing wi
 import torch
 
 from .. import _native
-from .._once import differentiated_once
+from .._once import differentiated_once, not_differentiated
 
 _EPS = 1e-6
 _CPU_CHUNK = 32
@@ -176,7 +176,7 @@ def gated_delta_rule(queries, keys, values, log_decay, beta, initial_state=None,
 def gated_delta_step(queries, keys, values, log_decay, beta, state, *, scale=None, normalize=False):
     """One token of every sequence: ``queries``, ``keys`` ``(N, Hk, E)``, ``values`` ``(N, H, M)``, ``log_decay``,
     ``beta`` ``(N, H)``; ``state`` ``(N, H, E, M)`` float32, updated in place (views of a larger buffer are fine, rows
-    along M contiguous).  Returns the outputs ``(N, H, M)`` in the values' type.  Not differentiable; one launch."""
+    along M contiguous).  Returns the outputs ``(N, H, M)`` in the values' type, whose gradient is an error; one launch."""
     if queries.dim() != 3:
         raise RuntimeError("gated_delta_step: expected queries (N, Hk, E), got %s" % (tuple(queries.shape),))
     on_gpu = queries.device.type == "cuda"
@@ -191,5 +191,6 @@ def gated_delta_step(queries, keys, values, log_decay, beta, state, *, scale=Non
             out, after = _cpu_rule(*(t.unsqueeze(2) for t in (queries, keys, values, log_decay, beta)), state, None,
                                    scale, normalize)
             state.copy_(after)
-        return out.squeeze(2)
+        return not_differentiated("gated_delta_step: the result cannot be differentiated", out.squeeze(2),
+                                  (queries, keys, values, log_decay, beta))
     return _native.host().delta_step(queries, keys, values, log_decay, beta, state, scale, normalize)

@@ -720,6 +720,19 @@ void no_tangents(const char *what, std::initializer_list<const Tensor *> inputs)
 }
 const Tensor *given(const OptTensor &t) { return t ? &*t : nullptr; }
 
+// Tensors as functions of all that they were made of, whose own gradient is an error
+struct NotDifferentiated : torch::autograd::Function<NotDifferentiated> {
+    static variable_list forward(AutogradContext *ctx, const char *error, at::TensorList tensors, at::TensorList) {
+        ctx->saved_data["error"] = std::string(error);
+        variable_list same;
+        for (const Tensor &t : tensors) same.push_back(t.variable_data());
+        return same;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list) {
+        TORCH_CHECK(false, ctx->saved_data["error"].toStringRef());
+    }
+};
+
 // ---- the gated delta rule (delta_rule/__init__.py) ----
 // Its memory comes from torch's allocator with every call (in a captured graph from the graph's own pool), so
 // calls on different streams and replays of different graphs never share any.
@@ -871,8 +884,8 @@ ftc_tensor4 delta_token(const Tensor &t, int64_t dims, const char *name, const T
     return d;
 }
 // One token: queries, keys (N, Hk, E), values (N, H, M), log_decay, beta (N, H), state (N, H, E, M) in place
-Tensor delta_step(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &log_decay,
-                  const Tensor &beta, const Tensor &state, double scale, bool normalize) {
+Tensor delta_step_result(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &log_decay,
+                         const Tensor &beta, const Tensor &state, double scale, bool normalize) {
     const at::NoGradGuard no_grad;
     if (torch::jit::tracer::isTracing()) error("gated_delta_step: a trace would not see the state change");
     no_tangents("gated_delta_step", {&queries, &keys, &values, &log_decay, &beta, &state});
@@ -896,6 +909,14 @@ Tensor delta_step(const Tensor &queries, const Tensor &keys, const Tensor &value
     if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
     return out;
 }
+Tensor delta_step(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &log_decay,
+                  const Tensor &beta, const Tensor &state, double scale, bool normalize) {
+    const Tensor out = delta_step_result(queries, keys, values, log_decay, beta, state, scale, normalize);
+    if (!differentiated({&queries, &keys, &values, &log_decay, &beta})) return out;
+    const Tensor made_of[] = {queries, keys, values, log_decay, beta};
+    return NotDifferentiated::apply("gated_delta_step: the result cannot be differentiated", at::TensorList(out),
+                                    at::TensorList(made_of))[0];
+}
 
 // The differentiable rule as a function of the C++ engine, as above for the attention: a step of a few short sequences
 // is bound by the host.
@@ -913,20 +934,8 @@ bool plain_or_none(py::handle h, OptTensor &to) {
     return true;
 }
 
-// Gradients of an operator that is differentiated once: where the caller will differentiate them again
-// (create_graph) they are functions of all that they were made of, whose own gradient is an error.
-struct Again : torch::autograd::Function<Again> {
-    static variable_list forward(AutogradContext *ctx, const char *what, at::TensorList grads, at::TensorList) {
-        ctx->saved_data["what"] = std::string(what);
-        variable_list same;
-        for (const Tensor &t : grads) same.push_back(t.variable_data());
-        return same;
-    }
-    static variable_list backward(AutogradContext *ctx, variable_list) {
-        const std::string what = ctx->saved_data["what"].toStringRef();
-        TORCH_CHECK(false, what, ": the gradients cannot be differentiated again");
-    }
-};
+// Gradients of an operator that is differentiated once: where the caller will differentiate them again (create_graph)
+// their own gradient is an error.
 void once(variable_list &grads, const char *what, const variable_list &saved, const variable_list &above) {
     if (!at::GradMode::is_enabled()) return;
     variable_list there, made_of;
@@ -935,7 +944,8 @@ void once(variable_list &grads, const char *what, const variable_list &saved, co
     for (const variable_list *list : {&saved, &above})
         for (const Tensor &t : *list)
             if (t.defined()) made_of.push_back(t);
-    const variable_list marked = Again::apply(what, at::TensorList(there), at::TensorList(made_of));
+    const std::string error = std::string(what) + ": the gradients cannot be differentiated again";
+    const variable_list marked = NotDifferentiated::apply(error.c_str(), at::TensorList(there), at::TensorList(made_of));
     size_t next = 0;
     for (Tensor &t : grads)
         if (t.defined()) t = marked[next++];

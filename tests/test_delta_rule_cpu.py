@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import delta_reference as ref
-from fast_transformers_amd.delta_rule import gated_delta_rule
+from fast_transformers_amd.delta_rule import gated_delta_rule, gated_delta_step
 
 
 def gradients(args, go, gs, rule=gated_delta_rule, **options):
@@ -52,3 +52,19 @@ def test_no_value_heads(L):
     assert out.shape == (2, 0, L, 4) and state.shape == (2, 0, 8, 4)
     grads = torch.autograd.grad(out.sum() + state.sum(), [q, k], allow_unused=True)
     assert all(grad is None or not grad.any() for grad in grads)
+
+
+@pytest.mark.parametrize("needs", range(5))
+def test_a_steps_result_has_no_derivative(needs):
+    q, k, v, g, b, s = ref.inputs(1, 2, 1, 1, 8, 6)
+    args = [q[:, :, 0], k[:, :, 0], v[:, :, 0], g[:, :, 0], b[:, :, 0]]
+    states = [s.clone(), s.clone()]
+    want = gated_delta_step(*args, states[0])
+    assert not want.requires_grad
+    args[needs] = args[needs].clone().requires_grad_(True)
+    out = gated_delta_step(*args, states[1])
+    assert torch.equal(out, want) and torch.equal(*states) and not states[1].requires_grad
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        out.sum().backward()
+    with torch.no_grad():
+        assert not gated_delta_step(*args, states[1]).requires_grad

@@ -90,3 +90,23 @@ def test_traces_see_the_calls():
         one = (q[:, :, 0], k[:, :, 0], v[:, :, 0], g[:, :, 0], b[:, :, 0], s)
         with pytest.raises(RuntimeError, match="trace"):
             torch.jit.trace(lambda *a: gated_delta_step(*a), one, check_trace=False)
+
+
+@pytest.mark.parametrize("needs", [None, 0, 1, 2, 3, 4])
+def test_a_steps_result_has_no_derivative(needs):
+    q, k, v, g, b, s = rule_inputs(1)
+    args = [q[:, :, 0], k[:, :, 0], v[:, :, 0], g[:, :, 0], b[:, :, 0]]
+    states = [s.clone(), s.clone()]
+    with torch.no_grad():
+        want = gated_delta_step(*args, states[0])
+    if needs is not None:
+        args[needs] = args[needs].clone().requires_grad_(True)
+    out = gated_delta_step(*args, states[1])
+    assert torch.equal(out, want) and torch.equal(*states) and not states[1].requires_grad
+    if needs is None:
+        assert not out.requires_grad
+    else:
+        with pytest.raises(RuntimeError, match="cannot be differentiated"):
+            (out * out).sum().backward()
+    with torch.no_grad():
+        assert not gated_delta_step(*args, states[1]).requires_grad
