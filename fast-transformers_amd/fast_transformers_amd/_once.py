@@ -24,6 +24,12 @@ def not_differentiated(error, result, made_of):
     return result
 
 
+def check_factor(factor, what):
+    """A factor that the kernels take as a number: a tensor's gradient would be lost."""
+    if isinstance(factor, torch.Tensor) and factor.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(what + ": scale is a number, not a tensor that requires a gradient")
+
+
 def differentiated_once(what):
     """Decorator of a Function's backward: where the gradients are to be differentiated again (``create_graph``), their
     own gradient is an error, also with respect to saved tensors (which torch's ``once_differentiable`` passes over)."""
@@ -43,4 +49,4 @@ def differentiated_once(what):
     return wrap
 
 
-__all__ = ["differentiated_once", "not_differentiated"]
+__all__ = ["check_factor", "differentiated_once", "not_differentiated"]

@@ -15,7 +15,7 @@ take an implementation of their own in torch operations, which shares nothing wi
 import torch
 
 from .. import _native
-from .._once import differentiated_once, not_differentiated
+from .._once import check_factor, differentiated_once, not_differentiated
 
 _EPS = 1e-6
 _CPU_CHUNK = 32
@@ -154,6 +154,8 @@ def gated_delta_rule(queries, keys, values, log_decay, beta, initial_state=None,
         _check(queries, keys, values, log_decay, beta, initial_state, "gated_delta_rule")
     if scale is None:
         scale = max(1, queries.shape[3]) ** -0.5
+    elif queries.device.type == "cuda":
+        check_factor(scale, "gated_delta_rule")
     if lengths is not None:
         if lengths.shape != values.shape[:1]:
             raise RuntimeError("gated_delta_rule: expected %d lengths, got shape %s"
@@ -186,6 +188,8 @@ def gated_delta_step(queries, keys, values, log_decay, beta, state, *, scale=Non
         raise RuntimeError("gated_delta_step: the state is updated in place and cannot be differentiated")
     if scale is None:
         scale = max(1, queries.shape[2]) ** -0.5
+    elif on_gpu:
+        check_factor(scale, "gated_delta_step")
     if not on_gpu:
         with torch.no_grad():
             out, after = _cpu_rule(*(t.unsqueeze(2) for t in (queries, keys, values, log_decay, beta)), state, None,

@@ -9,7 +9,7 @@
 import torch
 
 from .. import _native
-from .._once import differentiated_once
+from .._once import check_factor, differentiated_once
 
 _KINDS = {"rms": 1, "layer": 2}
 _ACTIVATIONS = {None: 0, "sigmoid": 1, "silu": 2}
@@ -105,6 +105,8 @@ def residual_norm(block, residual=None, gate=None, *, after=None, before=None, s
     dimension.  ``after``, ``before``: None, or ``("rms" or "layer", weight, bias)`` with weight and bias optional.
     ``activation`` of the gate: None, ``"sigmoid"`` or ``"silu"``.  ``h`` is the norm of ``x`` before ``x`` is rounded to its type.
     Differentiable once, in reverse, with respect to all tensors."""
+    if type(scale) is not float and block.is_cuda:
+        check_factor(scale, "residual_norm")
     if block.is_cuda and not torch.compiler.is_compiling():  # (calls as they mostly are, checked by the native code)
         pair = _native.host().residual_norm_plain(block, residual, gate, after, before, scale, activation, eps)
         if pair is not None:

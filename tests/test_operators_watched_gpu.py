@@ -110,3 +110,19 @@ def test_a_steps_result_has_no_derivative(needs):
             (out * out).sum().backward()
     with torch.no_grad():
         assert not gated_delta_step(*args, states[1]).requires_grad
+
+
+def test_factors_that_would_be_differentiated_are_refused():
+    scale = torch.tensor(0.5, device="cuda", requires_grad=True)
+    args = rule_inputs()
+    x = torch.randn(4, 32, device="cuda")
+    with pytest.raises(RuntimeError, match="scale"):
+        gated_delta_rule(*args, scale=scale)
+    with pytest.raises(RuntimeError, match="scale"):
+        residual_norm(x, x, before="rms", scale=scale)
+    q, k, v, g, b, s = rule_inputs(1)
+    with pytest.raises(RuntimeError, match="scale"):
+        gated_delta_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], g[:, :, 0], b[:, :, 0], s, scale=scale)
+    assert torch.equal(gated_delta_rule(*args, scale=scale.detach()), gated_delta_rule(*args, scale=0.5))
+    with torch.no_grad():
+        assert torch.equal(residual_norm(x, x, scale=scale)[0], residual_norm(x, x, scale=0.5)[0])
