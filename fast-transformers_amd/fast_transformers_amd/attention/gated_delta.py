@@ -16,7 +16,8 @@ from ..norms import residual_norm
 class GatedDeltaLayer(Module):
     """Projections to queries, keys, values, decays, write strengths and gates, the gated delta rule, the gated norm of
     every head's output, and the projection back.  ``n_key_heads`` (default ``n_heads``) key heads serve ``n_heads``
-    value heads."""
+    value heads.  ``d_keys`` (default ``d_model // n_heads``) is at most 128; ``d_values`` (the same) is 3 to 512: every
+    head's output is normalised."""
 
     def __init__(self, d_model, n_heads, d_keys=None, d_values=None, n_key_heads=None, eps=1e-6):
         super().__init__()
@@ -25,6 +26,8 @@ class GatedDeltaLayer(Module):
         n_key_heads = n_key_heads or n_heads
         if n_heads % n_key_heads:
             raise ValueError("n_heads must be a multiple of n_key_heads")
+        if not (1 <= d_keys <= 128 and 3 <= d_values <= 512):
+            raise ValueError("takes d_keys from 1 to 128 and d_values from 3 to 512, got %d and %d" % (d_keys, d_values))
         self.n_heads, self.n_key_heads, self.d_keys, self.d_values, self.eps = n_heads, n_key_heads, d_keys, d_values, eps
         self.query_projection = Linear(d_model, n_key_heads * d_keys, bias=False)
         self.key_projection = Linear(d_model, n_key_heads * d_keys, bias=False)
@@ -81,6 +84,8 @@ class GatedDeltaEncoder(Module):
                  eps=1e-6, stream_type=torch.float32):
         super().__init__()
         d_ff = d_ff or 4 * d_model
+        if not 3 <= d_model <= 16384:
+            raise ValueError("takes d_model from 3 to 16384, got %d" % d_model)
         self.attentions = ModuleList(GatedDeltaLayer(d_model, n_heads, d_keys, d_values, n_key_heads, eps)
                                      for _ in range(n_layers))
         self.up = ModuleList(Linear(d_model, d_ff) for _ in range(n_layers))
