@@ -1,5 +1,6 @@
 // C ABI entry points of the gated delta rule (include/ftc_causal_product.h): argument checking, workspaces and the
 // sequence of launches.  The kernels: ftc_delta_{prepare,scan,outputs,gradients,step}.hip.
+#include <algorithm>
 #include <cstdio>
 
 #include "ftc_delta_kernel.h"
@@ -102,6 +103,18 @@ int check_state(const ftc_tensor4 *t, const char *name, const Sizes &s) {
     return FTC_OK;
 }
 
+// Whether two rows of a tensor may share memory: in the order of the strides, each has to pass all that the smaller ones reach
+bool overlaps_itself(const ftc_tensor4 *t) {
+    int order[] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return t->stride[a] < t->stride[b]; });
+    int64_t reach = t->size[3];
+    for (int i : order) {
+        if (t->size[i] < 2) continue;
+        if (t->stride[i] < reach) return true;
+        reach += t->stride[i] * (t->size[i] - 1);
+    }
+    return false;
+}
 bool reads_wide(const Operand &o) {
     const int bytes = o.dtype == FTC_F32 ? 4 : 2, lot = 16 / bytes;
     return o.width % lot == 0 && ((uintptr_t)o.ptr & 15) == 0 && o.stride_n % lot == 0 && o.stride_h % lot == 0 &&
@@ -305,8 +318,7 @@ int ftc_gated_delta_step(const ftc_tensor4 *queries, const ftc_tensor4 *keys, co
     if (!state_in_out) return fail(FTC_ERR_INVALID, "state is null");
     if (int rc = check_state(state_in_out, "state", s)) return rc;
     if (s.N * s.H == 0 || s.L == 0) return FTC_OK;
-    if ((s.N > 1 && state_in_out->stride[0] == 0) || (s.H > 1 && state_in_out->stride[1] == 0) ||
-        (s.E > 1 && state_in_out->stride[2] < s.M))
+    if (overlaps_itself(state_in_out))
         return fail(FTC_ERR_INVALID, "state is written and must not overlap itself");
     p.out = rows_out(out), p.initial = p.final_ = state(state_in_out);
     p.scale = scale, p.normalize = normalize != 0;

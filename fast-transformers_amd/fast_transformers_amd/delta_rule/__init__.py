@@ -191,6 +191,11 @@ def gated_delta_step(queries, keys, values, log_decay, beta, state, *, scale=Non
     elif on_gpu:
         check_factor(scale, "gated_delta_step")
     if not on_gpu:
+        reach = state.shape[3]
+        for stride, size in sorted(zip(state.stride()[:3], state.shape[:3])):
+            if size > 1 and stride < reach:
+                raise RuntimeError("gated_delta_step: state is written and must not overlap itself")
+            reach += stride * (size - 1)
         with torch.no_grad():
             out, after = _cpu_rule(*(t.unsqueeze(2) for t in (queries, keys, values, log_decay, beta)), state, None,
                                    scale, normalize)
