@@ -21,9 +21,9 @@
 // 64 x 64 matrices with the rows.  What is not rows is in three pieces for bf16
 // rows too: of a normalised row's gradient what lies along the row is taken away again, and may be nearly all of it.
 //
-// What bounds it: the instructions that cut values into pieces and LDS, each about a third of the time with two workgroups a compute
-// unit, beside 2.2 GB of states, their gradients, Z, dE and rows.  Measured: 8192 chunks of 128 x 128 on 4096 of
-// key heads, bf16, 740 to 780 us (2.9 TB/s); 1280 of 64 x 64, fp32, 94.
+// What bounds it: vector instructions, most of them cutting values into pieces (46 % of the time), LDS (35 %) and the matrix cores
+// (25 %), two workgroups a compute unit, beside 2.2 GB of states, their gradients, Z, dE and rows.  Measured: 8192 chunks of
+// 128 x 128 on 4096 of key heads, bf16, 860 to 910 us (2.5 TB/s; in two pieces 740 to 780); 1280 of 64 x 64, fp32, 94 to 97.
 #include <type_traits>
 
 #include "ftc_delta_kernel.h"
@@ -33,8 +33,8 @@ namespace delta {
 namespace {
 
 constexpr int kSlice = 64;  // key columns of a workgroup
-// Wavefronts of a workgroup: four, two workgroups to a compute unit; three pieces leave LDS for one workgroup, of eight.  (1280 chunks
-// of 64 x 64, fp32: 94 us, with four 111.  8192 of 128 x 128, bf16: 817, with four 780: as many wavefronts read operands twice.)
+// Wavefronts of a workgroup: four, two workgroups to a compute unit; rows in three pieces leave LDS for one workgroup, of eight.  (1280
+// chunks of 64 x 64, fp32: 94 us, with four 111.  8192 of 128 x 128, bf16: 1224 with eight, with four 863.)
 template <typename T>
 constexpr int kWaves = Elem<T>::kPieces == 1 ? 4 : 8;
 

@@ -178,7 +178,8 @@ __device__ __forceinline__ void products(const Frag (&a)[TILES][NA], const Frag 
 }
 // Lets the last products' results arrive before a branch.  The compiler counts the instructions between a matrix
 // product and the first use of its result, but where a branch skips a block it counts those of the block on the path
-// without them too (seen in a listing: a result read two instructions after its product, and wrong rows).
+// without them too (seen in a listing: a result read two instructions after its product, and wrong rows).  Where it has to
+// stand is checked on the listings of all kernels, by tests/test_matrix_results.py.
 __device__ __forceinline__ void settle() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 15");

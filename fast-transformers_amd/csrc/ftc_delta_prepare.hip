@@ -8,7 +8,8 @@
 //
 // What bounds it: the steps of the inverse one after the other, and what it writes (36 KB of T and its transpose a chunk, 32 KB of
 // the keys' fragments).  T lies where k was, so that three workgroups fit a compute unit.  Measured: 8192 chunks
-// of 128 key columns, bf16, 181 us (2.5 TB/s written; two workgroups a compute unit 220); 1280 of 64, fp32, 38.
+// of 128 key columns, bf16, 181 us (2.5 TB/s written; two workgroups a compute unit 220; 250
+// to 300 where a backward follows and every chunk has betas of zero, since T is then made twice); 1280 of 64, fp32, 38.
 #include "ftc_delta_kernel.h"
 
 namespace ftc {
