@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
         for (int id = wave; id < 10; id += 4) {
             const int ti = id < 1 ? 0 : id < 3 ? 1 : id < 6 ? 2 : 3, tj = id - ti * (ti + 1) / 2;
             f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    #pragma unroll
+#pragma unroll
             for (int s = 0; s < KE; s++) {
                 Frag a[PIECES], b[PIECES];
                 rows_of<RB>(kp, ti, s, c, q, a);
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
                 acc = product(a, b, acc);
             }
             const int j = 16 * tj + c;
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int i = 16 * ti + 4 * q + r;
                 const float d = expf((high_mem[i] - high_mem[j]) + (low_mem[i] - low_mem[j]));
@@ -160,14 +160,14 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
         if (lane < 16) {
             const lds_float *const m = Mx + 16 * wave * kStride + 16 * wave;
             float x[16];
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 16; r++) {
                 float sum = r == lane ? 1.f : 0.f;
-    #pragma unroll
+#pragma unroll
                 for (int s = 0; s < r; s++) sum = fmaf(-m[r * kStride + s], x[s], sum);
                 x[r] = sum;
             }
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 16; r++) Tm[(16 * wave + r) * kStride + 16 * wave + lane] = x[r];
         }
         __syncthreads();
@@ -176,12 +176,12 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
         if (wave < 2) {
             const int r0 = 32 * wave + 16, c0 = 32 * wave;
             f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 4; r++)
                 x = mfma_f32(Mx[(r0 + c) * kStride + c0 + 4 * q + r], Tm[(c0 + 4 * q + r) * kStride + c0 + c], x);
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 4; r++) y = mfma_f32(Tm[(r0 + c) * kStride + r0 + 4 * q + r], x[r], y);
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 4; r++) Tm[(r0 + 4 * q + r) * kStride + c0 + c] = -y[r];
         }
         __syncthreads();
@@ -189,29 +189,29 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(DeltaArgs p) {
         {
             const int a = wave >> 1, b = wave & 1;
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    #pragma unroll
+#pragma unroll
             for (int kt = 0; kt < 2; kt++)
-    #pragma unroll
+#pragma unroll
                 for (int r = 0; r < 4; r++)
                     x = mfma_f32(Mx[(32 + 16 * a + c) * kStride + 16 * kt + 4 * q + r],
                                  Tm[(16 * kt + 4 * q + r) * kStride + 16 * b + c], x);
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 4; r++) X[(16 * a + 4 * q + r) * kStride + 16 * b + c] = x[r];
             __syncthreads();
             f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    #pragma unroll
+#pragma unroll
             for (int kt = 0; kt < 2; kt++)
-    #pragma unroll
+#pragma unroll
                 for (int r = 0; r < 4; r++)
                     y = mfma_f32(Tm[(32 + 16 * a + c) * kStride + 32 + 16 * kt + 4 * q + r],
                                  X[(16 * kt + 4 * q + r) * kStride + 16 * b + c], y);
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 4; r++) Tm[(32 + 16 * a + 4 * q + r) * kStride + 16 * b + c] = -y[r];
         }
         __syncthreads();
         // T in pieces where M was, and from there its fragments
         lds_char *const tp = (lds_char *)m_mem;
-    #pragma unroll
+#pragma unroll
         for (int i = 0; i < 4; i++) {
             const int u = tid + kThreads * i, row = u / 16, slot = u % 16;
             const lds_float *const x = Tm + row * kStride + 4 * slot;
