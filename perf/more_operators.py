@@ -10,11 +10,10 @@ past a sequence's length left out (``ragged``).
 
 The dropout behind a block, per value i (counted over the block's rows, one after the other):
 
-    x_i = residual_i + keep_i act(block_i + bias) / (1 - p),   keep_i = half_i >= p 2^16
+    x_i = residual_i + keep_i act(block_i + bias) / (1 - p),   keep_i = word_i >= p 2^32
 
-where half_i is the half word i % 8, low halves first, of the four words of Philox4x32-10 (Salmon, Moraes, Dror and Shaw,
-2011) with the seed as its key and (i // 8, offset) as its counter, 64 bits each, and p a multiple of 2^-16: the one
-next to the share that is asked for.
+where word_i is the word i % 4 of Philox4x32-10 (Salmon, Moraes, Dror and Shaw, 2011) with the seed as its key and
+(i // 4, offset) as its counter, 64 bits each.
 
 Cases are dicts of plain values.  ``kind``: "prefill" (the attention in inference, state in and out), "train" (forward
 and backward; with ``carry`` a state comes in and its gradient goes out), "step" (one token, state in place),
@@ -216,10 +215,10 @@ def _plain_step(q, k, v, g, state, scale):
     return (S * (scale * q)[..., None]).sum(2).to(dtype)
 
 
-def _plain_halves(count, seed, offset, device):
-    """The generator's first ``count`` half words as whole numbers of 64 bits."""
+def _plain_words(count, seed, offset, device):
+    """The generator's first ``count`` words as whole numbers of 64 bits."""
     low = 0xFFFFFFFF
-    at = torch.arange((count + 7) // 8, dtype=torch.int64, device=device)
+    at = torch.arange((count + 3) // 4, dtype=torch.int64, device=device)
     c = [at & low, at >> 32, torch.full_like(at, offset & low), torch.full_like(at, offset >> 32 & low)]
     key = [seed & low, seed >> 32 & low]
     for _ in range(10):
@@ -227,7 +226,7 @@ def _plain_halves(count, seed, offset, device):
         a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
         c = [(b >> 32 & low) ^ c[1] ^ key[0], b & low, (a >> 32 & low) ^ c[3] ^ key[1], a & low]
         key = [(key[0] + 0x9E3779B9) & low, (key[1] + 0xBB67AE85) & low]
-    return torch.stack([half for word in c for half in (word & 0xFFFF, word >> 16)], -1).reshape(-1)[:count]
+    return torch.stack(c, -1).reshape(-1)[:count]
 
 
 def _plain_dropout(s, case):
@@ -241,9 +240,8 @@ def _plain_dropout(s, case):
         a = 0.5 * a * (1 + torch.erf(a * math.sqrt(0.5)))
     elif case["activation"] == "silu":
         a = a / (1 + torch.exp(-a))
-    border = round(p * 2 ** 16)
-    keep = _plain_halves(block.numel(), s["seed"], s["offset"], block.device).view(block.shape) >= border
-    x = torch.where(keep, a * (2 ** 16 / (2 ** 16 - border)), 0.0)
+    keep = _plain_words(block.numel(), s["seed"], s["offset"], block.device).view(block.shape) >= round(p * 2 ** 32)
+    x = torch.where(keep, a * (1 / (1 - p)), 0.0)
     if s["residual"] is not None:
         x = s["residual"].float() + x
     return x.to(block.dtype if s["residual"] is None else s["residual"].dtype)
@@ -299,7 +297,7 @@ def work(case):
         values = case["N"] * case["L"] * case["D"]
         stream = b if case["stream"] == "none" else size[case["stream"]]
         residual = 0 if case["stream"] == "none" else stream
-        # block and residual in, x out; ten rounds of two products for every eight values, and the activation
+        # block and residual in, x out; ten rounds of two products for every four values, and the activation
         one, bias = values * (b + residual + stream), 4 * case["D"] * case["bias"]
         if case["kind"] == "dropout":
             return {"bytes": float(one + bias), "flops": 20.0 * values}
@@ -378,8 +376,8 @@ def _exact_step(case, s):
 def _exact_keep(case, s):
     """Which values are kept, from the generator in whole numbers without a sign, four words at a time."""
     count = s["block"].numel()
-    u16, u32, u64 = numpy.uint16, numpy.uint32, numpy.uint64
-    at = numpy.arange((count + 7) // 8, dtype=u64)
+    u32, u64 = numpy.uint32, numpy.uint64
+    at = numpy.arange((count + 3) // 4, dtype=u64)
     x0, x1 = at.astype(u32), (at >> u64(32)).astype(u32)
     x2, x3 = (numpy.full(at.shape, s["offset"] >> shift & 0xFFFFFFFF, dtype=u32) for shift in (0, 32))
     for turn in range(10):
@@ -387,8 +385,7 @@ def _exact_keep(case, s):
         left, right = x0.astype(u64) * u64(0xD2511F53), x2.astype(u64) * u64(0xCD9E8D57)
         x0, x2 = (right >> u64(32)).astype(u32) ^ x1 ^ u32(k0), (left >> u64(32)).astype(u32) ^ x3 ^ u32(k1)
         x1, x3 = right.astype(u32), left.astype(u32)
-    words = numpy.stack([x0, x1, x2, x3], -1).astype("<u4").view("<u2").reshape(-1)[:count]
-    keep = words >= u16(round(case["p"] * 2 ** 16))
+    keep = numpy.stack([x.astype(u64) >= u64(round(case["p"] * 2 ** 32)) for x in (x0, x1, x2, x3)], -1).reshape(-1)[:count]
     return torch.from_numpy(keep).to(s["block"].device).view(s["block"].shape)
 
 
@@ -410,7 +407,7 @@ def _exact_dropout(case, s):
         else:
             sigmoid = torch.sigmoid(z)
             a, slope = z * sigmoid, sigmoid * (1 + z * (1 - sigmoid))
-        factor = keep[lo:lo + part].double() / (1 - round(case["p"] * 2 ** 16) / 2 ** 16)
+        factor = keep[lo:lo + part].double() / (1 - case["p"])
         x = a * factor
         got = {"x": x if residual is None else x + residual[lo:lo + part].double()}
         if gx is not None:
