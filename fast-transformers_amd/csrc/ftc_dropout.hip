@@ -1,17 +1,17 @@
 // The dropout behind a block, with the block's bias, activation and residual in the same pass over the rows, and its gradients
 // (include/ftc_causal_product.h).
 //
-//   x_i = residual_i + keep_i act(z_i) / (1 - p),   z_i = block_i + bias,   keep_i = half_i >= p 2^16
+//   x_i = residual_i + keep_i act(z_i) / (1 - p),   z_i = block_i + bias,   keep_i = word_i >= p 2^32
 //   grad_block_i = keep_i act'(z_i) grad_x_i / (1 - p),   grad_bias = its sums over the rows,   grad_residual = grad_x
 //
-// No mask is stored: half_i comes from a generator that is a function of i, the value's number among the rows' values, one row
+// No mask is stored: word_i comes from a generator that is a function of i, the value's number among the rows' values, one row
 // after the other, wherever they lie.  It is Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2,
-// 3; 2011): ten rounds on a counter of four words, (i / 8, offset), with the seed as the key,
+// 3; 2011): ten rounds on a counter of four words, (i / 4, offset), with the seed as the key,
 //
 //   c <- (high(m1 c2) ^ c1 ^ k0, low(m1 c2), high(m0 c0) ^ c3 ^ k1, low(m0 c0)),   k0 += w0, k1 += w1
 //
-// whose eight half words, low halves first, are those of values 8 (i / 8) to 8 (i / 8) + 7.  Half a word decides a value, which
-// halves the generator's share: p is a multiple of 2^-16, the nearest one, and the factor belongs to that one.
+// whose four words are those of values 4 (i / 4) to 4 (i / 4) + 3.  A value has a word of 32 bits: p is a multiple of 2^-32, the nearest
+// one, and the factor belongs to that one.
 //
 // A lane takes eight values of a row at a time; the last eight of a row whose width is no multiple of eight overlap those before,
 // both lanes write the same.  All arithmetic is fp32, results are rounded once.  The sums for the bias: a workgroup walks rows with
@@ -37,7 +37,7 @@ constexpr int kThreads = 256;
 // 13.6, 40960 x 512 (fp32) 85 us in both directions instead of 82.
 constexpr int kAtOnce = 2;
 constexpr int64_t kMostWidth = 1 << 18;
-constexpr uint32_t kAll = 1 << 16;
+constexpr uint32_t kAll = 1 << 16;  // of the parts that p is counted in, each of 2^16 smaller ones
 
 struct Args {
     Rows block, residual, x, grad_x, grad_block;
@@ -46,7 +46,8 @@ struct Args {
     int64_t rows;
     int32_t D, lots;      // lots: of a row
     uint32_t magic;       // n / lots = high(n magic), n up to lots + 2^10; 0: one lot
-    uint32_t border;      // p 2^16
+    uint32_t gone;        // p 2^32 - 1, the largest word of a value that is dropped
+    int32_t drops;        // whether any is
     float factor;         // 1 / (1 - p), or 0
     uint32_t seed[2], offset[2];
     const int64_t *seeds;  // seed and offset on the device, or null
@@ -170,25 +171,32 @@ __device__ __forceinline__ u32x4 philox(uint64_t number, Key k) {
     }
     return u32x4{c0, c1, c2, c3};
 }
-// The half words of eight values from number `at` on, two to a word.  WHOLE: at is a multiple of eight.
+// The words of eight values from number `at` on.  WHOLE: at is a multiple of four.
+struct Words {
+    uint32_t w[kLot];
+};
 template <bool WHOLE>
-__device__ __forceinline__ u32x4 halves(uint64_t at, const Key &k) {
-    const u32x4 here = philox(at >> 3, k);
-    if (WHOLE) return here;
-    const u32x4 next = philox((at >> 3) + 1, k);
-    uint32_t w[8] = {here.x, here.y, here.z, here.w, next.x, next.y, next.z, next.w};
-    const bool four = at & 4, two = at & 2, one = at & 1;
-    auto pick = [](bool other, uint32_t a, uint32_t b) { return other ? a : b; };
+__device__ __forceinline__ Words words(uint64_t at, const Key &k) {
+    constexpr int kCounters = WHOLE ? 2 : 3;
+    uint32_t w[4 * kCounters];
 #pragma unroll
-    for (int i = 0; i < 6; i++) w[i] = pick(four, w[i + 2], w[i]);
+    for (int j = 0; j < kCounters; j++) {
+        const u32x4 four = philox((at >> 2) + j, k);
 #pragma unroll
-    for (int i = 0; i < 5; i++) w[i] = pick(two, w[i + 1], w[i]);
+        for (int i = 0; i < 4; i++) w[4 * j + i] = four[i];
+    }
+    if constexpr (!WHOLE) {
+        const bool two = at & 2, one = at & 1;
+        auto pick = [](bool other, uint32_t a, uint32_t b) { return other ? a : b; };
 #pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = pick(one, w[i] >> 16 | w[i + 1] << 16, w[i]);
-    return u32x4{w[0], w[1], w[2], w[3]};
-}
-__device__ __forceinline__ bool keeps(const u32x4 &halves, int i, uint32_t border) {
-    return (i % 2 ? halves[i / 2] >> 16 : halves[i / 2] & 0xffffu) >= border;
+        for (int i = 0; i < kLot + 1; i++) w[i] = pick(two, w[i + 2], w[i]);
+#pragma unroll
+        for (int i = 0; i < kLot; i++) w[i] = pick(one, w[i + 1], w[i]);
+    }
+    Words r;
+#pragma unroll
+    for (int i = 0; i < kLot; i++) r.w[i] = w[i];
+    return r;
 }
 
 // ---- activations ----
@@ -283,15 +291,15 @@ __device__ __forceinline__ Place place_of(const Args &p, int64_t row0, uint32_t 
 // One lot's result
 template <bool WHOLE, bool SHORT, bool FAST>
 __device__ __forceinline__ void lot_forward(const Args &p, const Place &at, const Key &key, Lot &z, const Lot &bias, const Lot &onto) {
-    const u32x4 half = halves<WHOLE>((uint64_t)(at.row * p.D + at.col), key);
+    const Words word = words<WHOLE>((uint64_t)(at.row * p.D + at.col), key);
 #pragma unroll
     for (int i = 0; i < kLot; i++) z.x[i] += bias.x[i];
     activate<FAST>(z, p.activation);
 #pragma unroll
-    for (int i = 0; i < kLot; i++) z.x[i] = (keeps(half, i, p.border) ? z.x[i] * p.factor : 0.f) + onto.x[i];
+    for (int i = 0; i < kLot; i++) z.x[i] = (!p.drops || word.w[i] > p.gone ? z.x[i] * p.factor : 0.f) + onto.x[i];
 }
 
-// T: the block's type, X: that of x.  WHOLE: widths are multiples of eight, SHORT: rows of fewer than eight.
+// T: the block's type, X: that of x.  WHOLE: widths are multiples of four, SHORT: rows of fewer than eight.
 template <typename T, typename X, bool WHOLE, bool SHORT>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(Args p) {
     const int64_t first = (int64_t)blockIdx.x * (kThreads * kAtOnce), row0 = first / p.lots;
@@ -352,7 +360,7 @@ __global__ __launch_bounds__(kThreads) void dropout_bias_kernel(Args p) {
 // One lot's gradient
 template <bool WHOLE, bool SHORT, bool FAST>
 __device__ __forceinline__ void lot_back(const Args &p, const Place &at, const Key &key, Lot z, const Lot &bias, Lot &grad) {
-    const u32x4 half = halves<WHOLE>((uint64_t)(at.row * p.D + at.col), key);
+    const Words word = words<WHOLE>((uint64_t)(at.row * p.D + at.col), key);
     if (p.activation != FTC_ACTIVATION_NONE) {
 #pragma unroll
         for (int i = 0; i < kLot; i++) z.x[i] += bias.x[i];
@@ -361,7 +369,7 @@ __device__ __forceinline__ void lot_back(const Args &p, const Place &at, const K
         for (int i = 0; i < kLot; i++) grad.x[i] *= z.x[i];
     }
 #pragma unroll
-    for (int i = 0; i < kLot; i++) grad.x[i] = keeps(half, i, p.border) ? grad.x[i] * p.factor : 0.f;
+    for (int i = 0; i < kLot; i++) grad.x[i] = !p.drops || word.w[i] > p.gone ? grad.x[i] * p.factor : 0.f;
 }
 
 template <typename T, typename X, bool WHOLE, bool SHORT>
@@ -456,7 +464,8 @@ int read_call(const ftc_residual_dropout_call *c, bool back, Args *p) {
         return fail(FTC_ERR_UNSUPPORTED, "rows of up to %lld values are supported, 2^35 values in all", (long long)kMostWidth);
     if (c->activation < FTC_ACTIVATION_NONE || c->activation > FTC_ACTIVATION_SILU)
         return fail(FTC_ERR_INVALID, "the activation has code %d", (int)c->activation);
-    if (c->dropped > kAll) return fail(FTC_ERR_INVALID, "%u parts in 65536 cannot be dropped", (unsigned)c->dropped);
+    if (c->dropped > kAll || c->dropped_rest >= kAll || (c->dropped == kAll && c->dropped_rest))
+        return fail(FTC_ERR_INVALID, "%u parts in 65536 and %u in 2^32 cannot be dropped", (unsigned)c->dropped, (unsigned)c->dropped_rest);
     if (c->bias && c->bias_dtype != FTC_F32 && c->bias_dtype != FTC_BF16)
         return fail(FTC_ERR_INVALID, "the bias has dtype code %d", (int)c->bias_dtype);
     const bool reads = !back || c->activation != FTC_ACTIVATION_NONE;
@@ -465,8 +474,9 @@ int read_call(const ftc_residual_dropout_call *c, bool back, Args *p) {
     p->bias = c->bias, p->bias_dtype = c->bias_dtype, p->activation = c->activation;
     p->rows = c->rows, p->D = (int32_t)c->width, p->lots = (p->D + kLot - 1) / kLot;
     p->magic = p->lots == 1 ? 0 : (uint32_t)(((uint64_t)1 << 32) / (uint32_t)p->lots + 1);
-    p->border = c->dropped;
-    p->factor = c->dropped == kAll ? 0.f : (float)(65536.0 / (65536.0 - c->dropped));
+    const uint64_t all = (uint64_t)kAll * kAll, border = (uint64_t)c->dropped * kAll + c->dropped_rest;
+    p->gone = (uint32_t)(border - 1), p->drops = border > 0;
+    p->factor = border == all ? 0.f : (float)((double)all / (double)(all - border));
     p->seed[0] = (uint32_t)c->seed, p->seed[1] = (uint32_t)(c->seed >> 32);
     p->offset[0] = (uint32_t)c->offset, p->offset[1] = (uint32_t)(c->offset >> 32);
     p->seeds = c->seeds;
@@ -505,9 +515,9 @@ void dispatch(const Args &p, bool block_f32, bool x_f32, int what, hipStream_t s
     auto widths = [&](auto t, auto x) {
         using T = decltype(t);
         using X = decltype(x);
-        if (p.D % kLot == 0) run<T, X, true, false>(p, what, stream);
-        else if (p.D > kLot) run<T, X, false, false>(p, what, stream);
-        else run<T, X, false, true>(p, what, stream);
+        if (p.D < kLot) run<T, X, false, true>(p, what, stream);
+        else if (p.D % 4 == 0) run<T, X, true, false>(p, what, stream);
+        else run<T, X, false, false>(p, what, stream);
     };
     if (block_f32) x_f32 ? widths(float(), float()) : widths(float(), uint16_t());
     else x_f32 ? widths(uint16_t(), float()) : widths(uint16_t(), uint16_t());

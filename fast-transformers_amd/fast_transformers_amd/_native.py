@@ -87,7 +87,7 @@ class ResidualNormCall(ctypes.Structure):
 class ResidualDropoutCall(ctypes.Structure):
     _fields_ = [("block", Rows), ("residual", Rows), ("bias", ctypes.c_void_p), ("rows", ctypes.c_int64), ("width", ctypes.c_int64),
                 ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("seeds", ctypes.c_void_p), ("bias_dtype", ctypes.c_int32),
-                ("activation", ctypes.c_int32), ("dropped", ctypes.c_uint32)]
+                ("activation", ctypes.c_int32), ("dropped", ctypes.c_uint32), ("dropped_rest", ctypes.c_uint32)]
 
 
 class Tensor4(ctypes.Structure):

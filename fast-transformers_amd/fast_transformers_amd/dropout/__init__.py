@@ -3,9 +3,9 @@
     x = residual + keep act(block + bias) / (1 - p)
 
 No mask is stored: whether value ``i`` is kept, counted over the block's values in the order of its shape, is a function of the
-seed, the offset and ``i``, and the backward makes it again.  It is half word ``i % 8``, low halves first, of the four words of
-Philox4x32-10 (Salmon, Moraes, Dror and Shaw, 2011) with the seed as its key and ``(i // 8, offset)`` as its counter, against
-``p 2^16``.  On the GPU it is one HIP kernel forward and one or two backward (``csrc/ftc_dropout.hip``); without the library a GPU tensor
+seed, the offset and ``i``, and the backward makes it again.  It is word ``i % 4`` of Philox4x32-10 (Salmon, Moraes, Dror and
+Shaw, 2011) with the seed as its key and ``(i // 4, offset)`` as its counter, against ``p 2^32``.  On the GPU it is one HIP kernel
+forward and one or two backward (``csrc/ftc_dropout.hip``); without the library a GPU tensor
 raises.  CPU tensors take torch operations, with the same values kept.
 """
 from operator import index
@@ -17,7 +17,7 @@ from .._once import differentiated_once
 
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
 _TYPES = (torch.float32, torch.bfloat16)
-_ALL = 1 << 16
+_ALL = 1 << 32
 _LOW = 0xFFFFFFFF
 
 
@@ -50,9 +50,9 @@ class ResidualDropout(torch.autograd.Function):
         return _native.host().residual_dropout_backward(block, ctx.block_type, bias, seeds, grad_x, *ctx.options, needs_block, needs_bias)
 
 
-def _cpu_halves(count, seed, offset):
-    """The generator's first ``count`` half words."""
-    at = torch.arange((count + 7) // 8, dtype=torch.int64)
+def _cpu_words(count, seed, offset):
+    """The generator's first ``count`` words."""
+    at = torch.arange((count + 3) // 4, dtype=torch.int64)
     c0, c1 = at & _LOW, at >> 32
     c2, c3 = (torch.full_like(at, offset >> shift & _LOW) for shift in (0, 32))
     k0, k1 = seed & _LOW, seed >> 32 & _LOW
@@ -61,8 +61,7 @@ def _cpu_halves(count, seed, offset):
         a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57
         c0, c1, c2, c3 = (b >> 32 & _LOW) ^ c1 ^ k0, b & _LOW, (a >> 32 & _LOW) ^ c3 ^ k1, a & _LOW
         k0, k1 = k0 + 0x9E3779B9 & _LOW, k1 + 0xBB67AE85 & _LOW
-    words = torch.stack((c0, c1, c2, c3), -1)
-    return torch.stack((words & 0xFFFF, words >> 16), -1).reshape(-1)[:count]
+    return torch.stack((c0, c1, c2, c3), -1).reshape(-1)[:count]
 
 
 def _cpu_dropout(block, residual, bias, seeds, activation, dropped, seed, offset):
@@ -70,7 +69,7 @@ def _cpu_dropout(block, residual, bias, seeds, activation, dropped, seed, offset
         seed, offset = (int(n) & (1 << 64) - 1 for n in seeds)
     z = block.float() if bias is None else block.float() + bias.float()
     z = {0: lambda t: t, 1: torch.relu, 2: torch.nn.functional.gelu, 3: torch.nn.functional.silu}[activation](z)
-    keep = _cpu_halves(block.numel(), seed, offset).view(block.shape) >= dropped
+    keep = _cpu_words(block.numel(), seed, offset).view(block.shape) >= dropped
     x = torch.where(keep, z * (_ALL / max(1, _ALL - dropped)), 0.0)
     return (x if residual is None else residual.float() + x).to(block.dtype if residual is None else residual.dtype)
 
@@ -95,7 +94,7 @@ def residual_dropout(block, residual=None, *, p, seed, offset=0, bias=None, acti
     ``block``: rows of up to 262144 values, float32 or bfloat16, in any number of dimensions; ``residual``: None, or of the block's
     shape in either type (``x`` has the residual's type, or the block's without one); ``bias``: None, or a vector of the rows' width
     in either type.  ``activation``: None, ``"relu"``, ``"gelu"`` (by the error function) or ``"silu"``.  ``p``: from 0 to 1; a multiple of
-    2^-16 is what counts, the nearest one, and 1 leaves the residual.  A dropped value is not looked at: NaN and infinity go
+    2^-32 is what counts, the nearest one, and 1 leaves the residual.  A dropped value is not looked at: NaN and infinity go
     as well.
 
     ``seed``, ``offset``: whole numbers of 64 bits; the same two drop the same values, whatever the strides, types and device, and two

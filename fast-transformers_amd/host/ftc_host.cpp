@@ -1434,7 +1434,7 @@ py::object residual_norm_plain(py::handle block, py::handle residual, py::handle
 // ---- the dropout behind a block (dropout/__init__.py) ----
 constexpr const char *kDropout = "residual_dropout";
 struct DropoutOptions {
-    int64_t activation, dropped;
+    int64_t activation, dropped;  // dropped: p 2^32
     uint64_t seed, offset;
 };
 struct DropoutCall {
@@ -1461,7 +1461,7 @@ struct DropoutCall {
             seeds = *numbers, call.seeds = seeds.const_data_ptr<int64_t>();
         }
         call.block = block.r, call.residual = residual.r;
-        call.activation = (int32_t)o.activation, call.dropped = (uint32_t)o.dropped, call.seed = o.seed, call.offset = o.offset;
+        call.activation = (int32_t)o.activation, call.dropped = (uint32_t)(o.dropped >> 16), call.dropped_rest = (uint32_t)(o.dropped & 0xffff), call.seed = o.seed, call.offset = o.offset;
     }
 };
 Tensor residual_dropout(const Tensor &block, const OptTensor &residual, const OptTensor &bias, const OptTensor &seeds,

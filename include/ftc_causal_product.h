@@ -500,8 +500,8 @@ int ftc_residual_norm_backward(const ftc_residual_norm_call *call, const float *
  *
  *   x = residual + keep act(block + bias) / (1 - p)
  *
- * dropped: p in parts of 65536, from 0 to 65536 (all).  keep of value i, counted over the rows one after the other, is half_i >=
- * dropped, half_i the half word i % 8, low halves first, of the four words of Philox4x32-10 with the seed as its key and (i / 8,
+ * p is dropped / 2^16 + dropped_rest / 2^32: dropped from 0 to 65536 (all), dropped_rest from 0 to 65535 (0 where all are dropped).  keep of value
+ * i, counted over the rows one after the other, is word_i >= p 2^32, word_i word i % 4 of Philox4x32-10 with the seed as its key and (i / 4,
  * offset) as its counter, 64 bits each.  seeds: NULL, or seed and offset as two values on the device, which take the place of
  * the call's (a captured graph then drops anew with every replay).  A dropped value is not looked at: NaN and infinity
  * go as well.  block and x (with the residual's dtype) are FTC_F32 or FTC_BF16 by themselves, rows of contiguous values `stride`
@@ -515,7 +515,7 @@ typedef struct ftc_residual_dropout_call {
     uint64_t seed, offset;
     const int64_t *seeds;
     int32_t bias_dtype, activation;
-    uint32_t dropped;
+    uint32_t dropped, dropped_rest;
 } ftc_residual_dropout_call;
 int ftc_residual_dropout(const ftc_residual_dropout_call *call, const ftc_rows *x, void *stream);
 /*
