@@ -46,7 +46,7 @@ struct Args {
     int64_t rows;
     int32_t D, lots;      // lots: of a row
     uint32_t magic;       // n / lots = high(n magic), n up to lots + 2^10; 0: one lot
-    uint32_t gone;        // p 2^32 - 1, the largest word of a value that is dropped
+    uint32_t gone;        // p 2^32 - 1, the largest word of a value that is dropped (0 where none is)
     int32_t drops;        // whether any is
     float factor;         // 1 / (1 - p), or 0
     uint32_t seed[2], offset[2];
@@ -151,6 +151,10 @@ __device__ __forceinline__ Lot load_bias(const Args &p, int col) {
     return widen(r);
 }
 
+struct Place {
+    int64_t row;
+    int col;
+};
 // ---- the generator ----
 struct Key {
     uint32_t k0, k1, o0, o1;
@@ -171,12 +175,19 @@ __device__ __forceinline__ u32x4 philox(uint64_t number, Key k) {
     }
     return u32x4{c0, c1, c2, c3};
 }
-// The words of eight values from number `at` on.  WHOLE: at is a multiple of four.
+// The words of eight values from number `at` on, or the largest ones where nothing is dropped.  WHOLE: at is a multiple of four.
 struct Words {
     uint32_t w[kLot];
 };
 template <bool WHOLE>
-__device__ __forceinline__ Words words(uint64_t at, const Key &k) {
+__device__ __forceinline__ Words words(const Args &p, const Place &place, const Key &k) {
+    Words r;
+    if (!p.drops) {  // (as in evaluation: no generator)
+#pragma unroll
+        for (int i = 0; i < kLot; i++) r.w[i] = ~0u;
+        return r;
+    }
+    const uint64_t at = (uint64_t)(place.row * p.D + place.col);
     constexpr int kCounters = WHOLE ? 2 : 3;
     uint32_t w[4 * kCounters];
 #pragma unroll
@@ -193,7 +204,6 @@ __device__ __forceinline__ Words words(uint64_t at, const Key &k) {
 #pragma unroll
         for (int i = 0; i < kLot; i++) w[i] = pick(one, w[i + 1], w[i]);
     }
-    Words r;
 #pragma unroll
     for (int i = 0; i < kLot; i++) r.w[i] = w[i];
     return r;
@@ -277,10 +287,6 @@ __device__ __forceinline__ void slopes(Lot &z, int activation) {
     }
 }
 
-struct Place {
-    int64_t row;
-    int col;
-};
 // the lane's u-th lot of its workgroup's
 __device__ __forceinline__ Place place_of(const Args &p, int64_t row0, uint32_t lot0, int u) {
     const uint32_t n = lot0 + threadIdx.x + kThreads * u;
@@ -291,12 +297,12 @@ __device__ __forceinline__ Place place_of(const Args &p, int64_t row0, uint32_t 
 // One lot's result
 template <bool WHOLE, bool SHORT, bool FAST>
 __device__ __forceinline__ void lot_forward(const Args &p, const Place &at, const Key &key, Lot &z, const Lot &bias, const Lot &onto) {
-    const Words word = words<WHOLE>((uint64_t)(at.row * p.D + at.col), key);
+    const Words word = words<WHOLE>(p, at, key);
 #pragma unroll
     for (int i = 0; i < kLot; i++) z.x[i] += bias.x[i];
     activate<FAST>(z, p.activation);
 #pragma unroll
-    for (int i = 0; i < kLot; i++) z.x[i] = (!p.drops || word.w[i] > p.gone ? z.x[i] * p.factor : 0.f) + onto.x[i];
+    for (int i = 0; i < kLot; i++) z.x[i] = (word.w[i] > p.gone ? z.x[i] * p.factor : 0.f) + onto.x[i];
 }
 
 // T: the block's type, X: that of x.  WHOLE: widths are multiples of four, SHORT: rows of fewer than eight.
@@ -360,7 +366,7 @@ __global__ __launch_bounds__(kThreads) void dropout_bias_kernel(Args p) {
 // One lot's gradient
 template <bool WHOLE, bool SHORT, bool FAST>
 __device__ __forceinline__ void lot_back(const Args &p, const Place &at, const Key &key, Lot z, const Lot &bias, Lot &grad) {
-    const Words word = words<WHOLE>((uint64_t)(at.row * p.D + at.col), key);
+    const Words word = words<WHOLE>(p, at, key);
     if (p.activation != FTC_ACTIVATION_NONE) {
 #pragma unroll
         for (int i = 0; i < kLot; i++) z.x[i] += bias.x[i];
@@ -369,7 +375,7 @@ __device__ __forceinline__ void lot_back(const Args &p, const Place &at, const K
         for (int i = 0; i < kLot; i++) grad.x[i] *= z.x[i];
     }
 #pragma unroll
-    for (int i = 0; i < kLot; i++) grad.x[i] = !p.drops || word.w[i] > p.gone ? grad.x[i] * p.factor : 0.f;
+    for (int i = 0; i < kLot; i++) grad.x[i] = word.w[i] > p.gone ? grad.x[i] * p.factor : 0.f;
 }
 
 template <typename T, typename X, bool WHOLE, bool SHORT>
@@ -475,7 +481,7 @@ int read_call(const ftc_residual_dropout_call *c, bool back, Args *p) {
     p->rows = c->rows, p->D = (int32_t)c->width, p->lots = (p->D + kLot - 1) / kLot;
     p->magic = p->lots == 1 ? 0 : (uint32_t)(((uint64_t)1 << 32) / (uint32_t)p->lots + 1);
     const uint64_t all = (uint64_t)kAll * kAll, border = (uint64_t)c->dropped * kAll + c->dropped_rest;
-    p->gone = (uint32_t)(border - 1), p->drops = border > 0;
+    p->drops = border > 0, p->gone = border > 0 ? (uint32_t)(border - 1) : 0;
     p->factor = border == all ? 0.f : (float)((double)all / (double)(all - border));
     p->seed[0] = (uint32_t)c->seed, p->seed[1] = (uint32_t)(c->seed >> 32);
     p->offset[0] = (uint32_t)c->offset, p->offset[1] = (uint32_t)(c->offset >> 32);
