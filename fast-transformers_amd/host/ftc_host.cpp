@@ -1035,6 +1035,11 @@ struct DecayedTensors {
         } else {
             if (log_decay.dim() != 3 || log_decay.device() != queries.device())
                 error("decayed_attention: log_decay must be 3-dimensional (N, H, L), on the device of the queries");
+            // (the library takes (1, H, 1, 1) as one for each head; a tensor of three dimensions is never meant so)
+            if (log_decay.size(0) != N || log_decay.size(1) != H || log_decay.size(2) != L)
+                error("decayed_attention: log_decay has shape (" + std::to_string(log_decay.size(0)) + ", " + std::to_string(log_decay.size(1)) +
+                      ", " + std::to_string(log_decay.size(2)) + "), expected (" + std::to_string(N) + ", " + std::to_string(H) + ", " +
+                      std::to_string(L) + ")");
             g = log_decay.size(2) > 1 && log_decay.stride(2) > (1 << 22) ? log_decay.contiguous() : log_decay;
         }
         dq = delta_describe(q, "queries", kDecayed), dk = delta_describe(k, "keys", kDecayed), dv = delta_describe(v, "values", kDecayed);
@@ -1136,6 +1141,8 @@ Tensor decayed_step_result(const Tensor &queries, const Tensor &keys, const Tens
     const bool per_head = log_decay.dim() == 1;
     if (per_head && (log_decay.size(0) != v.size(1) || log_decay.device() != q.device()))
         error("decayed_attention_step: log_decay must have one value for each head, on the device of the queries");
+    if (log_decay.dim() == 2 && (log_decay.size(0) != v.size(0) || log_decay.size(1) != v.size(1)))
+        error("decayed_attention_step: log_decay must have one value for each head of every sequence, (N, H)");
     const ftc_tensor4 dg = per_head ? describe_decays(log_decay) : delta_token(log_decay, 2, "log_decay", q, what);
     const c10::DeviceGuard guard(q.device());
     if (state.dim() != 4 || (state.size(3) > 1 && state.stride(3) != 1))
