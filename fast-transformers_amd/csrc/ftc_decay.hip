@@ -16,6 +16,8 @@ namespace {
 constexpr int64_t kStepMost = 8;
 constexpr int64_t kMostRowStride = 1 << 22;  // elements between positions: a chunk's offsets stay below 2 GiB
 
+constexpr int64_t kMostLanes = 0xffffffff;  // of a launch
+
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
 struct Sizes {
@@ -87,9 +89,24 @@ struct Sizes {
     bool pairs() const { return bf16() && group() % 2 == 0; }
     int64_t shares_of_keys() const { return group() / (pairs() ? 2 : 1); }
     int64_t part() const { return shares_of_keys() > 1 ? up(N * Hk * shares_of_keys() * L * E, 64) : 0; }
+    // Whether every launch of a route has fewer than 2^32 lanes (ftc_decay_scan_kernel.h, ftc_decay_finish.hip)
+    static int64_t scan_lanes(int64_t units, int64_t columns) { return up(units, 8) * 4 * columns_at_once((int)columns); }
+    bool borders_fit(bool keep) const {
+        const int64_t n = segments(keep);
+        return scan_lanes(chains() * (n - 1), width()) <= kMostLanes && (n <= 2 || chains() * up(up(E, 4) * width() / 4, 256) <= kMostLanes);
+    }
+    bool forward_fits(bool keep) const {
+        return scan_lanes(chains() * (walks(keep) ? 1 : segments(keep)), width()) <= kMostLanes && (walks(keep) || borders_fit(keep));
+    }
+    bool backward_fits() const {
+        const int64_t n = segments(true), heads = pairs() ? 2 : 1;
+        return borders_fit(true) && scan_lanes(chains() * n, width()) <= kMostLanes &&
+               2 * heads * scan_lanes(chains() / heads * n, E) <= kMostLanes && N * H * n * seg_len(true) <= kMostLanes;
+    }
     int64_t backward() const { return 4 * (slots(true) + totals(true) + anchors() + 2 * dots() + sums() + 2 * part()); }
 };
 
+int too_many() { return fail(FTC_ERR_UNSUPPORTED, "too many chains, positions and columns for one call"); }
 int check_sizes(Sizes &s) {
     if (s.N < 0 || s.H < 0 || s.Hk < 0 || s.L < 0 || s.E < 0 || s.M < 0) return fail(FTC_ERR_INVALID, "negative size");
     if (s.H > 0 && (s.Hk == 0 || s.H % s.Hk != 0))
@@ -98,14 +115,16 @@ int check_sizes(Sizes &s) {
     if (s.E < 1 || s.E > kMaxE || s.M < 1 || s.M > 512)
         return fail(FTC_ERR_UNSUPPORTED, "decayed attention takes key rows of 1 to 128 values and value rows of 1 to "
                     "512, got %lld and %lld", (long long)s.E, (long long)s.M);
-    // (a launch has fewer than 2^32 lanes: 2^23 workgroups of 512)
-    constexpr int64_t kMost = 0x7fffff;
-    const bool few = s.N <= kMost && s.H <= kMost && s.L <= 0x7fffff00 && s.N * s.H <= kMost;
-    if (few) s.settle();
-    if (!few || (s.N * s.H > 0 && (s.chains() > kMost / std::max<int64_t>(64, 4 * (s.segments(true) + 8)))))
-        return fail(FTC_ERR_UNSUPPORTED, "too many chains, positions and columns for one call");
+    constexpr int64_t kMost = 0xffffff;  // (workgroups of 256, the smallest that own a chain)
+    if (s.N > kMost || s.H > kMost || s.L > 0x7fffff00 || s.N * s.H > kMost) return too_many();
+    s.settle();
     return FTC_OK;
 }
+// ... and whether a route's launches have room for them
+int check_forward(const Sizes &s, bool keep) {  // (what is kept is for a backward)
+    return s.N * s.H == 0 || (s.forward_fits(keep) && (!keep || s.backward_fits())) ? FTC_OK : too_many();
+}
+int check_steps(int64_t lanes) { return lanes <= kMostLanes ? FTC_OK : too_many(); }
 int check_rows(const ftc_tensor4 *t, const char *name, int64_t N, int64_t H, int64_t L, int64_t X, int dtype) {
     if (!t) return fail(FTC_ERR_INVALID, "%s is null", name);
     if (t->dtype != FTC_F32 && t->dtype != FTC_BF16)
@@ -215,6 +234,10 @@ int64_t bytes_of(int64_t N, int64_t H, int64_t Hk, int64_t L, int64_t E, int64_t
     if (dtype != FTC_F32 && dtype != FTC_BF16) return fail(FTC_ERR_INVALID, "unknown dtype code %d", (int)dtype);
     if (int rc = check_sizes(s)) return rc;
     if (N * H == 0) return 0;
+    if (what == 0 && L > kStepMost)
+        if (int rc = check_forward(s, false)) return rc;
+    if (what != 0)
+        if (int rc = check_forward(s, true)) return rc;
     return what == 2 ? s.backward() : what == 1 ? s.forward_bytes(true) : L <= kStepMost ? 0 : s.forward_bytes(false);
 }
 
@@ -246,9 +269,11 @@ int ftc_decayed_attention_plan(int64_t N, int64_t H, int64_t Hk, int64_t L, int6
     if (int rc = check_sizes(s)) return rc;
     if (N * H == 0) return FTC_OK;
     if (L == 0 || (!keep && L <= kStepMost)) {
+        if (int rc = check_steps(decay_step_lanes(N * H, M, M % 4 == 0))) return rc;
         snprintf(text, text_bytes, "steps");
         return FTC_OK;
     }
+    if (int rc = check_forward(s, keep)) return rc;
     const int64_t segments = s.segments(keep);
     snprintf(text, text_bytes, "segments %lld of %lld%s, slices %lld", (long long)segments, (long long)s.seg_len(keep),
              segments > 1 && s.walks(keep) ? " one after the other" : "", (long long)s.slices());
@@ -271,10 +296,12 @@ int ftc_decayed_attention(const ftc_tensor4 *queries, const ftc_tensor4 *keys, c
     if (s.L == 0 || (!kept && s.L <= kStepMost)) {
         StepArgs p = {as_operand(queries), as_operand(keys), as_operand(values), in.g, lengths, state(initial_state), state(final_state),
                       as_operand_out(out), (int32_t)s.N, (int32_t)s.H, (int32_t)s.Hk, (int32_t)s.L, (int32_t)s.E, (int32_t)s.M, scale};
+        if (int rc = check_steps(decay_step_lanes(s.N * s.H, s.M, decay_step_vec(p)))) return rc;
         decay_steps(p, on);
         return launched("decay_step_kernel");
     }
     const bool keep = kept != nullptr;
+    if (int rc = check_forward(s, keep)) return rc;
     const int64_t need = s.forward_bytes(keep);
     void *const at = keep ? kept : workspace;
     if (need > 0 && (!at || (int64_t)(keep ? kept_bytes : workspace_bytes) < need))
@@ -322,6 +349,7 @@ int ftc_decayed_attention_backward(const ftc_tensor4 *queries, const ftc_tensor4
     if (int rc = check_apart(initial_state, "initial_state", grad_initial_state, "grad_initial_state")) return rc;
     if (s.N * s.H == 0 || (s.L == 0 && !grad_initial_state)) return FTC_OK;
     if (s.L == 0) return fail(FTC_ERR_INVALID, "a call of no positions has no backward");
+    if (int rc = check_forward(s, true)) return rc;
     if (!kept || (int64_t)kept_bytes < s.forward_bytes(true))
         return fail(FTC_ERR_WORKSPACE, "ftc_decayed_attention_backward needs the %lld bytes that the forward kept", (long long)s.forward_bytes(true));
     if (!workspace || (int64_t)workspace_bytes < s.backward())
@@ -413,6 +441,7 @@ int ftc_decayed_attention_step(const ftc_tensor4 *queries, const ftc_tensor4 *ke
     if (overlaps_itself(state_in_out)) return fail(FTC_ERR_INVALID, "state is written and must not overlap itself");
     StepArgs p = {as_operand(queries), as_operand(keys), as_operand(values), in.g, nullptr, state(state_in_out), state(state_in_out),
                   as_operand_out(out), (int32_t)s.N, (int32_t)s.H, (int32_t)s.Hk, (int32_t)s.L, (int32_t)s.E, (int32_t)s.M, scale};
+    if (int rc = check_steps(decay_step_lanes(s.N * s.H, s.M, decay_step_vec(p)))) return rc;
     decay_steps(p, (hipStream_t)stream);
     return launched("decay_step_kernel");
 }

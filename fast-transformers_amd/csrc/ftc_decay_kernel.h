@@ -124,6 +124,8 @@ struct StepArgs {
     float scale;
 };
 void decay_steps(const StepArgs &p, hipStream_t stream);
+bool decay_step_vec(const StepArgs &p);  // whether states are read and written 16 bytes at a time
+int64_t decay_step_lanes(int64_t chains, int64_t M, bool vec);
 
 }  // namespace decay
 }  // namespace ftc

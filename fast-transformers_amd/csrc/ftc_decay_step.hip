@@ -114,10 +114,11 @@ bool state_vec(const State &s) {
 
 }  // namespace
 
+bool decay_step_vec(const StepArgs &p) { return p.M % 4 == 0 && state_vec(p.first) && state_vec(p.last); }
+int64_t decay_step_lanes(int64_t chains, int64_t M, bool vec) { return chains * ((M + kBlock - 1) / kBlock) * (kGroups * kBlock / (vec ? 4 : 1)); }
 void decay_steps(const StepArgs &p, hipStream_t stream) {
     const dim3 grid((uint32_t)p.N * (uint32_t)p.H * (uint32_t)((p.M + kBlock - 1) / kBlock));
-    const bool vec = p.M % 4 == 0 && state_vec(p.first) && state_vec(p.last);
-    if (vec) {
+    if (decay_step_vec(p)) {
         if (p.E <= 64) decay_step_kernel<4, 4><<<grid, 256, 0, stream>>>(p);
         else decay_step_kernel<4, 8><<<grid, 256, 0, stream>>>(p);
     } else {

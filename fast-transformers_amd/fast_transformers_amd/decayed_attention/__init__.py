@@ -119,7 +119,9 @@ def decayed_attention(queries, keys, values, log_decay, initial_state=None, *, s
     leave the state as it is, are not looked at, and have outputs and gradients of zero.
 
     Returns the outputs, ``(N, H, L, M)`` in the values' type, and with ``return_state`` also the state after the
-    last position, float32.  E is at most 128, M at most 512.  Differentiable once, in reverse, with respect to everything
+    last position, float32.  E is at most 128, M at most 512; N H ceil(M / 128) is below 2^23 on the GPU, and in
+    a call that will be differentiated below 2^20 and, times ceil(L / 1024), below 2^22.
+    Differentiable once, in reverse, with respect to everything
     but ``lengths`` and ``scale``; a call that will be differentiated keeps the states every 1024 positions or fewer.  Log decays are
     meant to be at most zero; the gradient of one of ``-inf`` is zero.  Chunks of positions are worked on as a whole: NaN or infinity in a
     row within its length also reaches the outputs of up to 63 positions before it."""
@@ -152,7 +154,8 @@ def decayed_attention(queries, keys, values, log_decay, initial_state=None, *, s
 def decayed_attention_step(queries, keys, values, log_decay, state, *, scale=None):
     """One token of every sequence: ``queries``, ``keys`` ``(N, Hk, E)``, ``values`` ``(N, H, M)``, ``log_decay`` ``(N, H)`` or
     ``(H,)``; ``state`` ``(N, H, E, M)`` float32, updated in place (views of a larger buffer are fine, rows along M
-    contiguous).  Returns the outputs ``(N, H, M)`` in the values' type, whose gradient is an error; one launch."""
+    contiguous).  Returns the outputs ``(N, H, M)`` in the values' type, whose gradient is an error; one launch.  On the GPU
+    N H ceil(M / 64) is below 2^22."""
     if queries.dim() != 3:
         raise RuntimeError("decayed_attention_step: expected queries (N, Hk, E), got %s" % (tuple(queries.shape),))
     on_gpu = queries.device.type == "cuda"

@@ -406,8 +406,10 @@ int ftc_gated_delta_step(const ftc_tensor4 *queries, const ftc_tensor4 *keys, co
  * for each head.  lengths: N int64 values on the device, or NULL; positions at or past lengths[n] leave the state as it is,
  * their rows are not looked at and their outputs are zero.  initial_state (NULL: zeros), final_state (NULL: not wanted):
  * (N,H,E,M), FTC_F32, unit stride along M.  Results must not overlap the inputs: parts of a sequence run side by side.  Log
- * decays may be -infinity (the state is forgotten).  Sizes: E from 1 to 128, M from 1 to 512, L from 0 on; rows at most 2^22 elements apart; anything else
- * returns FTC_ERR_UNSUPPORTED.
+ * decays may be -infinity (the state is forgotten).  Sizes: E from 1 to 128, M from 1 to 512, L from 0 on; rows at most 2^22 elements apart; and no
+ * launch of 2^32 lanes: up to 8 positions that keep nothing, and the step below, N H ceil(M/64) below 2^22 (2^24 where states can be
+ * accessed 16 bytes at a time), longer calls that keep nothing N H ceil(M/128) below 2^23, with a backward below 2^20, and with ceil(L/1024) times
+ * that below 2^22, at least.  Anything else returns FTC_ERR_UNSUPPORTED.
  *
  * kept: memory of ftc_decayed_attention_kept_bytes that the backward reads (states every 1024 positions or fewer), or NULL for a
  * forward without one, which then needs `workspace`.  Neither needs initialisation, both are 256-byte aligned.
