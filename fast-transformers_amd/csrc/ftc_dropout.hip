@@ -210,11 +210,12 @@ __device__ __forceinline__ Words words(const Args &p, const Place &place, const 
 }
 
 // ---- activations ----
-// The complement of the normal distribution, 1 - Phi(|z|), for results of bf16: t P(t) e^{-x^2}, t = 1 / (1 + c x), x = |z| / sqrt 2, whose
-// exponential serves for the density as well.  P was fitted for the least largest error relative to the value (x up to 14), so that
-// the tail keeps its bits: of degree 7 to 1.6e-7, for gradients, which are added up in 32 bits for the bias; of degree 5 to 6.1e-6, a
-// six hundredth of what rounding a result to bf16 may cost.  (16384 x 8192, forward: 148 us with degree 7 there as well; 136 and 163 with
-// a fit of degree 4 to an absolute error of 1.5e-7, which loses gelu(-6) by 0.4 %, as much as a rounding to bf16 may.)
+// The complement of the normal distribution, 1 - Phi(|z|): t P(t) e^{-x^2}, t = 1 / (1 + c x), x = |z| / sqrt 2, whose exponential serves for
+// the density as well.  P was fitted for the least largest error relative to the value (x up to 14), so that the tail keeps its bits, which 1 + erf
+// does not (fp32: 4 % at -5, nothing left at -5.5).  For results of fp32 of degree 9 to 4.5e-9 (its roundings in 32 bits come to 3.8e-7 at most, 7.5e-8
+// in the mean); for gradients of bf16, which are added up in 32 bits for the bias, of degree 7 to 1.6e-7; for results of bf16 of degree 5 to 6.1e-6, a
+// six hundredth of what rounding a result to bf16 may cost.  (16384 x 8192, fp32, with a bias, forward and with its backward: 239 and 524 us; 255 and 545
+// with 1 + erf, 294 and 609 with erfc.)
 template <int N>
 __device__ __forceinline__ float behind(float z, float e, const float (&p)[N], float c) {
     const float t = __builtin_amdgcn_rcpf(fmaf(c, fabsf(z) * 0.70710678f, 1.f));
@@ -226,15 +227,13 @@ __device__ __forceinline__ float behind(float z, float e, const float (&p)[N], f
 // Phi(z) and its density
 template <bool FAST, bool SLOPE>
 __device__ __forceinline__ float normal(float z, float &density) {
-    if (!FAST) {
-        density = 0.39894228f * expf(-0.5f * z * z);
-        return 0.5f * (1.f + erff(z * 0.70710678f));
-    }
     const float e = __builtin_amdgcn_exp2f(z * z * -0.72134752f);
     density = 0.39894228f * e;
     constexpr float kSlope[] = {0.246796984f, 0.24770522f, 0.214494871f, 0.222751164f, -0.035136425f, 0.317385559f, -0.285824239f, 0.0718269597f},
                     kValue[] = {0.249892868f, 0.245066311f, 0.258995474f, 0.0543220965f, 0.335150677f, -0.143433497f};
-    const float half = SLOPE ? behind(z, e, kSlope, 0.4375f) : behind(z, e, kValue, 0.4425f);
+    constexpr float kFull[] = {0.190403491f,  0.190687627f,  0.176482618f, 0.17770642f,   0.0470097065f,
+                               0.303873807f, -0.316098958f, 0.435148358f, -0.256638408f, 0.0514253378f};
+    const float half = !FAST ? behind(z, e, kFull, 0.3375f) : SLOPE ? behind(z, e, kSlope, 0.4375f) : behind(z, e, kValue, 0.4425f);
     return z < 0.f ? half : 1.f - half;
 }
 // 1 / (1 + e^{-z}), and what it lacks to one, from e^{-|z|}: neither is lost where the other is next to one
