@@ -268,7 +268,7 @@ template <bool FAST>
 __device__ __forceinline__ void slopes(Lot &z, int activation) {
     if (activation == FTC_ACTIVATION_RELU) {
 #pragma unroll
-        for (int i = 0; i < kLot; i++) z.x[i] = z.x[i] > 0.f ? 1.f : 0.f;
+        for (int i = 0; i < kLot; i++) z.x[i] = z.x[i] <= 0.f ? 0.f : 1.f;  // (NaN passes it on, as it stays above)
     } else if (activation == FTC_ACTIVATION_GELU) {
 #pragma unroll
         for (int i = 0; i < kLot; i++) {

@@ -35,3 +35,22 @@ def test_tails_in_fp32(device, dtype, activation):
     slope, half = first + second, torch.finfo(dtype).eps / 2
     # (bf16 slopes' polynomials, 1.6e-7, are three of the half steps)
     assert ((grad.double().cpu() - slope).abs() <= half * slope.abs() + room * (first.abs() + second.abs()) + 1e-37).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [24, 21, 5])
+def test_nan_that_is_kept_stays_in_the_gradient_of_relu(device, dtype, width):
+    """Results of NaN pass the gradient on, as torch's relu does: it is zero where the result is."""
+    block = torch.randn(6, width, generator=torch.Generator().manual_seed(1))
+    block[2], block[:, 1], block[4, 0], block[4, 2] = float("nan"), float("nan"), float("inf"), -float("inf")
+    block = block.to(dtype).to(device).requires_grad_(True)
+    bias = torch.zeros(width, device=device, requires_grad=True)
+    gx = torch.randn(6, width, generator=torch.Generator().manual_seed(2)).to(dtype).to(device)
+    keep = ref.kept(block.numel(), 9, 0, 0.5).view(block.shape).to(device)
+    x = residual_dropout(block, p=0.5, seed=9, bias=bias, activation="relu")
+    assert torch.equal(torch.isnan(x), torch.isnan(block) & keep)
+    wanted = torch.where(keep & ~(block <= 0), 2 * gx, 0.0)
+    for leaves in ([block], [block, bias]):
+        grads = torch.autograd.grad(x, leaves, gx, retain_graph=True)
+        assert torch.equal(grads[0], wanted)
