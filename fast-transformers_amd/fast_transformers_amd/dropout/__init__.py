@@ -67,12 +67,13 @@ def _cpu_words(count, seed, offset):
 def _cpu_dropout(block, residual, bias, seeds, activation, dropped, seed, offset):
     if seeds is not None:
         seed, offset = (int(n) & (1 << 64) - 1 for n in seeds)
+    keep = _cpu_words(block.numel(), seed, offset).view(block.shape) >= dropped
     z = block.float() if bias is None else block.float() + bias.float()
+    z = torch.where(keep, z, 0.0)  # (before anything is made of them: gradients of what is dropped afterwards may be 0 x NaN)
     if activation == 2:  # (torch's gelu takes 1 + erf, which loses the tail)
         z = z * (0.5 * torch.special.erfc(z * -(0.5 ** 0.5)))
     else:
         z = {0: lambda t: t, 1: torch.relu, 3: torch.nn.functional.silu}[activation](z)
-    keep = _cpu_words(block.numel(), seed, offset).view(block.shape) >= dropped
     x = torch.where(keep, z * (_ALL / max(1, _ALL - dropped)), 0.0)
     return (x if residual is None else residual.float() + x).to(block.dtype if residual is None else residual.dtype)
 

@@ -54,3 +54,23 @@ def test_nan_that_is_kept_stays_in_the_gradient_of_relu(device, dtype, width):
     for leaves in ([block], [block, bias]):
         grads = torch.autograd.grad(x, leaves, gx, retain_graph=True)
         assert torch.equal(grads[0], wanted)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("activation", [None, "relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_do_not_look_at_dropped_values(device, dtype, activation):
+    gen = torch.Generator().manual_seed(3)
+    block, gx = (torch.randn(20, 33, generator=gen).to(dtype).to(device) for _ in range(2))
+    bias = torch.randn(33, generator=gen).to(device)
+    gone = ~ref.kept(block.numel(), 3, 0, 0.5).view(block.shape).to(device)
+    odd = torch.arange(33, device=device) % 2 == 0
+    spoiled, spoiled_gx = block.clone(), gx.clone()
+    spoiled[gone], spoiled_gx[gone & odd] = float("nan"), float("nan")
+    spoiled[gone & odd], spoiled_gx[gone & ~odd] = -float("inf"), float("inf")
+    results = []
+    for b, g in ((block, gx), (spoiled, spoiled_gx)):
+        leaves = [t.clone().requires_grad_(True) for t in (b, bias)]
+        x = residual_dropout(leaves[0], p=0.5, seed=3, bias=leaves[1], activation=activation)
+        results.append([x.detach(), *torch.autograd.grad(x, leaves, g)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
