@@ -105,6 +105,8 @@ def _cpu_attention(queries, keys, values, log_decay, state, lengths, scale):
         outs.append(scale * (rise * torch.matmul(qc, S) + torch.matmul(A, vc)))
         S = rise[:, :, -1:] * S + torch.matmul((fall * kc).transpose(-1, -2), vc)
     out = torch.cat(outs, 2) if outs else v.new_zeros((N, H, 0, M))
+    if lengths is not None:  # (a state or a row without numbers does not reach them, nor their gradients what is before)
+        out = torch.where(valid[..., None], out, 0.0)
     return out.to(values.dtype), S if outs or state is None else S.clone()
 
 
