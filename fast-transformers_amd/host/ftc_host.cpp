@@ -1227,6 +1227,7 @@ struct NormRows {
     ftc_rows r{nullptr, 0, FTC_F32};
     NormRows(const OptTensor &from, const char *name, const char *what = "residual_norm") {
         if (!from) return;
+        if (from->dim() == 0) error(std::string(what) + ": " + name + " has no dimensions, expected rows");
         width = from->size(-1), rows = width ? from->numel() / width : 0;
         int64_t stride = width;
         if (from->is_contiguous()) {  // (as it is: a view costs half a microsecond)
