@@ -123,7 +123,7 @@ def residual_dropout(block, residual=None, *, p, seed, offset=0, bias=None, acti
             raise RuntimeError("residual_dropout: %s must be a whole number of 64 bits, got %r" % (name, n))
     if not on_gpu and any(t is not None and t.device != block.device for t in (residual, bias, seeds)):
         raise RuntimeError("residual_dropout: all tensors must be on one device")
-    options = (_ACTIVATIONS[activation], int(round(p * _ALL)), index(seed) & (1 << 64) - 1, index(offset) & (1 << 64) - 1)
+    options = (_ACTIVATIONS[activation], int(round(float(p) * _ALL)), index(seed) & (1 << 64) - 1, index(offset) & (1 << 64) - 1)
     if block.device.type == "cpu":
         return _cpu_dropout(block, residual, bias, seeds, *options)
     if not torch.compiler.is_compiling():
