@@ -42,11 +42,12 @@ struct Sizes {
     }
     // The times of launches in n segments side by side, us: a scan's chunks and a start, and where there are several, the states at the
     // borders and their sums.  Measured by the number of segments, the one that this picks first:
-    //   forward: 64 chains of 2048 x 128 x 128, bf16  8: 74 (2 112, 4 75, 6 85)       8 of 4096 x 64 x 64, bf16   32: 32 (8 51, 64 38)
-    //            128 of 4096 x 128 x 128, bf16        4: 202 (1 272, 2 224, 8 242)    256 of 4096 x 64 x 64, bf16  3: 168 (1 201, 2 179, 4 190)
-    //            256 of 1024 x 128 x 128, bf16        1: 75 (2 99, 4 131)             192 of 2048 x 64 x 64, fp32  4: 156 (1 190, 2 170, 8 166)
-    //   with its backward: 80 of 1000 x 64 x 64, fp32 6: 179 (2 235, 4 181, 16 221)   16 of 16384 x 64 x 64, bf16 43: 245 (16 294, 32 248, 128 300)
-    //            64 of 2048 x 128 x 128, bf16         4: 261 (8 279)                  32 of 1024 x 128 x 128, fp32 8: 181 (1 480, 4 219, 16 247)
+    //   forward: 64 chains of 2048 x 128 x 128, bf16  8: 78 (2 116, 4 79, 6 88)       8 of 4096 x 64 x 64, bf16   32: 31 (8 49, 64 38)
+    //            128 of 4096 x 128 x 128, bf16        4: 219 (1 285, 2 234, 8 248)    256 of 4096 x 64 x 64, bf16  3: 180 (1 202, 2 189, 4 194)
+    //            256 of 1024 x 128 x 128, bf16        1: 79 (2 79, 4 80, walked)      192 of 2048 x 64 x 64, fp32  4: 160 (1 193, 2 176, 8 164)
+    //   with its backward: 80 of 1000 x 64 x 64, fp32 6: 174 (2 226, 4 193, 16 216)   16 of 16384 x 64 x 64, bf16 43: 238 (16 280, 32 245, 128 294)
+    //            64 of 2048 x 128 x 128, bf16         4: 262 (8 277)                  32 of 1024 x 128 x 128, fp32 8: 186 (1 456, 4 212, 16 244)
+    //            128 on 64 of keys, 4096 x 128 x 128, bf16  4: 782 to 800 (5 913, 8 886)
     double scan(int64_t n, int64_t tasks) const {
         const double all = (double)(tasks * chains() * n);
         return (double)((chunks() + n - 1) / n) * chunk(all) + 5 * std::ceil(all / (256.0 * held()));

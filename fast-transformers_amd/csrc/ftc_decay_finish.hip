@@ -1,8 +1,8 @@
 // Decayed linear attention, behind the scans: the states at the segments' borders from what each segment writes, the gradients of
 // the log decays from what every position receives and sends, and the gradients of shared queries and keys from their shares.
-// Formulas: ftc_decay_kernel.h.  All sums are in a fixed order.  What bounds them is latency: borders 9.7 us for 128 chains of four segments
-// of 128 x 128 (50 MB, 5.2 TB/s), 10.2 for 16 of 43 of 64 x 64 (six reads of eight, one after the other); the gradients of log decays 18 us for 128 chains
-// of 4096 positions (9.5 MB; sums in 64 bits), 6.6 for 80 of 1000, and 4 where they are those of heads.
+// Formulas: ftc_decay_kernel.h.  All sums are in a fixed order.  What bounds them is latency: borders 8.3 us for 128 chains of four segments
+// of 128 x 128 (50 MB, 6.1 TB/s, some of it from the last cache), 10.2 for 16 of 43 of 64 x 64 (six reads of eight, one after the other); the gradients of log decays 15 us for 128 chains
+// of 4096 positions (9.5 MB; sums in 64 bits), 6.4 for 80 of 1000, and 4.6 more where they are those of heads.
 #include "ftc_decay_kernel.h"
 
 namespace ftc {

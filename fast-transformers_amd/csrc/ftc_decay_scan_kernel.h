@@ -9,12 +9,14 @@
 // Pieces.  Products of rows are exact on the bf16 matrix cores, of fp32 rows in three pieces.  The state that is written
 // takes three pieces of what it adds, and so does whatever becomes a gradient of the decays: those are results of fp32.
 // What only becomes a result of bf16 takes two (to 2^-17, where its own rounding is 2^-8): 128 chains of 4096 x 128 x 128, bf16, take
-// 235 us forward with two and 253 with three.
+// 225 us forward with two and 238 with three.
 //
 // What bounds it: vector instructions (cuts into pieces, factors, addresses) and what a chunk's phases wait for each other, not memory.  A
-// launch of that size takes 174 us (403 MB of rows, 2.3 TB/s; vector instructions 57 % of a SIMD's cycles, matrix instructions 36 %, LDS 33 %
-// of a compute unit's), one that makes the states alone 77 (201 MB), the queries' and keys' gradients together 480 to 520.  80 chains of 1000 x 64 x 64,
-// fp32: 36, 15 and 69 us, 480 workgroups (of four wavefronts) that walk three chunks each: 5.7 us a chunk by themselves, 9 for two of them.
+// launch of that size takes 138 us (403 MB of rows, 2.9 TB/s; vector instructions 57 % of a SIMD's cycles, matrix instructions 36 %, LDS 33 %
+// of a compute unit's), one that makes the states alone 60 (201 MB), the queries' and keys' gradients together 360.  (So they take in a row of passes;
+// the first ones, before the card is at its clocks, take up to 30 % longer, in as many cycles.)  80 chains of 1000 x 64 x 64,
+// fp32: 32, 15 and 63 us, 480 workgroups (of four wavefronts) that walk three chunks each: 5.7 us a chunk by themselves, 9 for two of them.
+// Figures that stand side by side in these comments are of one card, taken in turn.
 //
 // Tried: wavefronts in two groups, one for the state and one for A, for fp32 rows (52 us forward as before, 227 with the gradients
 // instead of 182: registers); operands of two columns of wavefronts read once (spills); first remainders of pieces as dot products (they have

@@ -18,7 +18,8 @@
 // a lane's columns staying the same, and leaves them in the workspace for a second kernel, which adds them up in a fixed order.
 //
 // What bounds it: memory, for 40960 x 512 of fp32 onto a stream 48 us (252 MB, 5.2 TB/s) and back 32 (168 MB, 5.2 TB/s); with gelu the vector
-// unit as well, 16384 x 8192 of bf16 140 us (537 MB, 3.8 TB/s) and back 174 (805 MB and 17 of sums, 4.7 TB/s), then 6 to add them up.
+// unit as well, 16384 x 8192 of bf16 147 to 152 us (537 MB, 3.6 TB/s) and back 176 (805 MB and 17 of sums, 4.7 TB/s), then 6 to add them up.  Without
+// the generator, p = 0, the former is 8 to 12 % faster.
 #include <algorithm>
 
 #include "ftc_norm_kernel.h"
@@ -33,8 +34,8 @@ using norm::Rows;
 using norm::u32x4;
 
 constexpr int kThreads = 256;
-// Lots of a lane that are on their way at a time.  One: 16384 x 8192 148 and 186 us instead of 140 and 175; four: 5411 x 1001 14.8 instead of
-// 13.6, 40960 x 512 (fp32) 85 us in both directions instead of 82.
+// Lots of a lane that are on their way at a time.  Forward and backward, us, with one, two and four: 16384 x 8192 (bf16, bias, gelu) 336, 329, 336; 5411 x
+// 1001 (bf16 onto fp32, bias, relu) 29.8, 30.1, 32.8; 40960 x 512 (fp32) 78, 78.5, 82.5.
 constexpr int kAtOnce = 2;
 constexpr int64_t kMostWidth = 1 << 18;
 constexpr uint32_t kAll = 1 << 16;  // of the parts that p is counted in, each of 2^16 smaller ones
@@ -330,8 +331,8 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(Args p) {
     }
 }
 
-// ... with a bias: a workgroup's lanes keep their columns and walk the rows.  (Measured, 16384 x 8192, bf16, gelu: 158 us with the bias
-// loaded with every lot.)
+// ... with a bias: a workgroup's lanes keep their columns and walk the rows.  (us, and with the bias loaded with every lot: 5411 x 1001 13.7, 14.9;
+// 16384 x 8192 147, 148; 20000 x 768 25.7, 22.7.)
 template <typename T, typename X, bool WHOLE, bool SHORT>
 __global__ __launch_bounds__(kThreads) void dropout_bias_kernel(Args p) {
     const int across = p.across, teams = kThreads / across, lane = threadIdx.x % across, team = threadIdx.x / across;
@@ -488,9 +489,9 @@ int read_call(const ftc_residual_dropout_call *c, bool back, Args *p) {
     return FTC_OK;
 }
 // Workgroups that walk rows: 2048, eight a compute unit, but not so many that a team has fewer than four rows (each leaves a row of sums,
-// which are added up later), down to 512.  Measured, forward and backward, us, by the least number of rows, 1, 2, 4, 8: 5411 x 1001 35.6, 33.0,
-// 29.1, 29.5; 1000 x 4096 33.9, 26.7, 23.6, 23.7; 20000 x 768 44.6, 44.6, 44.8, 42.5; 16384 x 8192 (512 parts of four) 313 to 319, and 340 with
-// 256 parts.
+// which are added up later), down to 512.  Measured, forward and backward, us, by the least number of rows, 1, 2, 4, 8: 5411 x 1001 (bf16 onto fp32,
+// relu) 35.3, 33.5, 30.1, 31.4; of bf16 with gelu 1000 x 4096 34.2, 27.6, 24.9, 25.0; 20000 x 768 60.5, 61.0, 60.6, 61.1; 16384 x 8192 (512 parts of
+// four columns of workgroups) 328 to 337 whichever.
 void plan_walk(Args *p) {
     p->across = 1;
     while (p->across < p->lots && p->across < kThreads) p->across *= 2;
