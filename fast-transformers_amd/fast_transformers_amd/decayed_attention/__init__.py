@@ -121,7 +121,7 @@ def decayed_attention(queries, keys, values, log_decay, initial_state=None, *, s
     leave the state as it is, are not looked at, and have outputs and gradients of zero.
 
     Returns the outputs, ``(N, H, L, M)`` in the values' type, and with ``return_state`` also the state after the
-    last position, float32.  E is at most 128, M at most 512; N H ceil(M / 128) is below 2^23 on the GPU, and in
+    last position, float32.  E is at most 128, M at most 512; N H ceil(M / 128) is below 2^21 on the GPU, and in
     a call that will be differentiated below 2^20 and, times ceil(L / 1024), below 2^22.
     Differentiable once, in reverse, with respect to everything
     but ``lengths`` and ``scale``; a call that will be differentiated keeps the states every 1024 positions or fewer.  Log decays are
